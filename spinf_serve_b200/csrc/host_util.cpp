@@ -1,5 +1,7 @@
 #include "host_util.h"
 
+#include "paged_pool.h"
+
 #include <mutex>
 
 namespace spinf {
@@ -58,6 +60,22 @@ int make_tmap_3d(CUtensorMap* out, CUtensorMapDataType dt, int elem_bytes, const
   cuuint32_t box[3] = {b0, b1, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(out, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : SPINF_ERR_TENSORMAP;
+}
+
+// (64 dims, rows of a page, 64-dim slabs of a head's row, heads, pages): rank 5, the most a tensor map has
+int make_tmap_pages(CUtensorMap* out, const PagedPool& p, uint32_t box_rows, uint32_t box_slabs) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return SPINF_ERR_TENSORMAP;
+  if ((reinterpret_cast<uintptr_t>(p.base) & 15) || (p.s_row & 7) || (p.s_head & 7) || (p.s_page & 7) || p.dim % 64 || p.s_row < p.dim)
+    return SPINF_ERR_TENSORMAP;
+  cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(p.page), static_cast<cuuint64_t>(p.dim / 64), static_cast<cuuint64_t>(p.heads),
+                        static_cast<cuuint64_t>(p.n_pages)};
+  cuuint64_t strides[4] = {static_cast<cuuint64_t>(p.s_row) * 2, 128, static_cast<cuuint64_t>(p.s_head) * 2, static_cast<cuuint64_t>(p.s_page) * 2};
+  cuuint32_t box[5] = {64, box_rows, box_slabs, 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(p.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : SPINF_ERR_TENSORMAP;
 }

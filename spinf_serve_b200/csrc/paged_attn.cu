@@ -1,0 +1,660 @@
+// Attention of new tokens over the paged K/V cache: out = softmax(scale q K^T) V over the slots a row sees.
+//
+//   paged_rows_kernel     sequences with few rows per key / value head (at most 64 = tokens x heads that share it): a decoding step,
+//                         a question branch. Bound by reading K and V once.
+//   paged_join_kernel     joins the splits of a sequence: out = sum_c e^(m_c - m) O_c / sum_c e^(m_c - m) l_c
+//   paged_weight_kernel   adds each key's attention weight, sum over rows and heads of p, from the scores the first kernel kept
+//
+// paged_rows_kernel: persistent CTAs, one per SM; an item is (sequence, 64-row tile, kv head, split of the keys). One producer lane
+// brings K and V pages in with TMA, 64 keys at a time, into one ring that runs ahead across items; eight warps work on tiles of 128
+// keys. S: each warp takes 16 keys of the tile against all rows (warp-level mma.sync: at most 64 rows, so the products are far from
+// bounding: a tile of 128 keys takes about 5 700 cycles to arrive at an SM's share of HBM). The row maxima are exchanged through
+// shared memory, P goes to shared memory as bf16, and for P V each warp takes an eighth of the head dimensions over all 128 keys, so
+// the output needs no exchange and K and V are read from shared memory once. Running maximum and sum in fp32; P is rounded to bf16
+// for the product (its operands are 16 bit), which adds about what rounding the output to bf16 adds; the sum takes p unrounded.
+#include "gdn_mma.cuh"
+#include "paged.cuh"
+
+#include <atomic>
+
+namespace spinf {
+
+static constexpr int RT = 64;            // query rows per item
+static constexpr int ROWS_THREADS = 288;  // eight warps and the producer
+
+template <int D>
+struct RowsSmem {
+  static constexpr int SLABS = D / 64;
+  static constexpr int STAGE = 64 * D * 2;  // 64 keys of K or V
+  static constexpr int NST = D == 256 ? 5 : 10;
+  static constexpr int Q_OFF = NST * STAGE;
+  static constexpr int P_OFF = Q_OFF + RT * D * 2;
+  static constexpr int RED_OFF = P_OFF + RT * PG_TILE * 2;  // [64][8] floats, twice: row maxima, row sums
+  static constexpr int PRE_OFF = RED_OFF + 2 * RT * 8 * 4;
+  static constexpr int BAR_OFF = PRE_OFF + (PG_MAX_SEQS + 2) * 4;
+  static constexpr int TOTAL = BAR_OFF + 2 * NST * 8 + 16 + 1024;
+};
+static_assert(RowsSmem<256>::TOTAL <= 232448 && RowsSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
+static_assert(RowsSmem<256>::PRE_OFF % 8 == 0 && RowsSmem<256>::BAR_OFF % 8 == 0 && RowsSmem<128>::BAR_OFF % 8 == 0, "alignment");
+
+struct PagedAttnArgs {
+  const __nv_bfloat16* q;
+  int64_t q_pitch;
+  __nv_bfloat16* out;
+  int64_t out_pitch;
+  int H, h, group, window;
+  float scale_log2;
+  // joined later: part_o [B][seq_parts][D], part_ml [B][seq_parts][2] (maximum in log2 units, sum)
+  float* part_o;
+  float2* part_ml;
+  int64_t seq_parts;
+  float* lse;     // [n][H] log2 units, or null: what the weights are normalised with
+  float* scores;  // [B][tok_cap][H][score_pitch] log2 units, or null: kept for the weights
+  int64_t score_pitch;
+  int tok_cap;
+};
+
+// the rule for the few-row kernel
+__device__ __forceinline__ bool rows_class(const PagedSeq& q, int group) { return q.nq > 0; }
+__device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
+  const int rt = (q.nq * a.group + RT - 1) / RT;
+  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 1);
+}
+__device__ __forceinline__ int rows_items(const PagedSeqs& s, const PagedAttnArgs& a, int b, int* status) {
+  const PagedSeq q = paged_seq(s, b, status);
+  if (!rows_class(q, a.group)) return 0;
+  const PagedCut c = rows_cut(q, a);
+  return a.h * c.row_tiles * c.splits;
+}
+
+struct RowsItem {
+  int b, g, rt, split;
+  PagedSeq q;
+  PagedCut c;
+  int r0, rows;    // first row of the tile within the sequence's rows of the head (token * group + head in group), rows of the tile
+  int lo, hi;      // slots that some row of the tile sees
+  int t0, t1;      // key tiles of this split that hold some of them
+};
+
+__device__ __forceinline__ RowsItem rows_item(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int it, int* status) {
+  RowsItem w;
+  w.b = paged_find(pre, s.B, it);
+  w.q = paged_seq(s, w.b, status);
+  w.c = rows_cut(w.q, a);
+  int x = it - pre[w.b];
+  w.rt = x % w.c.row_tiles;
+  x /= w.c.row_tiles;
+  w.g = x % a.h;
+  w.split = x / a.h;
+  w.r0 = w.rt * RT;
+  const int all = w.q.nq * a.group;
+  w.rows = all - w.r0 < RT ? all - w.r0 : RT;
+  const int first = w.q.len - w.q.nq + w.r0 / a.group, last = w.q.len - w.q.nq + (w.r0 + w.rows - 1) / a.group;
+  w.lo = a.window > 0 && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
+  w.hi = last + 1 > 0 ? last + 1 : 0;
+  const int s0 = w.c.t_lo + w.split * w.c.tiles_per_split, s1 = s0 + w.c.tiles_per_split;
+  const int e0 = w.lo / PG_TILE, e1 = (w.hi + PG_TILE - 1) / PG_TILE;
+  w.t0 = s0 > e0 ? s0 : e0;
+  w.t1 = s1 < e1 ? s1 : e1;
+  if (w.t1 > w.c.t_hi) w.t1 = w.c.t_hi;
+  return w;
+}
+
+// byte offset of (key, 16-byte chunk of its row) in a stage: boxes of 2^br rows x all slabs, 128-byte swizzled
+template <int D>
+__device__ __forceinline__ uint32_t stage_offset(int key, int chunk, int br) {
+  const int box = key >> br, row = key & ((1 << br) - 1);
+  return box * (D * 2 << br) + ((chunk >> 3) * 128 << br) + sw128_offset(row, chunk & 7);
+}
+
+template <int D, int MT>
+__device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArgs& a, const RowsItem& w, uint8_t* smem, uint64_t* full,
+                                          uint64_t* empty, uint32_t& cnt, const WaitCtx& wc, int br) {
+  using L = RowsSmem<D>;
+  constexpr int KS = D / 16;       // 16-dimension steps of S
+  constexpr int DW = D / 8;        // head dimensions a warp takes in P V
+  constexpr int NT = DW / 8;       // 8-column tiles of them
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
+  float* red_m = reinterpret_cast<float*>(smem + L::RED_OFF);
+  float* red_l = red_m + RT * 8;
+  const uint32_t q_base = smem_u32(smem + L::Q_OFF), p_base = smem_u32(smem + L::P_OFF);
+
+  // Q rows of the item, zero behind the last one
+  for (int x = threadIdx.x; x < MT * 16 * (D / 8); x += 256) {
+    const int r = x / (D / 8), c = x % (D / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < w.rows) {
+      const int rr = w.r0 + r, tok = rr / a.group, hd = w.g * a.group + rr % a.group;
+      v = *reinterpret_cast<const uint4*>(a.q + (w.q.row0 + tok) * a.q_pitch + static_cast<int64_t>(hd) * D + c * 8);
+    }
+    *reinterpret_cast<uint4*>(smem + L::Q_OFF + (c >> 3) * (RT * 128) + sw128_offset(r, c & 7)) = v;
+  }
+  // this thread's rows: 16 m + lane / 4 and 8 more; the slots each sees
+  int lo_r[MT][2], hi_r[MT][2];
+  int lo_max = 0, hi_min = 0x7fffffff;
+  {
+    const int base = w.q.len - w.q.nq;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        int r = m * 16 + (lane >> 2) + 8 * x;
+        r = r < w.rows ? r : w.rows - 1;
+        const int slot = base + (w.r0 + r) / a.group;
+        hi_r[m][x] = slot;
+        lo_r[m][x] = a.window > 0 ? slot - a.window + 1 : 0;
+      }
+    lo_max = a.window > 0 ? base + (w.r0 + w.rows - 1) / a.group - a.window + 1 : 0;
+    hi_min = base + w.r0 / a.group;
+  }
+  float o[MT][NT][4];
+  float m_run[MT][2], l_run[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[m][t][x] = 0.f;
+    m_run[m][0] = m_run[m][1] = -INFINITY;
+    l_run[m][0] = l_run[m][1] = 0.f;
+  }
+  named_bar_sync(1, 256);
+
+  for (int t = w.t0; t < w.t1; ++t, cnt += 4) {
+    // ---- S of this warp's 16 keys
+    const int hf = warp >> 2, key0 = (warp & 3) * 16;  // stage of the tile, first key within it
+    bool ok = true;
+    {
+      const uint32_t c = cnt + hf;
+      ok = mbar_wait(wc, &full[c % L::NST], (c / L::NST) & 1u, ST_TIMEOUT_FULL);
+    }
+    float sc[MT][2][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sc[m][0][x] = sc[m][1][x] = 0.f;
+    if (ok) {
+      const uint32_t k_base = smem_u32(smem) + ((cnt + hf) % L::NST) * L::STAGE;
+      const int kk = key0 + ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t kf[4];
+        const uint32_t ka = k_base + stage_offset<D>(kk, ks * 2 + ((lane >> 3) & 1), br);
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(kf[0]), "=r"(kf[1]), "=r"(kf[2]), "=r"(kf[3]) : "r"(ka));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint32_t qf[4];
+          const int chunk = ks * 2 + (lane >> 4);
+          const uint32_t qa = q_base + (chunk >> 3) * (RT * 128) + sw128_offset(m * 16 + (lane & 15), chunk & 7);
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(qf[0]), "=r"(qf[1]), "=r"(qf[2]), "=r"(qf[3]) : "r"(qa));
+          mma_bf16(sc[m][0], qf, kf[0], kf[1]);
+          mma_bf16(sc[m][1], qf, kf[2], kf[3]);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) {  // this warp has read its keys of the two K stages (it used one of them)
+      mbar_arrive(&empty[cnt % L::NST]);
+      mbar_arrive(&empty[(cnt + 1) % L::NST]);
+    }
+    // ---- mask, row maxima
+    const int j0 = t * PG_TILE + hf * 64 + key0 + quad * 2;
+    const bool masked = (t + 1) * PG_TILE - 1 > hi_min || t * PG_TILE < lo_max;
+    float mx[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      mx[m][0] = mx[m][1] = -INFINITY;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float v = sc[m][nt][x] * a.scale_log2;
+          const int j = j0 + nt * 8 + (x & 1);
+          if (masked && (j > hi_r[m][x >> 1] || j < lo_r[m][x >> 1])) v = -INFINITY;
+          sc[m][nt][x] = v;
+          mx[m][x >> 1] = fmaxf(mx[m][x >> 1], v);
+        }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        mx[m][x] = fmaxf(mx[m][x], __shfl_xor_sync(0xffffffffu, mx[m][x], 1));
+        mx[m][x] = fmaxf(mx[m][x], __shfl_xor_sync(0xffffffffu, mx[m][x], 2));
+        if (quad == 0) red_m[(m * 16 + (lane >> 2) + 8 * x) * 8 + warp] = mx[m][x];
+      }
+    }
+    if (a.scores) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = m * 16 + (lane >> 2) + 8 * x;
+          if (r < w.rows) {
+            const int rr = w.r0 + r;
+            float* dst = a.scores + ((static_cast<int64_t>(w.b) * a.tok_cap + rr / a.group) * a.H + w.g * a.group + rr % a.group) * a.score_pitch + j0;
+            *reinterpret_cast<float2*>(dst) = make_float2(sc[m][0][2 * x], sc[m][0][2 * x + 1]);
+            *reinterpret_cast<float2*>(dst + 8) = make_float2(sc[m][1][2 * x], sc[m][1][2 * x + 1]);
+          }
+        }
+    }
+    if (!bar_red_and(1, 256, ok)) return false;
+    // ---- new maxima, P
+    float alpha[MT][2];
+    bool moved = false;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = m * 16 + (lane >> 2) + 8 * x;
+        const float4 u = *reinterpret_cast<const float4*>(red_m + r * 8), v = *reinterpret_cast<const float4*>(red_m + r * 8 + 4);
+        const float m_new = fmaxf(m_run[m][x], fmaxf(fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w)), fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
+        alpha[m][x] = m_new == m_run[m][x] ? 1.f : fast_exp2(m_run[m][x] - m_new);  // (equal covers a row that has seen nothing yet)
+        moved |= alpha[m][x] != 1.f;
+        m_run[m][x] = m_new;
+        const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const float p0 = fast_exp2(sc[m][nt][2 * x] + neg_m), p1 = fast_exp2(sc[m][nt][2 * x + 1] + neg_m);
+          sum += p0 + p1;
+          const int col = hf * 64 + key0 + nt * 8;  // key of the tile
+          const uint32_t off = (col >> 6) * (RT * 128) + sw128_offset(r, (col >> 3) & 7) + quad * 4;
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(p_base + off), "r"(pack_bf16x2(p0, p1)) : "memory");
+        }
+        l_run[m][x] = l_run[m][x] * alpha[m][x] + sum;
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[m][nt][x] *= alpha[m][x >> 1];
+    }
+    named_bar_sync(1, 256);
+    // ---- O += P V over this warp's head dimensions
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t c = cnt + 2 + half, st = c % L::NST;
+      ok = ok && mbar_wait(wc, &full[st], (c / L::NST) & 1u, ST_TIMEOUT_FULL);
+      if (ok) {
+        const int j_first = t * PG_TILE + half * 64;
+        if (j_first < w.lo || j_first + 64 > w.hi) {
+          // slots no row of the tile sees may hold anything (or were not copied): p is 0 there, but 0 * inf is not. Each warp clears
+          // what it reads.
+          for (int x = lane; x < 64 * (DW / 8); x += 32) {
+            const int key = x / (DW / 8), ch = warp * (DW / 8) + x % (DW / 8);
+            if (j_first + key < w.lo || j_first + key >= w.hi)
+              *reinterpret_cast<uint4*>(smem + st * L::STAGE + stage_offset<D>(key, ch, br)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();  // the stage is refilled by the copy engine
+          __syncwarp();
+        }
+        const uint32_t v_base = smem_u32(smem) + st * L::STAGE;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          uint32_t pf[MT][4];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint32_t pa = p_base + half * (RT * 128) + sw128_offset(m * 16 + (lane & 15), kk * 2 + (lane >> 4));
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(pf[m][0]), "=r"(pf[m][1]), "=r"(pf[m][2]), "=r"(pf[m][3]) : "r"(pa));
+          }
+          const int key = kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+          for (int np = 0; np < NT / 2; ++np) {
+            uint32_t vf[4];
+            const uint32_t va = v_base + stage_offset<D>(key, warp * (DW / 8) + np * 2 + (lane >> 4), br);
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(vf[0]), "=r"(vf[1]), "=r"(vf[2]), "=r"(vf[3]) : "r"(va));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              mma_bf16(o[m][2 * np], pf[m], vf[0], vf[1]);
+              mma_bf16(o[m][2 * np + 1], pf[m], vf[2], vf[3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    if (!ok) *wc.abort_flag = 1;  // the next barrier with a vote ends the CTA's warps together
+  }
+  // ---- row sums over the warps' keys, then the rows out
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float l = l_run[m][x];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (quad == 0) red_l[(m * 16 + (lane >> 2) + 8 * x) * 8 + warp] = l;
+    }
+  if (!bar_red_and(1, 256, !*wc.abort_flag)) return false;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = m * 16 + (lane >> 2) + 8 * x;
+      if (r >= w.rows) continue;
+      const float4 u = *reinterpret_cast<const float4*>(red_l + r * 8), v = *reinterpret_cast<const float4*>(red_l + r * 8 + 4);
+      const float l = ((u.x + u.y) + (u.z + u.w)) + ((v.x + v.y) + (v.z + v.w));
+      const int rr = w.r0 + r, tok = rr / a.group, hd = w.g * a.group + rr % a.group;
+      if (w.c.splits == 1) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row that sees nothing: 0; a NaN sum stays NaN
+        __nv_bfloat16* dst = a.out + (w.q.row0 + tok) * a.out_pitch + static_cast<int64_t>(hd) * D + warp * DW + quad * 2;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<uint32_t*>(dst + nt * 8) = pack_bf16x2(o[m][nt][2 * x] * inv, o[m][nt][2 * x + 1] * inv);
+        if (a.lse && warp == 0 && quad == 0) a.lse[static_cast<int64_t>(w.q.row0 + tok) * a.H + hd] = m_run[m][x] + log2f(l);
+      } else {
+        const int64_t at = w.b * a.seq_parts + (static_cast<int64_t>(w.split) * a.h + w.g) * (w.q.nq * a.group) + rr;
+        float* dst = a.part_o + at * D + warp * DW + quad * 2;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(o[m][nt][2 * x], o[m][nt][2 * x + 1]);
+        if (warp == 0 && quad == 0) a.part_ml[at] = make_float2(m_run[m][x], l);
+      }
+    }
+  return true;
+}
+
+template <int D>
+__global__ void __launch_bounds__(ROWS_THREADS, 1)
+paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedSeqs s, const PagedAttnArgs a,
+                  int* __restrict__ status) {
+  using L = RowsSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* empty = full + L::NST;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + L::NST);
+  const WaitCtx wc{abort_flag, status};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::NST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 8);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  paged_item_prefix(s.B, pre, ROWS_THREADS, [&](int b) { return rows_items(s, a, b, status); });
+  const int total = pre[s.B];
+  const int br = s.page_log2 < 6 ? s.page_log2 : 6;  // log2 of a box's rows
+
+  if (warp == 8) {
+    if (lane == 0) {
+      uint32_t cnt = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+        const RowsItem w = rows_item(s, a, pre, it, status);
+        const int32_t* pages = s.table + w.b * s.table_pitch;
+        for (int t = w.t0; t < w.t1 && ok; ++t)
+          for (int part = 0; part < 4; ++part, ++cnt) {
+            const uint32_t st = cnt % L::NST;
+            if (!mbar_wait(wc, &empty[st], ((cnt / L::NST) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+            const int j_first = t * PG_TILE + (part & 1) * 64;
+            const int box_rows = 1 << br;
+            // boxes that hold a slot some row sees; the others stay as they are (masked for K, cleared for V)
+            int bytes = 0;
+            uint32_t got = 0;
+            int pg[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int j = j_first + x * box_rows;
+              pg[x] = -1;
+              if (x * box_rows < 64 && j < w.hi && j + box_rows > w.lo) {
+                pg[x] = pages[j >> s.page_log2];
+                if (pg[x] < 0 || pg[x] >= s.n_pages) {
+                  atomicCAS(status, 0, ST_BAD_INDEX);
+                  pg[x] = -1;
+                } else {
+                  got |= 1u << x;
+                  bytes += box_rows * D * 2;
+                }
+              }
+            }
+            mbar_expect_tx(&full[st], bytes);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (got & (1u << x))
+                tma_load_5d(smem + st * L::STAGE + x * box_rows * D * 2, part < 2 ? &tmK : &tmV, 0, (j_first + x * box_rows) & ((1 << s.page_log2) - 1), 0,
+                            w.g, pg[x], &full[st]);
+          }
+      }
+      if (*abort_flag)  // bounded wait for copies that may still be in flight
+        for (uint32_t c = cnt > static_cast<uint32_t>(L::NST) ? cnt - L::NST : 0; c < cnt; ++c)
+          for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % L::NST], (c / L::NST) & 1u); ++spin) {}
+    }
+  } else {
+    uint32_t cnt = 0;
+    for (int it = blockIdx.x; it < total; it += gridDim.x) {
+      const RowsItem w = rows_item(s, a, pre, it, status);
+      bool ok;
+      switch ((w.rows + 15) >> 4) {
+        case 1: ok = rows_work<D, 1>(s, a, w, smem, full, empty, cnt, wc, br); break;
+        case 2: ok = rows_work<D, 2>(s, a, w, smem, full, empty, cnt, wc, br); break;
+        case 3: ok = rows_work<D, 3>(s, a, w, smem, full, empty, cnt, wc, br); break;
+        default: ok = rows_work<D, 4>(s, a, w, smem, full, empty, cnt, wc, br); break;
+      }
+      if (!ok) break;
+    }
+  }
+  __syncthreads();
+}
+
+// one warp per (row, head) whose sequence was split
+template <int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int V = D / 128;  // float4 per lane
+  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedSeq q = paged_seq(s, b, status);
+  if (!rows_class(q, a.group)) return;
+  const PagedCut c = rows_cut(q, a);
+  if (c.splits == 1) return;
+  const int all = q.nq * a.group;
+  for (int64_t x = blockIdx.x * 8 + warp; x < static_cast<int64_t>(q.nq) * a.H; x += gridDim.x * 8) {
+    const int tok = static_cast<int>(x / a.H), hd = static_cast<int>(x % a.H), g = hd / a.group, rr = tok * a.group + hd % a.group;
+    const int64_t at = b * a.seq_parts + static_cast<int64_t>(g) * all + rr, step = static_cast<int64_t>(a.h) * all;
+    float m = -INFINITY;
+    for (int i = lane; i < c.splits; i += 32) m = fmaxf(m, a.part_ml[at + i * step].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f;
+    float4 acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float neg_m = m == -INFINITY ? 0.f : -m;
+#pragma unroll 4
+    for (int i = 0; i < c.splits; ++i) {
+      const float2 ml = a.part_ml[at + i * step];
+      const float f = fast_exp2(ml.x + neg_m);
+      l = fmaf(f, ml.y, l);
+      const float4* src = reinterpret_cast<const float4*>(a.part_o + (at + i * step) * D);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float4 u = src[v * 32 + lane];
+        acc[v].x = fmaf(f, u.x, acc[v].x), acc[v].y = fmaf(f, u.y, acc[v].y), acc[v].z = fmaf(f, u.z, acc[v].z), acc[v].w = fmaf(f, u.w, acc[v].w);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    __nv_bfloat16* dst = a.out + (q.row0 + tok) * a.out_pitch + static_cast<int64_t>(hd) * D;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
+          make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv), pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
+    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd] = m + log2f(l);
+  }
+}
+
+struct PagedWeightArgs {
+  const float* in;  // [B][h][cap] fp32
+  float* out;
+  int64_t in_seq, in_head, out_seq, out_head;  // strides
+  float decay;                                 // 0: `in` is not read
+};
+
+// weights_out[b][g][j] = decay weights[b][g][j] + sum over the sequence's rows of kv head g of p(row, j), for j < len; a thread owns a
+// key and adds its rows in order
+__global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, const PagedAttnArgs a, const PagedWeightArgs w, int* __restrict__ status) {
+  pdl_wait();
+  const int b = blockIdx.z, g = blockIdx.y;
+  const PagedSeq q = paged_seq(s, b, status);
+  const int first = blockIdx.x * 1024;
+  if (first >= q.len) return;
+  const int all = rows_class(q, a.group) ? q.nq * a.group : 0, base = q.len - q.nq;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < all; ++r) {
+    const int tok = r / a.group, hd = g * a.group + r % a.group, hi = base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;
+    const float lse = a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd];
+    const float* src = a.scores + ((static_cast<int64_t>(b) * a.tok_cap + tok) * a.H + hd) * a.score_pitch + first + threadIdx.x;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int j = first + threadIdx.x + x * 256;
+      if (j <= hi && j >= lo) sum[x] += fast_exp2(src[x * 256] - lse);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int j = first + threadIdx.x + x * 256;
+    if (j < q.len) {
+      const float old = w.decay != 0.f ? w.in[b * w.in_seq + g * w.in_head + j] * w.decay : 0.f;
+      w.out[b * w.out_seq + g * w.out_head + j] = old + sum[x];
+    }
+  }
+}
+
+// what a call needs: sizes of the workspace's parts in bytes (256-byte multiples)
+struct PagedSizes {
+  int64_t seq_parts, part_o, part_ml, lse, scores, total;
+  int64_t score_pitch;
+  int tok_cap;
+};
+static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights) {
+  PagedSizes z = {};
+  const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
+  const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
+  if (slots > 1) {
+    const int64_t by_rows = max_q * H * slots;             // every row in every split
+    const int64_t by_items = static_cast<int64_t>(PG_SMS) * RT;  // every free slot one full row tile
+    z.seq_parts = by_rows < by_items ? by_rows : by_items;
+  }
+  z.part_o = up256(B * z.seq_parts * D * 4);
+  z.part_ml = up256(B * z.seq_parts * 8);
+  if (weights) {
+    z.lse = up256(n * H * 4);
+    z.score_pitch = tiles * PG_TILE;
+    z.tok_cap = static_cast<int>(max_q);
+    z.scores = up256(B * z.tok_cap * H * z.score_pitch * 4);
+  }
+  z.total = z.part_o + z.part_ml + z.lse + z.scores;
+  return z;
+}
+
+template <int D>
+static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+                        int max_splits, cudaStream_t st, int dev, int* status) {
+  CUtensorMap tmK, tmV;
+  int r;
+  const uint32_t box = kp.page < 64 ? static_cast<uint32_t>(kp.page) : 64u;
+  if ((r = make_tmap_pages(&tmK, kp, box, D / 64)) || (r = make_tmap_pages(&tmV, vp, box, D / 64))) return r;
+  auto kern = paged_rows_kernel<D>;
+  static std::atomic<bool> attr_set[64];
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    SPINF_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D>::TOTAL));
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  kern<<<static_cast<unsigned>(sm_count()), ROWS_THREADS, RowsSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+  SPINF_CUDA_OK(cudaGetLastError());
+  if (max_splits > 1) {
+    int64_t gx = (max_q * a.H + 7) / 8;
+    if (gx > 4096) gx = 4096;
+    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, s, a, status));
+  }
+  if (w)
+    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, s, a, *w, status));
+  return 0;
+}
+
+}  // namespace spinf
+
+using namespace spinf;
+
+extern "C" int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
+                                                         int32_t weights) {
+  if (n < 0 || B < 0 || B > PG_MAX_SEQS || H <= 0 || Hkv <= 0 || H % Hkv || (D != 128 && D != 256) || max_q < 0 || max_len < 0) return SPINF_ERR_BAD_ARGUMENT;
+  return paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0).total;
+}
+
+extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* k_pages,
+                                     const void* v_pages, int64_t n_pages, int32_t page, const int64_t* k_strides_host,
+                                     const int64_t* v_strides_host, const int32_t* table, int64_t table_pitch, const int32_t* lens,
+                                     const int32_t* cu, int32_t B, int64_t max_q, int64_t max_len, int32_t window, float scale,
+                                     const float* weights_in, float* weights_out, const int64_t* weight_strides_host, float decay,
+                                     void* out, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (B == 0 || (n == 0 && !weights_out)) return 0;  // nothing to do: the row pointers may be null
+  SPINF_CHECK_ARG(k_pages && v_pages && k_strides_host && v_strides_host && table && lens && cu && n >= 0 && B > 0);
+  SPINF_CHECK_ARG(n == 0 || (q && out));
+  SPINF_CHECK_ARG(H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 1024 && (D == 128 || D == 256) && n < (1ll << 31) / H);
+  SPINF_CHECK_ARG(q_pitch >= static_cast<int64_t>(H) * D && out_pitch >= static_cast<int64_t>(H) * D && q_pitch % 8 == 0 && out_pitch % 8 == 0);
+  SPINF_CHECK_ARG(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0);
+  SPINF_CHECK_ARG(page >= 16 && page <= 256 && (page & (page - 1)) == 0 && n_pages > 0 && n_pages < (1ll << 31));
+  SPINF_CHECK_ARG(max_q >= 0 && max_len >= 0 && max_len <= table_pitch * page && max_len < (1ll << 30) && window >= 0 && scale > 0.f);
+  SPINF_CHECK_ARG(!weights_out || (weight_strides_host && (weights_in || decay == 0.f)));
+  if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
+  const int64_t mq = max_q < n ? max_q : n;
+  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr);
+  SPINF_CHECK_ARG(z.total == 0 || (workspace && workspace_bytes >= z.total && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0));
+  int dev = 0;
+  SPINF_CUDA_OK(cudaGetDevice(&dev));
+  int* status = status_word(dev);
+  if (!status) return SPINF_ERR_CUDA;
+  PagedSeqs s;
+  s.table = table;
+  s.table_pitch = table_pitch;
+  s.lens = lens;
+  s.cu = cu;
+  s.B = B;
+  s.n_pages = static_cast<int>(n_pages);
+  s.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
+  s.max_len = static_cast<int>(max_len);
+  s.max_q = static_cast<int>(mq);
+  s.n = n;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PagedAttnArgs a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_pitch = q_pitch;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.out_pitch = out_pitch;
+  a.H = H;
+  a.h = Hkv;
+  a.group = H / Hkv;
+  a.window = window;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.seq_parts = z.seq_parts;
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + z.part_o);
+  if (weights_out) {
+    a.lse = reinterpret_cast<float*>(ws + z.part_o + z.part_ml);
+    a.scores = reinterpret_cast<float*>(ws + z.part_o + z.part_ml + z.lse);
+    a.score_pitch = z.score_pitch;
+    a.tok_cap = z.tok_cap;
+  }
+  PagedWeightArgs w;
+  if (weights_out) {
+    w.in = weights_in;
+    w.out = weights_out;
+    w.in_seq = weight_strides_host[0], w.in_head = weight_strides_host[1];
+    w.out_seq = weight_strides_host[2], w.out_head = weight_strides_host[3];
+    w.decay = decay;
+  }
+  const PagedPool kp = {k_pages, n_pages, page, Hkv, D, k_strides_host[0], k_strides_host[1], k_strides_host[2]};
+  const PagedPool vp = {v_pages, n_pages, page, Hkv, D, v_strides_host[0], v_strides_host[1], v_strides_host[2]};
+  const int max_splits = z.seq_parts ? 2 : 1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return D == 256 ? launch_paged<256>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, st, dev, status)
+                  : launch_paged<128>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, st, dev, status);
+}

@@ -603,3 +603,182 @@ def embed_scale(ids, emb, scale):
     )
     COUNTS["launches"] += 1
     return out
+
+
+# ---- paged K/V cache
+def _pages(k_pages, v_pages, what):
+    """the pools of a paged call, [pages, kv heads, page, D] with unit stride over D -> their shape and the strides of both"""
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.bfloat16 or t.dim() != 4 or t.stride(3) != 1:
+            raise SpinfError(f"{what}: {name} must be a CUDA bf16 [pages, kv heads, page, D] tensor (or view) with unit stride over D")
+    if v_pages.shape != k_pages.shape or v_pages.device != k_pages.device:
+        raise SpinfError(f"{what}: k_pages and v_pages must agree in shape and device")
+    page, D = k_pages.shape[2], k_pages.shape[3]
+    if page < 16 or page > 256 or page & (page - 1) or D not in (128, 256):
+        raise SpinfError(f"{what}: pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {page} of {D}")
+    _lib.init(k_pages.device)
+    i64x3 = ctypes.c_int64 * 3
+    return tuple(k_pages.shape), i64x3(*k_pages.stride()[:3]), i64x3(*v_pages.stride()[:3])
+
+
+def _paged_index(t, name, what, device, shape, pitched=False):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != len(shape):
+        raise SpinfError(f"{what}: {name} must be an int32 tensor of {len(shape)} dimensions on the pages' device")
+    if any(s is not None and s != have for s, have in zip(shape, t.shape)):
+        raise SpinfError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1 or not pitched and not t.is_contiguous():
+        raise SpinfError(f"{what}: {name} must be contiguous")
+
+
+def _table_pitch(table):
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=None, cos=None, sin=None, eps=1e-6, plus1=False, norm_v=False):
+    """a step's rows into the paged cache: qkv [n, (H + 2 Hkv) D] bf16 (rows of any pitch) -> q [n, H, D]; k and v go to the slots of
+    their sequences (spinf_paged_append in include/spinf_b200.h has the layout). wq, wk [D]: head norms of q and k (plus1: weights
+    1 + w); norm_v: norm of v without weight; cos, sin [n, R/2] bf16 (rope_table): rotary embedding over the first R dimensions.
+    Without norms and rotation the returned q is a view of qkv."""
+    what = "paged_append"
+    (n_pages, h, page, Dp), ks, vs = _pages(k_pages, v_pages, what)
+    dev = k_pages.device
+    if not isinstance(qkv, torch.Tensor) or qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise SpinfError(f"{what}: qkv must be a bf16 [n, (H + 2 Hkv) D] tensor on the pages' device with unit stride over its columns")
+    n = qkv.shape[0]
+    if h != Hkv or Dp != D or qkv.shape[1] != (H + 2 * Hkv) * D:
+        raise SpinfError(f"{what}: qkv {tuple(qkv.shape)} and pages {tuple(k_pages.shape)} do not fit {H} / {Hkv} heads of {D}")
+    if (wq is None) != (wk is None) or (cos is None) != (sin is None):
+        raise SpinfError(f"{what}: wq and wk, cos and sin come together")
+    for name, t, shape in (("wq", wq, (D,)), ("wk", wk, (D,)), ("cos", cos, None), ("sin", sin, None)):
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16 or t.device != dev or not t.is_contiguous() or (shape and tuple(t.shape) != shape):
+            raise SpinfError(f"{what}: {name} must be a contiguous bf16 tensor on the pages' device" + (f" of shape {shape}" if shape else ""))
+    rot = 0
+    if cos is not None:
+        rot = 2 * cos.shape[-1]
+        if tuple(cos.shape) != (n, rot // 2) or sin.shape != cos.shape or rot > D or rot % 16:
+            raise SpinfError(f"{what}: cos and sin must be [n, R/2] with R a multiple of 16 of at most D, got {tuple(cos.shape)}")
+    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
+    _paged_index(lens, "lens", what, dev, (None,))
+    _paged_index(cu, "cu", what, dev, (B + 1,))
+    _paged_index(table, "table", what, dev, (B, None), pitched=True)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin, eps, plus1, norm_v)
+    q = qkv[:, : H * D].view(n, H, D) if wq is None and not rot else torch.empty((n, H, D), dtype=torch.bfloat16, device=dev)
+    pitch = qkv.stride(0) if n > 1 else qkv.shape[1]
+    check(
+        _lib.lib().spinf_paged_append(
+            ptr(qkv), pitch, n, H, Hkv, D, ptr(wq), ptr(wk), ptr(cos) if rot else None, ptr(sin) if rot else None, rot, eps, int(plus1), int(norm_v),
+            None if wq is None and not rot else ptr(q), ptr(k_pages), ptr(v_pages), n_pages, page, ks, vs, ptr(table), _table_pitch(table),
+            table.shape[1], ptr(lens), ptr(cu), B, stream_ptr(),
+        ),
+        what,
+    )
+    COUNTS["launches"] += 1
+    return q
+
+
+def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=None, weights=None, weights_out=None, decay=1.0, max_len=None,
+                    out=None, workspace=None):
+    """attention of new tokens over the paged cache: q [n, H, D] bf16 (a view with contiguous heads and any row pitch), sequence b's
+    rows cu[b] .. cu[b + 1] over its lens[b] cached tokens, of which its own rows are the last; causal, with a window only the last
+    `window` slots of a row -> [n, H, D] (rows behind cu[B]: undefined in a new tensor, untouched in `out`; a row that sees nothing:
+    0). max_q, max_len: no sequence has more rows / tokens (max_len None: what the table can hold).
+    weights (fp32 [B, Hkv, cap], cap >= max_len): each slot's accumulated attention weight, weights_out = decay * weights + this
+    call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
+    tensor reused between calls on one stream."""
+    what = "paged_attention"
+    (n_pages, h, page, D), ks, vs = _pages(k_pages, v_pages, what)
+    dev = k_pages.device
+    if not isinstance(q, torch.Tensor) or q.dtype != torch.bfloat16 or q.device != dev or q.dim() != 3 or q.shape[2] != D:
+        raise SpinfError(f"{what}: q must be a bf16 [n, H, {D}] tensor on the pages' device")
+    n, H = q.shape[0], q.shape[1]
+    if H % h or H == 0:
+        raise SpinfError(f"{what}: {H} query heads do not share {h} key / value heads evenly")
+    if out is None:
+        out = torch.empty((n, H, D), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.device != dev or out.shape != q.shape:
+        raise SpinfError(f"{what}: out must be a bf16 tensor of q's shape on the pages' device")
+    for name, t in (("q", q), ("out", out)):
+        if n and (t.stride(2) != 1 or (H > 1 and t.stride(1) != D)):
+            raise SpinfError(f"{what}: {name} needs contiguous heads (any row pitch)")
+    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
+    _paged_index(lens, "lens", what, dev, (None,))
+    _paged_index(cu, "cu", what, dev, (B + 1,))
+    _paged_index(table, "table", what, dev, (B, None), pitched=True)
+    room = table.shape[1] * page
+    max_len = room if max_len is None else max_len
+    if max_len < 0 or max_len > room or max_q < 0:
+        raise SpinfError(f"{what}: max_len {max_len} and max_q {max_q} must not be negative, nor max_len above what the table holds ({room})")
+    if window is not None and window < 1:
+        raise SpinfError(f"{what}: a window has at least one slot (None: no window)")
+    strides = None
+    if weights is None and weights_out is not None:
+        raise SpinfError(f"{what}: weights_out comes with weights")
+    if weights is not None:
+        weights_out = weights if weights_out is None else weights_out
+        for name, t in (("weights", weights), ("weights_out", weights_out)):
+            if t.dtype != torch.float32 or t.device != dev or t.dim() != 3 or tuple(t.shape[:2]) != (B, h) or t.shape[2] < max_len or (t.shape[2] > 1 and t.stride(2) != 1):
+                raise SpinfError(f"{what}: {name} must be an fp32 [{B}, {h}, at least {max_len}] tensor on the pages' device, contiguous over slots")
+        strides = (ctypes.c_int64 * 4)(weights.stride(0), weights.stride(1), weights_out.stride(0), weights_out.stride(1))
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace)
+    lib = _lib.lib()
+    need = lib.spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, weights is not None)
+    check(need, what)
+    if need and (workspace is None or workspace.numel() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    check(
+        lib.spinf_paged_attention(
+            ptr(q), q.stride(0) if n > 1 else H * D, n, H, h, D, ptr(k_pages), ptr(v_pages), n_pages, page, ks, vs, ptr(table), _table_pitch(table),
+            ptr(lens), ptr(cu), B, max_q, max_len, window or 0, scale, ptr(weights), ptr(weights_out), strides, decay, ptr(out),
+            out.stride(0) if n > 1 else H * D, ptr(workspace) if need else None, need, stream_ptr(),
+        ),
+        what,
+    )
+    COUNTS["launches"] += 2 if weights is None else 3
+    return out
+
+
+def paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table, max_len=None):
+    """cuts every sequence back to `keep` cached tokens per kv head: the last `recent` slots and, of the others, those with the largest
+    accumulated weight (weights fp32 [B, Hkv, cap] as paged_attention keeps them; None: the last `keep` slots stay; ties: the lowest
+    slot). What stays is copied in slot order to the pages of new_table int32 [B, at least keep / page], none of which `table` may
+    name -> (new lens int32 [B], kept int32 [B, Hkv, keep]: the old slots, -1 behind the last, their weights [B, Hkv, keep] or None).
+    The old pages are the caller's to reuse."""
+    what = "paged_evict"
+    (n_pages, h, page, D), ks, vs = _pages(k_pages, v_pages, what)
+    dev = k_pages.device
+    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
+    _paged_index(lens, "lens", what, dev, (None,))
+    _paged_index(table, "table", what, dev, (B, None), pitched=True)
+    _paged_index(new_table, "new_table", what, dev, (B, None), pitched=True)
+    if keep < 1 or recent < 0 or recent > keep or keep > new_table.shape[1] * page:
+        raise SpinfError(f"{what}: keep {keep} needs at least one token and as many as new_table holds at most, recent {recent} between 0 and keep")
+    room = table.shape[1] * page
+    if weights is not None:
+        if weights.dtype != torch.float32 or weights.device != dev or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, h) or (weights.shape[2] > 1 and weights.stride(2) != 1):
+            raise SpinfError(f"{what}: weights must be an fp32 [{B}, {h}, cap] tensor on the pages' device, contiguous over slots")
+        room = min(room, weights.shape[2])
+    max_len = room if max_len is None else max_len
+    if max_len < 0 or max_len > room:
+        raise SpinfError(f"{what}: max_len {max_len} is more than the table and the weights hold ({room})")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table, max_len)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    kept = torch.empty((B, h, keep), dtype=torch.int32, device=dev)
+    w_out = None if weights is None else torch.empty((B, h, keep), dtype=torch.float32, device=dev)
+    check(
+        _lib.lib().spinf_paged_evict(
+            ptr(k_pages), ptr(v_pages), n_pages, page, h, D, ks, vs, ptr(table), _table_pitch(table), ptr(lens), B, max_len, ptr(weights),
+            0 if weights is None else weights.stride(0), 0 if weights is None else weights.stride(1), keep, keep if weights is None else recent,
+            ptr(new_table), _table_pitch(new_table), ptr(new_lens), ptr(kept), ptr(w_out), stream_ptr(),
+        ),
+        what,
+    )
+    COUNTS["launches"] += 2
+    return new_lens, kept, w_out

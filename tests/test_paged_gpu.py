@@ -1,0 +1,337 @@
+"""GPU parity of the paged K/V cache's operators (append, attention, eviction) against their definitions in 64 bits, with every slot
+that no row sees filled with NaN; streams, captured graphs, batch invariance and far offsets."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import paged as OP
+from spinf_serve_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+BF = 2.0**-8  # half a step of bf16, relative
+
+
+class Call:
+    """one call's tensors: NaN everywhere in the pools but in the sequences' slots; pages handed out in random order"""
+
+    def __init__(self, dev, H, h, D, page, seqs, seed=0, token_major=False, spare=3, extra_rows=0, shared_tokens=0, loud=0.5):
+        g = torch.Generator().manual_seed(seed)
+        self.H, self.h, self.D, self.page, self.dev = H, h, D, page, dev
+        self.lens, news = [L for L, _ in seqs], [n for _, n in seqs]
+        B = len(seqs)
+        shared = shared_tokens // page
+        need = [max(0, -(-L // page) - shared) for L in self.lens]
+        self.n_pages = sum(need) + shared + spare
+        order = torch.randperm(self.n_pages, generator=g).to(torch.int32)
+        width = max(1, max(-(-L // page) for L in self.lens))
+        self.table = torch.full((B, width), -7, dtype=torch.int32)  # entries behind a sequence's pages are never used
+        at = shared
+        for b in range(B):
+            self.table[b, :shared] = order[:shared]
+            self.table[b, shared : shared + need[b]] = order[at : at + need[b]]
+            at += need[b]
+        self.free = order[at:]
+        shape = (self.n_pages, page, h, D) if token_major else (self.n_pages, h, page, D)
+        k, v = (torch.full(shape, math.nan, dtype=torch.bfloat16) for _ in range(2))
+        if token_major:
+            k, v = k.transpose(1, 2), v.transpose(1, 2)
+        for b in range(B):
+            for s in range(self.lens[b]):
+                pg = int(self.table[b, s // page])
+                if math.isnan(float(k[pg, 0, s % page, 0])):
+                    size = 1 + loud * torch.randn((h, 1), generator=g).abs()
+                    k[pg, :, s % page] = (torch.randn((h, D), generator=g) * size).to(torch.bfloat16)
+                    v[pg, :, s % page] = torch.randn((h, D), generator=g).to(torch.bfloat16)
+        self.k, self.v = k, v
+        cu = [0]
+        for n in news:
+            cu.append(cu[-1] + n)
+        self.cu, self.n = torch.tensor(cu, dtype=torch.int32), cu[-1] + extra_rows
+        self.max_q = max(news)
+        self.q = torch.randn((self.n, H, D), generator=g).to(torch.bfloat16)
+        self.gen = g
+        self.lens_t = torch.tensor(self.lens, dtype=torch.int32)
+        self.on = {x: getattr(self, x).to(dev) for x in ("table", "cu", "q", "lens_t")}
+        keep_layout = lambda t: t.transpose(1, 2).contiguous().to(dev).transpose(1, 2) if token_major else t.to(dev)  # noqa: E731
+        self.on["k"], self.on["v"] = keep_layout(k), keep_layout(v)
+
+    def attend(self, window=None, **kw):
+        o = self.on
+        return ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], self.max_q, self.D**-0.5, window=window, **kw)
+
+    def expect(self, window=None):
+        return OP.attention(self.q, self.k, self.v, self.table, self.lens, self.cu, self.D**-0.5, window)
+
+
+def score_noise(c, big, longest):
+    """relative error of a p from fp32 sums: scores of D products each (two sides of the softmax), then a sum over the keys"""
+    return torch.expm1(2 * (c.D + 8) * 2.0**-24 * big) + (longest + 64) * 2.0**-24 + 2.0**-21
+
+
+def check_out(c, got, want, mag, big):
+    rows = int(c.cu[-1])
+    got, want = got[:rows].double().cpu(), want[:rows]
+    rel = score_noise(c, big[:rows], max(c.lens))[..., None]
+    # the result's rounding, p's rounding to bf16 (each at most half a step), and the fp32 sums
+    tol = BF * want.abs() + (BF * (1 + BF) + rel) * mag[:rows] * (1 + BF) + 1e-30
+    off = (got - want).abs() / tol
+    assert not torch.isnan(got).any()
+    assert off.max() <= 1.0, f"{float(off.max())} of the tolerance at {off.argmax()}"
+
+
+LAYOUTS = [(16, 8, 256), (4, 2, 128), (6, 1, 256), (3, 3, 128), (8, 1, 128)]
+MIXES = [
+    [(1, 1)],
+    [(0, 0), (5, 5), (1, 1), (0, 0)],
+    [(127, 1), (128, 1), (129, 1), (255, 2), (16, 1)],
+    [(700, 3), (33, 33), (64, 0), (1000, 1)],
+    [(300, 40), (300, 17), (45, 45)],
+    [(2, 5), (0, 3), (40, 41)],  # more rows than cached tokens: the first rows see nothing
+]
+
+
+@pytest.mark.parametrize("mix", range(len(MIXES)))
+@pytest.mark.parametrize("H,h,D", LAYOUTS)
+def test_attention_against_the_definition(dev, H, h, D, mix):
+    page = (16, 32, 64, 128, 256)[(mix + H) % 5]
+    c = Call(dev, H, h, D, page, MIXES[mix], seed=mix * 100 + H, token_major=mix % 2 == 1, extra_rows=2)
+    out = torch.full((c.n, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    got = c.attend(out=out)
+    assert got.data_ptr() == out.data_ptr()
+    want, _, mag, big = c.expect()
+    check_out(c, got, want, mag, big)
+    assert (got[int(c.cu[-1]) :] == 7.0).all()  # rows behind the last sequence
+    for b, (L, n) in enumerate(MIXES[mix]):  # rows that see nothing
+        for i in range(max(0, n - L)):
+            assert (got[int(c.cu[b]) + i] == 0).all()
+
+
+@pytest.mark.parametrize("window", [1, 7, 64, 200])
+@pytest.mark.parametrize("H,h,D", LAYOUTS[:2])
+def test_attention_with_a_window(dev, H, h, D, window):
+    c = Call(dev, H, h, D, 32, [(900, 2), (150, 100), (64, 64), (1, 1), (513, 35), (30, 36)], seed=window)
+    want, _, mag, big = c.expect(window)
+    check_out(c, c.attend(window), want, mag, big)
+
+
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("H,h,D", LAYOUTS)
+def test_attention_keeps_the_slots_weights(dev, H, h, D, window):
+    seqs = [(400, 1), (130, 20), (77, 77), (50, 0), (3, 5), (257, 6)]
+    c = Call(dev, H, h, D, 64, seqs, seed=H + D, spare=0)
+    _, weights, _, big = c.expect(window)
+    cap = 513
+    old = torch.rand((len(seqs), h, cap), generator=c.gen)
+    w_in = old.to(dev)
+    w_out = torch.full((len(seqs), h, cap), -3.0, device=dev)
+    c.attend(window, weights=w_in, weights_out=w_out, decay=0.5)
+    assert (w_in.cpu() == old).all()
+    rel = float(score_noise(c, big, 400).max()) + 2.0**-21
+    for b, (L, _) in enumerate(seqs):
+        want = 0.5 * old[b, :, :L].double() + weights[b]
+        assert ((w_out[b, :, :L].double().cpu() - want).abs() <= rel * want + 1e-30).all()
+        assert (w_out[b, :, L:] == -3.0).all()
+    # in place, and with decay 0 (the old values are not read)
+    w2 = torch.full_like(w_in, math.nan)
+    c.attend(window, weights=w2, decay=0.0)
+    for b, (L, _) in enumerate(seqs):
+        assert ((w2[b, :, :L].double().cpu() - weights[b]).abs() <= rel * weights[b] + 1e-30).all()
+        assert torch.isnan(w2[b, :, L:]).all()
+
+
+@pytest.mark.parametrize("shared", [0, 256])
+def test_a_sequence_alone_equals_itself_in_a_batch(dev, shared):
+    seqs = [(600, 12), (300, 1), (2000, 1), (600, 300), (331, 5), (420, 100)]
+    c = Call(dev, 4, 2, 128, 64, seqs, seed=3, shared_tokens=shared)
+    w = torch.zeros((len(seqs), 2, c.table.shape[1] * 64), device=dev)
+    every = c.attend(weights=w)
+    for b in range(len(seqs)):
+        r0, r1 = int(c.cu[b]), int(c.cu[b + 1])
+        w1 = torch.zeros_like(w[:1])
+        cu = torch.tensor([0, r1 - r0], dtype=torch.int32, device=dev)
+        one = ops.paged_attention(c.on["q"][r0:r1], c.on["k"], c.on["v"], c.on["table"][b : b + 1], c.on["lens_t"][b : b + 1], cu, r1 - r0, 128**-0.5, weights=w1)
+        assert torch.equal(one, every[r0:r1]) and torch.equal(w1[0], w[b])
+
+
+def test_attention_long_cache_and_many_rows(dev):
+    """sizes of the splits' and row tiles' other side: a cache of many tiles per split, a chunk of many row tiles"""
+    for H, h, D, seqs in ((12, 2, 256, [(9000, 1), (5000, 70)]), (4, 4, 128, [(3000, 1100), (20000, 1)])):
+        c = Call(dev, H, h, D, 128, seqs, seed=D)
+        want, _, mag, big = c.expect()
+        check_out(c, c.attend(), want, mag, big)
+
+
+def test_attention_views_streams_and_a_graph(dev):
+    c = Call(dev, 8, 2, 128, 64, [(300, 3), (129, 1)], seed=5)
+    want, _, mag, big = c.expect()
+    wide = torch.randn((c.n, 8 * 128 + 320), dtype=torch.bfloat16, device=dev)  # q inside wider projection rows
+    wide[:, : 8 * 128] = c.on["q"].view(c.n, -1)
+    q = wide[:, : 8 * 128].view(c.n, 8, 128)
+    wide_out = torch.full((c.n, 8 * 128 + 64), 5.0, dtype=torch.bfloat16, device=dev)
+    out = wide_out[:, : 8 * 128].view(c.n, 8, 128)
+    o = c.on
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.paged_attention(q, o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 3, 128**-0.5, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    check_out(c, out, want, mag, big)
+    assert (wide_out[:, 8 * 128 :] == 5.0).all()
+    # two calls at once on two streams, each with a workspace of its own
+    plain = c.attend()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for st in (s1, s2) * 4:
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            got.append(c.attend())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, plain) for x in got)
+    # a captured call, replayed after the lengths have moved
+    lens = o["lens_t"].clone()
+    call = lambda: ops.paged_attention(o["q"], o["k"], o["v"], o["table"], lens, o["cu"], 3, 128**-0.5)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = call()
+    graph.replay()
+    assert torch.equal(res, plain)
+    lens -= torch.tensor([40, 2], dtype=torch.int32, device=dev)
+    graph.replay()
+    c.lens = [260, 127]
+    want, _, mag, big = c.expect()
+    check_out(c, res, want, mag, big)
+
+
+def test_far_offsets(dev):
+    """pools of more than 2^31 elements: pages at their far end"""
+    h, page, D = 8, 128, 256
+    n_pages = 2**31 // (h * page * D) + 40
+    k = torch.empty((n_pages, h, page, D), dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
+    c = Call(dev, 16, h, D, page, [(700, 2), (200, 30)], seed=11)
+    far = n_pages - c.n_pages
+    k[far:], v[far:] = c.on["k"], c.on["v"]
+    o = c.on
+    table = torch.where(o["table"] >= 0, o["table"] + far, o["table"])
+    got = ops.paged_attention(o["q"], k, v, table, o["lens_t"], o["cu"], c.max_q, D**-0.5)
+    assert torch.equal(got, c.attend())
+    # append and eviction there
+    qkv = torch.randn((32, 32 * D), dtype=torch.bfloat16, device=dev)
+    ops.paged_append(qkv, 16, h, D, k, v, table, o["lens_t"], o["cu"])
+    s = 699
+    assert torch.equal(k[int(table[0, s // page]), :, s % page], qkv[1, 16 * D : 24 * D].view(h, D))
+    new_table = torch.tensor([[0, 1], [2, n_pages - 1 - int(o["table"].max())]], dtype=torch.int32, device=dev)
+    lens, kept, _ = ops.paged_evict(k, v, table, o["lens_t"], None, 150, 150, new_table)
+    assert lens.tolist() == [150, 150] and kept[0, 0, 0] == 550
+    assert torch.equal(k[int(new_table[0, 1]), :, 149 - page], qkv[1, 16 * D : 24 * D].view(h, D))
+
+
+@pytest.mark.parametrize("H,h,D", LAYOUTS)
+@pytest.mark.parametrize("rot,norms,norm_v,plus1,page", [(1, True, True, False, 64), (64, True, False, True, 16), (96, False, False, False, 128), (0, True, True, False, 32), (0, False, False, False, 64), (0, False, True, False, 256)])
+def test_append_against_the_definition(dev, H, h, D, rot, norms, norm_v, plus1, page):
+    rot = D if rot == 1 else rot
+    seqs = [(37, 5), (1, 1), (9, 0), (300, 130), (64, 64)]
+    c = Call(dev, H, h, D, page, seqs, seed=H + rot, token_major=H % 3 == 0, extra_rows=3)
+    g = c.gen
+    wide = (torch.randn((c.n, (H + 2 * h) * D + 24), generator=g) * 2).to(torch.bfloat16)
+    qkv = wide[:, : (H + 2 * h) * D]
+    wq, wk = ((0.2 * torch.randn(D, generator=g) + (0 if plus1 else 1)).to(torch.bfloat16) for _ in range(2)) if norms else (None, None)
+    cos, sin = ((torch.cos if i else torch.sin)(torch.rand((c.n, rot // 2), generator=g) * 7).to(torch.bfloat16) for i in range(2)) if rot else (None, None)
+    to = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    o = c.on
+    k0, v0 = o["k"].clone(), o["v"].clone()
+    q = ops.paged_append(wide.to(dev)[:, : (H + 2 * h) * D], H, h, D, o["k"], o["v"], o["table"], o["lens_t"], o["cu"], wq=to(wq), wk=to(wk), cos=to(cos), sin=to(sin), plus1=plus1, norm_v=norm_v)
+    wq64, wk64, wv64, qs, ks = OP.append(qkv, H, h, D, wq, wk, cos, sin, 1e-6, plus1, norm_v)
+    near = lambda a, b, size: ((a.double().cpu() - b).abs() <= BF * b.abs() + 2.0**-19 * size).all()  # noqa: E731
+    assert near(q, wq64, qs)
+    for b, (L, n) in enumerate(seqs):
+        for i in range(n):
+            s, r = L - n + i, int(c.cu[b]) + i
+            pg = int(c.table[b, s // page])
+            assert near(o["k"][pg, :, s % page], wk64[r], ks[r]) and near(o["v"][pg, :, s % page], wv64[r], wv64[r].abs())
+            k0[pg, :, s % page], v0[pg, :, s % page] = o["k"][pg, :, s % page], o["v"][pg, :, s % page]
+    same = lambda a, b: torch.equal(a.view(torch.int16), b.view(torch.int16))  # noqa: E731
+    assert same(k0.contiguous(), o["k"].contiguous()) and same(v0.contiguous(), o["v"].contiguous())  # nothing else was written
+
+
+@pytest.mark.parametrize("keep,recent", [(64, 16), (100, 0), (33, 33), (1, 0), (500, 499)])
+@pytest.mark.parametrize("D,page", [(128, 16), (256, 64), (128, 256)])
+def test_evict_against_the_definition(dev, D, page, keep, recent):
+    h = 3
+    seqs = [(400, 0), (64, 0), (0, 0), (1, 0), (101, 0), (1333, 0)]
+    per = -(-keep // page)
+    c = Call(dev, h, h, D, page, seqs, seed=keep, spare=per * len(seqs), token_major=D == 256)
+    g = c.gen
+    w = torch.rand((len(seqs), h, 1400), generator=g) ** 4
+    w[:, 0, ::3] = 0.0                      # ties at zero
+    w[:, 1] = (w[:, 1] * 8).round() / 8     # ties everywhere
+    w[0, 2, 5:50] = math.nan
+    w[0, 2, 60:70] = math.inf
+    w[5, 2] = -w[5, 2]
+    w[5, 0, 7] = -0.0
+    new_table = c.free[: per * len(seqs)].view(len(seqs), per).to(dev)
+    o = c.on
+    k0, v0 = o["k"].clone(), o["v"].clone()
+    lens, kept, wo = ops.paged_evict(o["k"], o["v"], o["table"], o["lens_t"], w.to(dev), keep, recent, new_table)
+    assert lens.tolist() == [min(L, keep) for L, _ in seqs]
+    for b, (L, _) in enumerate(seqs):
+        for head in range(h):
+            want = OP.evict(w[b, head, :L], L, keep, recent)
+            m = len(want)
+            assert kept[b, head, :m].tolist() == want and (kept[b, head, m:] == -1).all()
+            assert torch.equal(wo[b, head, :m].cpu().nan_to_num(7.0), w[b, head, want].nan_to_num(7.0)) and (wo[b, head, m:] == 0).all()
+            for pages, before in ((o["k"], k0), (o["v"], v0)):
+                new = OP.gather(pages.cpu()[:, head : head + 1], new_table[b].cpu(), m)[0]
+                old = OP.gather(before.cpu()[:, head : head + 1], c.table[b], L)[0]
+                assert torch.equal(new, old[want])
+    used = torch.unique(new_table).tolist()
+    others = torch.tensor([x for x in range(c.n_pages) if x not in used], device=dev)
+    assert torch.equal(o["k"][others].view(torch.int16), k0[others].view(torch.int16))
+
+
+def test_evict_long_rows(dev):
+    """rows of many segments per warp, against a sort"""
+    B, h, L, keep, recent = 2, 4, 70001, 5000, 100
+    k = torch.randn((2 * 1100 + 2 * 79, h, 64, 128), dtype=torch.bfloat16, device=dev)
+    v = torch.randn_like(k)
+    table = torch.randperm(2 * 1100, device=dev).to(torch.int32).view(2, 1100)
+    new_table = (2200 + torch.arange(2 * 79, device=dev)).to(torch.int32).view(2, 79)
+    w = torch.rand((B, h, 1100 * 64), device=dev).mul(2000).round()  # many ties
+    lens = torch.tensor([L, L - 13], dtype=torch.int32, device=dev)
+    _, kept, _ = ops.paged_evict(k, v, table, lens, w, keep, recent, new_table)
+    for b in range(B):
+        m = int(lens[b]) - recent
+        for g in range(h):
+            first = torch.sort(w[b, g, :m], descending=True, stable=True).indices[: keep - recent].sort().values
+            assert torch.equal(kept[b, g, : keep - recent].long(), first)
+
+
+def test_out_of_range_entries_are_reported_not_followed(dev):
+    """a page index outside the pool, a length above max_len: the kernels' own checks skip the access and set the status word"""
+    c = Call(dev, 4, 2, 128, 64, [(200, 2), (100, 1)], seed=1)
+    o = c.on
+    good = c.attend()
+    _lib.last_status()
+    for bad in (c.n_pages, -1, 2**30):
+        table = o["table"].clone()
+        table[1, 0] = bad
+        got = ops.paged_attention(o["q"], o["k"], o["v"], table, o["lens_t"], o["cu"], 2, 128**-0.5)
+        assert _lib.last_status(raise_on_error=False) == 5
+        assert torch.equal(got[:2], good[:2])
+    lens = o["lens_t"].clone()
+    lens[1] = 70000
+    got = ops.paged_attention(o["q"], o["k"], o["v"], o["table"], lens, o["cu"], 2, 128**-0.5)
+    assert _lib.last_status(raise_on_error=False) == 5
+    assert torch.equal(got[:2], good[:2])
+    qkv = torch.zeros((3, 8 * 128), dtype=torch.bfloat16, device=dev)
+    table = o["table"].clone()
+    table[0] = c.n_pages
+    ops.paged_append(qkv, 4, 2, 128, o["k"], o["v"], table, o["lens_t"], o["cu"])
+    assert _lib.last_status(raise_on_error=False) == 5
+    ops.paged_evict(o["k"], o["v"], table, o["lens_t"], None, 64, 64, c.free[:2].view(2, 1).to(dev))
+    assert _lib.last_status(raise_on_error=False) == 5
