@@ -147,6 +147,8 @@ def init(device) -> None:
     """prepares `device` (a torch.device or index) once: status word, driver entry points"""
     import torch
 
+    if device in _inited:
+        return
     idx = torch.device(device).index if not isinstance(device, int) else device
     idx = torch.cuda.current_device() if idx is None else idx
     if idx in _inited:
@@ -160,6 +162,13 @@ def stream_ptr():
     import torch
 
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream(index: int) -> int:
+    """the current stream of device `index` as an integer (stream_ptr without making a Stream object: 0.1 us instead of 3)"""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def last_status(raise_on_error: bool = True) -> int:

@@ -120,10 +120,11 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, int
 
 // a launch that may start before the kernel ahead of it on the stream has ended (its pdl_wait holds it back)
 template <class... Params, class... Args>
-inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t st, Args... args) {
+inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t st, int smem, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

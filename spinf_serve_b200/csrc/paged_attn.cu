@@ -54,12 +54,16 @@ struct PagedAttnArgs {
   int tok_cap;
 };
 
-// the rule for the few-row kernel
-__device__ __forceinline__ bool rows_class(const PagedSeq& q, int group) { return q.nq > 0; }
+// which kernel takes a sequence, by its rows per kv head, and how its keys are cut into splits
+static constexpr int STEP_ROWS = 16;
+__device__ __forceinline__ bool step_class(const PagedSeq& q, int group) { return q.nq > 0 && q.nq * group <= STEP_ROWS; }
+__device__ __forceinline__ PagedCut step_cut(const PagedSeq& q, const PagedAttnArgs& a) { return paged_cut(q, a.window, 1, a.h, PG_SMS, 1); }
+__device__ __forceinline__ bool rows_class(const PagedSeq& q, int group) { return q.nq * group > STEP_ROWS; }
 __device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
   const int rt = (q.nq * a.group + RT - 1) / RT;
   return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 1);
 }
+__device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a.group) ? step_cut(q, a) : rows_cut(q, a); }
 __device__ __forceinline__ int rows_items(const PagedSeqs& s, const PagedAttnArgs& a, int b, int* status) {
   const PagedSeq q = paged_seq(s, b, status);
   if (!rows_class(q, a.group)) return 0;
@@ -440,6 +444,384 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       if (!ok) break;
     }
   }
+  if (threadIdx.x == 0) pdl_wait();  // the kernels behind this one need what the kernel ahead of it wrote, too
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------- few rows per kv head (at most 16): a decoding step
+static constexpr int SW = 7;                        // consumer warps; the eighth warp is the producer (8 warps: 255 registers a thread)
+static constexpr int STEP_THREADS = (SW + 1) * 32;
+
+template <int D>
+struct StepSmem {
+  static constexpr int STAGE = 64 * D * 2;          // 64 keys of K or V
+  static constexpr int NST = D == 256 ? 5 : 10;
+  static constexpr int Q_PITCH = D * 2 + 16;        // a row of q; the 16 bytes spread the rows over the banks
+  static constexpr int Q_SLOT = STEP_ROWS * Q_PITCH;
+  static constexpr int MR = D == 256 ? 4 : 8;       // rows merged at a time
+  static constexpr int Q_OFF = NST * STAGE;
+  static constexpr int MERGE_OFF = Q_OFF + 2 * Q_SLOT;
+  static constexpr int ML_OFF = MERGE_OFF + SW * MR * D * 4;  // [SW][16] maxima, [SW][16] sums, [16] joined maxima, [16] joined sums
+  static constexpr int ITEM_OFF = ML_OFF + (2 * SW + 2) * STEP_ROWS * 4;
+  static constexpr int PRE_OFF = ITEM_OFF + 2 * 64;
+  static constexpr int BAR_OFF = PRE_OFF + (PG_MAX_SEQS + 2) * 4;
+  static constexpr int TOTAL = BAR_OFF + (2 * NST + 4) * 8 + 16 + 1024;
+};
+static_assert(StepSmem<256>::TOTAL <= 232448 && StepSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
+static_assert(StepSmem<256>::BAR_OFF % 8 == 0 && StepSmem<128>::BAR_OFF % 8 == 0 && StepSmem<256>::MERGE_OFF % 16 == 0 &&
+                  StepSmem<128>::MERGE_OFF % 16 == 0 && StepSmem<256>::ITEM_OFF % 16 == 0 && StepSmem<128>::ITEM_OFF % 16 == 0, "alignment");
+
+// what the consumers need of an item; the producer writes it beside the rows of q
+struct StepItem {
+  int b, g, split, splits;
+  int row0, nq, base;  // first row of q, rows of the sequence, slot of the first
+  int lo, hi;          // slots that some row sees
+  int u0, u1;          // 64-key units
+};
+
+__device__ __forceinline__ void movmatrix_t(uint32_t& d, uint32_t s) {
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(s));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// NT: 8-row tiles of q. A row's arithmetic is the same for either.
+template <int D, int NT>
+__global__ void __launch_bounds__(STEP_THREADS, 1)
+paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedSeqs s, const PagedAttnArgs a,
+                  int* __restrict__ status) {
+  using L = StepSmem<D>;
+  constexpr int KS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* empty = full + L::NST;
+  uint64_t* q_full = empty + L::NST;
+  uint64_t* q_empty = q_full + 2;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(q_empty + 2);
+  const WaitCtx wc{abort_flag, status};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::NST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);  // a 64-key stage is four 16-key pieces
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], SW);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  paged_item_prefix(s.B, pre, STEP_THREADS, [&](int b) {
+    const PagedSeq q = paged_seq(s, b, status);
+    return step_class(q, a.group) ? a.h * step_cut(q, a).splits : 0;
+  });
+  const int total = pre[s.B];
+  const int br = s.page_log2 < 6 ? s.page_log2 : 6;  // log2 of a box's rows
+
+  if (warp == SW) {
+    if (lane == 0) {
+      uint32_t cnt = 0, item_n = 0;
+      bool ok = true;
+      const int box_rows = 1 << br;
+      for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++item_n) {
+        const int b = paged_find(pre, s.B, it);
+        const PagedSeq q = paged_seq(s, b, status);
+        const PagedCut c = step_cut(q, a);
+        const int x = it - pre[b];
+        StepItem w;
+        w.b = b, w.g = x % a.h, w.split = x / a.h, w.splits = c.splits;
+        w.row0 = q.row0, w.nq = q.nq, w.base = q.len - q.nq;
+        w.lo = a.window > 0 && w.base - a.window + 1 > 0 ? w.base - a.window + 1 : 0;
+        w.hi = q.len;
+        const int s0 = 2 * (c.t_lo + w.split * c.tiles_per_split), s1 = s0 + 2 * c.tiles_per_split;
+        const int e0 = w.lo / 64, e1 = (w.hi + 63) / 64;
+        w.u0 = s0 > e0 ? s0 : e0;
+        w.u1 = s1 < e1 ? s1 : e1;
+        const uint32_t qs = item_n & 1u;
+        if (!mbar_wait(wc, &q_empty[qs], ((item_n >> 1) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        *reinterpret_cast<StepItem*>(smem + L::ITEM_OFF + qs * 64) = w;
+        const int rows = q.nq * a.group;
+        mbar_expect_tx(&q_full[qs], rows * D * 2);  // (an arrival: releases the item's numbers to the consumers as well)
+        for (int r = 0; r < rows; ++r)
+          bulk_load(smem + L::Q_OFF + qs * L::Q_SLOT + r * L::Q_PITCH,
+                    a.q + (q.row0 + r / a.group) * a.q_pitch + static_cast<int64_t>(w.g * a.group + r % a.group) * D, D * 2, &q_full[qs]);
+        const int32_t* pages = s.table + b * s.table_pitch;
+        for (int u = w.u0; u < w.u1 && ok; ++u) {
+          // boxes that hold a slot some row sees; the others stay as they are (masked for K, cleared for V)
+          int bytes = 0, pg[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int j = u * 64 + y * box_rows;
+            pg[y] = -1;
+            if (y * box_rows < 64 && j < w.hi && j + box_rows > w.lo) {
+              pg[y] = pages[j >> s.page_log2];
+              if (pg[y] < 0 || pg[y] >= s.n_pages) {
+                atomicCAS(status, 0, ST_BAD_INDEX);
+                pg[y] = -1;
+              } else {
+                bytes += box_rows * D * 2;
+              }
+            }
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part, ++cnt) {
+            const uint32_t st = cnt % L::NST;
+            if (!mbar_wait(wc, &empty[st], ((cnt / L::NST) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+            mbar_expect_tx(&full[st], bytes);
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (pg[y] >= 0)
+                tma_load_5d(smem + st * L::STAGE + y * box_rows * D * 2, part ? &tmV : &tmK, 0, (u * 64 + y * box_rows) & ((1 << s.page_log2) - 1), 0, w.g,
+                            pg[y], &full[st]);
+          }
+        }
+      }
+      if (*abort_flag) {  // bounded wait for copies that may still be in flight
+        for (uint32_t c = cnt > static_cast<uint32_t>(L::NST) ? cnt - L::NST : 0; c < cnt; ++c)
+          for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % L::NST], (c / L::NST) & 1u); ++spin) {}
+        for (uint32_t c = item_n > 2u ? item_n - 2u : 0u; c <= item_n; ++c)
+          for (int spin = 0; spin < 4096 && !mbar_try_wait(&q_full[c & 1u], (c >> 1) & 1u); ++spin) {}
+      }
+    }
+  } else {
+    float* m_w = reinterpret_cast<float*>(smem + L::ML_OFF);  // [SW][16]
+    float* l_w = m_w + SW * STEP_ROWS;
+    float* m_all = l_w + SW * STEP_ROWS;
+    float* l_all = m_all + STEP_ROWS;
+    float* merge = reinterpret_cast<float*>(smem + L::MERGE_OFF);
+    const uint32_t ring = smem_u32(smem);
+    const int c4 = lane & 3, r8 = lane >> 2;
+    uint32_t cnt0 = 0, item_n = 0;  // stages before the item, items so far
+    for (int it = blockIdx.x; it < total; it += gridDim.x, ++item_n) {
+      const uint32_t qs = item_n & 1u;
+      bool ok = mbar_wait(wc, &q_full[qs], (item_n >> 1) & 1u, ST_TIMEOUT_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      const StepItem w = *reinterpret_cast<const StepItem*>(smem + L::ITEM_OFF + qs * 64);
+      const int rows = w.nq * a.group;
+      uint32_t qf[NT][KS][2];  // q as the B operand: rows 8 n + lane / 4, dimensions 16 ks + 2 (lane % 4) and 8 more
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+          uint32_t r[4];
+          ldsm4(r, smem_u32(smem + L::Q_OFF + qs * L::Q_SLOT) + (n * 8 + (lane & 7)) * L::Q_PITCH + ks * 32 + (lane >> 3) * 16);
+          qf[n][ks][0] = r[0], qf[n][ks][1] = r[1], qf[n][ks + 1][0] = r[2], qf[n][ks + 1][1] = r[3];
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[qs]);
+      if (!ok) {  // the other warps leave at the vote below too: the abort flag is up
+        bar_red_and(1, SW * 32, false);
+        break;
+      }
+      // this thread's rows: 8 n + 2 (lane % 4) and the next; the slots each sees
+      int hi_r[NT][2], lo_r[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          int r = n * 8 + 2 * c4 + x;
+          r = r < rows ? r : rows - 1;
+          hi_r[n][x] = w.base + r / a.group;
+          lo_r[n][x] = a.window > 0 ? hi_r[n][x] - a.window + 1 : 0;
+        }
+      const int hi_min = w.base, lo_max = a.window > 0 ? w.hi - a.window : 0;
+      float o[KS][NT][4];  // O^T: dimensions 16 i + lane / 4 and 8 more, rows as above
+      float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[i][n][x] = 0.f;
+        m_run[n][0] = m_run[n][1] = -INFINITY;
+        l_run[n][0] = l_run[n][1] = 0.f;
+      }
+      const int pieces = 4 * (w.u1 - w.u0);
+      for (int p = warp; p < pieces && ok; p += SW) {
+        const int u = p >> 2, key0 = (p & 3) * 16;
+        const uint32_t ck = cnt0 + 2 * u, stk = ck % L::NST, stv = (ck + 1) % L::NST;
+        const int j0 = (w.u0 + u) * 64 + key0;
+        ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stk], (ck / L::NST) & 1u, ST_TIMEOUT_FULL));
+        if (!ok) break;
+        float sc[2][NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[0][n][x] = sc[1][n][x] = 0.f;
+        {
+          const uint32_t k_base = ring + stk * L::STAGE;
+          const int key = key0 + (lane & 15);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t kf[4];
+            ldsm4(kf, k_base + stage_offset<D>(key, ks * 2 + (lane >> 4), br));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(sc[ks & 1][n], kf, qf[n][ks][0], qf[n][ks][1]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stk]);
+        const bool masked = j0 + 15 > hi_min || j0 < lo_max;
+        uint32_t pf[NT][2];
+        bool moved = false;
+        float alpha[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float v[4];  // (key, row): (r8, 0) (r8, 1) (r8 + 8, 0) (r8 + 8, 1)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            v[x] = (sc[0][n][x] + sc[1][n][x]) * a.scale_log2;
+            const int j = j0 + r8 + (x >> 1) * 8;
+            if (masked && (j > hi_r[n][x & 1] || j < lo_r[n][x & 1])) v[x] = -INFINITY;
+          }
+          if (a.scores) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int r = n * 8 + 2 * c4 + x;
+              if (r < rows) {
+                float* dst = a.scores + ((static_cast<int64_t>(w.b) * a.tok_cap + r / a.group) * a.H + w.g * a.group + r % a.group) * a.score_pitch + j0 + r8;
+                dst[0] = v[x];
+                dst[8] = v[2 + x];
+              }
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float mx = fmaxf(v[x], v[2 + x]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(m_run[n][x], mx);
+            alpha[n][x] = m_new == m_run[n][x] ? 1.f : fast_exp2(m_run[n][x] - m_new);
+            moved |= alpha[n][x] != 1.f;
+            m_run[n][x] = m_new;
+            const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+            v[x] = fast_exp2(v[x] + neg_m);
+            v[2 + x] = fast_exp2(v[2 + x] + neg_m);
+            l_run[n][x] = l_run[n][x] * alpha[n][x] + (v[x] + v[2 + x]);
+          }
+          // P^T (keys x rows) -> the B operand of O^T: 8 x 8 blocks transposed between lanes
+          movmatrix_t(pf[n][0], pack_bf16x2(v[0], v[1]));
+          movmatrix_t(pf[n][1], pack_bf16x2(v[2], v[3]));
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[i][n][x] *= alpha[n][x & 1];
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stv], ((ck + 1) / L::NST) & 1u, ST_TIMEOUT_FULL));
+        if (!ok) break;
+        if (j0 < w.lo || j0 + 16 > w.hi) {
+          // slots no row sees may hold anything (or were not copied): p is 0 there, but 0 * inf is not
+          for (int x = lane; x < 16 * (D / 8); x += 32) {
+            const int key = key0 + x / (D / 8);
+            const int j = (w.u0 + u) * 64 + key;
+            if (j < w.lo || j >= w.hi) *reinterpret_cast<uint4*>(smem + stv * L::STAGE + stage_offset<D>(key, x % (D / 8), br)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();  // the stage is refilled by the copy engine
+          __syncwarp();
+        }
+        {
+          const uint32_t v_base = ring + stv * L::STAGE;
+          const int key = key0 + ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            uint32_t vf[4];
+            ldsm4_t(vf, v_base + stage_offset<D>(key, i * 2 + ((lane >> 3) & 1), br));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(o[i][n], vf, pf[n][0], pf[n][1]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stv]);
+      }
+      cnt0 += 2 * (w.u1 > w.u0 ? w.u1 - w.u0 : 0);
+      // ---- the warps' shares joined, in warp order
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float l = l_run[n][x];
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+          if (r8 == 0) {
+            const int r = n * 8 + 2 * c4 + x;
+            m_w[warp * STEP_ROWS + r] = m_run[n][x];
+            l_w[warp * STEP_ROWS + r] = l;
+          }
+        }
+      if (!bar_red_and(1, SW * 32, ok)) break;
+      float f[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = n * 8 + 2 * c4 + x;
+          float m = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int y = 0; y < SW; ++y) m = fmaxf(m, m_w[y * STEP_ROWS + r]);
+          const float neg_m = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+          for (int y = 0; y < SW; ++y) l = fmaf(fast_exp2(m_w[y * STEP_ROWS + r] + neg_m), l_w[y * STEP_ROWS + r], l);
+          f[n][x] = fast_exp2(m_run[n][x] + neg_m);
+          if (warp == 0 && r8 == 0) m_all[r] = m, l_all[r] = l;
+        }
+      for (int rb = 0; rb < rows; rb += L::MR) {
+        if (rb) named_bar_sync(1, SW * 32);  // the rows before these have been read
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = n * 8 + 2 * c4 + x;
+            if (r >= rb && r < rb + L::MR && r < rows) {
+              float* dst = merge + (warp * L::MR + r - rb) * D + r8;
+#pragma unroll
+              for (int i = 0; i < KS; ++i) dst[i * 16] = o[i][n][x] * f[n][x], dst[i * 16 + 8] = o[i][n][2 + x] * f[n][x];
+            }
+          }
+        named_bar_sync(1, SW * 32);
+        const int n_rows = rows - rb < L::MR ? rows - rb : L::MR;
+        for (int x = threadIdx.x; x < n_rows * (D / 4); x += SW * 32) {
+          const int r = rb + x / (D / 4), d = (x % (D / 4)) * 4;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int y = 0; y < SW; ++y) {
+            const float4 v = *reinterpret_cast<const float4*>(merge + (y * L::MR + r - rb) * D + d);
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+          }
+          const int tok = r / a.group, hd = w.g * a.group + r % a.group;
+          if (w.splits == 1) {
+            const float l = l_all[r], inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row that sees nothing: 0; a NaN sum stays NaN
+            *reinterpret_cast<uint2*>(a.out + (w.row0 + tok) * a.out_pitch + static_cast<int64_t>(hd) * D + d) =
+                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+            if (a.lse && d == 0) a.lse[static_cast<int64_t>(w.row0 + tok) * a.H + hd] = m_all[r] + log2f(l);
+          } else {
+            const int64_t at = w.b * a.seq_parts + (static_cast<int64_t>(w.split) * a.h + w.g) * rows + r;
+            *reinterpret_cast<float4*>(a.part_o + at * D + d) = acc;
+            if (d == 0) a.part_ml[at] = make_float2(m_all[r], l_all[r]);
+          }
+        }
+      }
+    }
+  }
   __syncthreads();
 }
 
@@ -451,8 +833,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedSeqs s, cons
   constexpr int V = D / 128;  // float4 per lane
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSeq q = paged_seq(s, b, status);
-  if (!rows_class(q, a.group)) return;
-  const PagedCut c = rows_cut(q, a);
+  if (q.nq == 0) return;
+  const PagedCut c = attn_cut(q, a);
   if (c.splits == 1) return;
   const int all = q.nq * a.group;
   for (int64_t x = blockIdx.x * 8 + warp; x < static_cast<int64_t>(q.nq) * a.H; x += gridDim.x * 8) {
@@ -504,7 +886,7 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, co
   const PagedSeq q = paged_seq(s, b, status);
   const int first = blockIdx.x * 1024;
   if (first >= q.len) return;
-  const int all = rows_class(q, a.group) ? q.nq * a.group : 0, base = q.len - q.nq;
+  const int all = q.nq * a.group, base = q.len - q.nq;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int r = 0; r < all; ++r) {
     const int tok = r / a.group, hd = g * a.group + r % a.group, hi = base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;
@@ -561,21 +943,28 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   int r;
   const uint32_t box = kp.page < 64 ? static_cast<uint32_t>(kp.page) : 64u;
   if ((r = make_tmap_pages(&tmK, kp, box, D / 64)) || (r = make_tmap_pages(&tmV, vp, box, D / 64))) return r;
-  auto kern = paged_rows_kernel<D>;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    SPINF_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D>::TOTAL));
+    SPINF_CUDA_OK(cudaFuncSetAttribute(paged_step_kernel<D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepSmem<D>::TOTAL));
+    SPINF_CUDA_OK(cudaFuncSetAttribute(paged_step_kernel<D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepSmem<D>::TOTAL));
+    SPINF_CUDA_OK(cudaFuncSetAttribute(paged_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D>::TOTAL));
     attr_set[dev].store(true, std::memory_order_release);
   }
-  kern<<<static_cast<unsigned>(sm_count()), ROWS_THREADS, RowsSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+  const unsigned grid = static_cast<unsigned>(sm_count());
+  if (max_q * a.group <= 8)
+    paged_step_kernel<D, 1><<<grid, STEP_THREADS, StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+  else
+    paged_step_kernel<D, 2><<<grid, STEP_THREADS, StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
   SPINF_CUDA_OK(cudaGetLastError());
+  if (max_q * a.group > STEP_ROWS)
+    SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, tmK, tmV, s, a, status));
   if (max_splits > 1) {
     int64_t gx = (max_q * a.H + 7) / 8;
     if (gx > 4096) gx = 4096;
-    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, s, a, status));
+    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, s, a, status));
   }
   if (w)
-    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, s, a, *w, status));
+    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, s, a, *w, status));
   return 0;
 }
 

@@ -3,6 +3,7 @@ memory and streams are torch's), and enqueues one entry point of libspinf_b200.s
 the CPU or through another library: a tensor that is not on a CUDA device is an error."""
 
 import ctypes
+import functools
 
 import torch
 
@@ -605,74 +606,93 @@ def embed_scale(ids, emb, scale):
     return out
 
 
-# ---- paged K/V cache
-def _pages(k_pages, v_pages, what):
-    """the pools of a paged call, [pages, kv heads, page, D] with unit stride over D -> their shape and the strides of both"""
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.bfloat16 or t.dim() != 4 or t.stride(3) != 1:
-            raise SpinfError(f"{what}: {name} must be a CUDA bf16 [pages, kv heads, page, D] tensor (or view) with unit stride over D")
-    if v_pages.shape != k_pages.shape or v_pages.device != k_pages.device:
-        raise SpinfError(f"{what}: k_pages and v_pages must agree in shape and device")
-    page, D = k_pages.shape[2], k_pages.shape[3]
+# ---- paged K/V cache. A decoding step makes these calls once per layer, for a few microseconds of GPU work each: the checks are one
+# expression each on the way through, and say what is wrong only when one fails.
+_I32, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
+
+
+@functools.lru_cache(maxsize=256)
+def _page_layout(shape, k_stride, v_stride):
+    """a pool's shape and strides, checked -> (pages, kv heads, page, D, the strides of k and v for the C entry points)"""
+    n_pages, h, page, D = shape
     if page < 16 or page > 256 or page & (page - 1) or D not in (128, 256):
-        raise SpinfError(f"{what}: pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {page} of {D}")
-    _lib.init(k_pages.device)
+        raise SpinfError(f"pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {page} of {D}")
+    if k_stride[3] != 1 or v_stride[3] != 1 or any(x % 8 for x in k_stride[:3] + v_stride[:3]):
+        raise SpinfError(f"pages need unit stride over D and strides that are multiples of 8 elements, got {k_stride} and {v_stride}")
     i64x3 = ctypes.c_int64 * 3
-    return tuple(k_pages.shape), i64x3(*k_pages.stride()[:3]), i64x3(*v_pages.stride()[:3])
+    return n_pages, h, page, D, i64x3(*k_stride[:3]), i64x3(*v_stride[:3])
 
 
-def _paged_index(t, name, what, device, shape, pitched=False):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != len(shape):
-        raise SpinfError(f"{what}: {name} must be an int32 tensor of {len(shape)} dimensions on the pages' device")
-    if any(s is not None and s != have for s, have in zip(shape, t.shape)):
-        raise SpinfError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1 or not pitched and not t.is_contiguous():
-        raise SpinfError(f"{what}: {name} must be contiguous")
+def _pages(k_pages, v_pages, what):
+    """the pools of a paged call, [pages, kv heads, page, D] with unit stride over D -> device index and _page_layout"""
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not _BF16 or t.dim() != 4:
+            raise SpinfError(f"{what}: {name} must be a CUDA bf16 [pages, kv heads, page, D] tensor or view")
+    if v_pages.shape != k_pages.shape or v_pages.get_device() != k_pages.get_device():
+        raise SpinfError(f"{what}: k_pages and v_pages must agree in shape and device")
+    idx = k_pages.get_device()
+    _lib.init(idx)
+    return idx, _page_layout(k_pages.shape, k_pages.stride(), v_pages.stride())
 
 
-def _table_pitch(table):
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+def _paged_index(what, idx, lens, table, cu=None, new_table=None):
+    """the index tensors of a paged call: int32 on the pages' device, rows of the tables contiguous -> number of sequences"""
+    tensors = [x for x in (lens, table, cu, new_table) if x is not None]
+    if not all(isinstance(x, torch.Tensor) and x.dtype is _I32 and x.get_device() == idx for x in tensors):
+        raise SpinfError(f"{what}: lens, cu and the page tables must be int32 tensors on the pages' device")
+    B = lens.numel()
+    if lens.dim() != 1 or (cu is not None and (cu.dim() != 1 or cu.numel() != B + 1)):
+        raise SpinfError(f"{what}: lens must be [B] and cu [B + 1], got {tuple(lens.shape)}" + ("" if cu is None else f" and {tuple(cu.shape)}"))
+    for x in (table,) if new_table is None else (table, new_table):
+        if x.dim() != 2 or x.shape[0] != B or (x.shape[1] > 1 and x.stride(1) != 1) or (B > 1 and x.stride(0) < x.shape[1]):
+            raise SpinfError(f"{what}: a page table must be [B, pages] with contiguous rows for the {B} sequences of lens, got {tuple(x.shape)}, strides {x.stride()}")
+    if not lens.is_contiguous() or (cu is not None and not cu.is_contiguous()):
+        raise SpinfError(f"{what}: lens and cu must be contiguous")
+    return B
+
+
+def _row_pitch(t, width):
+    return t.stride(0) if t.shape[0] > 1 else width
 
 
 def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=None, cos=None, sin=None, eps=1e-6, plus1=False, norm_v=False):
     """a step's rows into the paged cache: qkv [n, (H + 2 Hkv) D] bf16 (rows of any pitch) -> q [n, H, D]; k and v go to the slots of
     their sequences (spinf_paged_append in include/spinf_b200.h has the layout). wq, wk [D]: head norms of q and k (plus1: weights
     1 + w); norm_v: norm of v without weight; cos, sin [n, R/2] bf16 (rope_table): rotary embedding over the first R dimensions.
-    Without norms and rotation the returned q is a view of qkv."""
+    Without norms of q and rotation the returned q is a view of qkv."""
     what = "paged_append"
-    (n_pages, h, page, Dp), ks, vs = _pages(k_pages, v_pages, what)
-    dev = k_pages.device
-    if not isinstance(qkv, torch.Tensor) or qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.stride(1) != 1:
+    idx, (n_pages, h, page, Dp, ks, vs) = _pages(k_pages, v_pages, what)
+    if not isinstance(qkv, torch.Tensor) or qkv.dtype is not _BF16 or qkv.get_device() != idx or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
         raise SpinfError(f"{what}: qkv must be a bf16 [n, (H + 2 Hkv) D] tensor on the pages' device with unit stride over its columns")
-    n = qkv.shape[0]
-    if h != Hkv or Dp != D or qkv.shape[1] != (H + 2 * Hkv) * D:
+    n, width = qkv.shape
+    if h != Hkv or Dp != D or H < 1 or width != (H + 2 * Hkv) * D:
         raise SpinfError(f"{what}: qkv {tuple(qkv.shape)} and pages {tuple(k_pages.shape)} do not fit {H} / {Hkv} heads of {D}")
     if (wq is None) != (wk is None) or (cos is None) != (sin is None):
         raise SpinfError(f"{what}: wq and wk, cos and sin come together")
-    for name, t, shape in (("wq", wq, (D,)), ("wk", wk, (D,)), ("cos", cos, None), ("sin", sin, None)):
-        if t is None:
-            continue
-        if t.dtype != torch.bfloat16 or t.device != dev or not t.is_contiguous() or (shape and tuple(t.shape) != shape):
-            raise SpinfError(f"{what}: {name} must be a contiguous bf16 tensor on the pages' device" + (f" of shape {shape}" if shape else ""))
+    if wq is not None:
+        for t in (wq, wk):
+            if t.dtype is not _BF16 or t.get_device() != idx or t.dim() != 1 or t.numel() != D or not t.is_contiguous():
+                raise SpinfError(f"{what}: wq and wk must be contiguous bf16 [{D}] tensors on the pages' device")
     rot = 0
     if cos is not None:
         rot = 2 * cos.shape[-1]
-        if tuple(cos.shape) != (n, rot // 2) or sin.shape != cos.shape or rot > D or rot % 16:
-            raise SpinfError(f"{what}: cos and sin must be [n, R/2] with R a multiple of 16 of at most D, got {tuple(cos.shape)}")
-    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
-    _paged_index(lens, "lens", what, dev, (None,))
-    _paged_index(cu, "cu", what, dev, (B + 1,))
-    _paged_index(table, "table", what, dev, (B, None), pitched=True)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+        if cos.shape != (n, rot // 2) or sin.shape != cos.shape or rot > D or rot % 16:
+            raise SpinfError(f"{what}: cos and sin must be [n, R/2] with R a multiple of 16 of at most D, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        for t in (cos, sin):
+            if t.dtype is not _BF16 or t.get_device() != idx or not t.is_contiguous():
+                raise SpinfError(f"{what}: cos and sin must be contiguous bf16 tensors on the pages' device")
+    B = _paged_index(what, idx, lens, table, cu)
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
             return paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin, eps, plus1, norm_v)
-    q = qkv[:, : H * D].view(n, H, D) if wq is None and not rot else torch.empty((n, H, D), dtype=torch.bfloat16, device=dev)
-    pitch = qkv.stride(0) if n > 1 else qkv.shape[1]
+    moved = wq is not None or rot > 0
+    q = qkv.new_empty((n, H, D)) if moved else qkv[:, : H * D].view(n, H, D)
     check(
         _lib.lib().spinf_paged_append(
-            ptr(qkv), pitch, n, H, Hkv, D, ptr(wq), ptr(wk), ptr(cos) if rot else None, ptr(sin) if rot else None, rot, eps, int(plus1), int(norm_v),
-            None if wq is None and not rot else ptr(q), ptr(k_pages), ptr(v_pages), n_pages, page, ks, vs, ptr(table), _table_pitch(table),
-            table.shape[1], ptr(lens), ptr(cu), B, stream_ptr(),
+            qkv.data_ptr(), _row_pitch(qkv, width), n, H, Hkv, D, wq.data_ptr() if wq is not None else None, wk.data_ptr() if wq is not None else None,
+            cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, rot, eps, plus1, norm_v, q.data_ptr() if moved else None,
+            k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(), _row_pitch(table, table.shape[1]), table.shape[1],
+            lens.data_ptr(), cu.data_ptr(), B, _lib.raw_stream(idx),
         ),
         what,
     )
@@ -690,52 +710,51 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
     tensor reused between calls on one stream."""
     what = "paged_attention"
-    (n_pages, h, page, D), ks, vs = _pages(k_pages, v_pages, what)
-    dev = k_pages.device
-    if not isinstance(q, torch.Tensor) or q.dtype != torch.bfloat16 or q.device != dev or q.dim() != 3 or q.shape[2] != D:
+    idx, (n_pages, h, page, D, ks, vs) = _pages(k_pages, v_pages, what)
+    if not isinstance(q, torch.Tensor) or q.dtype is not _BF16 or q.get_device() != idx or q.dim() != 3 or q.shape[2] != D:
         raise SpinfError(f"{what}: q must be a bf16 [n, H, {D}] tensor on the pages' device")
-    n, H = q.shape[0], q.shape[1]
+    n, H, _ = q.shape
     if H % h or H == 0:
         raise SpinfError(f"{what}: {H} query heads do not share {h} key / value heads evenly")
-    if out is None:
-        out = torch.empty((n, H, D), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.device != dev or out.shape != q.shape:
+    if out is not None and (out.dtype is not _BF16 or out.get_device() != idx or out.shape != q.shape):
         raise SpinfError(f"{what}: out must be a bf16 tensor of q's shape on the pages' device")
-    for name, t in (("q", q), ("out", out)):
+    for t in (q,) if out is None else (q, out):
         if n and (t.stride(2) != 1 or (H > 1 and t.stride(1) != D)):
-            raise SpinfError(f"{what}: {name} needs contiguous heads (any row pitch)")
-    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
-    _paged_index(lens, "lens", what, dev, (None,))
-    _paged_index(cu, "cu", what, dev, (B + 1,))
-    _paged_index(table, "table", what, dev, (B, None), pitched=True)
+            raise SpinfError(f"{what}: q and out need contiguous heads (any row pitch)")
+    B = _paged_index(what, idx, lens, table, cu)
     room = table.shape[1] * page
-    max_len = room if max_len is None else max_len
+    if max_len is None:
+        max_len = room
     if max_len < 0 or max_len > room or max_q < 0:
         raise SpinfError(f"{what}: max_len {max_len} and max_q {max_q} must not be negative, nor max_len above what the table holds ({room})")
     if window is not None and window < 1:
         raise SpinfError(f"{what}: a window has at least one slot (None: no window)")
-    strides = None
+    strides = w_in = w_out = None
     if weights is None and weights_out is not None:
         raise SpinfError(f"{what}: weights_out comes with weights")
     if weights is not None:
-        weights_out = weights if weights_out is None else weights_out
-        for name, t in (("weights", weights), ("weights_out", weights_out)):
-            if t.dtype != torch.float32 or t.device != dev or t.dim() != 3 or tuple(t.shape[:2]) != (B, h) or t.shape[2] < max_len or (t.shape[2] > 1 and t.stride(2) != 1):
-                raise SpinfError(f"{what}: {name} must be an fp32 [{B}, {h}, at least {max_len}] tensor on the pages' device, contiguous over slots")
+        if weights_out is None:
+            weights_out = weights
+        for t in (weights, weights_out):
+            if t.dtype is not _F32 or t.get_device() != idx or t.dim() != 3 or t.shape[:2] != (B, h) or t.shape[2] < max_len or (t.shape[2] > 1 and t.stride(2) != 1):
+                raise SpinfError(f"{what}: weights must be fp32 [{B}, {h}, at least {max_len}] tensors on the pages' device, contiguous over slots")
         strides = (ctypes.c_int64 * 4)(weights.stride(0), weights.stride(1), weights_out.stride(0), weights_out.stride(1))
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+        w_in, w_out = weights.data_ptr(), weights_out.data_ptr()
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
             return paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace)
+    if out is None:
+        out = q.new_empty((n, H, D))
     lib = _lib.lib()
-    need = lib.spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, weights is not None)
+    need = lib.spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_out is not None)
     check(need, what)
     if need and (workspace is None or workspace.numel() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = q.new_empty(need, dtype=torch.uint8)
     check(
         lib.spinf_paged_attention(
-            ptr(q), q.stride(0) if n > 1 else H * D, n, H, h, D, ptr(k_pages), ptr(v_pages), n_pages, page, ks, vs, ptr(table), _table_pitch(table),
-            ptr(lens), ptr(cu), B, max_q, max_len, window or 0, scale, ptr(weights), ptr(weights_out), strides, decay, ptr(out),
-            out.stride(0) if n > 1 else H * D, ptr(workspace) if need else None, need, stream_ptr(),
+            q.data_ptr(), _row_pitch(q, H * D), n, H, h, D, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(),
+            _row_pitch(table, table.shape[1]), lens.data_ptr(), cu.data_ptr(), B, max_q, max_len, window or 0, scale, w_in, w_out, strides, decay,
+            out.data_ptr(), _row_pitch(out, H * D), workspace.data_ptr() if need else None, need, _lib.raw_stream(idx),
         ),
         what,
     )
@@ -750,33 +769,32 @@ def paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table,
     name -> (new lens int32 [B], kept int32 [B, Hkv, keep]: the old slots, -1 behind the last, their weights [B, Hkv, keep] or None).
     The old pages are the caller's to reuse."""
     what = "paged_evict"
-    (n_pages, h, page, D), ks, vs = _pages(k_pages, v_pages, what)
-    dev = k_pages.device
-    B = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
-    _paged_index(lens, "lens", what, dev, (None,))
-    _paged_index(table, "table", what, dev, (B, None), pitched=True)
-    _paged_index(new_table, "new_table", what, dev, (B, None), pitched=True)
+    idx, (n_pages, h, page, D, ks, vs) = _pages(k_pages, v_pages, what)
+    B = _paged_index(what, idx, lens, table, None, new_table)
     if keep < 1 or recent < 0 or recent > keep or keep > new_table.shape[1] * page:
         raise SpinfError(f"{what}: keep {keep} needs at least one token and as many as new_table holds at most, recent {recent} between 0 and keep")
     room = table.shape[1] * page
+    w_in, w_seq, w_head = None, 0, 0
     if weights is not None:
-        if weights.dtype != torch.float32 or weights.device != dev or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, h) or (weights.shape[2] > 1 and weights.stride(2) != 1):
+        if weights.dtype is not _F32 or weights.get_device() != idx or weights.dim() != 3 or weights.shape[:2] != (B, h) or (weights.shape[2] > 1 and weights.stride(2) != 1):
             raise SpinfError(f"{what}: weights must be an fp32 [{B}, {h}, cap] tensor on the pages' device, contiguous over slots")
         room = min(room, weights.shape[2])
-    max_len = room if max_len is None else max_len
+        w_in, w_seq, w_head = weights.data_ptr(), weights.stride(0), weights.stride(1)
+    if max_len is None:
+        max_len = room
     if max_len < 0 or max_len > room:
         raise SpinfError(f"{what}: max_len {max_len} is more than the table and the weights hold ({room})")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
             return paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table, max_len)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    kept = torch.empty((B, h, keep), dtype=torch.int32, device=dev)
-    w_out = None if weights is None else torch.empty((B, h, keep), dtype=torch.float32, device=dev)
+    new_lens = lens.new_empty((B,))
+    kept = lens.new_empty((B, h, keep))
+    w_out = None if weights is None else weights.new_empty((B, h, keep))
     check(
         _lib.lib().spinf_paged_evict(
-            ptr(k_pages), ptr(v_pages), n_pages, page, h, D, ks, vs, ptr(table), _table_pitch(table), ptr(lens), B, max_len, ptr(weights),
-            0 if weights is None else weights.stride(0), 0 if weights is None else weights.stride(1), keep, keep if weights is None else recent,
-            ptr(new_table), _table_pitch(new_table), ptr(new_lens), ptr(kept), ptr(w_out), stream_ptr(),
+            k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, h, D, ks, vs, table.data_ptr(), _row_pitch(table, table.shape[1]), lens.data_ptr(), B,
+            max_len, w_in, w_seq, w_head, keep, keep if weights is None else recent, new_table.data_ptr(), _row_pitch(new_table, new_table.shape[1]),
+            new_lens.data_ptr(), kept.data_ptr(), None if w_out is None else w_out.data_ptr(), _lib.raw_stream(idx),
         ),
         what,
     )
