@@ -120,17 +120,20 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, int
 
 // a launch that may start before the kernel ahead of it on the stream has ended (its pdl_wait holds it back)
 template <class... Params, class... Args>
-inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t st, int smem, Args... args) {
+inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t st, int smem, int cluster, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

@@ -13,13 +13,12 @@
 // the output needs no exchange and K and V are read from shared memory once. Running maximum and sum in fp32; P is rounded to bf16
 // for the product (its operands are 16 bit), which adds about what rounding the output to bf16 adds; the sum takes p unrounded.
 #include "gdn_mma.cuh"
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 #include <atomic>
 
 namespace spinf {
 
-static constexpr int RT = 64;            // query rows per item
 static constexpr int ROWS_THREADS = 288;  // eight warps and the producer
 
 template <int D>
@@ -37,36 +36,9 @@ struct RowsSmem {
 static_assert(RowsSmem<256>::TOTAL <= 232448 && RowsSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
 static_assert(RowsSmem<256>::PRE_OFF % 8 == 0 && RowsSmem<256>::BAR_OFF % 8 == 0 && RowsSmem<128>::BAR_OFF % 8 == 0, "alignment");
 
-struct PagedAttnArgs {
-  const __nv_bfloat16* q;
-  int64_t q_pitch;
-  __nv_bfloat16* out;
-  int64_t out_pitch;
-  int H, h, group, window;
-  float scale_log2;
-  // joined later: part_o [B][seq_parts][D], part_ml [B][seq_parts][2] (maximum in log2 units, sum)
-  float* part_o;
-  float2* part_ml;
-  int64_t seq_parts;
-  float* lse;     // [n][H] log2 units, or null: what the weights are normalised with
-  float* scores;  // [B][tok_cap][H][score_pitch] log2 units, or null: kept for the weights
-  int64_t score_pitch;
-  int tok_cap;
-};
-
-// which kernel takes a sequence, by its rows per kv head, and how its keys are cut into splits
-static constexpr int STEP_ROWS = 16;
-__device__ __forceinline__ bool step_class(const PagedSeq& q, int group) { return q.nq > 0 && q.nq * group <= STEP_ROWS; }
-__device__ __forceinline__ PagedCut step_cut(const PagedSeq& q, const PagedAttnArgs& a) { return paged_cut(q, a.window, 1, a.h, PG_SMS, 1); }
-__device__ __forceinline__ bool rows_class(const PagedSeq& q, int group) { return q.nq * group > STEP_ROWS; }
-__device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
-  const int rt = (q.nq * a.group + RT - 1) / RT;
-  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 1);
-}
-__device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a.group) ? step_cut(q, a) : rows_cut(q, a); }
 __device__ __forceinline__ int rows_items(const PagedSeqs& s, const PagedAttnArgs& a, int b, int* status) {
   const PagedSeq q = paged_seq(s, b, status);
-  if (!rows_class(q, a.group)) return 0;
+  if (!rows_class(q, a)) return 0;
   const PagedCut c = rows_cut(q, a);
   return a.h * c.row_tiles * c.splits;
 }
@@ -833,7 +805,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedSeqs s, cons
   constexpr int V = D / 128;  // float4 per lane
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSeq q = paged_seq(s, b, status);
-  if (q.nq == 0) return;
+  if (q.nq == 0 || chunk_class(q, a)) return;
   const PagedCut c = attn_cut(q, a);
   if (c.splits == 1) return;
   const int all = q.nq * a.group;
@@ -908,31 +880,45 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, co
   }
 }
 
+static constexpr int CHUNK_ROWS = 128;  // rows per kv head from which on the chunk kernel takes a sequence
+
 // what a call needs: sizes of the workspace's parts in bytes (256-byte multiples)
 struct PagedSizes {
-  int64_t seq_parts, part_o, part_ml, lse, scores, total;
+  int64_t seq_parts, part_o, part_ml, chunk_o, chunk_ml, unit_pre, lse, scores, total;
   int64_t score_pitch;
-  int tok_cap;
+  int tok_cap, chunk_rows, max_units;
 };
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights) {
   PagedSizes z = {};
   const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
   const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
+  z.chunk_rows = weights ? 0x7fffffff : CHUNK_ROWS;
+  const int64_t group = H / h, most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
   if (slots > 1) {
-    const int64_t by_rows = max_q * H * slots;             // every row in every split
+    const int64_t by_rows = (max_q < most ? max_q : most) * H * slots;  // every row in every split
     const int64_t by_items = static_cast<int64_t>(PG_SMS) * RT;  // every free slot one full row tile
     z.seq_parts = by_rows < by_items ? by_rows : by_items;
   }
   z.part_o = up256(B * z.seq_parts * D * 4);
   z.part_ml = up256(B * z.seq_parts * 8);
+  if (max_q > most) {
+    const int64_t tok = 256 / chunk_heads(static_cast<int>(group)), work = (max_q + tok - 1) / tok * (H / (256 / tok)) * (tiles > 0 ? tiles : 1);
+    int64_t units = work / CHUNK_MIN_TILES;
+    units = units < 1 ? 1 : units > CHUNK_UNITS ? CHUNK_UNITS : units;
+    const int64_t seqs = n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
+    z.max_units = static_cast<int>(seqs * units);
+    z.chunk_o = up256(seqs * units * 512 * D * 4);
+    z.chunk_ml = up256(seqs * units * 512 * 8);
+    z.unit_pre = up256((B + 1) * 4);
+  }
   if (weights) {
     z.lse = up256(n * H * 4);
     z.score_pitch = tiles * PG_TILE;
     z.tok_cap = static_cast<int>(max_q);
     z.scores = up256(B * z.tok_cap * H * z.score_pitch * 4);
   }
-  z.total = z.part_o + z.part_ml + z.lse + z.scores;
+  z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.unit_pre + z.lse + z.scores;
   return z;
 }
 
@@ -957,14 +943,16 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
     paged_step_kernel<D, 2><<<grid, STEP_THREADS, StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
   SPINF_CUDA_OK(cudaGetLastError());
   if (max_q * a.group > STEP_ROWS)
-    SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, tmK, tmV, s, a, status));
+    SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, 1, tmK, tmV, s, a, status));
   if (max_splits > 1) {
-    int64_t gx = (max_q * a.H + 7) / 8;
-    if (gx > 4096) gx = 4096;
-    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, s, a, status));
+    const int64_t most = a.chunk_rows / a.group;  // tokens of a sequence that is not the chunk kernel's
+    int64_t gx = ((max_q < most ? max_q : most) * a.H + 7) / 8;
+    if (gx > 1024) gx = 1024;
+    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, s, a, status));
   }
+  if (max_q * a.group > a.chunk_rows && (r = paged_chunk_launch(D, kp, vp, s, a, max_q, st, dev, status))) return r;
   if (w)
-    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, s, a, *w, status));
+    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, 1, s, a, *w, status));
   return 0;
 }
 
@@ -1024,11 +1012,21 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.seq_parts = z.seq_parts;
-  a.part_o = reinterpret_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(ws + z.part_o);
+  a.chunk_rows = z.chunk_rows;
+  a.max_units = z.max_units;
+  auto take = [&](int64_t bytes) {
+    uint8_t* p = ws;
+    ws += bytes;
+    return p;
+  };
+  a.part_o = reinterpret_cast<float*>(take(z.part_o));
+  a.part_ml = reinterpret_cast<float2*>(take(z.part_ml));
+  a.chunk_o = reinterpret_cast<float*>(take(z.chunk_o));
+  a.chunk_ml = reinterpret_cast<float2*>(take(z.chunk_ml));
+  a.unit_pre = reinterpret_cast<int32_t*>(take(z.unit_pre));
   if (weights_out) {
-    a.lse = reinterpret_cast<float*>(ws + z.part_o + z.part_ml);
-    a.scores = reinterpret_cast<float*>(ws + z.part_o + z.part_ml + z.lse);
+    a.lse = reinterpret_cast<float*>(take(z.lse));
+    a.scores = reinterpret_cast<float*>(take(z.scores));
     a.score_pitch = z.score_pitch;
     a.tok_cap = z.tok_cap;
   }

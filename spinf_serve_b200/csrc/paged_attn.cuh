@@ -1,0 +1,102 @@
+// The paged attention's arguments and the rules by which its kernels share out a call: which kernel takes a sequence, and how the
+// sequence's work is cut. All rules look at the sequence's own lengths and the model's heads only.
+#pragma once
+#include "paged.cuh"
+
+namespace spinf {
+
+struct PagedAttnArgs {
+  const __nv_bfloat16* q;
+  int64_t q_pitch;
+  __nv_bfloat16* out;
+  int64_t out_pitch;
+  int H, h, group, window;
+  float scale_log2;
+  int chunk_rows;  // sequences with more query rows per kv head than this are the chunk kernel's
+  // split keys, few rows: part_o [B][seq_parts][D], part_ml [B][seq_parts] (maximum in log2 units, sum)
+  float* part_o;
+  float2* part_ml;
+  int64_t seq_parts;
+  // cut items of the chunk kernel: 256 rows twice per unit; unit_pre [B + 1] the sequences' first units
+  float* chunk_o;
+  float2* chunk_ml;
+  int32_t* unit_pre;
+  int max_units;  // units there is room for
+  float* lse;     // [n][H] log2 units, or null: what the weights are normalised with
+  float* scores;  // [B][tok_cap][H][score_pitch] log2 units, or null: kept for the weights
+  int64_t score_pitch;
+  int tok_cap;
+};
+
+static constexpr int RT = 64;         // query rows of an item of the few-row kernel
+static constexpr int STEP_ROWS = 16;  // rows per kv head a decoding step's kernel takes
+
+__device__ __forceinline__ bool step_class(const PagedSeq& q, int group) { return q.nq > 0 && q.nq * group <= STEP_ROWS; }
+__device__ __forceinline__ bool chunk_class(const PagedSeq& q, const PagedAttnArgs& a) { return q.nq * a.group > a.chunk_rows; }
+__device__ __forceinline__ bool rows_class(const PagedSeq& q, const PagedAttnArgs& a) { return q.nq * a.group > STEP_ROWS && !chunk_class(q, a); }
+__device__ __forceinline__ PagedCut step_cut(const PagedSeq& q, const PagedAttnArgs& a) { return paged_cut(q, a.window, 1, a.h, PG_SMS, 1); }
+__device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
+  const int rt = (q.nq * a.group + RT - 1) / RT;
+  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 1);
+}
+__device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a.group) ? step_cut(q, a) : rows_cut(q, a); }
+
+// ---- the chunk kernel: items of 256 rows (hp heads x 256 / hp tokens), their key tiles dealt out in equal units
+static constexpr int CHUNK_UNITS = PG_SMS / 2;  // CTA pairs
+static constexpr int CHUNK_MIN_TILES = 8;       // least (item, tile) pairs of a unit: below that a cut costs more than it spreads
+
+// heads of an item: the largest power of two that divides the group, at most 8 (16 rows of a head in one CTA); more heads per item
+// mean fewer tokens, so less of the causal triangle is padding
+__host__ __device__ constexpr int chunk_heads(int group) { return group % 8 == 0 ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1; }
+
+struct ChunkCut {
+  int hp, tok, ntt, per_tt;  // heads and tokens of an item, token tiles, items of a token tile
+  int64_t work;              // (item, key tile) pairs
+  int units;
+
+  __device__ __forceinline__ void slots(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& lo, int& hi) const {
+    const int base = q.len - q.nq, first = base + tt * tok, end = (tt + 1) * tok < q.nq ? (tt + 1) * tok : q.nq;
+    lo = a.window > 0 && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
+    hi = base + end > 0 ? base + end : 0;
+  }
+  // key tiles [t0, t0 + nt) of a token tile; one (fully masked) where nothing is seen, so that its rows are written
+  __device__ __forceinline__ void tiles(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& t0, int& nt) const {
+    int lo, hi;
+    slots(q, a, tt, lo, hi);
+    t0 = lo / PG_TILE;
+    nt = (hi + PG_TILE - 1) / PG_TILE - t0;
+    nt = nt > 0 ? nt : 1;
+  }
+  __device__ __forceinline__ int64_t begin(int u) const { return work * u / units; }
+  __device__ __forceinline__ int unit_of(int64_t w) const { return static_cast<int>(((w + 1) * units - 1) / work); }
+};
+__device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttnArgs& a) {
+  ChunkCut c;
+  c.hp = chunk_heads(a.group);
+  c.tok = 256 / c.hp;
+  c.ntt = (q.nq + c.tok - 1) / c.tok;
+  c.per_tt = a.H / c.hp;
+  c.work = 0;
+  for (int tt = 0; tt < c.ntt; ++tt) {
+    int t0, nt;
+    c.tiles(q, a, tt, t0, nt);
+    c.work += static_cast<int64_t>(nt) * c.per_tt;
+  }
+  const int64_t u = c.work / CHUNK_MIN_TILES;
+  c.units = u < 1 ? 1 : u > CHUNK_UNITS ? CHUNK_UNITS : static_cast<int>(u);
+  return c;
+}
+
+// page of the `rows` slots from j on, or one past the last page (the copy then brings zeros) where no row sees any of them
+__device__ __forceinline__ int chunk_page(const PagedSeqs& s, const int32_t* pages, int j, int rows, int lo, int hi, int* status) {
+  if (j >= hi || j + rows <= lo) return s.n_pages;
+  const int pg = pages[j >> s.page_log2];
+  if (pg >= 0 && pg < s.n_pages) return pg;
+  atomicCAS(status, 0, ST_BAD_INDEX);
+  return s.n_pages;
+}
+
+int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, int64_t max_q, cudaStream_t st, int dev,
+                       int* status);
+
+}  // namespace spinf

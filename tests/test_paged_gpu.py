@@ -164,6 +164,26 @@ def test_attention_long_cache_and_many_rows(dev):
         check_out(c, c.attend(), want, mag, big)
 
 
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (8, 4, 128), (6, 1, 256), (3, 3, 128), (8, 1, 128)])
+@pytest.mark.parametrize("window", [None, 150])
+def test_chunks_against_the_definition(dev, H, h, D, page, window):
+    """sequences of the chunk kernel: whole and cut items, pages that end inside a tile, a prompt from the start, a batch with single
+    tokens in between, more rows than cached tokens"""
+    for seqs in ([(130, 130)], [(700, 161), (1, 1), (259, 259), (520, 20), (0, 0), (150, 200)]):
+        c = Call(dev, H, h, D, page, seqs, seed=page + H, token_major=page == 32)
+        want, _, mag, big = c.expect(window)
+        got = c.attend(window)
+        check_out(c, got, want, mag, big)
+        for b, (L, n) in enumerate(seqs):
+            assert (got[int(c.cu[b]) : int(c.cu[b]) + max(0, n - L)] == 0).all()
+            if n:
+                cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+                o, rows = c.on, slice(int(c.cu[b]), int(c.cu[b]) + n)
+                one = ops.paged_attention(o["q"][rows], o["k"], o["v"], o["table"][b : b + 1], o["lens_t"][b : b + 1], cu, n, D**-0.5, window=window)
+                assert torch.equal(one, got[rows])
+
+
 def test_attention_views_streams_and_a_graph(dev):
     c = Call(dev, 8, 2, 128, 64, [(300, 3), (129, 1)], seed=5)
     want, _, mag, big = c.expect()
