@@ -843,21 +843,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedSeqs s, cons
   }
 }
 
-struct PagedWeightArgs {
-  const float* in;  // [B][h][cap] fp32
-  float* out;
-  int64_t in_seq, in_head, out_seq, out_head;  // strides
-  float decay;                                 // 0: `in` is not read
-};
-
 // weights_out[b][g][j] = decay weights[b][g][j] + sum over the sequence's rows of kv head g of p(row, j), for j < len; a thread owns a
 // key and adds its rows in order
 __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, const PagedAttnArgs a, const PagedWeightArgs w, int* __restrict__ status) {
+  pdl_trigger();
   pdl_wait();
   const int b = blockIdx.z, g = blockIdx.y;
   const PagedSeq q = paged_seq(s, b, status);
   const int first = blockIdx.x * 1024;
-  if (first >= q.len) return;
+  if (first >= q.len || chunk_class(q, a)) return;
   const int all = q.nq * a.group, base = q.len - q.nq;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int r = 0; r < all; ++r) {
@@ -893,7 +887,7 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   PagedSizes z = {};
   const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
   const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
-  z.chunk_rows = weights ? 0x7fffffff : CHUNK_ROWS;
+  z.chunk_rows = CHUNK_ROWS;
   const int64_t group = H / h, most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
   if (slots > 1) {
     const int64_t by_rows = (max_q < most ? max_q : most) * H * slots;  // every row in every split
@@ -915,7 +909,7 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   if (weights) {
     z.lse = up256(n * H * 4);
     z.score_pitch = tiles * PG_TILE;
-    z.tok_cap = static_cast<int>(max_q);
+    z.tok_cap = static_cast<int>(max_q < most ? max_q : most);
     z.scores = up256(B * z.tok_cap * H * z.score_pitch * 4);
   }
   z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.unit_pre + z.lse + z.scores;
@@ -950,7 +944,7 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
     if (gx > 1024) gx = 1024;
     SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, s, a, status));
   }
-  if (max_q * a.group > a.chunk_rows && (r = paged_chunk_launch(D, kp, vp, s, a, max_q, st, dev, status))) return r;
+  if (max_q * a.group > a.chunk_rows && (r = paged_chunk_launch(D, kp, vp, s, a, w, max_q, st, dev, status))) return r;
   if (w)
     SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, 1, s, a, *w, status));
   return 0;

@@ -28,6 +28,13 @@ struct PagedAttnArgs {
   int tok_cap;
 };
 
+struct PagedWeightArgs {
+  const float* in;  // [B][h][cap] fp32
+  float* out;
+  int64_t in_seq, in_head, out_seq, out_head;  // strides
+  float decay;                                 // 0: `in` is not read
+};
+
 static constexpr int RT = 64;         // query rows of an item of the few-row kernel
 static constexpr int STEP_ROWS = 16;  // rows per kv head a decoding step's kernel takes
 
@@ -96,7 +103,7 @@ __device__ __forceinline__ int chunk_page(const PagedSeqs& s, const int32_t* pag
   return s.n_pages;
 }
 
-int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, int64_t max_q, cudaStream_t st, int dev,
-                       int* status);
+int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+                       cudaStream_t st, int dev, int* status);
 
 }  // namespace spinf

@@ -4,8 +4,9 @@
 // An item is 256 query rows of one kv head: `hp` heads that share it x 256 / hp tokens, the first half of the tokens in one CTA of
 // the pair and the second in the other. The pair walks the key tiles some row sees, 128 keys at a time:
 //   warp 0     one lane: TMA loads of Q and of this CTA's 64 keys of K
-//   warp 10    TMA loads of this CTA's half of V's dimensions (all 128 keys). In a tile with slots that no row of the item sees (a
-//              page's end, the front of a window) it waits for the copy and clears those rows: P is 0 there, but 0 * inf is not
+//   warp 10    one lane: TMA loads of this CTA's half of V's dimensions (all 128 keys)
+//   warp 11    in a tile with slots that no row of the item sees (a page's end, the front of a window) it waits for the copy of V and
+//              clears those rows, while warp 10 goes on: P is 0 there, but 0 * inf is not
 //   warp 1     owns tensor memory; the leader's lane issues S = Q K^T (M = 256) into one of two buffers and O += P V with P read from
 //              tensor memory; S of tile t + 1 is issued before P V of tile t
 //   warps 2-9  two softmax groups of four warps, thread = row, group A the first 64 keys of the tile and B the others; the mask is
@@ -25,7 +26,7 @@ namespace spinf {
 
 static constexpr int CH_KH = 64;
 static constexpr float CH_RESCALE = 24.f;  // log2 units: the reference maximum moves when a row's maximum grew by more
-static constexpr int CHUNK_THREADS = 352;
+static constexpr int CHUNK_THREADS = 384;
 
 template <int D>
 struct ChunkSmem {
@@ -137,8 +138,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* p_ready = s_full + 2;
   uint64_t* o_done = p_ready + 1;
   uint64_t* o_free = o_done + 1;
-  uint64_t* v_edge = o_free + 1;  // copies of a boundary tile, in the CTA's own barrier
-  uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(v_edge + 1);
+  uint64_t* v_edge = o_free + 1;  // NS: a boundary tile's copies complete on the CTA's own barrier
+  uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(v_edge + NS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_p + 1);
   float* xchg = reinterpret_cast<float*>(smem + L::XCHG_OFF);
   int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
@@ -157,12 +158,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 2);  // one arrival of each CTA's V warp: the copies are queued, or the boundary tile is ready
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_edge[i], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
     mbar_init(p_ready, 16);  // one arrival per softmax warp of both CTAs
     mbar_init(o_done, 1);
     mbar_init(o_free, 16);
-    mbar_init(v_edge, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -230,61 +231,73 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
     }
   } else if (warp == 10) {
-    const int rows = s.page_log2 < 7 ? 1 << s.page_log2 : PG_TILE;  // rows of a V box
-    uint32_t cnt = 0, edges = 0;
-    bool ok = true;
-    for (int it = pair; it < total && ok; it += n_pairs) {
-      ChunkWalk wk;
-      wk.start(s, a, pre, it, status);
-      const int32_t* pages = s.table + wk.b * s.table_pitch;
-      ChunkSeg g;
-      while (ok && wk.next(a, g)) {
-        for (int t = g.ta; t < g.tb; ++t, ++cnt) {
-          const uint32_t st = cnt % NS;
-          const bool edge = t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi;
-          if (lane == 0) {
-            ok = mbar_wait(wc, &v_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
-            if (ok) {
-              if (edge)
-                mbar_expect_tx(v_edge, L::KV);
-              else if (rank == 0)
-                mbar_expect_tx(&v_full[st], 2 * L::KV);
-              else
-                mbar_arrive_cluster(map_to_cta(&v_full[st], 0));
-              const uint32_t bar = map_to_cta(&v_full[st], 0);
-              for (int x = 0; x < PG_TILE / rows; ++x) {
-                const int j = t * PG_TILE + x * rows;
-                const int pg = chunk_page(s, pages, j, rows, g.lo, g.hi, status);
-                uint8_t* dst = smem + L::V_OFF + st * L::KV + x * rows * 128;
-                for (int y = 0; y < (rows == PG_TILE ? 1 : V_SLABS); ++y) {
-                  const int slab = static_cast<int>(rank) * V_SLABS + y;
-                  if (edge)
-                    tma_load_5d(dst + y * PG_TILE * 128, &tmV, 0, j & in_page, slab, g.g, pg, v_edge);
-                  else
-                    tma_load_5d_pair(dst + y * PG_TILE * 128, &tmV, 0, j & in_page, slab, g.g, pg, bar);
-                }
+    if (lane == 0) {
+      const int rows = s.page_log2 < 7 ? 1 << s.page_log2 : PG_TILE;  // rows of a V box
+      uint32_t cnt = 0;
+      bool ok = true;
+      for (int it = pair; it < total && ok; it += n_pairs) {
+        ChunkWalk wk;
+        wk.start(s, a, pre, it, status);
+        const int32_t* pages = s.table + wk.b * s.table_pitch;
+        ChunkSeg g;
+        while (ok && wk.next(a, g)) {
+          for (int t = g.ta; t < g.tb; ++t, ++cnt) {
+            const uint32_t st = cnt % NS;
+            const bool edge = t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi;
+            if (!mbar_wait(wc, &v_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+            if (edge)
+              mbar_expect_tx(&v_edge[st], L::KV);
+            else if (rank == 0)
+              mbar_expect_tx(&v_full[st], 2 * L::KV);
+            else
+              mbar_arrive_cluster(map_to_cta(&v_full[st], 0));
+            const uint32_t bar = map_to_cta(&v_full[st], 0);
+            for (int x = 0; x < PG_TILE / rows; ++x) {
+              const int j = t * PG_TILE + x * rows;
+              const int pg = chunk_page(s, pages, j, rows, g.lo, g.hi, status);
+              uint8_t* dst = smem + L::V_OFF + st * L::KV + x * rows * 128;
+              for (int y = 0; y < (rows == PG_TILE ? 1 : V_SLABS); ++y) {
+                const int slab = static_cast<int>(rank) * V_SLABS + y;
+                if (edge)
+                  tma_load_5d(dst + y * PG_TILE * 128, &tmV, 0, j & in_page, slab, g.g, pg, &v_edge[st]);
+                else
+                  tma_load_5d_pair(dst + y * PG_TILE * 128, &tmV, 0, j & in_page, slab, g.g, pg, bar);
               }
-              if (edge) ok = mbar_wait(wc, v_edge, edges & 1u, ST_TIMEOUT_FULL);
             }
-          }
-          ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
-          if (!ok) break;
-          if (edge) {
-            ++edges;
-            for (int x = lane; x < PG_TILE * V_SLABS * 8; x += 32) {
-              const int key = (x >> 3) % PG_TILE, slab = (x >> 3) / PG_TILE, j = t * PG_TILE + key;
-              if (j < g.lo || j >= g.hi)
-                *reinterpret_cast<uint4*>(smem + L::V_OFF + st * L::KV + slab * PG_TILE * 128 + sw128_offset(key, x & 7)) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_release(map_to_cta(&v_full[st], 0));
           }
         }
       }
     }
-    if (*abort_flag && lane == 0)  // a boundary tile's copies complete here, not on the leader's barriers
-      for (int spin = 0; spin < 4096 && !mbar_try_wait(v_edge, edges & 1u); ++spin) {}
+  } else if (warp == 11) {
+    uint32_t cnt = 0, edges[NS];  // boundary tiles each stage has held
+#pragma unroll
+    for (int i = 0; i < NS; ++i) edges[i] = 0;
+    bool ok = true;
+    for (int it = pair; it < total && ok; it += n_pairs) {
+      ChunkWalk wk;
+      wk.start(s, a, pre, it, status);
+      ChunkSeg g;
+      while (ok && wk.next(a, g)) {
+        for (int t = g.ta; t < g.tb; ++t, ++cnt) {
+          if (t * PG_TILE >= g.lo && (t + 1) * PG_TILE <= g.hi) continue;
+          const uint32_t st = cnt % NS;
+          uint32_t turn = 0;
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+            if (static_cast<uint32_t>(i) == st) turn = edges[i]++;
+          ok = __all_sync(0xffffffffu, mbar_wait(wc, &v_edge[st], turn & 1u, ST_TIMEOUT_FULL));
+          if (!ok) break;
+          for (int x = lane; x < PG_TILE * V_SLABS * 8; x += 32) {
+            const int key = (x >> 3) % PG_TILE, slab = (x >> 3) / PG_TILE, j = t * PG_TILE + key;
+            if (j < g.lo || j >= g.hi)
+              *reinterpret_cast<uint4*>(smem + L::V_OFF + st * L::KV + slab * PG_TILE * 128 + sw128_offset(key, x & 7)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_release(map_to_cta(&v_full[st], 0));
+        }
+      }
+    }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t q_addr = smem_u32(smem);
@@ -562,9 +575,252 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s
   }
 }
 
+// ---------------------------------------------------------------- the keys' attention weights of a chunk
+// weights_out[j] = decay weights_in[j] + sum over rows p(row, j), p = exp2(s scale - lse(row)), with the rows' lse from above: a second
+// pass over Q K^T, this time with the keys as the rows of the product, so that a key's sum stays in one thread: S^T = K Q^T, thread =
+// key, 64 query rows a stage along its columns. No reduction across threads, no atomics: a key adds its rows in one fixed order.
+// Item = 256 keys of a (sequence, kv head), both tiles of K resident in shared memory while the rows that see any of them stream by.
+// Bound by the exponentials (256 x 64 a stage at 16 per cycle and SM: 1 024 cycles, the products 512 at D 128 and 1 024 at D 256).
 template <int D>
-static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, int64_t max_q, cudaStream_t st, int dev,
-                        int* status) {
+struct ChunkWeightSmem {
+  static constexpr int SLABS = D / 64;
+  static constexpr int K_TILE = SLABS * 128 * 128;  // 128 keys
+  static constexpr int NK = D == 256 ? 1 : 2;       // items whose keys are held (or being fetched)
+  static constexpr int Q_STAGE = SLABS * 64 * 128;  // 64 rows of q
+  static constexpr int NQ = D == 256 ? 2 : 4;
+  static constexpr int NS = 4;                      // S buffers of 128 columns, each with its rows' lse
+  static constexpr int Q_OFF = NK * 2 * K_TILE;
+  static constexpr int LSE_OFF = Q_OFF + NQ * Q_STAGE;
+  static constexpr int BAR_OFF = LSE_OFF + NS * 64 * 4;
+  static constexpr int PRE_OFF = BAR_OFF + 256;
+  static constexpr int TOTAL = PRE_OFF + (PG_MAX_SEQS + 2) * 4 + 1024;
+};
+static_assert(ChunkWeightSmem<256>::TOTAL <= 232448 && ChunkWeightSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
+static constexpr int CHUNK_WEIGHT_THREADS = 352;
+
+struct ChunkWeightItem {
+  PagedSeq q;
+  int b, g, j0;          // first key
+  int hp, tok, sets;     // heads and tokens of a stage of 64 rows, head sets of the kv head
+  int tt0, tt1;          // token tiles with rows that see some of the keys
+};
+__device__ __forceinline__ ChunkWeightItem chunk_weight_item(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int it, int* status) {
+  ChunkWeightItem w;
+  w.b = paged_find(pre, s.B, it);
+  w.q = paged_seq(s, w.b, status);
+  const int x = it - pre[w.b];
+  w.g = x % a.h;
+  w.j0 = x / a.h * 256;
+  w.hp = chunk_heads(a.group);
+  w.tok = 64 / w.hp;
+  w.sets = a.group / w.hp;
+  const int base = w.q.len - w.q.nq;
+  const int first = w.j0 > base ? w.j0 - base : 0;  // tokens before it sit before every key
+  int end = w.q.nq;
+  if (a.window > 0) {
+    const int64_t e = static_cast<int64_t>(w.j0) + 255 + a.window - base;  // tokens from it on see none of the keys
+    end = e < end ? (e > 0 ? static_cast<int>(e) : 0) : end;
+  }
+  w.tt0 = first / w.tok;
+  w.tt1 = end > first ? (end + w.tok - 1) / w.tok : w.tt0;
+  return w;
+}
+
+template <int D>
+__global__ void __launch_bounds__(CHUNK_WEIGHT_THREADS, 1)
+paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const PagedSeqs s, const PagedAttnArgs a,
+                          const PagedWeightArgs wa, int* __restrict__ status) {
+  using L = ChunkWeightSmem<D>;
+  constexpr int SLABS = L::SLABS, NK = L::NK, NQ = L::NQ, NS = L::NS;
+  constexpr uint32_t IDESC = make_idesc(FMT_BF16, FMT_BF16, 128, 64, 0, 0);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* k_empty = k_full + NK;
+  uint64_t* q_full = k_empty + NK;
+  uint64_t* q_empty = q_full + NQ;
+  uint64_t* s_full = q_empty + NQ;
+  uint64_t* s_empty = s_full + NS;
+  uint64_t* lse_full = s_empty + NS;
+  uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(lse_full + NS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_p + 1);
+  float* lse_ring = reinterpret_cast<float*>(smem + L::LSE_OFF);
+  int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WaitCtx wc{abort_flag, status};
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < NQ; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 8), mbar_init(&lse_full[i], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_base_p, 512);
+    tmem_relinquish();
+  }
+  paged_item_prefix(s.B, pre, CHUNK_WEIGHT_THREADS, [&](int b) {
+    const PagedSeq q = paged_seq(s, b, status);
+    return chunk_class(q, a) ? a.h * ((q.len + 255) / 256) : 0;
+  });
+  const int total = pre[s.B];
+  pdl_wait();  // lse is the kernels' ahead
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_p;
+  const int in_page = (1 << s.page_log2) - 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int rows = s.page_log2 < 7 ? 1 << s.page_log2 : PG_TILE;
+      uint32_t n = 0;
+      for (int it = blockIdx.x; it < total; it += gridDim.x, ++n) {
+        const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+        const int32_t* pages = s.table + w.b * s.table_pitch;
+        const uint32_t st = n % NK;
+        if (!mbar_wait(wc, &k_empty[st], ((n / NK) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) break;
+        mbar_expect_tx(&k_full[st], 2 * L::K_TILE);
+        for (int t = 0; t < 2; ++t)
+          for (int x = 0; x < PG_TILE / rows; ++x) {
+            const int j = w.j0 + t * PG_TILE + x * rows;
+            const int pg = chunk_page(s, pages, j, rows, 0, w.q.len, status);
+            uint8_t* dst = smem + (st * 2 + t) * L::K_TILE + x * rows * 128;
+            for (int y = 0; y < (rows == PG_TILE ? 1 : SLABS); ++y) tma_load_5d(dst + y * PG_TILE * 128, &tmK, 0, j & in_page, y, w.g, pg, &k_full[st]);
+          }
+      }
+      if (*abort_flag)  // bounded wait for copies that may still be in flight
+        for (uint32_t c = n > static_cast<uint32_t>(NK) ? n - NK : 0; c < n; ++c)
+          for (int spin = 0; spin < 4096 && !mbar_try_wait(&k_full[c % NK], (c / NK) & 1u); ++spin) {}
+    }
+  } else if (warp == 10) {
+    uint32_t n = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+      const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+      for (int set = 0; set < w.sets && ok; ++set)
+        for (int tt = w.tt0; tt < w.tt1; ++tt, ++n) {
+          const uint32_t st = n % NQ, sl = n % NS;
+          ok = __all_sync(0xffffffffu, mbar_wait(wc, &s_empty[sl], ((n / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY) &&
+                                           mbar_wait(wc, &q_empty[st], ((n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY));
+          if (!ok) break;
+          const int h0 = w.g * a.group + set * w.hp;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = lane + 32 * x, tok = tt * w.tok + r % w.tok;
+            float v = INFINITY;  // rows that are none, or see nothing, weigh nothing: exp2(s - inf) = 0
+            if (tok < w.q.nq) v = a.lse[static_cast<int64_t>(w.q.row0 + tok) * a.H + h0 + r / w.tok];
+            lse_ring[sl * 64 + r] = v == -INFINITY ? INFINITY : v;
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&lse_full[sl]);
+            mbar_expect_tx(&q_full[st], L::Q_STAGE);
+            for (int hh = 0; hh < w.hp; ++hh)
+              for (int x = 0; x < SLABS; ++x)
+                tma_load_2d(smem + L::Q_OFF + st * L::Q_STAGE + x * 64 * 128 + hh * w.tok * 128, &tmQ, (h0 + hh) * D + x * 64, w.q.row0 + tt * w.tok, &q_full[st]);
+          }
+        }
+    }
+    if (*abort_flag && lane == 0)
+      for (uint32_t c = n > static_cast<uint32_t>(NQ) ? n - NQ : 0; c < n; ++c)
+        for (int spin = 0; spin < 4096 && !mbar_try_wait(&q_full[c % NQ], (c / NQ) & 1u); ++spin) {}
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t n = 0, k = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+        const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+        if (!mbar_wait(wc, &k_full[k % NK], (k / NK) & 1u, ST_TIMEOUT_FULL)) break;
+        const uint32_t k_addr = smem_u32(smem) + (k % NK) * 2 * L::K_TILE;
+        const int stages = w.sets * (w.tt1 - w.tt0);
+        for (int i = 0; i < stages; ++i, ++n) {
+          if (!mbar_wait(wc, &s_empty[n % NS], ((n / NS) & 1u) ^ 1u, ST_TIMEOUT_TMEM)) { ok = false; break; }
+          if (!mbar_wait(wc, &q_full[n % NQ], (n / NQ) & 1u, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t q_addr = smem_u32(smem + L::Q_OFF + (n % NQ) * L::Q_STAGE);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < SLABS; ++x) {
+              const uint64_t ad = make_smem_desc_sw128(k_addr + t * L::K_TILE + x * 128 * 128, 16, 1024);
+              const uint64_t bd = make_smem_desc_sw128(q_addr + x * 64 * 128, 16, 1024);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) umma_f16_ss(tmem_base + (n % NS) * 128 + t * 64, ad + 2 * y, bd + 2 * y, IDESC, (x | y) != 0);
+            }
+          umma_commit(&q_empty[n % NQ]);
+          umma_commit(&s_full[n % NS]);
+        }
+        if (ok) umma_commit(&k_empty[k % NK]);
+      }
+    }
+  } else {
+    const int kt = (warp - 2) >> 2, qd = warp & 3;
+    const uint32_t lane_off = static_cast<uint32_t>(qd * 32) << 16;
+    uint32_t n = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+      const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+      const int j = w.j0 + kt * PG_TILE + qd * 32 + lane, base = w.q.len - w.q.nq;
+      const int j_end = a.window > 0 ? j + a.window : 0x7fffffff;  // slots [j, j_end) see the key
+      const int tile_lo = w.j0 + kt * PG_TILE;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int set = 0; set < w.sets && ok; ++set)
+        for (int tt = w.tt0; tt < w.tt1; ++tt, ++n) {
+          const uint32_t sl = n % NS;
+          ok = mbar_wait(wc, &s_full[sl], (n / NS) & 1u, ST_TIMEOUT_TMEM) && mbar_wait(wc, &lse_full[sl], (n / NS) & 1u, ST_TIMEOUT_FULL);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t v0[32], v1[32];
+          const uint32_t at = tmem_base + lane_off + sl * 128 + kt * 64;
+          tmem_ld_x32(at, v0);
+          tmem_ld_x32(at + 32, v1);
+          tmem_wait_ld();
+          const float4* lse = reinterpret_cast<const float4*>(lse_ring + sl * 64);
+          const int slot0 = base + tt * w.tok;  // of the stage's first token
+          const bool masked = slot0 < tile_lo + PG_TILE - 1 || (a.window > 0 && slot0 + w.tok - 1 >= tile_lo + a.window);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float4 z = lse[c];
+            const float zz[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int col = c * 4 + x;
+              const float sv = __uint_as_float(col < 32 ? v0[col & 31] : v1[col & 31]);
+              float p = fast_exp2(fmaf(sv, a.scale_log2, -zz[x]));
+              if (masked) {
+                const int slot = slot0 + (col & (w.tok - 1));  // w.tok is a power of two
+                p = slot >= j && slot < j_end ? p : 0.f;
+              }
+              sum[x] += p;
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[sl]);
+        }
+      if (ok && j < w.q.len) {
+        const float old = wa.decay != 0.f ? wa.in[w.b * wa.in_seq + w.g * wa.in_head + j] * wa.decay : 0.f;
+        wa.out[w.b * wa.out_seq + w.g * wa.out_head + j] = old + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int D>
+static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+                        cudaStream_t st, int dev, int* status) {
   using L = ChunkSmem<D>;
   CUtensorMap tmQ, tmK, tmV;
   const int hp = chunk_heads(a.group);
@@ -577,6 +833,7 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev].load(std::memory_order_acquire)) {
     SPINF_CUDA_OK(cudaFuncSetAttribute(paged_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+    SPINF_CUDA_OK(cudaFuncSetAttribute(paged_chunk_weight_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkWeightSmem<D>::TOTAL));
     attr_set[dev].store(true, std::memory_order_release);
   }
   SPINF_CUDA_OK(launch_after(paged_chunk_kernel<D>, dim3(static_cast<unsigned>(sm_count() / 2 * 2)), dim3(CHUNK_THREADS), st, L::TOTAL, 2, tmQ, tmK, tmV, s, a,
@@ -584,12 +841,18 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   int64_t gx = (max_q * a.H + 7) / 8;
   if (gx > 2048) gx = 2048;
   SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, s, a, status));
+  if (!w) return 0;
+  CUtensorMap tmQw, tmKw;
+  if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;
+  if ((r = make_tmap_pages(&tmKw, kp, vrows, vrows == PG_TILE ? D / 64 : 1))) return r;
+  SPINF_CUDA_OK(launch_after(paged_chunk_weight_kernel<D>, dim3(static_cast<unsigned>(sm_count())), dim3(CHUNK_WEIGHT_THREADS), st, ChunkWeightSmem<D>::TOTAL, 1,
+                             tmQw, tmKw, s, a, *w, status));
   return 0;
 }
 
-int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, int64_t max_q, cudaStream_t st, int dev,
-                       int* status) {
-  return D == 256 ? launch_chunk<256>(kp, vp, s, a, max_q, st, dev, status) : launch_chunk<128>(kp, vp, s, a, max_q, st, dev, status);
+int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+                       cudaStream_t st, int dev, int* status) {
+  return D == 256 ? launch_chunk<256>(kp, vp, s, a, w, max_q, st, dev, status) : launch_chunk<128>(kp, vp, s, a, w, max_q, st, dev, status);
 }
 
 }  // namespace spinf

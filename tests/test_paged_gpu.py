@@ -184,6 +184,23 @@ def test_chunks_against_the_definition(dev, H, h, D, page, window):
                 assert torch.equal(one, got[rows])
 
 
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (8, 4, 128), (6, 1, 256), (3, 3, 128), (8, 1, 128)])
+@pytest.mark.parametrize("window", [None, 150])
+def test_chunks_keep_the_slots_weights(dev, H, h, D, page, window):
+    seqs = [(700, 161), (259, 259), (9, 2), (520, 140), (150, 200), (90, 0)]
+    c = Call(dev, H, h, D, page, seqs, seed=page + H, spare=0)
+    want, weights, mag, big = c.expect(window)
+    w = torch.rand((len(seqs), h, 704), generator=c.gen)
+    on = w.to(dev)
+    check_out(c, c.attend(window, weights=on, max_len=700), want, mag, big)
+    rel = float(score_noise(c, big, 700).max()) + 2.0**-20  # (the slots' sums run over up to 1 600 rows)
+    for b, (L, _) in enumerate(seqs):
+        ref = w[b, :, :L].double() + weights[b]
+        assert ((on[b, :, :L].double().cpu() - ref).abs() <= rel * ref + 1600 * 2.0**-24 * ref).all()
+        assert torch.equal(on[b, :, L:].cpu(), w[b, :, L:])
+
+
 def test_attention_views_streams_and_a_graph(dev):
     c = Call(dev, 8, 2, 128, 64, [(300, 3), (129, 1)], seed=5)
     want, _, mag, big = c.expect()
