@@ -19,6 +19,7 @@
 
 namespace spinf {
 
+static constexpr int PLAN = 32;          // items planned at a time, one per lane of the producer warp
 static constexpr int ROWS_THREADS = 288;  // eight warps and the producer
 
 template <int D>
@@ -26,54 +27,152 @@ struct RowsSmem {
   static constexpr int SLABS = D / 64;
   static constexpr int STAGE = 64 * D * 2;  // 64 keys of K or V
   static constexpr int NST = D == 256 ? 5 : 10;
-  static constexpr int Q_OFF = NST * STAGE;
-  static constexpr int P_OFF = Q_OFF + RT * D * 2;
-  static constexpr int RED_OFF = P_OFF + RT * PG_TILE * 2;  // [64][8] floats, twice: row maxima, row sums
-  static constexpr int PRE_OFF = RED_OFF + 2 * RT * 8 * 4;
+  static constexpr int Q_PITCH = D * 2 + 16;  // a row of q; the 16 bytes spread the rows over the banks
+  static constexpr int Q_SLOT = RT * Q_PITCH;
+  static constexpr int P_OFF = NST * STAGE;
+  static constexpr int Q_OFF = P_OFF + RT * PG_TILE * 2;
+  static constexpr int RED_OFF = Q_OFF + Q_SLOT;  // [64][8] floats, twice: row maxima, row sums
+  static constexpr int ITEM_OFF = RED_OFF + 2 * RT * 8 * 4;
+  static constexpr int PRE_OFF = ITEM_OFF + (1 + PLAN) * 64;
   static constexpr int BAR_OFF = PRE_OFF + (PG_MAX_SEQS + 2) * 4;
-  static constexpr int TOTAL = BAR_OFF + 2 * NST * 8 + 16 + 1024;
+  static constexpr int TOTAL = BAR_OFF + (2 * NST + 2) * 8 + 16 + 1024;
 };
 static_assert(RowsSmem<256>::TOTAL <= 232448 && RowsSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
 static_assert(RowsSmem<256>::PRE_OFF % 8 == 0 && RowsSmem<256>::BAR_OFF % 8 == 0 && RowsSmem<128>::BAR_OFF % 8 == 0, "alignment");
 
-__device__ __forceinline__ int rows_items(const PagedSeqs& s, const PagedAttnArgs& a, int b, int* status) {
-  const PagedSeq q = paged_seq(s, b, status);
-  if (!rows_class(q, a)) return 0;
-  const PagedCut c = rows_cut(q, a);
-  return a.h * c.row_tiles * c.splits;
-}
-
-struct RowsItem {
-  int b, g, rt, split;
-  PagedSeq q;
-  PagedCut c;
-  int r0, rows;    // first row of the tile within the sequence's rows of the head (token * group + head in group), rows of the tile
-  int lo, hi;      // slots that some row of the tile sees
-  int t0, t1;      // key tiles of this split that hold some of them
+// what the consumers need of an item; the producer writes it beside the rows of q
+struct alignas(4) KeyItem {
+  int b, g, split, splits;
+  int row0, nq, base;  // first row of q, rows of the sequence, slot of the first
+  int r0, rows;        // rows of the item among the sequence's rows of the head (token * group + head in group)
+  int lo, hi;          // slots that some row of the item sees
+  int u0, u1;          // 64-key units
 };
 
-__device__ __forceinline__ RowsItem rows_item(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int it, int* status) {
-  RowsItem w;
+template <bool STEP>
+__device__ __forceinline__ int key_items(const PagedSeqs& s, const PagedAttnArgs& a, int b, int* status) {
+  const PagedSeq q = paged_seq(s, b, status);
+  if (!(STEP ? step_class(q, a.group) : rows_class(q, a))) return 0;
+  const PagedCut c = STEP ? step_cut(q, a) : rows_cut(q, a);
+  return a.h * c.row_tiles * c.splits;
+}
+template <bool STEP>
+__device__ __forceinline__ KeyItem key_item(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int it, int* status) {
+  KeyItem w;
   w.b = paged_find(pre, s.B, it);
-  w.q = paged_seq(s, w.b, status);
-  w.c = rows_cut(w.q, a);
+  const PagedSeq q = paged_seq(s, w.b, status);
+  const PagedCut c = STEP ? step_cut(q, a) : rows_cut(q, a);
   int x = it - pre[w.b];
-  w.rt = x % w.c.row_tiles;
-  x /= w.c.row_tiles;
+  w.r0 = STEP ? 0 : x % c.row_tiles * RT;
+  if (!STEP) x /= c.row_tiles;
   w.g = x % a.h;
   w.split = x / a.h;
-  w.r0 = w.rt * RT;
-  const int all = w.q.nq * a.group;
-  w.rows = all - w.r0 < RT ? all - w.r0 : RT;
-  const int first = w.q.len - w.q.nq + w.r0 / a.group, last = w.q.len - w.q.nq + (w.r0 + w.rows - 1) / a.group;
+  w.splits = c.splits;
+  w.row0 = q.row0, w.nq = q.nq, w.base = q.len - q.nq;
+  const int all = q.nq * a.group;
+  w.rows = STEP || all - w.r0 < RT ? all - w.r0 : RT;
+  const int first = w.base + w.r0 / a.group, last = w.base + (w.r0 + w.rows - 1) / a.group;
   w.lo = a.window > 0 && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
   w.hi = last + 1 > 0 ? last + 1 : 0;
-  const int s0 = w.c.t_lo + w.split * w.c.tiles_per_split, s1 = s0 + w.c.tiles_per_split;
+  const int s0 = c.t_lo + w.split * c.tiles_per_split, s1 = s0 + c.tiles_per_split < c.t_hi ? s0 + c.tiles_per_split : c.t_hi;
   const int e0 = w.lo / PG_TILE, e1 = (w.hi + PG_TILE - 1) / PG_TILE;
-  w.t0 = s0 > e0 ? s0 : e0;
-  w.t1 = s1 < e1 ? s1 : e1;
-  if (w.t1 > w.c.t_hi) w.t1 = w.c.t_hi;
+  w.u0 = 2 * (s0 > e0 ? s0 : e0);
+  w.u1 = 2 * (s1 < e1 ? s1 : e1);
+  if (STEP && w.u1 * 64 >= w.hi + 64) w.u1 -= 1;  // units one by one: the last tile's second half may lie behind the last slot
+  if (w.u1 < w.u0) w.u1 = w.u0;
   return w;
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// The producer warp of both few-row kernels. Items are planned 32 at a time, one per lane, and an item's page indexes are fetched by
+// the lanes together, the next item's while this one is copied, so that no step of the copy loop waits for a load of its own. Order of
+// the stages: K and V of a unit in turn (STEP), or the two K units of a 128-key tile and then its two V units.
+template <int D, bool STEP, int NST, int STAGE, int Q_PITCH, int Q_SLOT, int NQ>
+__device__ __forceinline__ void produce_keys(const PagedSeqs& s, const PagedAttnArgs& a, const CUtensorMap* tmK, const CUtensorMap* tmV, const int* pre,
+                                             int total, uint8_t* ring, uint8_t* q_slots, KeyItem* items, KeyItem* plan, uint64_t* full, uint64_t* empty,
+                                             uint64_t* q_full, uint64_t* q_empty, const WaitCtx& wc, int* status) {
+  const int lane = threadIdx.x & 31;
+  const int br = s.page_log2 < 6 ? s.page_log2 : 6, box_rows = 1 << br, in_page = (1 << s.page_log2) - 1;
+  uint32_t cnt = 0, item_n = 0;
+  bool ok = true;
+  // page of box x of an item (boxes of 2^br slots from its first unit on): -1 where no row sees any of them, -2 for a bad index
+  auto page_of = [&](const KeyItem& w, int x) -> int {
+    const int j = (w.u0 * 64) + (x << br);
+    if (j >= w.u1 * 64 || j >= w.hi || j + box_rows <= w.lo) return -1;
+    const int pg = s.table[w.b * s.table_pitch + (j >> s.page_log2)];
+    return pg >= 0 && pg < s.n_pages ? pg : -2;
+  };
+  for (int k0 = 0; ok && static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(k0) * gridDim.x < total; k0 += PLAN) {
+    const int64_t mine = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(k0 + lane) * gridDim.x;
+    __syncwarp();
+    if (mine < total) plan[lane] = key_item<STEP>(s, a, pre, static_cast<int>(mine), status);
+    const int n_plan = __popc(__ballot_sync(0xffffffffu, mine < total));
+    __syncwarp();
+    int pages_next = page_of(plan[0], lane);
+    for (int k = 0; k < n_plan && ok; ++k, ++item_n) {
+      const KeyItem w = plan[k];
+      int pages = pages_next;
+      if (k + 1 < n_plan) pages_next = page_of(plan[k + 1], lane);
+      const uint32_t qs = item_n % NQ;
+      if (lane == 0) {
+        ok = mbar_wait(wc, &q_empty[qs], ((item_n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+        if (ok) {
+          items[qs] = w;
+          mbar_expect_tx(&q_full[qs], w.rows * D * 2);  // (an arrival: releases the item's numbers to the consumers as well)
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      if (!ok) break;
+      for (int r = lane; r < w.rows; r += 32) {
+        const int rr = w.r0 + r;
+        bulk_load(q_slots + qs * Q_SLOT + r * Q_PITCH, a.q + (w.row0 + rr / a.group) * a.q_pitch + static_cast<int64_t>(w.g * a.group + rr % a.group) * D,
+                  D * 2, &q_full[qs]);
+      }
+      constexpr int UNITS = STEP ? 1 : 2;
+      const int boxes = 64 >> br;  // of a unit
+      for (int u = w.u0; u < w.u1 && ok; u += UNITS) {
+        const int x0 = (u - w.u0) * boxes;
+        if (x0 && (x0 & 31) == 0) pages = page_of(w, x0 + lane);
+        int pg[UNITS][4];
+#pragma unroll
+        for (int v = 0; v < UNITS; ++v)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) pg[v][y] = __shfl_sync(0xffffffffu, pages, (x0 + v * boxes + y) & 31);
+        if (lane == 0) {
+#pragma unroll
+          for (int part = 0; part < 2 * UNITS; ++part, ++cnt) {
+            const int v = part % UNITS;
+            const uint32_t st = cnt % NST;
+            if (!mbar_wait(wc, &empty[st], ((cnt / NST) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+            int bytes = 0;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              if (y >= boxes) continue;
+              if (pg[v][y] == -2) atomicCAS(status, 0, ST_BAD_INDEX);
+              bytes += pg[v][y] >= 0 ? box_rows * D * 2 : 0;
+            }
+            mbar_expect_tx(&full[st], bytes);  // boxes that no row sees stay as they are (masked for K, cleared for V)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (y < boxes && pg[v][y] >= 0)
+                tma_load_5d(ring + st * STAGE + y * box_rows * D * 2, part < UNITS ? tmK : tmV, 0, ((u + v) * 64 + y * box_rows) & in_page, 0, w.g, pg[v][y],
+                            &full[st]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      }
+    }
+  }
+  if (*wc.abort_flag && lane == 0) {  // bounded wait for copies that may still be in flight
+    for (uint32_t c = cnt > static_cast<uint32_t>(NST) ? cnt - NST : 0; c < cnt; ++c)
+      for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % NST], (c / NST) & 1u); ++spin) {}
+    for (uint32_t c = item_n > static_cast<uint32_t>(NQ) ? item_n - NQ : 0u; c <= item_n; ++c)
+      for (int spin = 0; spin < 4096 && !mbar_try_wait(&q_full[c % NQ], (c / NQ) & 1u); ++spin) {}
+  }
 }
 
 // byte offset of (key, 16-byte chunk of its row) in a stage: boxes of 2^br rows x all slabs, 128-byte swizzled
@@ -84,8 +183,8 @@ __device__ __forceinline__ uint32_t stage_offset(int key, int chunk, int br) {
 }
 
 template <int D, int MT>
-__device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArgs& a, const RowsItem& w, uint8_t* smem, uint64_t* full,
-                                          uint64_t* empty, uint32_t& cnt, const WaitCtx& wc, int br) {
+__device__ __forceinline__ bool rows_work(const PagedAttnArgs& a, const KeyItem& w, uint8_t* smem, uint64_t* full, uint64_t* empty, uint64_t* q_empty,
+                                          uint32_t& cnt, const WaitCtx& wc, int br) {
   using L = RowsSmem<D>;
   constexpr int KS = D / 16;       // 16-dimension steps of S
   constexpr int DW = D / 8;        // head dimensions a warp takes in P V
@@ -94,22 +193,13 @@ __device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArg
   float* red_m = reinterpret_cast<float*>(smem + L::RED_OFF);
   float* red_l = red_m + RT * 8;
   const uint32_t q_base = smem_u32(smem + L::Q_OFF), p_base = smem_u32(smem + L::P_OFF);
+  const int t0 = w.u0 / 2, t1 = w.u1 / 2;
 
-  // Q rows of the item, zero behind the last one
-  for (int x = threadIdx.x; x < MT * 16 * (D / 8); x += 256) {
-    const int r = x / (D / 8), c = x % (D / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < w.rows) {
-      const int rr = w.r0 + r, tok = rr / a.group, hd = w.g * a.group + rr % a.group;
-      v = *reinterpret_cast<const uint4*>(a.q + (w.q.row0 + tok) * a.q_pitch + static_cast<int64_t>(hd) * D + c * 8);
-    }
-    *reinterpret_cast<uint4*>(smem + L::Q_OFF + (c >> 3) * (RT * 128) + sw128_offset(r, c & 7)) = v;
-  }
   // this thread's rows: 16 m + lane / 4 and 8 more; the slots each sees
   int lo_r[MT][2], hi_r[MT][2];
   int lo_max = 0, hi_min = 0x7fffffff;
   {
-    const int base = w.q.len - w.q.nq;
+    const int base = w.base;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -134,9 +224,8 @@ __device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArg
     m_run[m][0] = m_run[m][1] = -INFINITY;
     l_run[m][0] = l_run[m][1] = 0.f;
   }
-  named_bar_sync(1, 256);
 
-  for (int t = w.t0; t < w.t1; ++t, cnt += 4) {
+  for (int t = t0; t < t1; ++t, cnt += 4) {
     // ---- S of this warp's 16 keys
     const int hf = warp >> 2, key0 = (warp & 3) * 16;  // stage of the tile, first key within it
     bool ok = true;
@@ -161,7 +250,7 @@ __device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArg
         for (int m = 0; m < MT; ++m) {
           uint32_t qf[4];
           const int chunk = ks * 2 + (lane >> 4);
-          const uint32_t qa = q_base + (chunk >> 3) * (RT * 128) + sw128_offset(m * 16 + (lane & 15), chunk & 7);
+          const uint32_t qa = q_base + (m * 16 + (lane & 15)) * L::Q_PITCH + chunk * 16;
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(qf[0]), "=r"(qf[1]), "=r"(qf[2]), "=r"(qf[3]) : "r"(qa));
           mma_bf16(sc[m][0], qf, kf[0], kf[1]);
           mma_bf16(sc[m][1], qf, kf[2], kf[3]);
@@ -172,6 +261,7 @@ __device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArg
     if (lane == 0) {  // this warp has read its keys of the two K stages (it used one of them)
       mbar_arrive(&empty[cnt % L::NST]);
       mbar_arrive(&empty[(cnt + 1) % L::NST]);
+      if (t == t1 - 1) mbar_arrive(q_empty);  // and q for the last time
     }
     // ---- mask, row maxima
     const int j0 = t * PG_TILE + hf * 64 + key0 + quad * 2;
@@ -292,6 +382,7 @@ __device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArg
     }
     if (!ok) *wc.abort_flag = 1;  // the next barrier with a vote ends the CTA's warps together
   }
+  if (t1 <= t0 && lane == 0) mbar_arrive(q_empty);
   // ---- row sums over the warps' keys, then the rows out
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -312,15 +403,15 @@ __device__ __forceinline__ bool rows_work(const PagedSeqs& s, const PagedAttnArg
       const float4 u = *reinterpret_cast<const float4*>(red_l + r * 8), v = *reinterpret_cast<const float4*>(red_l + r * 8 + 4);
       const float l = ((u.x + u.y) + (u.z + u.w)) + ((v.x + v.y) + (v.z + v.w));
       const int rr = w.r0 + r, tok = rr / a.group, hd = w.g * a.group + rr % a.group;
-      if (w.c.splits == 1) {
+      if (w.splits == 1) {
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row that sees nothing: 0; a NaN sum stays NaN
-        __nv_bfloat16* dst = a.out + (w.q.row0 + tok) * a.out_pitch + static_cast<int64_t>(hd) * D + warp * DW + quad * 2;
+        __nv_bfloat16* dst = a.out + (w.row0 + tok) * a.out_pitch + static_cast<int64_t>(hd) * D + warp * DW + quad * 2;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           *reinterpret_cast<uint32_t*>(dst + nt * 8) = pack_bf16x2(o[m][nt][2 * x] * inv, o[m][nt][2 * x + 1] * inv);
-        if (a.lse && warp == 0 && quad == 0) a.lse[static_cast<int64_t>(w.q.row0 + tok) * a.H + hd] = m_run[m][x] + log2f(l);
+        if (a.lse && warp == 0 && quad == 0) a.lse[static_cast<int64_t>(w.row0 + tok) * a.H + hd] = m_run[m][x] + log2f(l);
       } else {
-        const int64_t at = w.b * a.seq_parts + (static_cast<int64_t>(w.split) * a.h + w.g) * (w.q.nq * a.group) + rr;
+        const int64_t at = w.b * a.seq_parts + (static_cast<int64_t>(w.split) * a.h + w.g) * (w.nq * a.group) + rr;
         float* dst = a.part_o + at * D + warp * DW + quad * 2;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(o[m][nt][2 * x], o[m][nt][2 * x + 1]);
@@ -340,78 +431,43 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* empty = full + L::NST;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + L::NST);
+  uint64_t* q_full = empty + L::NST;
+  uint64_t* q_empty = q_full + 1;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(q_empty + 1);
   const WaitCtx wc{abort_flag, status};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 8);
     }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 8);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  paged_item_prefix(s.B, pre, ROWS_THREADS, [&](int b) { return rows_items(s, a, b, status); });
+  paged_item_prefix(s.B, pre, ROWS_THREADS, [&](int b) { return key_items<false>(s, a, b, status); });
   const int total = pre[s.B];
   const int br = s.page_log2 < 6 ? s.page_log2 : 6;  // log2 of a box's rows
+  KeyItem* items = reinterpret_cast<KeyItem*>(smem + L::ITEM_OFF);
 
   if (warp == 8) {
-    if (lane == 0) {
-      uint32_t cnt = 0;
-      bool ok = true;
-      for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
-        const RowsItem w = rows_item(s, a, pre, it, status);
-        const int32_t* pages = s.table + w.b * s.table_pitch;
-        for (int t = w.t0; t < w.t1 && ok; ++t)
-          for (int part = 0; part < 4; ++part, ++cnt) {
-            const uint32_t st = cnt % L::NST;
-            if (!mbar_wait(wc, &empty[st], ((cnt / L::NST) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-            const int j_first = t * PG_TILE + (part & 1) * 64;
-            const int box_rows = 1 << br;
-            // boxes that hold a slot some row sees; the others stay as they are (masked for K, cleared for V)
-            int bytes = 0;
-            uint32_t got = 0;
-            int pg[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int j = j_first + x * box_rows;
-              pg[x] = -1;
-              if (x * box_rows < 64 && j < w.hi && j + box_rows > w.lo) {
-                pg[x] = pages[j >> s.page_log2];
-                if (pg[x] < 0 || pg[x] >= s.n_pages) {
-                  atomicCAS(status, 0, ST_BAD_INDEX);
-                  pg[x] = -1;
-                } else {
-                  got |= 1u << x;
-                  bytes += box_rows * D * 2;
-                }
-              }
-            }
-            mbar_expect_tx(&full[st], bytes);
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (got & (1u << x))
-                tma_load_5d(smem + st * L::STAGE + x * box_rows * D * 2, part < 2 ? &tmK : &tmV, 0, (j_first + x * box_rows) & ((1 << s.page_log2) - 1), 0,
-                            w.g, pg[x], &full[st]);
-          }
-      }
-      if (*abort_flag)  // bounded wait for copies that may still be in flight
-        for (uint32_t c = cnt > static_cast<uint32_t>(L::NST) ? cnt - L::NST : 0; c < cnt; ++c)
-          for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % L::NST], (c / L::NST) & 1u); ++spin) {}
-    }
+    produce_keys<D, false, L::NST, L::STAGE, L::Q_PITCH, L::Q_SLOT, 1>(s, a, &tmK, &tmV, pre, total, smem, smem + L::Q_OFF, items, items + 1, full, empty,
+                                                                       q_full, q_empty, wc, status);
   } else {
-    uint32_t cnt = 0;
-    for (int it = blockIdx.x; it < total; it += gridDim.x) {
-      const RowsItem w = rows_item(s, a, pre, it, status);
+    uint32_t cnt = 0, item_n = 0;
+    for (int it = blockIdx.x; it < total; it += gridDim.x, ++item_n) {
+      if (!bar_red_and(1, 256, mbar_wait(wc, q_full, item_n & 1u, ST_TIMEOUT_FULL))) break;  // (also: the last item's sums have been read)
+      const KeyItem w = items[0];
       bool ok;
       switch ((w.rows + 15) >> 4) {
-        case 1: ok = rows_work<D, 1>(s, a, w, smem, full, empty, cnt, wc, br); break;
-        case 2: ok = rows_work<D, 2>(s, a, w, smem, full, empty, cnt, wc, br); break;
-        case 3: ok = rows_work<D, 3>(s, a, w, smem, full, empty, cnt, wc, br); break;
-        default: ok = rows_work<D, 4>(s, a, w, smem, full, empty, cnt, wc, br); break;
+        case 1: ok = rows_work<D, 1>(a, w, smem, full, empty, q_empty, cnt, wc, br); break;
+        case 2: ok = rows_work<D, 2>(a, w, smem, full, empty, q_empty, cnt, wc, br); break;
+        case 3: ok = rows_work<D, 3>(a, w, smem, full, empty, q_empty, cnt, wc, br); break;
+        default: ok = rows_work<D, 4>(a, w, smem, full, empty, q_empty, cnt, wc, br); break;
       }
       if (!ok) break;
     }
@@ -435,21 +491,13 @@ struct StepSmem {
   static constexpr int MERGE_OFF = Q_OFF + 2 * Q_SLOT;
   static constexpr int ML_OFF = MERGE_OFF + SW * MR * D * 4;  // [SW][16] maxima, [SW][16] sums, [16] joined maxima, [16] joined sums
   static constexpr int ITEM_OFF = ML_OFF + (2 * SW + 2) * STEP_ROWS * 4;
-  static constexpr int PRE_OFF = ITEM_OFF + 2 * 64;
+  static constexpr int PRE_OFF = ITEM_OFF + (2 + PLAN) * 64;
   static constexpr int BAR_OFF = PRE_OFF + (PG_MAX_SEQS + 2) * 4;
   static constexpr int TOTAL = BAR_OFF + (2 * NST + 4) * 8 + 16 + 1024;
 };
 static_assert(StepSmem<256>::TOTAL <= 232448 && StepSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
 static_assert(StepSmem<256>::BAR_OFF % 8 == 0 && StepSmem<128>::BAR_OFF % 8 == 0 && StepSmem<256>::MERGE_OFF % 16 == 0 &&
                   StepSmem<128>::MERGE_OFF % 16 == 0 && StepSmem<256>::ITEM_OFF % 16 == 0 && StepSmem<128>::ITEM_OFF % 16 == 0, "alignment");
-
-// what the consumers need of an item; the producer writes it beside the rows of q
-struct StepItem {
-  int b, g, split, splits;
-  int row0, nq, base;  // first row of q, rows of the sequence, slot of the first
-  int lo, hi;          // slots that some row sees
-  int u0, u1;          // 64-key units
-};
 
 __device__ __forceinline__ void movmatrix_t(uint32_t& d, uint32_t s) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(s));
@@ -460,11 +508,6 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-
 // NT: 8-row tiles of q. A row's arithmetic is the same for either.
 template <int D, int NT>
 __global__ void __launch_bounds__(STEP_THREADS, 1)
@@ -497,78 +540,14 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  paged_item_prefix(s.B, pre, STEP_THREADS, [&](int b) {
-    const PagedSeq q = paged_seq(s, b, status);
-    return step_class(q, a.group) ? a.h * step_cut(q, a).splits : 0;
-  });
+  paged_item_prefix(s.B, pre, STEP_THREADS, [&](int b) { return key_items<true>(s, a, b, status); });
   const int total = pre[s.B];
   const int br = s.page_log2 < 6 ? s.page_log2 : 6;  // log2 of a box's rows
+  KeyItem* items = reinterpret_cast<KeyItem*>(smem + L::ITEM_OFF);
 
   if (warp == SW) {
-    if (lane == 0) {
-      uint32_t cnt = 0, item_n = 0;
-      bool ok = true;
-      const int box_rows = 1 << br;
-      for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++item_n) {
-        const int b = paged_find(pre, s.B, it);
-        const PagedSeq q = paged_seq(s, b, status);
-        const PagedCut c = step_cut(q, a);
-        const int x = it - pre[b];
-        StepItem w;
-        w.b = b, w.g = x % a.h, w.split = x / a.h, w.splits = c.splits;
-        w.row0 = q.row0, w.nq = q.nq, w.base = q.len - q.nq;
-        w.lo = a.window > 0 && w.base - a.window + 1 > 0 ? w.base - a.window + 1 : 0;
-        w.hi = q.len;
-        const int s0 = 2 * (c.t_lo + w.split * c.tiles_per_split), s1 = s0 + 2 * c.tiles_per_split;
-        const int e0 = w.lo / 64, e1 = (w.hi + 63) / 64;
-        w.u0 = s0 > e0 ? s0 : e0;
-        w.u1 = s1 < e1 ? s1 : e1;
-        const uint32_t qs = item_n & 1u;
-        if (!mbar_wait(wc, &q_empty[qs], ((item_n >> 1) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-        *reinterpret_cast<StepItem*>(smem + L::ITEM_OFF + qs * 64) = w;
-        const int rows = q.nq * a.group;
-        mbar_expect_tx(&q_full[qs], rows * D * 2);  // (an arrival: releases the item's numbers to the consumers as well)
-        for (int r = 0; r < rows; ++r)
-          bulk_load(smem + L::Q_OFF + qs * L::Q_SLOT + r * L::Q_PITCH,
-                    a.q + (q.row0 + r / a.group) * a.q_pitch + static_cast<int64_t>(w.g * a.group + r % a.group) * D, D * 2, &q_full[qs]);
-        const int32_t* pages = s.table + b * s.table_pitch;
-        for (int u = w.u0; u < w.u1 && ok; ++u) {
-          // boxes that hold a slot some row sees; the others stay as they are (masked for K, cleared for V)
-          int bytes = 0, pg[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int j = u * 64 + y * box_rows;
-            pg[y] = -1;
-            if (y * box_rows < 64 && j < w.hi && j + box_rows > w.lo) {
-              pg[y] = pages[j >> s.page_log2];
-              if (pg[y] < 0 || pg[y] >= s.n_pages) {
-                atomicCAS(status, 0, ST_BAD_INDEX);
-                pg[y] = -1;
-              } else {
-                bytes += box_rows * D * 2;
-              }
-            }
-          }
-#pragma unroll
-          for (int part = 0; part < 2; ++part, ++cnt) {
-            const uint32_t st = cnt % L::NST;
-            if (!mbar_wait(wc, &empty[st], ((cnt / L::NST) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-            mbar_expect_tx(&full[st], bytes);
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (pg[y] >= 0)
-                tma_load_5d(smem + st * L::STAGE + y * box_rows * D * 2, part ? &tmV : &tmK, 0, (u * 64 + y * box_rows) & ((1 << s.page_log2) - 1), 0, w.g,
-                            pg[y], &full[st]);
-          }
-        }
-      }
-      if (*abort_flag) {  // bounded wait for copies that may still be in flight
-        for (uint32_t c = cnt > static_cast<uint32_t>(L::NST) ? cnt - L::NST : 0; c < cnt; ++c)
-          for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % L::NST], (c / L::NST) & 1u); ++spin) {}
-        for (uint32_t c = item_n > 2u ? item_n - 2u : 0u; c <= item_n; ++c)
-          for (int spin = 0; spin < 4096 && !mbar_try_wait(&q_full[c & 1u], (c >> 1) & 1u); ++spin) {}
-      }
-    }
+    produce_keys<D, true, L::NST, L::STAGE, L::Q_PITCH, L::Q_SLOT, 2>(s, a, &tmK, &tmV, pre, total, smem, smem + L::Q_OFF, items, items + 2, full, empty,
+                                                                      q_full, q_empty, wc, status);
   } else {
     float* m_w = reinterpret_cast<float*>(smem + L::ML_OFF);  // [SW][16]
     float* l_w = m_w + SW * STEP_ROWS;
@@ -582,8 +561,8 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const uint32_t qs = item_n & 1u;
       bool ok = mbar_wait(wc, &q_full[qs], (item_n >> 1) & 1u, ST_TIMEOUT_FULL);
       ok = __all_sync(0xffffffffu, ok);
-      const StepItem w = *reinterpret_cast<const StepItem*>(smem + L::ITEM_OFF + qs * 64);
-      const int rows = w.nq * a.group;
+      const KeyItem w = items[qs];
+      const int rows = w.rows;
       uint32_t qf[NT][KS][2];  // q as the B operand: rows 8 n + lane / 4, dimensions 16 ks + 2 (lane % 4) and 8 more
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -797,49 +776,83 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __syncthreads();
 }
 
-// one warp per (row, head) whose sequence was split
+// Joins the splits of a (row, head). With few splits a warp takes one; with many the CTA does, its threads in groups of D / 4 that
+// share the splits out (a decoding step has few rows and many splits: read one after the other they would be a chain of latencies).
 template <int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+__global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+  constexpr int V = D / 128;       // float4 per lane of a warp
+  constexpr int G = 256 / (D / 4);  // groups of the CTA
+  __shared__ float4 part[G][D / 4];
+  __shared__ float part_l[G];
   pdl_trigger();
   pdl_wait();
-  constexpr int V = D / 128;  // float4 per lane
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSeq q = paged_seq(s, b, status);
   if (q.nq == 0 || chunk_class(q, a)) return;
   const PagedCut c = attn_cut(q, a);
   if (c.splits == 1) return;
-  const int all = q.nq * a.group;
-  for (int64_t x = blockIdx.x * 8 + warp; x < static_cast<int64_t>(q.nq) * a.H; x += gridDim.x * 8) {
-    const int tok = static_cast<int>(x / a.H), hd = static_cast<int>(x % a.H), g = hd / a.group, rr = tok * a.group + hd % a.group;
-    const int64_t at = b * a.seq_parts + static_cast<int64_t>(g) * all + rr, step = static_cast<int64_t>(a.h) * all;
+  const int all = q.nq * a.group, rows = q.nq * a.H;
+  const int64_t step = static_cast<int64_t>(a.h) * all;
+  const bool few = c.splits <= 4;
+  for (int x = few ? blockIdx.x * 8 + warp : blockIdx.x; x < rows; x += few ? gridDim.x * 8 : gridDim.x) {
+    const int tok = x / a.H, hd = x % a.H;
+    const int64_t at = b * a.seq_parts + static_cast<int64_t>(hd / a.group) * all + tok * a.group + hd % a.group;
     float m = -INFINITY;
     for (int i = lane; i < c.splits; i += 32) m = fmaxf(m, a.part_ml[at + i * step].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f;
-    float4 acc[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
     const float neg_m = m == -INFINITY ? 0.f : -m;
-#pragma unroll 4
-    for (int i = 0; i < c.splits; ++i) {
-      const float2 ml = a.part_ml[at + i * step];
-      const float f = fast_exp2(ml.x + neg_m);
-      l = fmaf(f, ml.y, l);
-      const float4* src = reinterpret_cast<const float4*>(a.part_o + (at + i * step) * D);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float4 u = src[v * 32 + lane];
-        acc[v].x = fmaf(f, u.x, acc[v].x), acc[v].y = fmaf(f, u.y, acc[v].y), acc[v].z = fmaf(f, u.z, acc[v].z), acc[v].w = fmaf(f, u.w, acc[v].w);
-      }
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     __nv_bfloat16* dst = a.out + (q.row0 + tok) * a.out_pitch + static_cast<int64_t>(hd) * D;
+    float l = 0.f;
+    if (few) {
+      float4 acc[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
-          make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv), pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
-    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd] = m + log2f(l);
+      for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < c.splits; ++i) {
+        const float2 ml = a.part_ml[at + i * step];
+        const float f = fast_exp2(ml.x + neg_m);
+        l = fmaf(f, ml.y, l);
+        const float4* src = reinterpret_cast<const float4*>(a.part_o + (at + i * step) * D);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float4 u = src[v * 32 + lane];
+          acc[v].x = fmaf(f, u.x, acc[v].x), acc[v].y = fmaf(f, u.y, acc[v].y), acc[v].z = fmaf(f, u.z, acc[v].z), acc[v].w = fmaf(f, u.w, acc[v].w);
+        }
+      }
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
+            make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv), pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
+      if (a.lse && lane == 0) a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd] = m + log2f(l);
+    } else {
+      const int grp = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int i = grp; i < c.splits; i += G) {
+        const float2 ml = a.part_ml[at + i * step];
+        const float f = fast_exp2(ml.x + neg_m);
+        l = fmaf(f, ml.y, l);
+        const float4 u = reinterpret_cast<const float4*>(a.part_o + (at + i * step) * D)[d];
+        acc.x = fmaf(f, u.x, acc.x), acc.y = fmaf(f, u.y, acc.y), acc.z = fmaf(f, u.z, acc.z), acc.w = fmaf(f, u.w, acc.w);
+      }
+      part[grp][d] = acc;
+      if (d == 0) part_l[grp] = l;
+      __syncthreads();
+      if (grp == 0) {
+        l = part_l[0];
+#pragma unroll
+        for (int y = 1; y < G; ++y) {
+          const float4 u = part[y][d];
+          acc.x += u.x, acc.y += u.y, acc.z += u.z, acc.w += u.w;
+          l += part_l[y];
+        }
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        *reinterpret_cast<uint2*>(dst + d * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        if (a.lse && d == 0) a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd] = m + log2f(l);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -940,7 +953,7 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
     SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, 1, tmK, tmV, s, a, status));
   if (max_splits > 1) {
     const int64_t most = a.chunk_rows / a.group;  // tokens of a sequence that is not the chunk kernel's
-    int64_t gx = ((max_q < most ? max_q : most) * a.H + 7) / 8;
+    int64_t gx = (max_q < most ? max_q : most) * a.H;
     if (gx > 1024) gx = 1024;
     SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, s, a, status));
   }

@@ -44,7 +44,7 @@ __device__ __forceinline__ bool rows_class(const PagedSeq& q, const PagedAttnArg
 __device__ __forceinline__ PagedCut step_cut(const PagedSeq& q, const PagedAttnArgs& a) { return paged_cut(q, a.window, 1, a.h, PG_SMS, 1); }
 __device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
   const int rt = (q.nq * a.group + RT - 1) / RT;
-  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 1);
+  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 4);  // splits of at least 4 tiles: up to 64 rows of partial results each
 }
 __device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a.group) ? step_cut(q, a) : rows_cut(q, a); }
 
@@ -60,6 +60,7 @@ struct ChunkCut {
   int hp, tok, ntt, per_tt;  // heads and tokens of an item, token tiles, items of a token tile
   int64_t work;              // (item, key tile) pairs
   int units;
+  bool whole;                // units take whole items: those that begin in their range
 
   __device__ __forceinline__ void slots(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& lo, int& hi) const {
     const int base = q.len - q.nq, first = base + tt * tok, end = (tt + 1) * tok < q.nq ? (tt + 1) * tok : q.nq;
@@ -91,6 +92,9 @@ __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttn
   }
   const int64_t u = c.work / CHUNK_MIN_TILES;
   c.units = u < 1 ? 1 : u > CHUNK_UNITS ? CHUNK_UNITS : static_cast<int>(u);
+  // many short items (a window): a cut would cost about as much as the imbalance it removes
+  const int64_t items = static_cast<int64_t>(c.ntt) * c.per_tt;
+  c.whole = items >= 2 * CHUNK_UNITS && c.work <= 24 * items;
   return c;
 }
 

@@ -3,8 +3,8 @@
 //
 // An item is 256 query rows of one kv head: `hp` heads that share it x 256 / hp tokens, the first half of the tokens in one CTA of
 // the pair and the second in the other. The pair walks the key tiles some row sees, 128 keys at a time:
-//   warp 0     one lane: TMA loads of Q and of this CTA's 64 keys of K
-//   warp 10    one lane: TMA loads of this CTA's half of V's dimensions (all 128 keys)
+//   warp 0     TMA loads of this CTA's 64 keys of K
+//   warp 10    TMA loads of Q and of this CTA's half of V's dimensions (all 128 keys)
 //   warp 11    in a tile with slots that no row of the item sees (a page's end, the front of a window) it waits for the copy of V and
 //              clears those rows, while warp 10 goes on: P is 0 there, but 0 * inf is not
 //   warp 1     owns tensor memory; the leader's lane issues S = Q K^T (M = 256) into one of two buffers and O += P V with P read from
@@ -34,7 +34,8 @@ struct ChunkSmem {
   static constexpr int Q_BYTES = SLABS * 128 * 128;
   static constexpr int KV = SLABS * CH_KH * 128;  // one stage: 64 keys of K, or 128 keys of half of V's dimensions
   static constexpr int NS = D == 256 ? 2 : 4;
-  static constexpr int K_OFF = Q_BYTES;
+  static constexpr int NQ = D == 256 ? 1 : 2;  // q of this segment and, where there is room, of the next
+  static constexpr int K_OFF = NQ * Q_BYTES;
   static constexpr int V_OFF = K_OFF + NS * KV;
   static constexpr int BAR_OFF = V_OFF + NS * KV;
   static constexpr int XCHG_OFF = BAR_OFF + 512;
@@ -85,6 +86,10 @@ struct ChunkWalk {
     first = true;
     tt = -1, w_tt = 0, nt = 0;
     advance(a);
+    if (c.whole) {
+      const int off = static_cast<int>((w - w_tt) % nt);
+      if (off) w += nt - off;
+    }
   }
   // to the token tile that holds pair w
   __device__ __forceinline__ void advance(const PagedAttnArgs& a) {
@@ -101,7 +106,7 @@ struct ChunkWalk {
     const int64_t in = w - w_tt;
     const int item = static_cast<int>(in / nt), off = static_cast<int>(in - static_cast<int64_t>(item) * nt);
     const int64_t left = w_end - w;
-    const int len = left < nt - off ? static_cast<int>(left) : nt - off;
+    const int len = !c.whole && left < nt - off ? static_cast<int>(left) : nt - off;
     const int sets = a.group / c.hp;
     g.g = item / sets;
     g.h0 = g.g * a.group + (item % sets) * c.hp;
@@ -116,12 +121,36 @@ struct ChunkWalk {
   }
 };
 
+// The pages of a segment's boxes in the order they are copied, 32 fetched at a time by the lanes of the producer warp and the next 32
+// ahead of use: the copy loop never waits for a table entry.
+struct PageRun {
+  int cur, nxt, x;       // box
+  int j0, nb_log2, rl;   // first slot of box 0; boxes per tile, rows of a box (log2)
+  __device__ __forceinline__ int fetch(const PagedSeqs& s, const int32_t* pages, const ChunkSeg& g, int box, int* status) const {
+    const int t = g.ta + (box >> nb_log2);
+    if (t >= g.tb) return s.n_pages;
+    return chunk_page(s, pages, t * PG_TILE + j0 + ((box & ((1 << nb_log2) - 1)) << rl), 1 << rl, g.lo, g.hi, status);
+  }
+  __device__ __forceinline__ void start(const PagedSeqs& s, const int32_t* pages, const ChunkSeg& g, int first, int boxes_log2, int rows_log2, int lane, int* status) {
+    x = 0, j0 = first, nb_log2 = boxes_log2, rl = rows_log2;
+    cur = fetch(s, pages, g, lane, status);
+    nxt = fetch(s, pages, g, 32 + lane, status);
+  }
+  __device__ __forceinline__ int get(const PagedSeqs& s, const int32_t* pages, const ChunkSeg& g, int lane, int* status) {
+    if (x && (x & 31) == 0) {
+      cur = nxt;
+      nxt = fetch(s, pages, g, x + 32 + lane, status);
+    }
+    return __shfl_sync(0xffffffffu, cur, x++ & 31);
+  }
+};
+
 template <int D>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
   using L = ChunkSmem<D>;
-  constexpr int SLABS = L::SLABS, NS = L::NS, V_SLABS = SLABS / 2;
+  constexpr int SLABS = L::SLABS, NS = L::NS, NQ = L::NQ, V_SLABS = SLABS / 2;
   constexpr uint32_t IDESC_S = make_idesc(FMT_BF16, FMT_BF16, 256, 128, 0, 0);
   constexpr uint32_t IDESC_O = make_idesc(FMT_BF16, FMT_BF16, 256, D, 0, 1);  // B = V, MN-major (head dimensions contiguous)
 
@@ -129,8 +158,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;
+  uint64_t* q_empty = bars + NQ;
+  uint64_t* k_full = bars + 2 * NQ;
   uint64_t* k_empty = k_full + NS;
   uint64_t* v_full = k_empty + NS;
   uint64_t* v_empty = v_full + NS;
@@ -151,8 +180,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   pdl_trigger();
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    for (int i = 0; i < NQ; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -193,32 +224,28 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   const int in_page = (1 << s.page_log2) - 1;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const int rows = s.page_log2 < 6 ? 1 << s.page_log2 : CH_KH;  // rows of a K box
-      uint32_t cnt = 0, seg_n = 0;
-      bool ok = true;
-      for (int it = pair; it < total && ok; it += n_pairs) {
-        ChunkWalk wk;
-        wk.start(s, a, pre, it, status);
-        const int32_t* pages = s.table + wk.b * s.table_pitch;
-        const int hp = wk.c.hp, qrows = 128 / hp;
-        ChunkSeg g;
-        while (ok && wk.next(a, g)) {
-          if (!mbar_wait(wc, q_empty, (seg_n & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(q_full, 2 * L::Q_BYTES);
-          const int row = wk.q.row0 + g.tok0 + static_cast<int>(rank) * qrows;
-          for (int hh = 0; hh < hp; ++hh)
-            for (int x = 0; x < SLABS; ++x)
-              tma_load_2d_pair(smem + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, row, map_to_cta(q_full, 0));
-          ++seg_n;
-          for (int t = g.ta; t < g.tb; ++t, ++cnt) {
-            const uint32_t st = cnt % NS;
-            if (!mbar_wait(wc, &k_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-            if (rank == 0) mbar_expect_tx(&k_full[st], 2 * L::KV);
-            const uint32_t bar = map_to_cta(&k_full[st], 0);
-            const int j0 = t * PG_TILE + static_cast<int>(rank) * CH_KH;
-            for (int x = 0; x < CH_KH / rows; ++x) {
-              const int pg = chunk_page(s, pages, j0 + x * rows, rows, g.lo, g.hi, status);
+    const int rl = s.page_log2 < 6 ? s.page_log2 : 6, rows = 1 << rl;  // rows of a K box
+    uint32_t cnt = 0;
+    bool ok = true;
+    for (int it = pair; it < total && ok; it += n_pairs) {
+      ChunkWalk wk;
+      wk.start(s, a, pre, it, status);
+      const int32_t* pages = s.table + wk.b * s.table_pitch;
+      ChunkSeg g;
+      while (ok && wk.next(a, g)) {
+        PageRun run;
+        run.start(s, pages, g, static_cast<int>(rank) * CH_KH, 6 - rl, rl, lane, status);
+        for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
+          const uint32_t st = cnt % NS;
+          if (lane == 0) {
+            ok = mbar_wait(wc, &k_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+            if (ok && rank == 0) mbar_expect_tx(&k_full[st], 2 * L::KV);
+          }
+          const int j0 = t * PG_TILE + static_cast<int>(rank) * CH_KH;
+          for (int x = 0; x < CH_KH >> rl; ++x) {
+            const int pg = run.get(s, pages, g, lane, status);
+            if (lane == 0 && ok) {
+              const uint32_t bar = map_to_cta(&k_full[st], 0);
               const int at = (j0 + x * rows) & in_page;
               uint8_t* dst = smem + L::K_OFF + st * L::KV + x * rows * 128;
               if (rows == CH_KH)
@@ -227,44 +254,67 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 for (int y = 0; y < SLABS; ++y) tma_load_5d_pair(dst + y * CH_KH * 128, &tmK, 0, at, y, g.g, pg, bar);
             }
           }
+          ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
         }
       }
     }
   } else if (warp == 10) {
-    if (lane == 0) {
-      const int rows = s.page_log2 < 7 ? 1 << s.page_log2 : PG_TILE;  // rows of a V box
-      uint32_t cnt = 0;
-      bool ok = true;
-      for (int it = pair; it < total && ok; it += n_pairs) {
-        ChunkWalk wk;
-        wk.start(s, a, pre, it, status);
-        const int32_t* pages = s.table + wk.b * s.table_pitch;
-        ChunkSeg g;
-        while (ok && wk.next(a, g)) {
-          for (int t = g.ta; t < g.tb; ++t, ++cnt) {
-            const uint32_t st = cnt % NS;
-            const bool edge = t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi;
-            if (!mbar_wait(wc, &v_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-            if (edge)
-              mbar_expect_tx(&v_edge[st], L::KV);
-            else if (rank == 0)
-              mbar_expect_tx(&v_full[st], 2 * L::KV);
-            else
-              mbar_arrive_cluster(map_to_cta(&v_full[st], 0));
-            const uint32_t bar = map_to_cta(&v_full[st], 0);
-            for (int x = 0; x < PG_TILE / rows; ++x) {
-              const int j = t * PG_TILE + x * rows;
-              const int pg = chunk_page(s, pages, j, rows, g.lo, g.hi, status);
+    const int rl = s.page_log2 < 7 ? s.page_log2 : 7, rows = 1 << rl;  // rows of a V box
+    uint32_t cnt = 0, seg_n = 0;
+    bool ok = true;
+    for (int it = pair; it < total && ok; it += n_pairs) {
+      ChunkWalk wk;
+      wk.start(s, a, pre, it, status);
+      const int32_t* pages = s.table + wk.b * s.table_pitch;
+      const int hp = wk.c.hp, qrows = 128 / hp;
+      ChunkSeg g;
+      while (ok && wk.next(a, g)) {
+        PageRun run;
+        run.start(s, pages, g, 0, 7 - rl, rl, lane, status);
+        // Q comes with this warp, not with K's: the next segment's K is then not held back until the last product has read Q
+        const uint32_t qs = seg_n % NQ;
+        if (lane == 0) {
+          ok = mbar_wait(wc, &q_empty[qs], ((seg_n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+          if (ok) {
+            if (rank == 0) mbar_expect_tx(&q_full[qs], 2 * L::Q_BYTES);
+            const int row = wk.q.row0 + g.tok0 + static_cast<int>(rank) * qrows;
+            for (int hh = 0; hh < hp; ++hh)
+              for (int x = 0; x < SLABS; ++x)
+                tma_load_2d_pair(smem + qs * L::Q_BYTES + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, row, map_to_cta(&q_full[qs], 0));
+          }
+        }
+        ++seg_n;
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+        for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
+          const uint32_t st = cnt % NS;
+          const bool edge = t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi;
+          if (lane == 0) {
+            ok = mbar_wait(wc, &v_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+            if (ok) {
+              if (edge)
+                mbar_expect_tx(&v_edge[st], L::KV);
+              else if (rank == 0)
+                mbar_expect_tx(&v_full[st], 2 * L::KV);
+              else
+                mbar_arrive_cluster(map_to_cta(&v_full[st], 0));
+            }
+          }
+          for (int x = 0; x < PG_TILE >> rl; ++x) {
+            const int pg = run.get(s, pages, g, lane, status);
+            if (lane == 0 && ok) {
+              const uint32_t bar = map_to_cta(&v_full[st], 0);
+              const int at = (t * PG_TILE + x * rows) & in_page;
               uint8_t* dst = smem + L::V_OFF + st * L::KV + x * rows * 128;
               for (int y = 0; y < (rows == PG_TILE ? 1 : V_SLABS); ++y) {
                 const int slab = static_cast<int>(rank) * V_SLABS + y;
                 if (edge)
-                  tma_load_5d(dst + y * PG_TILE * 128, &tmV, 0, j & in_page, slab, g.g, pg, &v_edge[st]);
+                  tma_load_5d(dst + y * PG_TILE * 128, &tmV, 0, at, slab, g.g, pg, &v_edge[st]);
                 else
-                  tma_load_5d_pair(dst + y * PG_TILE * 128, &tmV, 0, j & in_page, slab, g.g, pg, bar);
+                  tma_load_5d_pair(dst + y * PG_TILE * 128, &tmV, 0, at, slab, g.g, pg, bar);
               }
             }
           }
+          ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
         }
       }
     }
@@ -300,8 +350,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      const uint32_t q_addr = smem_u32(smem);
-      uint32_t kc = 0, vc = 0, gt = 0, seg_n = 0;
+      uint32_t q_addr = 0, kc = 0, vc = 0, gt = 0, seg_n = 0;
       bool ok = true;
       auto issue_s = [&](uint32_t g) -> bool {  // S of tile g into buffer g & 1
         const uint32_t st = kc % NS;
@@ -327,7 +376,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         ChunkSeg g;
         while (ok && wk.next(a, g)) {
           const int n_tiles = g.tb - g.ta;
-          if (!mbar_wait(wc, q_full, seg_n & 1u, ST_TIMEOUT_FULL)) { ok = false; break; }
+          const uint32_t qs = seg_n % NQ;
+          if (!mbar_wait(wc, &q_full[qs], (seg_n / NQ) & 1u, ST_TIMEOUT_FULL)) { ok = false; break; }
+          q_addr = smem_u32(smem) + qs * L::Q_BYTES;
           tc_fence_after();
           if (!issue_s(gt)) { ok = false; break; }
           for (int i = 0; i < n_tiles; ++i) {
@@ -335,7 +386,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (i + 1 < n_tiles) {
               if (!issue_s(gi + 1)) { ok = false; break; }  // buffer (gi + 1) & 1 last held P of tile gi - 1, whose P V was issued before
             } else {
-              umma_commit_pair_both(q_empty);
+              umma_commit_pair_both(&q_empty[qs]);
             }
             if (!mbar_wait(wc, p_ready, gi & 1u, ST_TIMEOUT_OTHER)) { ok = false; break; }
             if (i == 0 && seg_n > 0 && !mbar_wait(wc, o_free, (seg_n - 1) & 1u, ST_TIMEOUT_OTHER)) { ok = false; break; }
@@ -515,50 +566,54 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 }
 
 // ---------------------------------------------------------------- join of the cut items
-// one warp per (row, head); the pieces of its item are added in the order of the units
+// CTAs (it, y): the item that unit `it` begins inside of, if this is the first unit that does; 64 of its 256 rows, a warp per row, the
+// pieces added in the order of the units
 template <int D>
 __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
   pdl_trigger();
   pdl_wait();
   constexpr int V = D / 128;  // float4 per lane
-  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int it = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (it >= a.unit_pre[s.B] || it >= a.max_units) return;
+  const int b = paged_find(a.unit_pre, s.B, it);
+  const int u = it - a.unit_pre[b];
+  if (u == 0) return;
   const PagedSeq q = paged_seq(s, b, status);
-  if (!chunk_class(q, a)) return;
   const ChunkCut c = chunk_cut(q, a);
-  if (c.units == 1 || a.unit_pre[b + 1] > a.max_units) return;
-  // a CTA takes 8 rows (token, head) at a time, all of one token tile and one head where there are many tokens
+  if (c.whole) return;
+  const int64_t w = c.begin(u);
   int64_t w_tt = 0;
-  int tt = 0, t0 = 0, nt = 0;
+  int tt = 0, t0, nt;
   c.tiles(q, a, 0, t0, nt);
-  const int64_t all = static_cast<int64_t>(q.nq) * a.H;
-  for (int64_t x = blockIdx.x * 8 + warp; x < all; x += gridDim.x * 8) {
-    const int tok = static_cast<int>(x / a.H), head = static_cast<int>(x % a.H);
-    while (tt < tok / c.tok) {
-      w_tt += static_cast<int64_t>(nt) * c.per_tt;
-      ++tt;
-      c.tiles(q, a, tt, t0, nt);
-    }
-    const int g = head / a.group, hh = head % a.group, sets = a.group / c.hp;
-    const int64_t w0 = w_tt + static_cast<int64_t>(g * sets + hh / c.hp) * nt;
-    const int u0 = c.unit_of(w0), u1 = c.unit_of(w0 + nt - 1);
-    if (u0 == u1) continue;  // whole in one unit: already written
-    const int in_tile = tok - tt * c.tok, qrows = 128 / c.hp;
-    const int row = (in_tile / qrows) * 128 + (hh % c.hp) * qrows + in_tile % qrows;
-    float m = -INFINITY, l = 0.f;
-    auto slot = [&](int u) {  // the piece is the unit's first segment unless the item starts inside the unit
-      return ((a.unit_pre[b] + static_cast<int64_t>(u)) * 2 + (c.begin(u) < w0 ? 1 : 0)) * 256 + row;
-    };
-    for (int u = u0; u <= u1; ++u) m = fmaxf(m, a.chunk_ml[slot(u)].x);
+  while (w >= w_tt + static_cast<int64_t>(nt) * c.per_tt) {
+    w_tt += static_cast<int64_t>(nt) * c.per_tt;
+    c.tiles(q, a, ++tt, t0, nt);
+  }
+  const int item = static_cast<int>((w - w_tt) / nt);
+  const int64_t w0 = w_tt + static_cast<int64_t>(item) * nt;
+  if (w == w0 || c.begin(u - 1) > w0) return;  // the unit begins with an item, or an earlier one has cut it
+  const int u1 = c.unit_of(w0 + nt - 1);
+  if (it - u + u1 >= a.max_units) return;
+  const int sets = a.group / c.hp, qrows = 128 / c.hp;
+  const int h0 = item / sets * a.group + item % sets * c.hp;
+  const int64_t first = (static_cast<int64_t>(it - 1) * 2 + (c.begin(u - 1) < w0 ? 1 : 0)) * 256;  // the piece at the end of the unit before, or all of it
+  for (int r = blockIdx.y * 64 + warp; r < blockIdx.y * 64 + 64; r += 8) {
+    const int in = r & 127, tok = tt * c.tok + (r >> 7) * qrows + in % qrows, head = h0 + in / qrows;
+    if (tok >= q.nq) continue;
+    const int64_t at0 = first + r, at = static_cast<int64_t>(it) * 512 + r;  // further pieces: 512 rows apart
+    float m = a.chunk_ml[at0].x;
+    for (int y = 0; y <= u1 - u; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
     const float neg_m = m == -INFINITY ? 0.f : -m;
+    float l = 0.f;
     float4 acc[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int u = u0; u <= u1; ++u) {
-      const int64_t at = slot(u);
-      const float2 ml = a.chunk_ml[at];
+    for (int y = -1; y <= u1 - u; ++y) {
+      const int64_t from = y < 0 ? at0 : at + y * 512;
+      const float2 ml = a.chunk_ml[from];
       const float f = fast_exp2(ml.x + neg_m);
       l = fmaf(f, ml.y, l);
-      const float4* src = reinterpret_cast<const float4*>(a.chunk_o + at * D);
+      const float4* src = reinterpret_cast<const float4*>(a.chunk_o + from * D);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float4 z = src[v * 32 + lane];
@@ -838,9 +893,7 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   }
   SPINF_CUDA_OK(launch_after(paged_chunk_kernel<D>, dim3(static_cast<unsigned>(sm_count() / 2 * 2)), dim3(CHUNK_THREADS), st, L::TOTAL, 2, tmQ, tmK, tmV, s, a,
                              status));
-  int64_t gx = (max_q * a.H + 7) / 8;
-  if (gx > 2048) gx = 2048;
-  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, s, a, status));
+  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, s, a, status));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
   if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;
