@@ -912,7 +912,7 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   if (max_q > most) {
     const int64_t tok = 256 / chunk_heads(static_cast<int>(group)), work = (max_q + tok - 1) / tok * (H / (256 / tok)) * (tiles > 0 ? tiles : 1);
     int64_t units = work / CHUNK_MIN_TILES;
-    units = units < 1 ? 1 : units > CHUNK_UNITS ? CHUNK_UNITS : units;
+    units = units < 1 ? 1 : units > chunk_units_of(D) ? chunk_units_of(D) : units;
     const int64_t seqs = n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
     z.max_units = static_cast<int>(seqs * units);
     z.chunk_o = up256(seqs * units * 512 * D * 4);
@@ -1015,6 +1015,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.out_pitch = out_pitch;
   a.H = H;
   a.h = Hkv;
+  a.D = D;
   a.group = H / Hkv;
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;

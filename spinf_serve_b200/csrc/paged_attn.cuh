@@ -10,7 +10,7 @@ struct PagedAttnArgs {
   int64_t q_pitch;
   __nv_bfloat16* out;
   int64_t out_pitch;
-  int H, h, group, window;
+  int H, h, D, group, window;
   float scale_log2;
   int chunk_rows;  // sequences with more query rows per kv head than this are the chunk kernel's
   // split keys, few rows: part_o [B][seq_parts][D], part_ml [B][seq_parts] (maximum in log2 units, sum)
@@ -49,7 +49,8 @@ __device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnA
 __device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a.group) ? step_cut(q, a) : rows_cut(q, a); }
 
 // ---- the chunk kernel: items of 256 rows (hp heads x 256 / hp tokens), their key tiles dealt out in equal units
-static constexpr int CHUNK_UNITS = PG_SMS / 2;  // CTA pairs
+// units of a sequence: one per CTA pair (D 256) or CTA (D 128)
+__host__ __device__ constexpr int chunk_units_of(int D) { return D == 256 ? PG_SMS / 2 : PG_SMS; }
 static constexpr int CHUNK_MIN_TILES = 8;       // least (item, tile) pairs of a unit: below that a cut costs more than it spreads
 
 // heads of an item: the largest power of two that divides the group, at most 8 (16 rows of a head in one CTA); more heads per item
@@ -91,10 +92,11 @@ __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttn
     c.work += static_cast<int64_t>(nt) * c.per_tt;
   }
   const int64_t u = c.work / CHUNK_MIN_TILES;
-  c.units = u < 1 ? 1 : u > CHUNK_UNITS ? CHUNK_UNITS : static_cast<int>(u);
+  const int most = chunk_units_of(a.D);
+  c.units = u < 1 ? 1 : u > most ? most : static_cast<int>(u);
   // many short items (a window): a cut would cost about as much as the imbalance it removes
   const int64_t items = static_cast<int64_t>(c.ntt) * c.per_tt;
-  c.whole = items >= 2 * CHUNK_UNITS && c.work <= 24 * items;
+  c.whole = items >= 2 * most && c.work <= 24 * items;
   return c;
 }
 

@@ -1,20 +1,19 @@
-// Attention of a chunk of new tokens over the paged K/V cache (sequences with more than 64 query rows per kv head), tcgen05 + TMEM +
-// TMA as CTA pairs.
+// Attention of a chunk of new tokens over the paged K/V cache (sequences with more than 128 query rows per kv head), tcgen05 + TMEM +
+// TMA.
 //
-// An item is 256 query rows of one kv head: `hp` heads that share it x 256 / hp tokens, the first half of the tokens in one CTA of
-// the pair and the second in the other. The pair walks the key tiles some row sees, 128 keys at a time:
-//   warp 0     TMA loads of this CTA's 64 keys of K
-//   warp 10    TMA loads of Q and of this CTA's half of V's dimensions (all 128 keys)
-//   warp 11    in a tile with slots that no row of the item sees (a page's end, the front of a window) it waits for the copy of V and
-//              clears those rows, while warp 10 goes on: P is 0 there, but 0 * inf is not
-//   warp 1     owns tensor memory; the leader's lane issues S = Q K^T (M = 256) into one of two buffers and O += P V with P read from
-//              tensor memory; S of tile t + 1 is issued before P V of tile t
-//   warps 2-9  two softmax groups of four warps, thread = row, group A the first 64 keys of the tile and B the others; the mask is
-//              arithmetic on slots (a row sees the slots up to its own, with a window the last ones), evaluated on boundary tiles only
-// What bounds it: the tensor pipe (4 D flops per pair of row and key). The pair is there for K and V: 128 rows alone would need a
-// tile of 128 keys from L2 every 2 048 cycles (D 256), 64 bytes per cycle and SM, more than L2 delivers; 256 rows halve that.
+// An item is 256 query rows of one kv head in two tiles of 128: `hp` heads that share it x 256 / hp tokens, the first half of the
+// tokens in one tile and the second in the other. The key tiles some row sees are walked 128 keys at a time; S = Q K^T and O += P V
+// on the tensor cores with P read from tensor memory, the softmax thread per row in fp32 with P rounded to bf16 for the product.
+//   D 256 (paged_pair_kernel): a CTA pair, one tile of rows each (O takes half of tensor memory). The pair is there for K and V: 128
+//       rows alone would need 128 keys from L2 every 2 048 cycles, 64 bytes per cycle and SM, more than L2 delivers. Two S buffers; two
+//       groups of four softmax warps, each half the keys of every row.
+//   D 128 (paged_two_kernel): one CTA holds both tiles (S and O of each fill tensor memory) and a group of four softmax warps per tile.
+//       The exponentials take as long as the products here (128 x 128 at 16 per cycle and SM: 1 024 cycles); with two independent tiles
+//       one tile's softmax runs under the other's products and waits, where the pair form leaves its chain of waits exposed (2 434
+//       cycles per 128 x 128 and SM).
+// Bound by the tensor pipe (4 D flops per row and key).
 //
-// A sequence's work, the (item, key tile) pairs in order, is dealt out in equal contiguous units, one per CTA pair of the GPU
+// A sequence's work, the (item, key tile) pairs in order, is dealt out in equal contiguous units, one per CTA pair / CTA of the GPU
 // (fewer for little work): the causal triangle, ragged tails and few items of many tiles balance by themselves. An item cut by
 // a unit's border leaves partial rows (maximum, sum, O in fp32), which the join adds in order. The cut depends on the sequence's own
 // lengths only, so its results do not depend on the rest of the call.
@@ -26,22 +25,25 @@ namespace spinf {
 
 static constexpr int CH_KH = 64;
 static constexpr float CH_RESCALE = 24.f;  // log2 units: the reference maximum moves when a row's maximum grew by more
-static constexpr int CHUNK_THREADS = 384;
+static constexpr int CHUNK_THREADS = 384;  // 12 warps (three per scheduler: 168 registers a thread)
 
 template <int D>
 struct ChunkSmem {
   static constexpr int SLABS = D / 64;
-  static constexpr int Q_BYTES = SLABS * 128 * 128;
-  static constexpr int KV = SLABS * CH_KH * 128;  // one stage: 64 keys of K, or 128 keys of half of V's dimensions
-  static constexpr int NS = D == 256 ? 2 : 4;
-  static constexpr int NQ = D == 256 ? 1 : 2;  // q of this segment and, where there is room, of the next
-  static constexpr int K_OFF = NQ * Q_BYTES;
+  static constexpr int Q_BYTES = (D == 256 ? 1 : 2) * SLABS * 128 * 128;   // the CTA's rows of q
+  static constexpr int KV = (D == 256 ? CH_KH : PG_TILE) * SLABS * 128;     // one stage: the CTA's share of a tile of K, or of V
+  static constexpr int NS = 2;
+  static constexpr int SEGS = 8, PLAN = 8;  // segment ring; units planned at a time
+  static constexpr int K_OFF = Q_BYTES;
   static constexpr int V_OFF = K_OFF + NS * KV;
-  static constexpr int BAR_OFF = V_OFF + NS * KV;
+  static constexpr int OUT_OFF = V_OFF + NS * KV;   // 2 KB per softmax warp: rows of the output on their way to global memory
+  static constexpr int BAR_OFF = OUT_OFF + 8 * 2048;
   static constexpr int XCHG_OFF = BAR_OFF + 512;
-  static constexpr int PRE_OFF = XCHG_OFF + 3 * 2 * 128 * 4;
+  static constexpr int SEG_OFF = XCHG_OFF + 3 * 2 * 128 * 4;
+  static constexpr int PLAN_OFF = SEG_OFF + SEGS * 64;
+  static constexpr int PRE_OFF = PLAN_OFF + PLAN * 128;
   static constexpr int TOTAL = PRE_OFF + (PG_MAX_SEQS + 2) * 4 + 1024;
-  static constexpr int TMEM_COLS = 512;  // S: 2 x 128 columns, O: D columns from 256
+  static constexpr int TMEM_COLS = 512;  // D 256: S 2 x 128 columns, O 256; D 128: S of each tile, O of each tile
   static constexpr int O_COL = 256;
 };
 static_assert(ChunkSmem<256>::TOTAL <= 232448 && ChunkSmem<128>::TOTAL <= 232448, "shared memory of a CTA");
@@ -59,13 +61,15 @@ __device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_add
 
 // a segment: consecutive key tiles of one item
 struct ChunkSeg {
-  int g, h0, tok0;     // kv head, first query head, first token of the pair
-  int ta, tb;          // key tiles
-  int lo, hi;          // slots some row of the item sees
-  int64_t part;        // first row of the partial result (256 rows), or -1: the segment is the whole item
+  int b, row0, nq, base;  // sequence, its first row of q, its rows, the first one's slot
+  int g, h0, tok0, hp;    // kv head, first query head, first token, heads of the item
+  int ta, tb;             // key tiles (ta < 0: no more segments)
+  int lo, hi;             // slots some row of the item sees
+  int part;               // partial result (256 rows) to write, or -1: the segment is the whole item
 };
+static_assert(sizeof(ChunkSeg) <= 64, "slot of the segment ring");
 
-// walks the segments of a unit; every role of both CTAs walks the same
+// the walk over a unit's segments, as it is planned
 struct ChunkWalk {
   PagedSeq q;
   ChunkCut c;
@@ -75,16 +79,16 @@ struct ChunkWalk {
   int64_t w_tt;      // first pair of the token tile
   bool first;
 
-  __device__ __forceinline__ void start(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int it, int* status) {
-    b = paged_find(pre, s.B, it);
+  __device__ __forceinline__ void start(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int unit, int* status) {
+    b = paged_find(pre, s.B, unit);
     q = paged_seq(s, b, status);
     c = chunk_cut(q, a);
-    this->it = it;
-    const int u = it - pre[b];
+    it = unit;
+    const int u = unit - pre[b];
     w = c.begin(u);
     w_end = c.begin(u + 1);
     first = true;
-    tt = -1, w_tt = 0, nt = 0;
+    tt = -1, w_tt = 0, nt = 0, t0 = 0;
     advance(a);
     if (c.whole) {
       const int off = static_cast<int>((w - w_tt) % nt);
@@ -108,16 +112,80 @@ struct ChunkWalk {
     const int64_t left = w_end - w;
     const int len = !c.whole && left < nt - off ? static_cast<int>(left) : nt - off;
     const int sets = a.group / c.hp;
+    g.b = b, g.row0 = q.row0, g.nq = q.nq, g.base = q.len - q.nq;
     g.g = item / sets;
     g.h0 = g.g * a.group + (item % sets) * c.hp;
     g.tok0 = tt * c.tok;
+    g.hp = c.hp;
     g.ta = t0 + off;
     g.tb = g.ta + len;
     c.slots(q, a, tt, g.lo, g.hi);
-    g.part = len == nt ? -1 : (static_cast<int64_t>(it) * 2 + (first ? 0 : 1)) * 256;
+    g.part = len == nt ? -1 : it * 2 + (first ? 0 : 1);
     first = false;
     w += len;
     return true;
+  }
+};
+static_assert(sizeof(ChunkWalk) <= 128, "slot of the unit plan");
+
+// The segments reach the other warps through a ring in shared memory: units are planned several at a time, one per lane, so that none
+// of the searches and divisions stands between two segments.
+template <class L>
+struct SegRing {
+  ChunkSeg* slots;
+  uint64_t* full;
+  uint64_t* empty;
+  uint32_t n;
+  __device__ __forceinline__ bool next(const WaitCtx& wc, ChunkSeg& g) const {
+    if (!mbar_wait(wc, &full[n % L::SEGS], (n / L::SEGS) & 1u, ST_TIMEOUT_FULL)) return false;
+    g = *reinterpret_cast<const ChunkSeg*>(reinterpret_cast<const uint8_t*>(slots) + (n % L::SEGS) * 64);
+    return g.ta >= 0;
+  }
+  // one arrival per reading warp; the numbers are in registers from here on
+  __device__ __forceinline__ void done() { mbar_arrive(&empty[n++ % L::SEGS]); }
+};
+// the planning side (one warp): publish() puts the next segment into the ring, at the end the mark that there is none
+template <class L>
+struct SegPlan {
+  uint8_t* plan;   // L::PLAN walks of 128 bytes
+  int u, k, total, step;  // next unit to plan for, next walk
+  uint32_t n;
+  bool ended;
+  __device__ __forceinline__ bool publish(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, const SegRing<L>& ring, const WaitCtx& wc, int* status) {
+    if (ended) return true;
+    const int lane = threadIdx.x & 31;
+    for (;;) {
+      if (k == L::PLAN && u < total) {
+        __syncwarp();
+        const int mine = u + lane * step;
+        if (lane < L::PLAN && mine < total) reinterpret_cast<ChunkWalk*>(plan + lane * 128)->start(s, a, pre, mine, status);
+        __syncwarp();
+        k = 0;
+      }
+      const bool have = k < L::PLAN && u + k * step < total;
+      int put = 0;  // 1: a segment, 2: the walk has none left, 3: the ring does not empty
+      if (lane == 0) {
+        ChunkSeg g;
+        g.ta = -1;
+        put = !have || reinterpret_cast<ChunkWalk*>(plan + k * 128)->next(a, g) ? 1 : 2;
+        if (put == 1) {
+          if (mbar_wait(wc, &ring.empty[n % L::SEGS], ((n / L::SEGS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) {
+            *reinterpret_cast<ChunkSeg*>(reinterpret_cast<uint8_t*>(ring.slots) + (n % L::SEGS) * 64) = g;
+            mbar_arrive(&ring.full[n % L::SEGS]);
+          } else {
+            put = 3;
+          }
+        }
+      }
+      put = __shfl_sync(0xffffffffu, put, 0);
+      if (put == 2) {
+        if (++k == L::PLAN) u += L::PLAN * step;
+        continue;
+      }
+      ++n;
+      ended = !have;
+      return put == 1;
+    }
   }
 };
 
@@ -145,12 +213,169 @@ struct PageRun {
   }
 };
 
-template <int D>
+// 128 bytes of each of the warp's 32 rows (row = lane, words w) to global memory through 2 KB of shared memory, 16 rows at a time: a
+// store instruction then covers whole 128-byte lines of four rows instead of 16 bytes of 32 rows (15 000 -> cycles per segment).
+// dst(r): where row r's bytes go, or null.
+template <class Dst>
+__device__ __forceinline__ void store_lines(const uint32_t (&w)[32], uint8_t* stage, int lane, Dst dst) {
+  uint4* st = reinterpret_cast<uint4*>(stage);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncwarp();
+    if ((lane >> 4) == h) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) st[(lane & 15) * 8 + (x ^ (lane & 7))] = make_uint4(w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = k * 4 + (lane >> 3), ch = lane & 7;
+      uint8_t* to = dst(h * 16 + r);
+      if (to) *reinterpret_cast<uint4*>(to + ch * 16) = st[r * 8 + (ch ^ (r & 7))];
+    }
+  }
+}
+
+// O of 128 rows x COLS columns from tensor memory (from column `taddr`, head dimensions from d0 on): divided by the sums and rounded to
+// the output, or in fp32 to the segment's partial result. `free_o` is called when the last column is in registers.
+template <int D, int COLS, class Free>
+__device__ __forceinline__ void chunk_store(const PagedAttnArgs& a, const ChunkSeg& g, uint32_t taddr, int d0, int tile, int qd, int lane, float inv,
+                                            uint8_t* stage, Free free_o) {
+  const int qrows = 128 / g.hp;
+  auto tok_of = [&](int r) { return g.tok0 + tile * qrows + (qd * 32 + r) % qrows; };
+  if (g.part < 0) {
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += 64) {
+      uint32_t o[32], w[32];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        __syncwarp();
+        tmem_ld_x32(taddr + c + x * 32, o);
+        tmem_wait_ld();
+        if (x == 1 && c + 64 >= COLS) free_o();
+#pragma unroll
+        for (int y = 0; y < 16; ++y) w[x * 16 + y] = pack_bf16x2(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
+      }
+      store_lines(w, stage, lane, [&](int r) -> uint8_t* {
+        const int tok = tok_of(r), head = g.h0 + (qd * 32 + r) / qrows;
+        if (tok >= g.nq) return nullptr;
+        return reinterpret_cast<uint8_t*>(a.out + static_cast<int64_t>(g.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D + d0 + c);
+      });
+    }
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += 32) {
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld_x32(taddr + c, o);
+      tmem_wait_ld();
+      if (c + 32 >= COLS) free_o();
+      store_lines(o, stage, lane, [&](int r) -> uint8_t* {
+        if (tok_of(r) >= g.nq) return nullptr;
+        return reinterpret_cast<uint8_t*>(a.chunk_o + (static_cast<int64_t>(g.part) * 256 + tile * 128 + qd * 32 + r) * D + d0 + c);
+      });
+    }
+  }
+}
+__device__ __forceinline__ void chunk_store_stats(const PagedAttnArgs& a, const ChunkSeg& g, int tile, int row, int tok, int head, float m, float l) {
+  if (tok >= g.nq) return;
+  if (g.part >= 0)
+    a.chunk_ml[static_cast<int64_t>(g.part) * 256 + tile * 128 + row] = make_float2(m, l);
+  else if (a.lse)
+    a.lse[static_cast<int64_t>(g.row0 + tok) * a.H + head] = m + log2f(l);
+}
+
+// 64 scores of a row from tensor memory, hidden ones (slots outside [lo, hi], jb the first's slot) at -inf where the tile is a boundary
+__device__ __forceinline__ void chunk_scores(float (&sc)[64], uint32_t taddr, bool masked, int jb, int lo, int hi) {
+  uint32_t v0[32], v1[32];
+  tmem_ld_x32(taddr, v0);
+  tmem_ld_x32(taddr + 32, v1);
+  tmem_wait_ld();
+#pragma unroll
+  for (int c = 0; c < 32; ++c) sc[c] = __uint_as_float(v0[c]), sc[32 + c] = __uint_as_float(v1[c]);
+  if (masked) {
+    uint64_t bits = hi < jb ? 0ull : hi - jb >= 63 ? ~0ull : (2ull << (hi - jb)) - 1ull;
+    if (lo > jb) bits &= lo - jb > 63 ? 0ull : ~0ull << (lo - jb);
+    const uint32_t b_lo = static_cast<uint32_t>(bits), b_hi = static_cast<uint32_t>(bits >> 32);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      sc[c] = (b_lo & (1u << c)) ? sc[c] : -INFINITY;
+      sc[32 + c] = (b_hi & (1u << c)) ? sc[32 + c] : -INFINITY;
+    }
+  }
+}
+__device__ __forceinline__ float chunk_max(const float (&sc)[64]) {
+  float m[4] = {sc[0], sc[1], sc[2], sc[3]};  // four chains: one is 64 dependent instructions
+#pragma unroll
+  for (int c = 4; c < 64; ++c) m[c & 3] = fmaxf(m[c & 3], sc[c]);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// p = 2^(scale s - m), packed to bf16 pairs; returns their sum (unrounded)
+__device__ __forceinline__ float chunk_probs(const float (&sc)[64], float scale_log2, float neg_m, uint32_t (&pk)[32]) {
+  float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const float p0 = fast_exp2(fmaf(sc[2 * c], scale_log2, neg_m)), p1 = fast_exp2(fmaf(sc[2 * c + 1], scale_log2, neg_m));
+    sum0 += p0;
+    sum1 += p1;
+    pk[c] = pack_bf16x2(p0, p1);
+  }
+  return sum0 + sum1;
+}
+// COLS columns of O times alpha, in tensor memory
+template <int COLS>
+__device__ __forceinline__ void chunk_rescale(uint32_t taddr, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t o[32];
+    tmem_ld_x32(taddr + c, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+    tmem_st_x32(taddr + c, o);
+  }
+}
+// rows of a boundary tile of V (slabs of `slabs` x 64 dimensions, 128 keys each) that no row of the item sees
+__device__ __forceinline__ void chunk_clear(uint8_t* v, int slabs, int t, const ChunkSeg& g, int lane) {
+  for (int x = lane; x < PG_TILE * slabs * 8; x += 32) {
+    const int key = (x >> 3) % PG_TILE, slab = (x >> 3) / PG_TILE, j = t * PG_TILE + key;
+    if (j < g.lo || j >= g.hi) *reinterpret_cast<uint4*>(v + slab * PG_TILE * 128 + sw128_offset(key, x & 7)) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+__device__ __forceinline__ bool chunk_edge(const ChunkSeg& g, int t) { return t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi; }
+
+// unit counts of the sequences, and where the join finds them
+__device__ __forceinline__ int chunk_units(const PagedSeqs& s, const PagedAttnArgs& a, int* pre, int* status) {
+  paged_item_prefix(s.B, pre, CHUNK_THREADS, [&](int b) {
+    const PagedSeq q = paged_seq(s, b, status);
+    return chunk_class(q, a) ? chunk_cut(q, a).units : 0;
+  });
+  int total = pre[s.B];
+  if (total > a.max_units) {  // rows of q that several sequences claim: more units than n rows can make
+    total = a.max_units;
+    atomicCAS(status, 0, ST_BAD_INDEX);
+  }
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b <= s.B; b += CHUNK_THREADS) a.unit_pre[b] = pre[b];
+  return total;
+}
+
+// ---------------------------------------------------------------- D 256: CTA pairs
+//   warp 0      TMA loads of this CTA's 64 keys of K
+//   warp 1      owns tensor memory; the leader's lane issues S = Q K^T (M = 256) into one of two buffers and O += P V; S of tile t + 1
+//               before P V of tile t. A queued product blocks its issue slot until the pipe takes it, so whatever can be waited for
+//               earlier is (V before S), and a product's one commit serves the softmax and the copies: S done = its K stage free
+//   warps 2-9   softmax: thread = row, group A the first 64 keys of the tile, group B the others; maxima exchanged in shared memory
+//   warp 10     TMA loads of Q and of this CTA's half of V's dimensions (all 128 keys)
+//   warp 11     in a tile with slots that no row of the item sees (a page's end, the front of a window) it waits for the copy of V
+//               and clears those rows, while warp 10 goes on: P is 0 there, but 0 * inf is not. It also plans the segments
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
-paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+  constexpr int D = 256;
   using L = ChunkSmem<D>;
-  constexpr int SLABS = L::SLABS, NS = L::NS, NQ = L::NQ, V_SLABS = SLABS / 2;
+  constexpr int SLABS = L::SLABS, NS = L::NS, V_SLABS = SLABS / 2;
   constexpr uint32_t IDESC_S = make_idesc(FMT_BF16, FMT_BF16, 256, 128, 0, 0);
   constexpr uint32_t IDESC_O = make_idesc(FMT_BF16, FMT_BF16, 256, D, 0, 1);  // B = V, MN-major (head dimensions contiguous)
 
@@ -158,17 +383,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + NQ;
-  uint64_t* k_full = bars + 2 * NQ;
-  uint64_t* k_empty = k_full + NS;
-  uint64_t* v_full = k_empty + NS;
-  uint64_t* v_empty = v_full + NS;
-  uint64_t* s_full = v_empty + NS;  // 2 buffers
-  uint64_t* p_ready = s_full + 2;
-  uint64_t* o_done = p_ready + 1;
-  uint64_t* o_free = o_done + 1;
-  uint64_t* v_edge = o_free + 1;  // NS: a boundary tile's copies complete on the CTA's own barrier
-  uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(v_edge + NS);
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;        // NS
+  uint64_t* v_full = k_full + NS;     // NS
+  uint64_t* s_done = v_full + NS;     // NS: S of a tile is there, its K stage is free
+  uint64_t* o_done = s_done + NS;     // NS: P V of a tile is done, its V stage is free
+  uint64_t* v_edge = o_done + NS;     // NS: a boundary tile's copies complete on the CTA's own barrier
+  uint64_t* p_ready = v_edge + NS;
+  uint64_t* o_free = p_ready + 1;
+  uint64_t* seg_full = o_free + 1;    // SEGS
+  uint64_t* seg_empty = seg_full + L::SEGS;
+  uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(seg_empty + L::SEGS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_p + 1);
   float* xchg = reinterpret_cast<float*>(smem + L::XCHG_OFF);
   int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
@@ -180,21 +405,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   pdl_trigger();
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NQ; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 2);  // one arrival of each CTA's V warp: the copies are queued, or the boundary tile is ready
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_full[i], 2);  // one arrival of each CTA: the copies are queued, or the boundary tile is ready
+      mbar_init(&s_done[i], 1);
+      mbar_init(&o_done[i], 1);
       mbar_init(&v_edge[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
     mbar_init(p_ready, 16);  // one arrival per softmax warp of both CTAs
-    mbar_init(o_done, 1);
     mbar_init(o_free, 16);
+    for (int i = 0; i < L::SEGS; ++i) {
+      mbar_init(&seg_full[i], 1);
+      mbar_init(&seg_empty[i], rank == 0 ? 12 : 11);  // K, V, boundary, 8 softmax warps, and the leader's products
+    }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -205,159 +430,137 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     tmem_alloc_pair(tmem_base_p, L::TMEM_COLS);
     tmem_relinquish_pair();
   }
-  paged_item_prefix(s.B, pre, CHUNK_THREADS, [&](int b) {
-    const PagedSeq q = paged_seq(s, b, status);
-    return chunk_class(q, a) ? chunk_cut(q, a).units : 0;
-  });
-  int total = pre[s.B];
-  if (total > a.max_units) {  // rows of q that several sequences claim: more units than n rows can make
-    total = a.max_units;
-    atomicCAS(status, 0, ST_BAD_INDEX);
-  }
-  if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b <= s.B; b += CHUNK_THREADS) a.unit_pre[b] = pre[b];  // the join's index of the partial rows
+  const int total = chunk_units(s, a, pre, status);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers are initialised before any remote arrival or peer-signalled copy
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_p;
   const int in_page = (1 << s.page_log2) - 1;
+  SegRing<L> ring{reinterpret_cast<ChunkSeg*>(smem + L::SEG_OFF), seg_full, seg_empty, 0};
+  ChunkSeg g;
 
   if (warp == 0) {
     const int rl = s.page_log2 < 6 ? s.page_log2 : 6, rows = 1 << rl;  // rows of a K box
     uint32_t cnt = 0;
     bool ok = true;
-    for (int it = pair; it < total && ok; it += n_pairs) {
-      ChunkWalk wk;
-      wk.start(s, a, pre, it, status);
-      const int32_t* pages = s.table + wk.b * s.table_pitch;
-      ChunkSeg g;
-      while (ok && wk.next(a, g)) {
-        PageRun run;
-        run.start(s, pages, g, static_cast<int>(rank) * CH_KH, 6 - rl, rl, lane, status);
-        for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
-          const uint32_t st = cnt % NS;
-          if (lane == 0) {
-            ok = mbar_wait(wc, &k_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
-            if (ok && rank == 0) mbar_expect_tx(&k_full[st], 2 * L::KV);
-          }
-          const int j0 = t * PG_TILE + static_cast<int>(rank) * CH_KH;
-          for (int x = 0; x < CH_KH >> rl; ++x) {
-            const int pg = run.get(s, pages, g, lane, status);
-            if (lane == 0 && ok) {
-              const uint32_t bar = map_to_cta(&k_full[st], 0);
-              const int at = (j0 + x * rows) & in_page;
-              uint8_t* dst = smem + L::K_OFF + st * L::KV + x * rows * 128;
-              if (rows == CH_KH)
-                tma_load_5d_pair(dst, &tmK, 0, at, 0, g.g, pg, bar);
-              else
-                for (int y = 0; y < SLABS; ++y) tma_load_5d_pair(dst + y * CH_KH * 128, &tmK, 0, at, y, g.g, pg, bar);
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+    while (ok && ring.next(wc, g)) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      const int32_t* pages = s.table + g.b * s.table_pitch;
+      PageRun run;
+      run.start(s, pages, g, static_cast<int>(rank) * CH_KH, 6 - rl, rl, lane, status);
+      for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
+        const uint32_t st = cnt % NS;
+        if (lane == 0) {
+          ok = mbar_wait(wc, &s_done[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+          if (ok && rank == 0) mbar_expect_tx(&k_full[st], 2 * L::KV);
         }
+        const int j0 = t * PG_TILE + static_cast<int>(rank) * CH_KH;
+        for (int x = 0; x < CH_KH >> rl; ++x) {
+          const int pg = run.get(s, pages, g, lane, status);
+          if (lane == 0 && ok) {
+            const uint32_t bar = map_to_cta(&k_full[st], 0);
+            const int at = (j0 + x * rows) & in_page;
+            uint8_t* dst = smem + L::K_OFF + st * L::KV + x * rows * 128;
+            if (rows == CH_KH)
+              tma_load_5d_pair(dst, &tmK, 0, at, 0, g.g, pg, bar);
+            else
+              for (int y = 0; y < SLABS; ++y) tma_load_5d_pair(dst + y * CH_KH * 128, &tmK, 0, at, y, g.g, pg, bar);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       }
     }
   } else if (warp == 10) {
     const int rl = s.page_log2 < 7 ? s.page_log2 : 7, rows = 1 << rl;  // rows of a V box
     uint32_t cnt = 0, seg_n = 0;
     bool ok = true;
-    for (int it = pair; it < total && ok; it += n_pairs) {
-      ChunkWalk wk;
-      wk.start(s, a, pre, it, status);
-      const int32_t* pages = s.table + wk.b * s.table_pitch;
-      const int hp = wk.c.hp, qrows = 128 / hp;
-      ChunkSeg g;
-      while (ok && wk.next(a, g)) {
-        PageRun run;
-        run.start(s, pages, g, 0, 7 - rl, rl, lane, status);
-        // Q comes with this warp, not with K's: the next segment's K is then not held back until the last product has read Q
-        const uint32_t qs = seg_n % NQ;
+    while (ok && ring.next(wc, g)) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      const int32_t* pages = s.table + g.b * s.table_pitch;
+      PageRun run;
+      run.start(s, pages, g, 0, 7 - rl, rl, lane, status);
+      // Q comes with this warp, not with K's: the next segment's K is then not held back until the last product has read Q
+      if (lane == 0) {
+        ok = mbar_wait(wc, q_empty, (seg_n & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+        if (ok) {
+          if (rank == 0) mbar_expect_tx(q_full, 2 * L::Q_BYTES);
+          const int qrows = 128 / g.hp, row = g.row0 + g.tok0 + static_cast<int>(rank) * qrows;
+          for (int hh = 0; hh < g.hp; ++hh)
+            for (int x = 0; x < SLABS; ++x)
+              tma_load_2d_pair(smem + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, row, map_to_cta(q_full, 0));
+        }
+      }
+      ++seg_n;
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
+        const uint32_t st = cnt % NS;
+        const bool edge = chunk_edge(g, t);
         if (lane == 0) {
-          ok = mbar_wait(wc, &q_empty[qs], ((seg_n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+          ok = mbar_wait(wc, &o_done[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
           if (ok) {
-            if (rank == 0) mbar_expect_tx(&q_full[qs], 2 * L::Q_BYTES);
-            const int row = wk.q.row0 + g.tok0 + static_cast<int>(rank) * qrows;
-            for (int hh = 0; hh < hp; ++hh)
-              for (int x = 0; x < SLABS; ++x)
-                tma_load_2d_pair(smem + qs * L::Q_BYTES + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, row, map_to_cta(&q_full[qs], 0));
+            if (edge)
+              mbar_expect_tx(&v_edge[st], L::KV);
+            else if (rank == 0)
+              mbar_expect_tx(&v_full[st], 2 * L::KV);
+            else
+              mbar_arrive_cluster(map_to_cta(&v_full[st], 0));
           }
         }
-        ++seg_n;
-        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
-        for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
-          const uint32_t st = cnt % NS;
-          const bool edge = t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi;
-          if (lane == 0) {
-            ok = mbar_wait(wc, &v_empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
-            if (ok) {
+        for (int x = 0; x < PG_TILE >> rl; ++x) {
+          const int pg = run.get(s, pages, g, lane, status);
+          if (lane == 0 && ok) {
+            const uint32_t bar = map_to_cta(&v_full[st], 0);
+            const int at = (t * PG_TILE + x * rows) & in_page;
+            uint8_t* dst = smem + L::V_OFF + st * L::KV + x * rows * 128;
+            for (int y = 0; y < (rows == PG_TILE ? 1 : V_SLABS); ++y) {
+              const int slab = static_cast<int>(rank) * V_SLABS + y;
               if (edge)
-                mbar_expect_tx(&v_edge[st], L::KV);
-              else if (rank == 0)
-                mbar_expect_tx(&v_full[st], 2 * L::KV);
+                tma_load_5d(dst + y * PG_TILE * 128, &tmV, 0, at, slab, g.g, pg, &v_edge[st]);
               else
-                mbar_arrive_cluster(map_to_cta(&v_full[st], 0));
+                tma_load_5d_pair(dst + y * PG_TILE * 128, &tmV, 0, at, slab, g.g, pg, bar);
             }
           }
-          for (int x = 0; x < PG_TILE >> rl; ++x) {
-            const int pg = run.get(s, pages, g, lane, status);
-            if (lane == 0 && ok) {
-              const uint32_t bar = map_to_cta(&v_full[st], 0);
-              const int at = (t * PG_TILE + x * rows) & in_page;
-              uint8_t* dst = smem + L::V_OFF + st * L::KV + x * rows * 128;
-              for (int y = 0; y < (rows == PG_TILE ? 1 : V_SLABS); ++y) {
-                const int slab = static_cast<int>(rank) * V_SLABS + y;
-                if (edge)
-                  tma_load_5d(dst + y * PG_TILE * 128, &tmV, 0, at, slab, g.g, pg, &v_edge[st]);
-                else
-                  tma_load_5d_pair(dst + y * PG_TILE * 128, &tmV, 0, at, slab, g.g, pg, bar);
-              }
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
         }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       }
     }
   } else if (warp == 11) {
     uint32_t cnt = 0, edges[NS];  // boundary tiles each stage has held
 #pragma unroll
     for (int i = 0; i < NS; ++i) edges[i] = 0;
+    SegPlan<L> planner{smem + L::PLAN_OFF, pair, L::PLAN, total, n_pairs, 0, false};
     bool ok = true;
-    for (int it = pair; it < total && ok; it += n_pairs) {
-      ChunkWalk wk;
-      wk.start(s, a, pre, it, status);
-      ChunkSeg g;
-      while (ok && wk.next(a, g)) {
-        for (int t = g.ta; t < g.tb; ++t, ++cnt) {
-          if (t * PG_TILE >= g.lo && (t + 1) * PG_TILE <= g.hi) continue;
-          const uint32_t st = cnt % NS;
-          uint32_t turn = 0;
+    for (int i = 0; i + 1 < L::SEGS && ok; ++i) ok = planner.publish(s, a, pre, ring, wc, status);
+    while (ok && __all_sync(0xffffffffu, ring.next(wc, g))) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      for (int t = g.ta; t < g.tb; ++t, ++cnt) {
+        if (!chunk_edge(g, t)) continue;
+        const uint32_t st = cnt % NS;
+        uint32_t turn = 0;
 #pragma unroll
-          for (int i = 0; i < NS; ++i)
-            if (static_cast<uint32_t>(i) == st) turn = edges[i]++;
-          ok = __all_sync(0xffffffffu, mbar_wait(wc, &v_edge[st], turn & 1u, ST_TIMEOUT_FULL));
-          if (!ok) break;
-          for (int x = lane; x < PG_TILE * V_SLABS * 8; x += 32) {
-            const int key = (x >> 3) % PG_TILE, slab = (x >> 3) / PG_TILE, j = t * PG_TILE + key;
-            if (j < g.lo || j >= g.hi)
-              *reinterpret_cast<uint4*>(smem + L::V_OFF + st * L::KV + slab * PG_TILE * 128 + sw128_offset(key, x & 7)) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_release(map_to_cta(&v_full[st], 0));
-        }
+        for (int i = 0; i < NS; ++i)
+          if (static_cast<uint32_t>(i) == st) turn = edges[i]++;
+        ok = __all_sync(0xffffffffu, mbar_wait(wc, &v_edge[st], turn & 1u, ST_TIMEOUT_FULL));
+        if (!ok) break;
+        chunk_clear(smem + L::V_OFF + st * L::KV, V_SLABS, t, g, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_release(map_to_cta(&v_full[st], 0));
       }
+      ok = ok && planner.publish(s, a, pre, ring, wc, status);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      uint32_t q_addr = 0, kc = 0, vc = 0, gt = 0, seg_n = 0;
+      const uint32_t q_addr = smem_u32(smem);
+      uint32_t kc = 0, gt = 0, seg_n = 0;
       bool ok = true;
-      auto issue_s = [&](uint32_t g) -> bool {  // S of tile g into buffer g & 1
-        const uint32_t st = kc % NS;
-        if (!mbar_wait(wc, &k_full[st], (kc / NS) & 1u, ST_TIMEOUT_FULL)) return false;
+      auto issue_s = [&]() {  // S of the next tile into buffer kc & 1; its K is there
         tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + L::K_OFF + st * L::KV);
-        const uint32_t d_tmem = tmem_base + (g & 1u) * 128;
+        const uint32_t k_addr = smem_u32(smem + L::K_OFF + (kc % NS) * L::KV);
+        const uint32_t d_tmem = tmem_base + (kc & 1u) * 128;
 #pragma unroll
         for (int x = 0; x < SLABS; ++x) {
           const uint64_t ad = make_smem_desc_sw128(q_addr + x * 128 * 128, 16, 1024);
@@ -365,192 +568,112 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_f16_ss_pair(d_tmem, ad + 2 * k, bd + 2 * k, IDESC_S, (x | k) != 0);
         }
-        umma_commit_pair_both(&k_empty[st]);
-        umma_commit_pair_both(&s_full[g & 1u]);
+        umma_commit_pair_both(&s_done[kc % NS]);
         ++kc;
-        return true;
       };
-      for (int it = pair; it < total && ok; it += n_pairs) {
-        ChunkWalk wk;
-        wk.start(s, a, pre, it, status);
-        ChunkSeg g;
-        while (ok && wk.next(a, g)) {
-          const int n_tiles = g.tb - g.ta;
-          const uint32_t qs = seg_n % NQ;
-          if (!mbar_wait(wc, &q_full[qs], (seg_n / NQ) & 1u, ST_TIMEOUT_FULL)) { ok = false; break; }
-          q_addr = smem_u32(smem) + qs * L::Q_BYTES;
+      while (ok && ring.next(wc, g)) {
+        ring.done();
+        const int n_tiles = g.tb - g.ta;
+        ok = mbar_wait(wc, q_full, seg_n & 1u, ST_TIMEOUT_FULL) && mbar_wait(wc, &k_full[kc % NS], (kc / NS) & 1u, ST_TIMEOUT_FULL);
+        if (!ok) break;
+        issue_s();
+        for (int i = 0; i < n_tiles; ++i) {
+          const uint32_t gi = gt + i, st = gi % NS;
+          ok = i + 1 >= n_tiles || mbar_wait(wc, &k_full[kc % NS], (kc / NS) & 1u, ST_TIMEOUT_FULL);
+          ok = ok && mbar_wait(wc, &v_full[st], (gi / NS) & 1u, ST_TIMEOUT_FULL);
+          if (!ok) break;
+          if (i + 1 < n_tiles)
+            issue_s();  // buffer (gi + 1) & 1 last held P of tile gi - 1, whose P V was issued before
+          else
+            umma_commit_pair_both(q_empty);
+          ok = mbar_wait(wc, p_ready, gi & 1u, ST_TIMEOUT_OTHER);
+          if (ok && i == 0 && seg_n > 0) ok = mbar_wait(wc, o_free, (seg_n - 1) & 1u, ST_TIMEOUT_OTHER);
+          if (!ok) break;
           tc_fence_after();
-          if (!issue_s(gt)) { ok = false; break; }
-          for (int i = 0; i < n_tiles; ++i) {
-            const uint32_t gi = gt + i;
-            if (i + 1 < n_tiles) {
-              if (!issue_s(gi + 1)) { ok = false; break; }  // buffer (gi + 1) & 1 last held P of tile gi - 1, whose P V was issued before
-            } else {
-              umma_commit_pair_both(&q_empty[qs]);
-            }
-            if (!mbar_wait(wc, p_ready, gi & 1u, ST_TIMEOUT_OTHER)) { ok = false; break; }
-            if (i == 0 && seg_n > 0 && !mbar_wait(wc, o_free, (seg_n - 1) & 1u, ST_TIMEOUT_OTHER)) { ok = false; break; }
-            const uint32_t st = vc % NS;
-            if (!mbar_wait(wc, &v_full[st], (vc / NS) & 1u, ST_TIMEOUT_FULL)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t v_addr = smem_u32(smem + L::V_OFF + st * L::KV);
-            const uint64_t vd = make_smem_desc_sw128(v_addr, PG_TILE * 128, 1024);
+          const uint64_t vd = make_smem_desc_sw128(smem_u32(smem + L::V_OFF + st * L::KV), PG_TILE * 128, 1024);
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const uint32_t p_tmem = tmem_base + (gi & 1u) * 128 + hh * CH_KH;  // packed bf16 P: 16 keys per 8 columns
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16_ts_pair(tmem_base + L::O_COL, p_tmem + 8 * k, vd + 128 * (4 * hh + k), IDESC_O, (i | hh | k) != 0);
-            }
-            umma_commit_pair_both(&v_empty[st]);
-            umma_commit_pair_both(o_done);
-            ++vc;
-          }
-          gt += n_tiles;
-          ++seg_n;
+          for (int k = 0; k < 8; ++k)  // packed bf16 P: 16 keys per 8 columns, the second group's from column 64 on
+            umma_f16_ts_pair(tmem_base + L::O_COL, tmem_base + (gi & 1u) * 128 + (k >> 2) * CH_KH + 8 * (k & 3), vd + 128 * k, IDESC_O, (i | k) != 0);
+          umma_commit_pair_both(&o_done[st]);
         }
+        gt += n_tiles;
+        ++seg_n;
       }
     }
   } else {
-    // softmax warps 2..9
     const int wg = (warp - 2) >> 2;
     const int qd = warp & 3;  // TMEM lane quarter of this warp
     const int row = qd * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(qd * 32) << 16;
+    uint8_t* stage = smem + L::OUT_OFF + (warp - 2) * 2048;
+    const uint32_t p_bar = map_to_cta(p_ready, 0), free_bar = map_to_cta(o_free, 0);
     uint32_t gt = 0;
-    bool alive = true;
-    for (int it = pair; it < total && alive; it += n_pairs) {
-      ChunkWalk wk;
-      wk.start(s, a, pre, it, status);
-      const int hp = wk.c.hp, qrows = 128 / hp;
-      const int base = wk.q.len - wk.q.nq;
-      ChunkSeg g;
-      while (alive && wk.next(a, g)) {
-        const int n_tiles = g.tb - g.ta;
-        const int head = g.h0 + row / qrows;
-        const int tok_first = g.tok0 + static_cast<int>(rank) * qrows, tok = tok_first + row % qrows;
-        const int hi = base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;  // slots the row sees
-        const int hi_min = base + tok_first, lo_max = a.window > 0 ? hi_min + qrows - a.window : 0;
-        float m_ref = -INFINITY, l_run = 0.f;
-        for (int i = 0; i < n_tiles; ++i) {
-          const uint32_t gi = gt + i;
-          const int jb = (g.ta + i) * PG_TILE + wg * CH_KH;
-          bool got = mbar_wait(wc, &s_full[gi & 1u], (gi >> 1) & 1u, ST_TIMEOUT_TMEM);
-          float sc[CH_KH];
-          float mx = -INFINITY;
-          const uint32_t s_tmem = tmem_base + lane_off + (gi & 1u) * 128 + wg * CH_KH;
-          if (__all_sync(0xffffffffu, got)) {
+    while (__all_sync(0xffffffffu, ring.next(wc, g))) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      const int n_tiles = g.tb - g.ta, qrows = 128 / g.hp;
+      const int head = g.h0 + row / qrows;
+      const int tok_first = g.tok0 + static_cast<int>(rank) * qrows, tok = tok_first + row % qrows;
+      const int hi = g.base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;  // slots the row sees
+      const int hi_min = g.base + tok_first, lo_max = a.window > 0 ? hi_min + qrows - a.window : 0;
+      float m_ref = -INFINITY, l_run = 0.f;
+      bool alive = true;
+      for (int i = 0; i < n_tiles; ++i) {
+        const uint32_t gi = gt + i;
+        const int jb = (g.ta + i) * PG_TILE + wg * CH_KH;
+        bool got = mbar_wait(wc, &s_done[gi % NS], (gi / NS) & 1u, ST_TIMEOUT_TMEM);
+        float sc[CH_KH];
+        float mx = -INFINITY;
+        const uint32_t s_tmem = tmem_base + lane_off + (gi & 1u) * 128 + wg * CH_KH;
+        got = __all_sync(0xffffffffu, got);
+        if (got) {
+          tc_fence_after();
+          chunk_scores(sc, s_tmem, jb + CH_KH - 1 > hi_min || jb < lo_max, jb, lo, hi);
+          mx = chunk_max(sc);
+        }
+        float* xq = xchg + (gi & 1u) * 256;
+        xq[wg * 128 + row] = mx;
+        if (!bar_red_and(1 + qd, 64, got)) { alive = false; break; }  // the two warps that share these rows leave together
+        mx = fmaxf(mx, xq[(wg ^ 1) * 128 + row]) * a.scale_log2;
+        float alpha = 1.f;
+        if (mx - m_ref > CH_RESCALE) {  // false for NaN (-inf minus -inf): a row that has seen nothing yet
+          alpha = fast_exp2(m_ref - mx);
+          m_ref = mx;
+        }
+        uint32_t pk[CH_KH / 2];
+        l_run = l_run * alpha + chunk_probs(sc, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref, pk);
+        if (i > 0) {
+          const bool done = mbar_wait(wc, &o_done[(gi - 1) % NS], ((gi - 1) / NS) & 1u, ST_TIMEOUT_TMEM);
+          if (__any_sync(0xffffffffu, alpha != 1.f) && __all_sync(0xffffffffu, done)) {
+            // every P V so far has completed and none is issued until all warps have arrived on p_ready
             tc_fence_after();
-            uint32_t v0[32], v1[32];
-            tmem_ld_x32(s_tmem, v0);
-            tmem_ld_x32(s_tmem + 32, v1);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) sc[c] = __uint_as_float(v0[c]), sc[32 + c] = __uint_as_float(v1[c]);
-            if (jb + CH_KH - 1 > hi_min || jb < lo_max) {
-              uint64_t bits = hi < jb ? 0ull : hi - jb >= 63 ? ~0ull : (2ull << (hi - jb)) - 1ull;
-              if (lo > jb) bits &= lo - jb > 63 ? 0ull : ~0ull << (lo - jb);
-              const uint32_t b_lo = static_cast<uint32_t>(bits), b_hi = static_cast<uint32_t>(bits >> 32);
-#pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                sc[c] = (b_lo & (1u << c)) ? sc[c] : -INFINITY;
-                sc[32 + c] = (b_hi & (1u << c)) ? sc[32 + c] : -INFINITY;
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < CH_KH; ++c) mx = fmaxf(mx, sc[c]);
-          } else {
-            got = false;
-          }
-          float* xq = xchg + (gi & 1u) * 256;
-          xq[wg * 128 + row] = mx;
-          if (!bar_red_and(1 + qd, 64, got)) { alive = false; break; }  // the two warps that share these rows leave together
-          mx = fmaxf(mx, xq[(wg ^ 1) * 128 + row]) * a.scale_log2;
-          float alpha = 1.f;
-          if (mx - m_ref > CH_RESCALE) {  // false for NaN (-inf minus -inf): a row that has seen nothing yet
-            alpha = fast_exp2(m_ref - mx);
-            m_ref = mx;
-          }
-          const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-          float sum0 = 0.f, sum1 = 0.f;
-          uint32_t pk[CH_KH / 2];
-#pragma unroll
-          for (int c = 0; c < CH_KH / 2; ++c) {
-            const float p0 = fast_exp2(fmaf(sc[2 * c], a.scale_log2, neg_m)), p1 = fast_exp2(fmaf(sc[2 * c + 1], a.scale_log2, neg_m));
-            sum0 += p0;
-            sum1 += p1;
-            pk[c] = pack_bf16x2(p0, p1);
-          }
-          l_run = l_run * alpha + (sum0 + sum1);
-          if (i > 0) {
-            const bool done = mbar_wait(wc, o_done, (gi - 1) & 1u, ST_TIMEOUT_TMEM);
-            if (__any_sync(0xffffffffu, alpha != 1.f) && __all_sync(0xffffffffu, done)) {
-              tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < D / 64; ++c) {
-                uint32_t o[32];
-                const uint32_t o_tmem = tmem_base + lane_off + L::O_COL + wg * (D / 2) + c * 32;
-                tmem_ld_x32(o_tmem, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-                tmem_st_x32(o_tmem, o);
-              }
-            }
-          }
-          __syncwarp();
-          tmem_st_x32(s_tmem, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_to_cta(p_ready, 0));
-        }
-        if (!alive) break;
-        gt += n_tiles;
-
-        // end of the segment: O of this group's half of the columns
-        float* xq = xchg + 2 * 256;
-        xq[wg * 128 + row] = l_run;
-        const bool got = mbar_wait(wc, o_done, (gt - 1) & 1u, ST_TIMEOUT_TMEM);
-        if (!bar_red_and(1 + qd, 64, got)) { alive = false; break; }
-        tc_fence_after();
-        const float l = l_run + xq[(wg ^ 1) * 128 + row];
-        const bool live = tok < wk.q.nq;
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row that sees nothing: 0; a NaN sum stays NaN
-        __nv_bfloat16* dst = a.out + static_cast<int64_t>(wk.q.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D + wg * (D / 2);
-        const int64_t prow = g.part + static_cast<int64_t>(rank) * 128 + row;
-#pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t o[32];
-          __syncwarp();
-          tmem_ld_x32(tmem_base + lane_off + L::O_COL + wg * (D / 2) + c * 32, o);
-          tmem_wait_ld();
-          if (c == D / 64 - 1) {  // O is in registers: the next segment's first P V may overwrite it
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(o_free, 0));
-          }
-          if (!live) continue;
-          if (g.part < 0) {
-            uint32_t wv[16];
-#pragma unroll
-            for (int x = 0; x < 16; ++x) wv[x] = pack_bf16x2(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv);
-            uint4* to = reinterpret_cast<uint4*>(dst + c * 32);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) to[x] = make_uint4(wv[4 * x], wv[4 * x + 1], wv[4 * x + 2], wv[4 * x + 3]);
-          } else {
-            uint4* to = reinterpret_cast<uint4*>(a.chunk_o + prow * D + wg * (D / 2) + c * 32);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) to[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            chunk_rescale<D / 2>(tmem_base + lane_off + L::O_COL + wg * (D / 2), alpha);
           }
         }
-        if (live && wg == 0) {
-          if (g.part >= 0)
-            a.chunk_ml[prow] = make_float2(m_ref, l);
-          else if (a.lse)
-            a.lse[static_cast<int64_t>(wk.q.row0 + tok) * a.H + head] = m_ref + log2f(l);
-        }
+        __syncwarp();
+        tmem_st_x32(s_tmem, pk);  // P over the first 32 columns of the S half this thread has read
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(p_bar);
       }
+      if (!alive) break;
+      gt += n_tiles;
+
+      // end of the segment: O of this group's half of the columns
+      float* xq = xchg + 2 * 256;
+      xq[wg * 128 + row] = l_run;
+      const bool got = mbar_wait(wc, &o_done[(gt - 1) % NS], ((gt - 1) / NS) & 1u, ST_TIMEOUT_TMEM);
+      if (!bar_red_and(1 + qd, 64, got)) break;
+      tc_fence_after();
+      const float l = l_run + xq[(wg ^ 1) * 128 + row];
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row that sees nothing: 0; a NaN sum stays NaN
+      chunk_store<D, D / 2>(a, g, tmem_base + lane_off + L::O_COL + wg * (D / 2), wg * (D / 2), static_cast<int>(rank), qd, lane, inv, stage, [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(free_bar);
+      });
+      if (wg == 0) chunk_store_stats(a, g, static_cast<int>(rank), row, tok, head, m_ref, l);
     }
   }
 
@@ -562,6 +685,279 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     __syncwarp();
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, L::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- D 128: two tiles of rows in one CTA
+// The warps' parts as above; the products go round as P V of tile 0, S of tile 0 for the next keys, P V of tile 1, S of tile 1, so that
+// while one tile's softmax works the pipe has the other's products.
+__global__ void __launch_bounds__(CHUNK_THREADS, 1)
+paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+  constexpr int D = 128;
+  using L = ChunkSmem<D>;
+  constexpr int SLABS = L::SLABS, NS = L::NS;
+  constexpr uint32_t IDESC_S = make_idesc(FMT_BF16, FMT_BF16, 128, 128, 0, 0);
+  constexpr uint32_t IDESC_O = make_idesc(FMT_BF16, FMT_BF16, 128, D, 0, 1);  // B = V, MN-major
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;         // NS
+  uint64_t* v_full = k_full + NS;      // NS
+  uint64_t* v_edge = v_full + NS;      // NS
+  uint64_t* s_done = v_edge + NS;      // [tile][NS]: S is there; tile 1's: the K stage is free as well
+  uint64_t* o_done = s_done + 2 * NS;  // [tile][NS]: P V is done; tile 1's: the V stage is free as well
+  uint64_t* p_ready = o_done + 2 * NS;  // [tile]
+  uint64_t* o_free = p_ready + 2;       // [tile]
+  uint64_t* seg_full = o_free + 2;
+  uint64_t* seg_empty = seg_full + L::SEGS;
+  uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(seg_empty + L::SEGS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_p + 1);
+  int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WaitCtx wc{abort_flag, status};
+  pdl_trigger();
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_edge[i], 1);
+      for (int x = 0; x < 2; ++x) mbar_init(&s_done[x * NS + i], 1), mbar_init(&o_done[x * NS + i], 1);
+    }
+    for (int x = 0; x < 2; ++x) mbar_init(&p_ready[x], 4), mbar_init(&o_free[x], 4);
+    for (int i = 0; i < L::SEGS; ++i) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 12);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_base_p, L::TMEM_COLS);
+    tmem_relinquish();
+  }
+  const int total = chunk_units(s, a, pre, status);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_p;
+  const int in_page = (1 << s.page_log2) - 1;
+  SegRing<L> ring{reinterpret_cast<ChunkSeg*>(smem + L::SEG_OFF), seg_full, seg_empty, 0};
+  ChunkSeg g;
+
+  if (warp == 0 || warp == 10) {
+    const bool is_k = warp == 0;
+    const int rl = s.page_log2 < 7 ? s.page_log2 : 7, rows = 1 << rl;  // rows of a box
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = (is_k ? s_done : o_done) + NS;
+    const CUtensorMap* tm = is_k ? &tmK : &tmV;
+    uint8_t* stages = smem + (is_k ? L::K_OFF : L::V_OFF);
+    uint32_t cnt = 0, seg_n = 0;
+    bool ok = true;
+    while (ok && ring.next(wc, g)) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      const int32_t* pages = s.table + g.b * s.table_pitch;
+      PageRun run;
+      run.start(s, pages, g, 0, 7 - rl, rl, lane, status);
+      if (!is_k && lane == 0) {  // (K of the next segment is not held back until the last product has read Q)
+        ok = mbar_wait(wc, q_empty, (seg_n & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+        if (ok) {
+          mbar_expect_tx(q_full, L::Q_BYTES);
+          const int qrows = 128 / g.hp;
+          for (int tile = 0; tile < 2; ++tile)
+            for (int hh = 0; hh < g.hp; ++hh)
+              for (int x = 0; x < SLABS; ++x)
+                tma_load_2d(smem + tile * (L::Q_BYTES / 2) + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, g.row0 + g.tok0 + tile * qrows, q_full);
+        }
+      }
+      ++seg_n;
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      for (int t = g.ta; t < g.tb && ok; ++t, ++cnt) {
+        const uint32_t st = cnt % NS;
+        const bool edge = !is_k && chunk_edge(g, t);
+        uint64_t* bar = edge ? &v_edge[st] : &full[st];
+        if (lane == 0) {
+          ok = mbar_wait(wc, &empty[st], ((cnt / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
+          if (ok) mbar_expect_tx(bar, L::KV);
+        }
+        for (int x = 0; x < PG_TILE >> rl; ++x) {
+          const int pg = run.get(s, pages, g, lane, status);
+          if (lane == 0 && ok) {
+            uint8_t* dst = stages + st * L::KV + x * rows * 128;
+            for (int y = 0; y < (rows == PG_TILE ? 1 : SLABS); ++y)
+              tma_load_5d(dst + y * PG_TILE * 128, tm, 0, (t * PG_TILE + x * rows) & in_page, y, g.g, pg, bar);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      }
+    }
+    if (*abort_flag && lane == 0) {  // bounded wait for copies that may still be in flight
+      for (uint32_t c = cnt > static_cast<uint32_t>(NS) ? cnt - NS : 0; c <= cnt; ++c)
+        for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % NS], (c / NS) & 1u); ++spin) {}
+      for (int spin = 0; !is_k && seg_n && spin < 4096 && !mbar_try_wait(q_full, (seg_n - 1) & 1u); ++spin) {}
+    }
+  } else if (warp == 11) {
+    uint32_t cnt = 0, edges[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) edges[i] = 0;
+    SegPlan<L> planner{smem + L::PLAN_OFF, static_cast<int>(blockIdx.x), L::PLAN, total, static_cast<int>(gridDim.x), 0, false};
+    bool ok = true;
+    for (int i = 0; i + 1 < L::SEGS && ok; ++i) ok = planner.publish(s, a, pre, ring, wc, status);
+    while (ok && __all_sync(0xffffffffu, ring.next(wc, g))) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      for (int t = g.ta; t < g.tb; ++t, ++cnt) {
+        if (!chunk_edge(g, t)) continue;
+        const uint32_t st = cnt % NS;
+        uint32_t turn = 0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          if (static_cast<uint32_t>(i) == st) turn = edges[i]++;
+        ok = __all_sync(0xffffffffu, mbar_wait(wc, &v_edge[st], turn & 1u, ST_TIMEOUT_FULL));
+        if (!ok) break;
+        chunk_clear(smem + L::V_OFF + st * L::KV, SLABS, t, g, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
+      }
+      ok = ok && planner.publish(s, a, pre, ring, wc, status);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t gt = 0, seg_n = 0;
+      bool ok = true;
+      auto issue_s = [&](int tile, uint32_t gi) {
+        const uint32_t q_addr = smem_u32(smem) + tile * (L::Q_BYTES / 2), k_addr = smem_u32(smem + L::K_OFF + (gi % NS) * L::KV);
+#pragma unroll
+        for (int x = 0; x < SLABS; ++x) {
+          const uint64_t ad = make_smem_desc_sw128(q_addr + x * 128 * 128, 16, 1024);
+          const uint64_t bd = make_smem_desc_sw128(k_addr + x * PG_TILE * 128, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16_ss(tmem_base + tile * 128, ad + 2 * k, bd + 2 * k, IDESC_S, (x | k) != 0);
+        }
+        umma_commit(&s_done[tile * NS + gi % NS]);
+      };
+      while (ok && ring.next(wc, g)) {
+        ring.done();
+        const int n_tiles = g.tb - g.ta;
+        ok = mbar_wait(wc, q_full, seg_n & 1u, ST_TIMEOUT_FULL) && mbar_wait(wc, &k_full[gt % NS], (gt / NS) & 1u, ST_TIMEOUT_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        // S of tile x may replace P of the last segment's end: its P V was issued before
+        issue_s(0, gt);
+        issue_s(1, gt);
+        for (int i = 0; i < n_tiles && ok; ++i) {
+          const uint32_t gi = gt + i, st = gi % NS;
+          const bool more = i + 1 < n_tiles;
+          ok = mbar_wait(wc, &v_full[st], (gi / NS) & 1u, ST_TIMEOUT_FULL) &&
+               (!more || mbar_wait(wc, &k_full[(gi + 1) % NS], ((gi + 1) / NS) & 1u, ST_TIMEOUT_FULL));
+          if (!ok) break;
+          if (!more) umma_commit(q_empty);
+          const uint64_t vd = make_smem_desc_sw128(smem_u32(smem + L::V_OFF + st * L::KV), PG_TILE * 128, 1024);
+#pragma unroll
+          for (int tile = 0; tile < 2; ++tile) {
+            ok = ok && mbar_wait(wc, &p_ready[tile], gi & 1u, ST_TIMEOUT_OTHER);
+            if (ok && i == 0 && seg_n > 0) ok = mbar_wait(wc, &o_free[tile], (seg_n - 1) & 1u, ST_TIMEOUT_OTHER);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 8; ++k)  // packed bf16 P: 16 keys per 8 columns
+              umma_f16_ts(tmem_base + L::O_COL + tile * D, tmem_base + tile * 128 + (k >> 2) * CH_KH + 8 * (k & 3), vd + 128 * k, IDESC_O, (i | k) != 0);
+            umma_commit(&o_done[tile * NS + st]);
+            if (more) issue_s(tile, gi + 1);
+          }
+        }
+        gt += n_tiles;
+        ++seg_n;
+      }
+    }
+  } else {
+    const int tile = (warp - 2) >> 2;
+    const int qd = warp & 3;
+    const int row = qd * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(qd * 32) << 16;
+    uint8_t* stage = smem + L::OUT_OFF + (warp - 2) * 2048;
+    const uint32_t s_tmem = tmem_base + lane_off + tile * 128, o_tmem = tmem_base + lane_off + L::O_COL + tile * D;
+    uint32_t gt = 0;
+    bool alive = true;
+    while (alive && __all_sync(0xffffffffu, ring.next(wc, g))) {
+      __syncwarp();
+      if (lane == 0) ring.done(); else ++ring.n;
+      const int n_tiles = g.tb - g.ta, qrows = 128 / g.hp;
+      const int head = g.h0 + row / qrows;
+      const int tok_first = g.tok0 + tile * qrows, tok = tok_first + row % qrows;
+      const int hi = g.base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;
+      const int hi_min = g.base + tok_first, lo_max = a.window > 0 ? hi_min + qrows - a.window : 0;
+      float m_ref = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < n_tiles; ++i) {
+        const uint32_t gi = gt + i;
+        const int jb = (g.ta + i) * PG_TILE;
+        alive = __all_sync(0xffffffffu, mbar_wait(wc, &s_done[tile * NS + gi % NS], (gi / NS) & 1u, ST_TIMEOUT_TMEM));
+        if (!alive) break;
+        tc_fence_after();
+        const bool masked = jb + PG_TILE - 1 > hi_min || jb < lo_max;
+        float sc[CH_KH];
+        // the maximum first; the second half's scores stay in registers, the first half's are read again (128 at once would spill)
+        chunk_scores(sc, s_tmem, masked, jb, lo, hi);
+        float mx = chunk_max(sc);
+        chunk_scores(sc, s_tmem + CH_KH, masked, jb + CH_KH, lo, hi);
+        mx = fmaxf(mx, chunk_max(sc)) * a.scale_log2;
+        float alpha = 1.f;
+        if (mx - m_ref > CH_RESCALE) {  // false for NaN (-inf minus -inf): a row that has seen nothing yet
+          alpha = fast_exp2(m_ref - mx);
+          m_ref = mx;
+        }
+        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+        if (i > 0) {
+          const bool done = mbar_wait(wc, &o_done[tile * NS + (gi - 1) % NS], ((gi - 1) / NS) & 1u, ST_TIMEOUT_TMEM);
+          if (__any_sync(0xffffffffu, alpha != 1.f) && __all_sync(0xffffffffu, done)) {
+            tc_fence_after();
+            chunk_rescale<D>(o_tmem, alpha);
+          }
+        }
+        uint32_t pk[CH_KH / 2];
+        float sum = chunk_probs(sc, a.scale_log2, neg_m, pk);
+        __syncwarp();
+        tmem_st_x32(s_tmem + CH_KH, pk);  // P of keys 64 .. 127 over their own scores
+        chunk_scores(sc, s_tmem, masked, jb, lo, hi);
+        sum += chunk_probs(sc, a.scale_log2, neg_m, pk);
+        l_run = l_run * alpha + sum;
+        __syncwarp();
+        tmem_st_x32(s_tmem, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[tile]);
+      }
+      if (!alive) break;
+      gt += n_tiles;
+      alive = __all_sync(0xffffffffu, mbar_wait(wc, &o_done[tile * NS + (gt - 1) % NS], ((gt - 1) / NS) & 1u, ST_TIMEOUT_TMEM));
+      if (!alive) break;
+      tc_fence_after();
+      const float inv = l_run > 0.f ? 1.f / l_run : (l_run == 0.f ? 0.f : l_run);
+      chunk_store<D, D>(a, g, o_tmem, 0, tile, qd, lane, inv, stage, [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[tile]);
+      });
+      chunk_store_stats(a, g, tile, row, tok, head, m_ref, l_run);
+    }
+  }
+
+  if (threadIdx.x == 0) pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::TMEM_COLS);
   }
 }
 
@@ -883,16 +1279,20 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   const uint32_t krows = kp.page < CH_KH ? static_cast<uint32_t>(kp.page) : static_cast<uint32_t>(CH_KH);
   const uint32_t vrows = kp.page < PG_TILE ? static_cast<uint32_t>(kp.page) : static_cast<uint32_t>(PG_TILE);
   if ((r = make_tmap_2d(&tmQ, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 128 / hp))) return r;
-  if ((r = make_tmap_pages(&tmK, kp, krows, krows == CH_KH ? D / 64 : 1))) return r;
-  if ((r = make_tmap_pages(&tmV, vp, vrows, vrows == PG_TILE ? D / 128 : 1))) return r;
+  if (D == 256) {  // a CTA's 64 keys of K, its half of V's dimensions
+    if ((r = make_tmap_pages(&tmK, kp, krows, krows == CH_KH ? D / 64 : 1)) || (r = make_tmap_pages(&tmV, vp, vrows, vrows == PG_TILE ? D / 128 : 1))) return r;
+  } else if ((r = make_tmap_pages(&tmK, kp, vrows, vrows == PG_TILE ? D / 64 : 1)) || (r = make_tmap_pages(&tmV, vp, vrows, vrows == PG_TILE ? D / 64 : 1))) {
+    return r;
+  }
+  auto kern = D == 256 ? paged_pair_kernel : paged_two_kernel;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    SPINF_CUDA_OK(cudaFuncSetAttribute(paged_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+    SPINF_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
     SPINF_CUDA_OK(cudaFuncSetAttribute(paged_chunk_weight_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkWeightSmem<D>::TOTAL));
     attr_set[dev].store(true, std::memory_order_release);
   }
-  SPINF_CUDA_OK(launch_after(paged_chunk_kernel<D>, dim3(static_cast<unsigned>(sm_count() / 2 * 2)), dim3(CHUNK_THREADS), st, L::TOTAL, 2, tmQ, tmK, tmV, s, a,
-                             status));
+  SPINF_CUDA_OK(launch_after(kern, dim3(static_cast<unsigned>(D == 256 ? sm_count() / 2 * 2 : sm_count())), dim3(CHUNK_THREADS), st, L::TOTAL,
+                             D == 256 ? 2 : 1, tmQ, tmK, tmV, s, a, status));
   SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, s, a, status));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
