@@ -891,9 +891,10 @@ static constexpr int CHUNK_ROWS = 128;  // rows per kv head from which on the ch
 
 // what a call needs: sizes of the workspace's parts in bytes (256-byte multiples)
 struct PagedSizes {
-  int64_t seq_parts, part_o, part_ml, chunk_o, chunk_ml, unit_pre, lse, scores, total;
+  int64_t seq_parts, part_o, part_ml, chunk_o, chunk_ml, joins, lse, scores, total;
   int64_t score_pitch;
   int tok_cap, chunk_rows, max_units;
+  bool too_large;
 };
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights) {
@@ -910,14 +911,16 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   z.part_o = up256(B * z.seq_parts * D * 4);
   z.part_ml = up256(B * z.seq_parts * 8);
   if (max_q > most) {
-    const int64_t tok = 256 / chunk_heads(static_cast<int>(group)), work = (max_q + tok - 1) / tok * (H / (256 / tok)) * (tiles > 0 ? tiles : 1);
+    const int hl = chunk_heads_log2(static_cast<int>(group)), tl = 8 - hl;
+    const int64_t work = ((max_q + (1 << tl) - 1) >> tl) * (H >> hl) * (tiles > 0 ? tiles : 1);
+    if (work >= (1ll << 31)) z.too_large = true;  // the chunk kernels count (item, key tile) pairs in 32 bits
     int64_t units = work / CHUNK_MIN_TILES;
     units = units < 1 ? 1 : units > chunk_units_of(D) ? chunk_units_of(D) : units;
     const int64_t seqs = n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
     z.max_units = static_cast<int>(seqs * units);
     z.chunk_o = up256(seqs * units * 512 * D * 4);
     z.chunk_ml = up256(seqs * units * 512 * 8);
-    z.unit_pre = up256((B + 1) * 4);
+    z.joins = up256(seqs * units * static_cast<int64_t>(sizeof(ChunkJoin)) + 16);
   }
   if (weights) {
     z.lse = up256(n * H * 4);
@@ -925,7 +928,7 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
     z.tok_cap = static_cast<int>(max_q < most ? max_q : most);
     z.scores = up256(B * z.tok_cap * H * z.score_pitch * 4);
   }
-  z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.unit_pre + z.lse + z.scores;
+  z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.joins + z.lse + z.scores;
   return z;
 }
 
@@ -970,7 +973,8 @@ using namespace spinf;
 extern "C" int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
                                                          int32_t weights) {
   if (n < 0 || B < 0 || B > PG_MAX_SEQS || H <= 0 || Hkv <= 0 || H % Hkv || (D != 128 && D != 256) || max_q < 0 || max_len < 0) return SPINF_ERR_BAD_ARGUMENT;
-  return paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0).total;
+  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0);
+  return z.too_large ? SPINF_ERR_TOO_LARGE : z.total;
 }
 
 extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* k_pages,
@@ -991,6 +995,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
   const int64_t mq = max_q < n ? max_q : n;
   const PagedSizes z = paged_sizes(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr);
+  if (z.too_large) return SPINF_ERR_TOO_LARGE;
   SPINF_CHECK_ARG(z.total == 0 || (workspace && workspace_bytes >= z.total && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0));
   int dev = 0;
   SPINF_CUDA_OK(cudaGetDevice(&dev));
@@ -1018,6 +1023,8 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.D = D;
   a.group = H / Hkv;
   a.window = window;
+  a.hp_log2 = chunk_heads_log2(a.group);
+  a.sets = a.group >> a.hp_log2;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.seq_parts = z.seq_parts;
   a.chunk_rows = z.chunk_rows;
@@ -1031,7 +1038,8 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.part_ml = reinterpret_cast<float2*>(take(z.part_ml));
   a.chunk_o = reinterpret_cast<float*>(take(z.chunk_o));
   a.chunk_ml = reinterpret_cast<float2*>(take(z.chunk_ml));
-  a.unit_pre = reinterpret_cast<int32_t*>(take(z.unit_pre));
+  a.n_units = reinterpret_cast<int32_t*>(take(z.joins));
+  a.joins = reinterpret_cast<ChunkJoin*>(a.n_units + 4);
   if (weights_out) {
     a.lse = reinterpret_cast<float*>(take(z.lse));
     a.scores = reinterpret_cast<float*>(take(z.scores));

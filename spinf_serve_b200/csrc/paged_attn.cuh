@@ -5,22 +5,26 @@
 
 namespace spinf {
 
+struct ChunkJoin;
+
 struct PagedAttnArgs {
   const __nv_bfloat16* q;
   int64_t q_pitch;
   __nv_bfloat16* out;
   int64_t out_pitch;
   int H, h, D, group, window;
+  int hp_log2, sets;  // chunk kernels: heads of an item, items of a kv head and token tile
   float scale_log2;
   int chunk_rows;  // sequences with more query rows per kv head than this are the chunk kernel's
   // split keys, few rows: part_o [B][seq_parts][D], part_ml [B][seq_parts] (maximum in log2 units, sum)
   float* part_o;
   float2* part_ml;
   int64_t seq_parts;
-  // cut items of the chunk kernel: 256 rows twice per unit; unit_pre [B + 1] the sequences' first units
+  // cut items of the chunk kernel: 256 rows twice per unit, and what to join
   float* chunk_o;
   float2* chunk_ml;
-  int32_t* unit_pre;
+  ChunkJoin* joins;  // [max_units]
+  int32_t* n_units;
   int max_units;  // units there is room for
   float* lse;     // [n][H] log2 units, or null: what the weights are normalised with
   float* scores;  // [B][tok_cap][H][score_pitch] log2 units, or null: kept for the weights
@@ -53,52 +57,64 @@ __device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnA
 __host__ __device__ constexpr int chunk_units_of(int D) { return D == 256 ? PG_SMS / 2 : PG_SMS; }
 static constexpr int CHUNK_MIN_TILES = 8;       // least (item, tile) pairs of a unit: below that a cut costs more than it spreads
 
-// heads of an item: the largest power of two that divides the group, at most 8 (16 rows of a head in one CTA); more heads per item
-// mean fewer tokens, so less of the causal triangle is padding
-__host__ __device__ constexpr int chunk_heads(int group) { return group % 8 == 0 ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1; }
+// heads of an item, as a power of two: the largest that divides the group, at most 8 (16 rows of a head in one tile); more heads per
+// item mean fewer tokens, so less of the causal triangle is padding
+__host__ __device__ constexpr int chunk_heads_log2(int group) { return group % 8 == 0 ? 3 : group % 4 == 0 ? 2 : group % 2 == 0 ? 1 : 0; }
 
 struct ChunkCut {
-  int hp, tok, ntt, per_tt;  // heads and tokens of an item, token tiles, items of a token tile
-  int64_t work;              // (item, key tile) pairs
-  int units;
-  bool whole;                // units take whole items: those that begin in their range
+  int tok_log2, ntt, per_tt;  // tokens of an item, token tiles, items of a token tile
+  int work;                   // (item, key tile) pairs
+  int units, quot, rem;       // unit u takes quot pairs, the first `rem` units one more
+  bool whole;                 // units take whole items: those that begin in their range
 
   __device__ __forceinline__ void slots(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& lo, int& hi) const {
-    const int base = q.len - q.nq, first = base + tt * tok, end = (tt + 1) * tok < q.nq ? (tt + 1) * tok : q.nq;
+    const int base = q.len - q.nq, first = base + (tt << tok_log2);
+    const int end = (tt + 1) << tok_log2 < q.nq ? base + ((tt + 1) << tok_log2) : q.len;
     lo = a.window > 0 && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
-    hi = base + end > 0 ? base + end : 0;
+    hi = end > 0 ? end : 0;
   }
   // key tiles [t0, t0 + nt) of a token tile; one (fully masked) where nothing is seen, so that its rows are written
   __device__ __forceinline__ void tiles(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& t0, int& nt) const {
     int lo, hi;
     slots(q, a, tt, lo, hi);
-    t0 = lo / PG_TILE;
-    nt = (hi + PG_TILE - 1) / PG_TILE - t0;
+    t0 = lo >> 7;
+    nt = ((hi + PG_TILE - 1) >> 7) - t0;
     nt = nt > 0 ? nt : 1;
   }
-  __device__ __forceinline__ int64_t begin(int u) const { return work * u / units; }
-  __device__ __forceinline__ int unit_of(int64_t w) const { return static_cast<int>(((w + 1) * units - 1) / work); }
+  __device__ __forceinline__ int begin(int u) const { return u * quot + (u < rem ? u : rem); }
+  __device__ __forceinline__ int unit_of(int w) const {
+    const int edge = rem * (quot + 1);
+    return w < edge ? w / (quot + 1) : rem + (w - edge) / quot;
+  }
 };
+static_assert(PG_TILE == 128, "key tiles are counted by shifts");
 __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttnArgs& a) {
   ChunkCut c;
-  c.hp = chunk_heads(a.group);
-  c.tok = 256 / c.hp;
-  c.ntt = (q.nq + c.tok - 1) / c.tok;
-  c.per_tt = a.H / c.hp;
-  c.work = 0;
+  c.tok_log2 = 8 - a.hp_log2;
+  c.ntt = (q.nq + (1 << c.tok_log2) - 1) >> c.tok_log2;
+  c.per_tt = a.H >> a.hp_log2;
+  int tiles = 0;
   for (int tt = 0; tt < c.ntt; ++tt) {
     int t0, nt;
     c.tiles(q, a, tt, t0, nt);
-    c.work += static_cast<int64_t>(nt) * c.per_tt;
+    tiles += nt;
   }
-  const int64_t u = c.work / CHUNK_MIN_TILES;
-  const int most = chunk_units_of(a.D);
-  c.units = u < 1 ? 1 : u > most ? most : static_cast<int>(u);
+  c.work = tiles * c.per_tt;  // (the host has checked that this fits)
+  const int u = c.work / CHUNK_MIN_TILES, most = chunk_units_of(a.D);
+  c.units = u < 1 ? 1 : u > most ? most : u;
+  c.quot = c.work / c.units;
+  c.rem = c.work - c.quot * c.units;
   // many short items (a window): a cut would cost about as much as the imbalance it removes
-  const int64_t items = static_cast<int64_t>(c.ntt) * c.per_tt;
-  c.whole = items >= 2 * most && c.work <= 24 * items;
+  c.whole = c.ntt * c.per_tt >= 2 * most && tiles <= 24 * c.ntt;
   return c;
 }
+
+// what the join has to do for a unit that is the first to begin inside of an item (pieces 0: nothing)
+struct alignas(16) ChunkJoin {
+  int pieces;             // partial results of the item, the first of them not the unit's own
+  int first;              // the one before (in units of 256 rows); the others are 2 it, 2 it + 2, ..
+  int row0, nq, tok0, h0;
+};
 
 // page of the `rows` slots from j on, or one past the last page (the copy then brings zeros) where no row sees any of them
 __device__ __forceinline__ int chunk_page(const PagedSeqs& s, const int32_t* pages, int j, int rows, int lo, int hi, int* status) {

@@ -62,7 +62,7 @@ __device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_add
 // a segment: consecutive key tiles of one item
 struct ChunkSeg {
   int b, row0, nq, base;  // sequence, its first row of q, its rows, the first one's slot
-  int g, h0, tok0, hp;    // kv head, first query head, first token, heads of the item
+  int g, h0, tok0;        // kv head, first query head, first token
   int ta, tb;             // key tiles (ta < 0: no more segments)
   int lo, hi;             // slots some row of the item sees
   int part;               // partial result (256 rows) to write, or -1: the segment is the whole item
@@ -74,9 +74,9 @@ struct ChunkWalk {
   PagedSeq q;
   ChunkCut c;
   int b, it;
-  int64_t w, w_end;  // (item, tile) pairs of the unit still to do
+  int w, w_end;      // (item, tile) pairs of the unit still to do
   int tt, nt, t0;    // token tile, its key tiles, the first of them
-  int64_t w_tt;      // first pair of the token tile
+  int w_tt;          // first pair of the token tile
   bool first;
 
   __device__ __forceinline__ void start(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int unit, int* status) {
@@ -88,35 +88,42 @@ struct ChunkWalk {
     w = c.begin(u);
     w_end = c.begin(u + 1);
     first = true;
-    tt = -1, w_tt = 0, nt = 0, t0 = 0;
+    tt = 0, w_tt = 0;
+    c.tiles(q, a, 0, t0, nt);
     advance(a);
-    if (c.whole) {
-      const int off = static_cast<int>((w - w_tt) % nt);
-      if (off) w += nt - off;
+    const int item = (w - w_tt) / nt, off = w - w_tt - item * nt;
+    ChunkJoin join;
+    join.pieces = 0;
+    if (off) {
+      if (c.whole) {
+        w += nt - off;
+      } else if (c.begin(u - 1) <= w - off) {  // the first unit that begins inside this item
+        const int w0 = w - off;
+        join.pieces = c.unit_of(w0 + nt - 1) - u + 2;
+        join.first = (unit - 1) * 2 + (c.begin(u - 1) < w0 ? 1 : 0);
+        join.row0 = q.row0, join.nq = q.nq;
+        join.tok0 = tt << c.tok_log2;
+        join.h0 = item / a.sets * a.group + (item % a.sets << a.hp_log2);
+      }
     }
+    a.joins[unit] = join;
   }
   // to the token tile that holds pair w
   __device__ __forceinline__ void advance(const PagedAttnArgs& a) {
-    while (w >= w_tt + static_cast<int64_t>(nt) * c.per_tt) {
-      w_tt += static_cast<int64_t>(nt) * c.per_tt;
-      ++tt;
-      if (tt >= c.ntt) return;
-      c.tiles(q, a, tt, t0, nt);
+    while (w >= w_tt + nt * c.per_tt && tt + 1 < c.ntt) {
+      w_tt += nt * c.per_tt;
+      c.tiles(q, a, ++tt, t0, nt);
     }
   }
   __device__ __forceinline__ bool next(const PagedAttnArgs& a, ChunkSeg& g) {
     if (w >= w_end) return false;
     advance(a);
-    const int64_t in = w - w_tt;
-    const int item = static_cast<int>(in / nt), off = static_cast<int>(in - static_cast<int64_t>(item) * nt);
-    const int64_t left = w_end - w;
-    const int len = !c.whole && left < nt - off ? static_cast<int>(left) : nt - off;
-    const int sets = a.group / c.hp;
+    const int item = (w - w_tt) / nt, off = w - w_tt - item * nt;
+    const int len = !c.whole && w_end - w < nt - off ? w_end - w : nt - off;
     g.b = b, g.row0 = q.row0, g.nq = q.nq, g.base = q.len - q.nq;
-    g.g = item / sets;
-    g.h0 = g.g * a.group + (item % sets) * c.hp;
-    g.tok0 = tt * c.tok;
-    g.hp = c.hp;
+    g.g = item / a.sets;
+    g.h0 = g.g * a.group + ((item - g.g * a.sets) << a.hp_log2);
+    g.tok0 = tt << c.tok_log2;
     g.ta = t0 + off;
     g.tb = g.ta + len;
     c.slots(q, a, tt, g.lo, g.hi);
@@ -158,7 +165,11 @@ struct SegPlan {
       if (k == L::PLAN && u < total) {
         __syncwarp();
         const int mine = u + lane * step;
-        if (lane < L::PLAN && mine < total) reinterpret_cast<ChunkWalk*>(plan + lane * 128)->start(s, a, pre, mine, status);
+        if (lane < L::PLAN && mine < total) {
+          ChunkWalk wk;
+          wk.start(s, a, pre, mine, status);
+          *reinterpret_cast<ChunkWalk*>(plan + lane * 128) = wk;
+        }
         __syncwarp();
         k = 0;
       }
@@ -167,7 +178,12 @@ struct SegPlan {
       if (lane == 0) {
         ChunkSeg g;
         g.ta = -1;
-        put = !have || reinterpret_cast<ChunkWalk*>(plan + k * 128)->next(a, g) ? 1 : 2;
+        put = 1;
+        if (have) {
+          ChunkWalk wk = *reinterpret_cast<const ChunkWalk*>(plan + k * 128);
+          put = wk.next(a, g) ? 1 : 2;
+          *reinterpret_cast<ChunkWalk*>(plan + k * 128) = wk;
+        }
         if (put == 1) {
           if (mbar_wait(wc, &ring.empty[n % L::SEGS], ((n / L::SEGS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) {
             *reinterpret_cast<ChunkSeg*>(reinterpret_cast<uint8_t*>(ring.slots) + (n % L::SEGS) * 64) = g;
@@ -241,8 +257,8 @@ __device__ __forceinline__ void store_lines(const uint32_t (&w)[32], uint8_t* st
 template <int D, int COLS, class Free>
 __device__ __forceinline__ void chunk_store(const PagedAttnArgs& a, const ChunkSeg& g, uint32_t taddr, int d0, int tile, int qd, int lane, float inv,
                                             uint8_t* stage, Free free_o) {
-  const int qrows = 128 / g.hp;
-  auto tok_of = [&](int r) { return g.tok0 + tile * qrows + (qd * 32 + r) % qrows; };
+  const int ql = 7 - a.hp_log2;  // log2 of a head's rows in a tile
+  auto tok_of = [&](int r) { return g.tok0 + (tile << ql) + ((qd * 32 + r) & ((1 << ql) - 1)); };
   if (g.part < 0) {
 #pragma unroll 1
     for (int c = 0; c < COLS; c += 64) {
@@ -257,7 +273,7 @@ __device__ __forceinline__ void chunk_store(const PagedAttnArgs& a, const ChunkS
         for (int y = 0; y < 16; ++y) w[x * 16 + y] = pack_bf16x2(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
       }
       store_lines(w, stage, lane, [&](int r) -> uint8_t* {
-        const int tok = tok_of(r), head = g.h0 + (qd * 32 + r) / qrows;
+        const int tok = tok_of(r), head = g.h0 + ((qd * 32 + r) >> ql);
         if (tok >= g.nq) return nullptr;
         return reinterpret_cast<uint8_t*>(a.out + static_cast<int64_t>(g.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D + d0 + c);
       });
@@ -345,7 +361,7 @@ __device__ __forceinline__ void chunk_clear(uint8_t* v, int slabs, int t, const 
 }
 __device__ __forceinline__ bool chunk_edge(const ChunkSeg& g, int t) { return t * PG_TILE < g.lo || (t + 1) * PG_TILE > g.hi; }
 
-// unit counts of the sequences, and where the join finds them
+// unit counts of the sequences, and for the join their sum
 __device__ __forceinline__ int chunk_units(const PagedSeqs& s, const PagedAttnArgs& a, int* pre, int* status) {
   paged_item_prefix(s.B, pre, CHUNK_THREADS, [&](int b) {
     const PagedSeq q = paged_seq(s, b, status);
@@ -356,8 +372,7 @@ __device__ __forceinline__ int chunk_units(const PagedSeqs& s, const PagedAttnAr
     total = a.max_units;
     atomicCAS(status, 0, ST_BAD_INDEX);
   }
-  if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b <= s.B; b += CHUNK_THREADS) a.unit_pre[b] = pre[b];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_units = total;
   return total;
 }
 
@@ -487,8 +502,8 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = mbar_wait(wc, q_empty, (seg_n & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
         if (ok) {
           if (rank == 0) mbar_expect_tx(q_full, 2 * L::Q_BYTES);
-          const int qrows = 128 / g.hp, row = g.row0 + g.tok0 + static_cast<int>(rank) * qrows;
-          for (int hh = 0; hh < g.hp; ++hh)
+          const int qrows = 128 >> a.hp_log2, row = g.row0 + g.tok0 + static_cast<int>(rank) * qrows;
+          for (int hh = 0; hh < 1 << a.hp_log2; ++hh)
             for (int x = 0; x < SLABS; ++x)
               tma_load_2d_pair(smem + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, row, map_to_cta(q_full, 0));
         }
@@ -611,9 +626,9 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     while (__all_sync(0xffffffffu, ring.next(wc, g))) {
       __syncwarp();
       if (lane == 0) ring.done(); else ++ring.n;
-      const int n_tiles = g.tb - g.ta, qrows = 128 / g.hp;
-      const int head = g.h0 + row / qrows;
-      const int tok_first = g.tok0 + static_cast<int>(rank) * qrows, tok = tok_first + row % qrows;
+      const int n_tiles = g.tb - g.ta, qrows = 128 >> a.hp_log2;
+      const int head = g.h0 + (row >> (7 - a.hp_log2));
+      const int tok_first = g.tok0 + static_cast<int>(rank) * qrows, tok = tok_first + (row & (qrows - 1));
       const int hi = g.base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;  // slots the row sees
       const int hi_min = g.base + tok_first, lo_max = a.window > 0 ? hi_min + qrows - a.window : 0;
       float m_ref = -INFINITY, l_run = 0.f;
@@ -771,9 +786,9 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ok = mbar_wait(wc, q_empty, (seg_n & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
         if (ok) {
           mbar_expect_tx(q_full, L::Q_BYTES);
-          const int qrows = 128 / g.hp;
+          const int qrows = 128 >> a.hp_log2;
           for (int tile = 0; tile < 2; ++tile)
-            for (int hh = 0; hh < g.hp; ++hh)
+            for (int hh = 0; hh < 1 << a.hp_log2; ++hh)
               for (int x = 0; x < SLABS; ++x)
                 tma_load_2d(smem + tile * (L::Q_BYTES / 2) + x * 128 * 128 + hh * qrows * 128, &tmQ, (g.h0 + hh) * D + x * 64, g.row0 + g.tok0 + tile * qrows, q_full);
         }
@@ -890,9 +905,9 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     while (alive && __all_sync(0xffffffffu, ring.next(wc, g))) {
       __syncwarp();
       if (lane == 0) ring.done(); else ++ring.n;
-      const int n_tiles = g.tb - g.ta, qrows = 128 / g.hp;
-      const int head = g.h0 + row / qrows;
-      const int tok_first = g.tok0 + tile * qrows, tok = tok_first + row % qrows;
+      const int n_tiles = g.tb - g.ta, qrows = 128 >> a.hp_log2;
+      const int head = g.h0 + (row >> (7 - a.hp_log2));
+      const int tok_first = g.tok0 + tile * qrows, tok = tok_first + (row & (qrows - 1));
       const int hi = g.base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;
       const int hi_min = g.base + tok_first, lo_max = a.window > 0 ? hi_min + qrows - a.window : 0;
       float m_ref = -INFINITY, l_run = 0.f;
@@ -962,49 +977,32 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 // ---------------------------------------------------------------- join of the cut items
-// CTAs (it, y): the item that unit `it` begins inside of, if this is the first unit that does; 64 of its 256 rows, a warp per row, the
-// pieces added in the order of the units
+// CTAs (it, y): the item that unit `it` is the first to begin inside of, as the planning warps have left word; 64 of its 256 rows, a
+// warp per row, the pieces added in the order of the units
 template <int D>
-__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
+__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedAttnArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int V = D / 128;  // float4 per lane
   const int it = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (it >= a.unit_pre[s.B] || it >= a.max_units) return;
-  const int b = paged_find(a.unit_pre, s.B, it);
-  const int u = it - a.unit_pre[b];
-  if (u == 0) return;
-  const PagedSeq q = paged_seq(s, b, status);
-  const ChunkCut c = chunk_cut(q, a);
-  if (c.whole) return;
-  const int64_t w = c.begin(u);
-  int64_t w_tt = 0;
-  int tt = 0, t0, nt;
-  c.tiles(q, a, 0, t0, nt);
-  while (w >= w_tt + static_cast<int64_t>(nt) * c.per_tt) {
-    w_tt += static_cast<int64_t>(nt) * c.per_tt;
-    c.tiles(q, a, ++tt, t0, nt);
-  }
-  const int item = static_cast<int>((w - w_tt) / nt);
-  const int64_t w0 = w_tt + static_cast<int64_t>(item) * nt;
-  if (w == w0 || c.begin(u - 1) > w0) return;  // the unit begins with an item, or an earlier one has cut it
-  const int u1 = c.unit_of(w0 + nt - 1);
-  if (it - u + u1 >= a.max_units) return;
-  const int sets = a.group / c.hp, qrows = 128 / c.hp;
-  const int h0 = item / sets * a.group + item % sets * c.hp;
-  const int64_t first = (static_cast<int64_t>(it - 1) * 2 + (c.begin(u - 1) < w0 ? 1 : 0)) * 256;  // the piece at the end of the unit before, or all of it
+  const int total = *a.n_units;
+  const ChunkJoin join = a.joins[it];  // (read with the count, used only below it)
+  if (it >= total || join.pieces == 0) return;
+  const int last = it + join.pieces - 2 < a.max_units ? join.pieces - 2 : a.max_units - 1 - it;
+  const int ql = 7 - a.hp_log2;
+  const int64_t first = static_cast<int64_t>(join.first) * 256;
   for (int r = blockIdx.y * 64 + warp; r < blockIdx.y * 64 + 64; r += 8) {
-    const int in = r & 127, tok = tt * c.tok + (r >> 7) * qrows + in % qrows, head = h0 + in / qrows;
-    if (tok >= q.nq) continue;
+    const int in = r & 127, tok = join.tok0 + ((r >> 7) << ql) + (in & ((1 << ql) - 1)), head = join.h0 + (in >> ql);
+    if (tok >= join.nq) continue;
     const int64_t at0 = first + r, at = static_cast<int64_t>(it) * 512 + r;  // further pieces: 512 rows apart
     float m = a.chunk_ml[at0].x;
-    for (int y = 0; y <= u1 - u; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
+    for (int y = 0; y <= last; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
     const float neg_m = m == -INFINITY ? 0.f : -m;
     float l = 0.f;
     float4 acc[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int y = -1; y <= u1 - u; ++y) {
+    for (int y = -1; y <= last; ++y) {
       const int64_t from = y < 0 ? at0 : at + y * 512;
       const float2 ml = a.chunk_ml[from];
       const float f = fast_exp2(ml.x + neg_m);
@@ -1017,12 +1015,12 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s
       }
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    __nv_bfloat16* dst = a.out + (q.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D;
+    __nv_bfloat16* dst = a.out + (join.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D;
 #pragma unroll
     for (int v = 0; v < V; ++v)
       *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
           make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv), pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
-    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + head] = m + log2f(l);
+    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(join.row0 + tok) * a.H + head] = m + log2f(l);
   }
 }
 
@@ -1062,9 +1060,9 @@ __device__ __forceinline__ ChunkWeightItem chunk_weight_item(const PagedSeqs& s,
   const int x = it - pre[w.b];
   w.g = x % a.h;
   w.j0 = x / a.h * 256;
-  w.hp = chunk_heads(a.group);
-  w.tok = 64 / w.hp;
-  w.sets = a.group / w.hp;
+  w.hp = 1 << a.hp_log2;
+  w.tok = 64 >> a.hp_log2;
+  w.sets = a.sets;
   const int base = w.q.len - w.q.nq;
   const int first = w.j0 > base ? w.j0 - base : 0;  // tokens before it sit before every key
   int end = w.q.nq;
@@ -1274,7 +1272,7 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
                         cudaStream_t st, int dev, int* status) {
   using L = ChunkSmem<D>;
   CUtensorMap tmQ, tmK, tmV;
-  const int hp = chunk_heads(a.group);
+  const int hp = 1 << a.hp_log2;
   int r;
   const uint32_t krows = kp.page < CH_KH ? static_cast<uint32_t>(kp.page) : static_cast<uint32_t>(CH_KH);
   const uint32_t vrows = kp.page < PG_TILE ? static_cast<uint32_t>(kp.page) : static_cast<uint32_t>(PG_TILE);
@@ -1293,7 +1291,7 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   }
   SPINF_CUDA_OK(launch_after(kern, dim3(static_cast<unsigned>(D == 256 ? sm_count() / 2 * 2 : sm_count())), dim3(CHUNK_THREADS), st, L::TOTAL,
                              D == 256 ? 2 : 1, tmQ, tmK, tmV, s, a, status));
-  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, s, a, status));
+  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, a));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
   if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;
