@@ -529,7 +529,7 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NST; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);  // a 64-key stage is four 16-key pieces
+      mbar_init(&empty[i], SW);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
@@ -601,13 +601,21 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         m_run[n][0] = m_run[n][1] = -INFINITY;
         l_run[n][0] = l_run[n][1] = 0.f;
       }
-      const int pieces = 4 * (w.u1 - w.u0);
-      for (int p = warp; p < pieces && ok; p += SW) {
-        const int u = p >> 2, key0 = (p & 3) * 16;
+      // A unit is four pieces of 16 keys, piece after piece to the warps in turn. Every warp waits for every stage and lets it go, also
+      // where it has no piece: a barrier's parity tells a phase only from its neighbours, so no warp may be a phase ahead of one.
+      const int units = w.u1 - w.u0;
+      int turn = warp;  // pieces from the unit's first on to this warp's next
+      for (int u = 0; u < units && ok; ++u, turn = turn < 4 ? turn + SW - 4 : turn - 4) {
         const uint32_t ck = cnt0 + 2 * u, stk = ck % L::NST, stv = (ck + 1) % L::NST;
-        const int j0 = (w.u0 + u) * 64 + key0;
         ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stk], (ck / L::NST) & 1u, ST_TIMEOUT_FULL));
         if (!ok) break;
+        if (turn >= 4) {
+          if (lane == 0) mbar_arrive(&empty[stk]);
+          ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stv], ((ck + 1) / L::NST) & 1u, ST_TIMEOUT_FULL));
+          if (ok && lane == 0) mbar_arrive(&empty[stv]);
+          continue;
+        }
+        const int key0 = turn * 16, j0 = (w.u0 + u) * 64 + key0;
         float sc[2][NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)

@@ -94,6 +94,7 @@ __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttn
   c.ntt = (q.nq + (1 << c.tok_log2) - 1) >> c.tok_log2;
   c.per_tt = a.H >> a.hp_log2;
   int tiles = 0;
+#pragma unroll 1
   for (int tt = 0; tt < c.ntt; ++tt) {
     int t0, nt;
     c.tiles(q, a, tt, t0, nt);

@@ -110,6 +110,7 @@ struct ChunkWalk {
   }
   // to the token tile that holds pair w
   __device__ __forceinline__ void advance(const PagedAttnArgs& a) {
+#pragma unroll 1
     while (w >= w_tt + nt * c.per_tt && tt + 1 < c.ntt) {
       w_tt += nt * c.per_tt;
       c.tiles(q, a, ++tt, t0, nt);
@@ -229,67 +230,55 @@ struct PageRun {
   }
 };
 
-// 128 bytes of each of the warp's 32 rows (row = lane, words w) to global memory through 2 KB of shared memory, 16 rows at a time: a
-// store instruction then covers whole 128-byte lines of four rows instead of 16 bytes of 32 rows (15 000 -> cycles per segment).
-// dst(r): where row r's bytes go, or null.
-template <class Dst>
-__device__ __forceinline__ void store_lines(const uint32_t (&w)[32], uint8_t* stage, int lane, Dst dst) {
-  uint4* st = reinterpret_cast<uint4*>(stage);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    __syncwarp();
-    if ((lane >> 4) == h) {
-#pragma unroll
-      for (int x = 0; x < 8; ++x) st[(lane & 15) * 8 + (x ^ (lane & 7))] = make_uint4(w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = k * 4 + (lane >> 3), ch = lane & 7;
-      uint8_t* to = dst(h * 16 + r);
-      if (to) *reinterpret_cast<uint4*>(to + ch * 16) = st[r * 8 + (ch ^ (r & 7))];
-    }
-  }
-}
-
 // O of 128 rows x COLS columns from tensor memory (from column `taddr`, head dimensions from d0 on): divided by the sums and rounded to
-// the output, or in fp32 to the segment's partial result. `free_o` is called when the last column is in registers.
+// the output, or in fp32 to the segment's partial result. `free_o` is called when the last column is in registers. A warp's 32 rows go
+// through 2 KB of shared memory, so that a store instruction covers whole sectors side by side (8 rows x 64 bytes, 4 rows x 128 bytes)
+// instead of 16 bytes of 32 rows. The loops stay rolled: this runs once a segment, and code that is not in the instruction cache
+// costs more than the loop.
 template <int D, int COLS, class Free>
 __device__ __forceinline__ void chunk_store(const PagedAttnArgs& a, const ChunkSeg& g, uint32_t taddr, int d0, int tile, int qd, int lane, float inv,
                                             uint8_t* stage, Free free_o) {
   const int ql = 7 - a.hp_log2;  // log2 of a head's rows in a tile
-  auto tok_of = [&](int r) { return g.tok0 + (tile << ql) + ((qd * 32 + r) & ((1 << ql) - 1)); };
-  if (g.part < 0) {
+  uint4* st = reinterpret_cast<uint4*>(stage);
 #pragma unroll 1
-    for (int c = 0; c < COLS; c += 64) {
-      uint32_t o[32], w[32];
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    tmem_ld_x32(taddr + c, o);
+    tmem_wait_ld();
+    if (c + 32 >= COLS) free_o();
+    if (g.part < 0) {  // 64 bytes of every row
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        __syncwarp();
-        tmem_ld_x32(taddr + c + x * 32, o);
-        tmem_wait_ld();
-        if (x == 1 && c + 64 >= COLS) free_o();
-#pragma unroll
-        for (int y = 0; y < 16; ++y) w[x * 16 + y] = pack_bf16x2(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
-      }
-      store_lines(w, stage, lane, [&](int r) -> uint8_t* {
-        const int tok = tok_of(r), head = g.h0 + ((qd * 32 + r) >> ql);
-        if (tok >= g.nq) return nullptr;
-        return reinterpret_cast<uint8_t*>(a.out + static_cast<int64_t>(g.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D + d0 + c);
-      });
-    }
-  } else {
-#pragma unroll 1
-    for (int c = 0; c < COLS; c += 32) {
-      uint32_t o[32];
+      for (int x = 0; x < 4; ++x)
+        st[lane * 4 + (x ^ ((lane >> 1) & 3))] =
+            make_uint4(pack_bf16x2(__uint_as_float(o[8 * x]) * inv, __uint_as_float(o[8 * x + 1]) * inv),
+                       pack_bf16x2(__uint_as_float(o[8 * x + 2]) * inv, __uint_as_float(o[8 * x + 3]) * inv),
+                       pack_bf16x2(__uint_as_float(o[8 * x + 4]) * inv, __uint_as_float(o[8 * x + 5]) * inv),
+                       pack_bf16x2(__uint_as_float(o[8 * x + 6]) * inv, __uint_as_float(o[8 * x + 7]) * inv));
       __syncwarp();
-      tmem_ld_x32(taddr + c, o);
-      tmem_wait_ld();
-      if (c + 32 >= COLS) free_o();
-      store_lines(o, stage, lane, [&](int r) -> uint8_t* {
-        if (tok_of(r) >= g.nq) return nullptr;
-        return reinterpret_cast<uint8_t*>(a.chunk_o + (static_cast<int64_t>(g.part) * 256 + tile * 128 + qd * 32 + r) * D + d0 + c);
-      });
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        const int r = k * 8 + (lane >> 2), ch = lane & 3, rr = qd * 32 + r;
+        const int tok = g.tok0 + (tile << ql) + (rr & ((1 << ql) - 1)), head = g.h0 + (rr >> ql);
+        if (tok < g.nq)
+          *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(g.row0 + tok) * a.out_pitch + head * D + d0 + c + ch * 8) = st[r * 4 + (ch ^ ((r >> 1) & 3))];
+      }
+    } else {  // 128 bytes of every row, 16 rows at a time
+      float* to = a.chunk_o + (static_cast<int64_t>(g.part) * 256 + tile * 128 + qd * 32) * D + d0 + c;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if ((lane >> 4) == h) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) st[(lane & 15) * 8 + (x ^ (lane & 7))] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = k * 4 + (lane >> 3), ch = lane & 7;
+          *reinterpret_cast<uint4*>(to + (h * 16 + r) * D + ch * 4) = st[r * 8 + (ch ^ (r & 7))];
+        }
+        __syncwarp();
+      }
     }
   }
 }
@@ -338,6 +327,58 @@ __device__ __forceinline__ float chunk_probs(const float (&sc)[64], float scale_
   }
   return sum0 + sum1;
 }
+// the same over the 128 scores of a row, 32 at a time
+__device__ __forceinline__ uint32_t slot_bits(int jb, int lo, int hi) {  // which of the 32 slots from jb on lie in [lo, hi]
+  uint32_t bits = hi < jb ? 0u : hi - jb >= 31 ? ~0u : (2u << (hi - jb)) - 1u;
+  if (lo > jb) bits &= lo - jb > 31 ? 0u : ~0u << (lo - jb);
+  return bits;
+}
+__device__ __forceinline__ float chunk_row_max(uint32_t taddr, bool masked, int jb, int lo, int hi) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int x = 0; x < 4; ++x) {
+    uint32_t v[32];
+    tmem_ld_x32(taddr + x * 32, v);
+    tmem_wait_ld();
+    const uint32_t bits = masked ? slot_bits(jb + x * 32, lo, hi) : ~0u;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) m[c & 3] = fmaxf(m[c & 3], (bits & (1u << c)) ? __uint_as_float(v[c]) : -INFINITY);
+  }
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+__device__ __forceinline__ float chunk_row_probs(uint32_t taddr, bool masked, int jb, int lo, int hi, float scale_log2, float neg_m, uint32_t (&pk)[64],
+                                                 float& sum) {
+  float m[2] = {-INFINITY, -INFINITY}, s[2] = {0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    uint32_t u[32];
+    tmem_ld_x32(taddr + x * 32, u);
+    tmem_wait_ld();
+    if (masked) {
+      const uint32_t bits = slot_bits(jb + x * 32, lo, hi);
+#pragma unroll
+      for (int c = 0; c < 32; ++c) u[c] = (bits & (1u << c)) ? u[c] : 0xff800000u;  // -inf
+    }
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const float s0 = __uint_as_float(u[2 * c]), s1 = __uint_as_float(u[2 * c + 1]);
+      m[0] = fmaxf(m[0], s0);
+      m[1] = fmaxf(m[1], s1);
+      const float p0 = fast_exp2(fmaf(s0, scale_log2, neg_m)), p1 = fast_exp2(fmaf(s1, scale_log2, neg_m));
+      s[0] += p0;
+      s[1] += p1;
+      pk[x * 16 + c] = pack_bf16x2(p0, p1);
+    }
+  }
+  sum = s[0] + s[1];
+  return fmaxf(m[0], m[1]);
+}
+__device__ __forceinline__ void tmem_st_x64(uint32_t taddr, const uint32_t (&r)[64]) {
+  const uint32_t (&lo)[32] = *reinterpret_cast<const uint32_t (*)[32]>(&r[0]);
+  const uint32_t (&hi)[32] = *reinterpret_cast<const uint32_t (*)[32]>(&r[32]);
+  tmem_st_x32(taddr, lo);
+  tmem_st_x32(taddr + 32, hi);
+}
 // COLS columns of O times alpha, in tensor memory
 template <int COLS>
 __device__ __forceinline__ void chunk_rescale(uint32_t taddr, float alpha) {
@@ -381,10 +422,10 @@ __device__ __forceinline__ int chunk_units(const PagedSeqs& s, const PagedAttnAr
 //   warp 1      owns tensor memory; the leader's lane issues S = Q K^T (M = 256) into one of two buffers and O += P V; S of tile t + 1
 //               before P V of tile t. A queued product blocks its issue slot until the pipe takes it, so whatever can be waited for
 //               earlier is (V before S), and a product's one commit serves the softmax and the copies: S done = its K stage free
-//   warps 2-9   softmax: thread = row, group A the first 64 keys of the tile, group B the others; maxima exchanged in shared memory
-//   warp 10     TMA loads of Q and of this CTA's half of V's dimensions (all 128 keys)
-//   warp 11     in a tile with slots that no row of the item sees (a page's end, the front of a window) it waits for the copy of V
-//               and clears those rows, while warp 10 goes on: P is 0 there, but 0 * inf is not. It also plans the segments
+//   warps 4-11  softmax: thread = row, group A the first 64 keys of the tile, group B the others; maxima exchanged in shared memory
+//   warp 2      TMA loads of Q and of this CTA's half of V's dimensions (all 128 keys)
+//   warp 3      in a tile with slots that no row of the item sees (a page's end, the front of a window) it waits for the copy of V
+//               and clears those rows, while warp 2 goes on: P is 0 there, but 0 * inf is not. It also plans the segments
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
@@ -487,7 +528,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == 2) {
     const int rl = s.page_log2 < 7 ? s.page_log2 : 7, rows = 1 << rl;  // rows of a V box
     uint32_t cnt = 0, seg_n = 0;
     bool ok = true;
@@ -542,7 +583,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       }
     }
-  } else if (warp == 11) {
+  } else if (warp == 3) {
     uint32_t cnt = 0, edges[NS];  // boundary tiles each stage has held
 #pragma unroll
     for (int i = 0; i < NS; ++i) edges[i] = 0;
@@ -616,11 +657,11 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     }
   } else {
-    const int wg = (warp - 2) >> 2;
+    const int wg = (warp - 4) >> 2;
     const int qd = warp & 3;  // TMEM lane quarter of this warp
     const int row = qd * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(qd * 32) << 16;
-    uint8_t* stage = smem + L::OUT_OFF + (warp - 2) * 2048;
+    uint8_t* stage = smem + L::OUT_OFF + (warp - 4) * 2048;
     const uint32_t p_bar = map_to_cta(p_ready, 0), free_bar = map_to_cta(o_free, 0);
     uint32_t gt = 0;
     while (__all_sync(0xffffffffu, ring.next(wc, g))) {
@@ -767,7 +808,7 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   SegRing<L> ring{reinterpret_cast<ChunkSeg*>(smem + L::SEG_OFF), seg_full, seg_empty, 0};
   ChunkSeg g;
 
-  if (warp == 0 || warp == 10) {
+  if (warp == 0 || warp == 2) {
     const bool is_k = warp == 0;
     const int rl = s.page_log2 < 7 ? s.page_log2 : 7, rows = 1 << rl;  // rows of a box
     uint64_t* full = is_k ? k_full : v_full;
@@ -819,7 +860,7 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % NS], (c / NS) & 1u); ++spin) {}
       for (int spin = 0; !is_k && seg_n && spin < 4096 && !mbar_try_wait(q_full, (seg_n - 1) & 1u); ++spin) {}
     }
-  } else if (warp == 11) {
+  } else if (warp == 3) {
     uint32_t cnt = 0, edges[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) edges[i] = 0;
@@ -884,7 +925,7 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 8; ++k)  // packed bf16 P: 16 keys per 8 columns
-              umma_f16_ts(tmem_base + L::O_COL + tile * D, tmem_base + tile * 128 + (k >> 2) * CH_KH + 8 * (k & 3), vd + 128 * k, IDESC_O, (i | k) != 0);
+              umma_f16_ts(tmem_base + L::O_COL + tile * D, tmem_base + tile * 128 + 8 * k, vd + 128 * k, IDESC_O, (i | k) != 0);
             umma_commit(&o_done[tile * NS + st]);
             if (more) issue_s(tile, gi + 1);
           }
@@ -894,11 +935,11 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
     }
   } else {
-    const int tile = (warp - 2) >> 2;
+    const int tile = (warp - 4) >> 2;
     const int qd = warp & 3;
     const int row = qd * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(qd * 32) << 16;
-    uint8_t* stage = smem + L::OUT_OFF + (warp - 2) * 2048;
+    uint8_t* stage = smem + L::OUT_OFF + (warp - 4) * 2048;
     const uint32_t s_tmem = tmem_base + lane_off + tile * 128, o_tmem = tmem_base + lane_off + L::O_COL + tile * D;
     uint32_t gt = 0;
     bool alive = true;
@@ -918,18 +959,27 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!alive) break;
         tc_fence_after();
         const bool masked = jb + PG_TILE - 1 > hi_min || jb < lo_max;
-        float sc[CH_KH];
-        // the maximum first; the second half's scores stay in registers, the first half's are read again (128 at once would spill)
-        chunk_scores(sc, s_tmem, masked, jb, lo, hi);
-        float mx = chunk_max(sc);
-        chunk_scores(sc, s_tmem + CH_KH, masked, jb + CH_KH, lo, hi);
-        mx = fmaxf(mx, chunk_max(sc)) * a.scale_log2;
-        float alpha = 1.f;
-        if (mx - m_ref > CH_RESCALE) {  // false for NaN (-inf minus -inf): a row that has seen nothing yet
-          alpha = fast_exp2(m_ref - mx);
+        // p against the reference maximum as it stands, the tile's own maximum found on the way: no pass over the scores before the
+        // exponentials. Only where a row outgrew the threshold (or has no maximum yet) is the tile done again.
+        uint32_t pk[PG_TILE / 2];
+        float alpha = 1.f, sum = 0.f;
+        bool again = i == 0;
+        if (again) {
+          const float mx = chunk_row_max(s_tmem, masked, jb, lo, hi) * a.scale_log2;
           m_ref = mx;
         }
-        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+#pragma unroll 1
+        for (;;) {
+          const float mx = chunk_row_probs(s_tmem, masked, jb, lo, hi, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref, pk, sum) * a.scale_log2;
+          const bool grown = !again && mx - m_ref > CH_RESCALE;  // false for NaN (-inf minus -inf): a row that has seen nothing yet
+          if (!__any_sync(0xffffffffu, grown)) break;
+          if (grown) {
+            alpha = fast_exp2(m_ref - mx);
+            m_ref = mx;
+          }
+          again = true;
+        }
+        l_run = l_run * alpha + sum;
         if (i > 0) {
           const bool done = mbar_wait(wc, &o_done[tile * NS + (gi - 1) % NS], ((gi - 1) / NS) & 1u, ST_TIMEOUT_TMEM);
           if (__any_sync(0xffffffffu, alpha != 1.f) && __all_sync(0xffffffffu, done)) {
@@ -937,15 +987,8 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             chunk_rescale<D>(o_tmem, alpha);
           }
         }
-        uint32_t pk[CH_KH / 2];
-        float sum = chunk_probs(sc, a.scale_log2, neg_m, pk);
         __syncwarp();
-        tmem_st_x32(s_tmem + CH_KH, pk);  // P of keys 64 .. 127 over their own scores
-        chunk_scores(sc, s_tmem, masked, jb, lo, hi);
-        sum += chunk_probs(sc, a.scale_log2, neg_m, pk);
-        l_run = l_run * alpha + sum;
-        __syncwarp();
-        tmem_st_x32(s_tmem, pk);
+        tmem_st_x64(s_tmem, pk);  // P over the first half of the scores' columns
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();

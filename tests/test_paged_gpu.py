@@ -201,6 +201,33 @@ def test_chunks_keep_the_slots_weights(dev, H, h, D, page, window):
         assert torch.equal(on[b, :, L:].cpu(), w[b, :, L:])
 
 
+@pytest.mark.parametrize("H,h,D,page", [(32, 16, 256, 16), (32, 16, 128, 128), (96, 16, 256, 64), (64, 16, 128, 32), (16, 16, 256, 128)])
+def test_long_items_of_a_step(dev, H, h, D, page):
+    """many stages per work item: the ring goes round dozens of times, with warps that have no keys in some stages"""
+    L, B = 30011, 2
+    width = -(-L // page)
+    g = torch.Generator(device=dev).manual_seed(H + D)
+    k, v = (torch.randn((B * width, h, page, D), generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    q = torch.randn((B, H, D), generator=g, device=dev, dtype=torch.bfloat16)
+    table = torch.randperm(B * width, generator=g, device=dev).to(torch.int32).view(B, width)
+    lens = torch.tensor([L, L - 700], dtype=torch.int32, device=dev)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=dev)
+    run = lambda: ops.paged_attention(q, k, v, table, lens, cu, 1, D**-0.5)  # noqa: E731
+    first = run()
+    for _ in range(20):
+        assert torch.equal(run(), first)
+    for b in range(B):
+        n = int(lens[b])
+        kk = k[table[b].long()].transpose(0, 1).reshape(h, -1, D)[:, :n].double()
+        vv = v[table[b].long()].transpose(0, 1).reshape(h, -1, D)[:, :n].double()
+        qq = q[b].double().view(h, H // h, D)
+        p = torch.softmax(qq @ kk.transpose(1, 2) * D**-0.5, -1)
+        want, mag = p @ vv, p @ vv.abs()
+        rel = math.expm1(2 * (D + 8) * 2.0**-24 * float((qq.abs() @ kk.abs().transpose(1, 2)).max()) * D**-0.5) + (n + 64) * 2.0**-24
+        tol = BF * want.abs() + (BF * (1 + BF) + rel) * mag * (1 + BF)
+        assert ((first[b].double().view_as(want) - want).abs() <= tol).all()
+
+
 def test_attention_views_streams_and_a_graph(dev):
     c = Call(dev, 8, 2, 128, 64, [(300, 3), (129, 1)], seed=5)
     want, _, mag, big = c.expect()
