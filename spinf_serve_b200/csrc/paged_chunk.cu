@@ -327,33 +327,21 @@ __device__ __forceinline__ float chunk_probs(const float (&sc)[64], float scale_
   }
   return sum0 + sum1;
 }
-// the same over the 128 scores of a row, 32 at a time
 __device__ __forceinline__ uint32_t slot_bits(int jb, int lo, int hi) {  // which of the 32 slots from jb on lie in [lo, hi]
   uint32_t bits = hi < jb ? 0u : hi - jb >= 31 ? ~0u : (2u << (hi - jb)) - 1u;
   if (lo > jb) bits &= lo - jb > 31 ? 0u : ~0u << (lo - jb);
   return bits;
 }
-__device__ __forceinline__ float chunk_row_max(uint32_t taddr, bool masked, int jb, int lo, int hi) {
-  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-  for (int x = 0; x < 4; ++x) {
-    uint32_t v[32];
-    tmem_ld_x32(taddr + x * 32, v);
-    tmem_wait_ld();
-    const uint32_t bits = masked ? slot_bits(jb + x * 32, lo, hi) : ~0u;
-#pragma unroll
-    for (int c = 0; c < 32; ++c) m[c & 3] = fmaxf(m[c & 3], (bits & (1u << c)) ? __uint_as_float(v[c]) : -INFINITY);
-  }
-  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-}
-__device__ __forceinline__ float chunk_row_probs(uint32_t taddr, bool masked, int jb, int lo, int hi, float scale_log2, float neg_m, uint32_t (&pk)[64],
-                                                 float& sum) {
+// P of 64 keys of a row from their scores in tensor memory, and on the way the largest score; sum: of p, unrounded
+__device__ __forceinline__ float chunk_half(uint32_t taddr, bool masked, int jb, int lo, int hi, float scale_log2, float neg_m, uint32_t (&pk)[32], float& sum) {
   float m[2] = {-INFINITY, -INFINITY}, s[2] = {0.f, 0.f};
+  uint32_t v0[32], v1[32];
+  tmem_ld_x32(taddr, v0);
+  tmem_ld_x32(taddr + 32, v1);
+  tmem_wait_ld();
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    uint32_t u[32];
-    tmem_ld_x32(taddr + x * 32, u);
-    tmem_wait_ld();
+  for (int x = 0; x < 2; ++x) {
+    uint32_t (&u)[32] = x ? v1 : v0;
     if (masked) {
       const uint32_t bits = slot_bits(jb + x * 32, lo, hi);
 #pragma unroll
@@ -371,13 +359,7 @@ __device__ __forceinline__ float chunk_row_probs(uint32_t taddr, bool masked, in
     }
   }
   sum = s[0] + s[1];
-  return fmaxf(m[0], m[1]);
-}
-__device__ __forceinline__ void tmem_st_x64(uint32_t taddr, const uint32_t (&r)[64]) {
-  const uint32_t (&lo)[32] = *reinterpret_cast<const uint32_t (*)[32]>(&r[0]);
-  const uint32_t (&hi)[32] = *reinterpret_cast<const uint32_t (*)[32]>(&r[32]);
-  tmem_st_x32(taddr, lo);
-  tmem_st_x32(taddr + 32, hi);
+  return fmaxf(m[0], m[1]) * scale_log2;
 }
 // COLS columns of O times alpha, in tensor memory
 template <int COLS>
@@ -925,7 +907,7 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 8; ++k)  // packed bf16 P: 16 keys per 8 columns
-              umma_f16_ts(tmem_base + L::O_COL + tile * D, tmem_base + tile * 128 + 8 * k, vd + 128 * k, IDESC_O, (i | k) != 0);
+              umma_f16_ts(tmem_base + L::O_COL + tile * D, tmem_base + tile * 128 + (k >> 2) * CH_KH + 8 * (k & 3), vd + 128 * k, IDESC_O, (i | k) != 0);
             umma_commit(&o_done[tile * NS + st]);
             if (more) issue_s(tile, gi + 1);
           }
@@ -959,36 +941,44 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!alive) break;
         tc_fence_after();
         const bool masked = jb + PG_TILE - 1 > hi_min || jb < lo_max;
-        // p against the reference maximum as it stands, the tile's own maximum found on the way: no pass over the scores before the
-        // exponentials. Only where a row outgrew the threshold (or has no maximum yet) is the tile done again.
-        uint32_t pk[PG_TILE / 2];
-        float alpha = 1.f, sum = 0.f;
-        bool again = i == 0;
-        if (again) {
-          const float mx = chunk_row_max(s_tmem, masked, jb, lo, hi) * a.scale_log2;
-          m_ref = mx;
-        }
+        // p against the reference maximum as it stands, the scores' own maximum found on the way: no pass over the scores before the
+        // exponentials. Only where a row outgrew the threshold (or has no maximum yet) is the half done again. The reference is a whole
+        // number, so what was computed against the old one is scaled by a power of two, exactly.
+        float alpha = 1.f;
 #pragma unroll 1
-        for (;;) {
-          const float mx = chunk_row_probs(s_tmem, masked, jb, lo, hi, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref, pk, sum) * a.scale_log2;
-          const bool grown = !again && mx - m_ref > CH_RESCALE;  // false for NaN (-inf minus -inf): a row that has seen nothing yet
-          if (!__any_sync(0xffffffffu, grown)) break;
-          if (grown) {
-            alpha = fast_exp2(m_ref - mx);
-            m_ref = mx;
+        for (int half = 1; half >= 0; --half) {
+          uint32_t pk[32];
+          float sum;
+          const uint32_t at = s_tmem + half * CH_KH;
+          const int jh = jb + half * CH_KH;
+          const float mx = chunk_half(at, masked, jh, lo, hi, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref, pk, sum);
+          const bool grown = mx - m_ref > CH_RESCALE;  // false for NaN (-inf minus -inf): a row that has seen nothing yet
+          if (__any_sync(0xffffffffu, grown)) {
+            float f = 1.f;
+            if (grown) {
+              const float m_new = ceilf(mx);
+              f = fast_exp2(m_ref - m_new);
+              m_ref = m_new;
+            }
+            alpha *= f;
+            l_run *= f;
+            if (half == 0) {  // the other half's P is in tensor memory already
+              const uint32_t f2 = pack_bf16x2(f, f);
+              tmem_wait_st();
+              tmem_ld_x32(at + CH_KH, pk);
+              tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) pk[c] = bf2_mul(pk[c], f2);
+              tmem_st_x32(at + CH_KH, pk);
+            }
+            chunk_half(at, masked, jh, lo, hi, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref, pk, sum);
           }
-          again = true;
+          l_run += sum;
+          __syncwarp();
+          tmem_st_x32(at, pk);  // over the scores this thread has read
         }
-        l_run = l_run * alpha + sum;
-        if (i > 0) {
-          const bool done = mbar_wait(wc, &o_done[tile * NS + (gi - 1) % NS], ((gi - 1) / NS) & 1u, ST_TIMEOUT_TMEM);
-          if (__any_sync(0xffffffffu, alpha != 1.f) && __all_sync(0xffffffffu, done)) {
-            tc_fence_after();
-            chunk_rescale<D>(o_tmem, alpha);
-          }
-        }
-        __syncwarp();
-        tmem_st_x64(s_tmem, pk);  // P over the first half of the scores' columns
+        // (S of this tile was issued behind P V of the last: that has completed, and none is in flight until this warp has arrived)
+        if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) chunk_rescale<D>(o_tmem, alpha);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
