@@ -233,21 +233,28 @@ struct PageRun {
 // O of 128 rows x COLS columns from tensor memory (from column `taddr`, head dimensions from d0 on): divided by the sums and rounded to
 // the output, or in fp32 to the segment's partial result. `free_o` is called when the last column is in registers. A warp's 32 rows go
 // through 2 KB of shared memory, so that a store instruction covers whole sectors side by side (8 rows x 64 bytes, 4 rows x 128 bytes)
-// instead of 16 bytes of 32 rows. The loops stay rolled: this runs once a segment, and code that is not in the instruction cache
-// costs more than the loop.
+// instead of 16 bytes of 32 rows; where the rows go is worked out once for all columns.
 template <int D, int COLS, class Free>
 __device__ __forceinline__ void chunk_store(const PagedAttnArgs& a, const ChunkSeg& g, uint32_t taddr, int d0, int tile, int qd, int lane, float inv,
                                             uint8_t* stage, Free free_o) {
-  const int ql = 7 - a.hp_log2;  // log2 of a head's rows in a tile
   uint4* st = reinterpret_cast<uint4*>(stage);
+  if (g.part < 0) {
+    const int ql = 7 - a.hp_log2;  // log2 of a head's rows in a tile
+    __nv_bfloat16* to[4];          // rows lane / 4, + 8, + 16, + 24 of the warp (null: none of the sequence's)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int rr = qd * 32 + k * 8 + (lane >> 2);
+      const int tok = g.tok0 + (tile << ql) + (rr & ((1 << ql) - 1)), head = g.h0 + (rr >> ql);
+      to[k] = tok < g.nq ? a.out + static_cast<int64_t>(g.row0 + tok) * a.out_pitch + head * D + d0 + (lane & 3) * 8 : nullptr;
+    }
+    const int rd = (lane >> 2) * 4 + ((lane & 3) ^ ((lane >> 3) & 3));  // (rows 8 apart swizzle alike)
 #pragma unroll 1
-  for (int c = 0; c < COLS; c += 32) {
-    uint32_t o[32];
-    __syncwarp();
-    tmem_ld_x32(taddr + c, o);
-    tmem_wait_ld();
-    if (c + 32 >= COLS) free_o();
-    if (g.part < 0) {  // 64 bytes of every row
+    for (int c = 0; c < COLS; c += 32) {
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld_x32(taddr + c, o);
+      tmem_wait_ld();
+      if (c + 32 >= COLS) free_o();
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         st[lane * 4 + (x ^ ((lane >> 1) & 3))] =
@@ -256,27 +263,34 @@ __device__ __forceinline__ void chunk_store(const PagedAttnArgs& a, const ChunkS
                        pack_bf16x2(__uint_as_float(o[8 * x + 4]) * inv, __uint_as_float(o[8 * x + 5]) * inv),
                        pack_bf16x2(__uint_as_float(o[8 * x + 6]) * inv, __uint_as_float(o[8 * x + 7]) * inv));
       __syncwarp();
+      uint4 w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = st[k * 32 + rd];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (to[k]) *reinterpret_cast<uint4*>(to[k] + c) = w[k];
+    }
+  } else {
+    float* to = a.chunk_o + (static_cast<int64_t>(g.part) * 256 + tile * 128 + qd * 32 + (lane >> 3)) * D + d0 + (lane & 7) * 4;
 #pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        const int r = k * 8 + (lane >> 2), ch = lane & 3, rr = qd * 32 + r;
-        const int tok = g.tok0 + (tile << ql) + (rr & ((1 << ql) - 1)), head = g.h0 + (rr >> ql);
-        if (tok < g.nq)
-          *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(g.row0 + tok) * a.out_pitch + head * D + d0 + c + ch * 8) = st[r * 4 + (ch ^ ((r >> 1) & 3))];
-      }
-    } else {  // 128 bytes of every row, 16 rows at a time
-      float* to = a.chunk_o + (static_cast<int64_t>(g.part) * 256 + tile * 128 + qd * 32) * D + d0 + c;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
+    for (int c = 0; c < COLS; c += 32) {
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld_x32(taddr + c, o);
+      tmem_wait_ld();
+      if (c + 32 >= COLS) free_o();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // 128 bytes of 16 rows at a time
         if ((lane >> 4) == h) {
 #pragma unroll
           for (int x = 0; x < 8; ++x) st[(lane & 15) * 8 + (x ^ (lane & 7))] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
         }
         __syncwarp();
+        uint4 w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = k * 4 + (lane >> 3), ch = lane & 7;
-          *reinterpret_cast<uint4*>(to + (h * 16 + r) * D + ch * 4) = st[r * 8 + (ch ^ (r & 7))];
-        }
+        for (int k = 0; k < 4; ++k) w[k] = st[k * 32 + (lane & ~7) + ((lane & 7) ^ ((k * 4 + (lane >> 3)) & 7))];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + c + (h * 16 + k * 4) * D) = w[k];
         __syncwarp();
       }
     }
