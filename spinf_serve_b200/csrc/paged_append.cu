@@ -3,7 +3,7 @@
 //   r = rsqrt(mean(x^2) + eps),  y = x r w,  y1' = y1 cos - y2 sin,  y2' = y2 cos + y1 sin  (halves of the rotary dimensions)
 // Everything in fp32 with one rounding at the end. (qkv_norm_rope rounds after every module's output, as the module code it stands
 // in for does; nothing else reads what this writes before the attention, so the intermediate roundings would only lose bits.)
-// A group of D / 8 lanes owns one head's row, 16 bytes a lane.
+// A group of D / 8 lanes owns one head's row, 16 bytes a lane. Bound by HBM.
 #include "common.cuh"
 #include "host_util.h"
 #include "paged.cuh"
@@ -34,90 +34,125 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
   for (int i = 0; i < 4; ++i) x[2 * i] = bf2_lo(w[i]), x[2 * i + 1] = bf2_hi(w[i]);
 }
 
+// A CTA walks tokens: 256 at a time it first works out where their rows go (a thread per token), then takes them one by one, all heads
+// at once, four rows to a group of lanes; the next token's rows are on their way while this one's are worked on. The norm weights
+// stay in registers, the rotary table is read once per token and lane.
 template <int D>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, const PagedSeqs s, int* __restrict__ status) {
+__global__ void __launch_bounds__(256, 2) paged_append_kernel(const AppendArgs a, const PagedSeqs s, int* __restrict__ status) {
   constexpr int LANES = D / 8;         // lanes of a head's row
   constexpr int GROUPS = 256 / LANES;  // rows a CTA works on at once
-  constexpr int IPT = 4;               // rows a group has in flight
-  const int lane = threadIdx.x & 31, sub = lane % LANES, group = threadIdx.x / LANES;
+  constexpr int RPT = 4;               // rows a group has in flight
+  __shared__ int s_page[256], s_row[256];
+  const int lane = threadIdx.x & 31, sub = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const uint32_t gmask = LANES == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
-  const int heads = a.skip_q ? 2 * a.h : a.H + 2 * a.h;
-  const int64_t items = s.n * heads;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * GROUPS + group) * IPT;
-  uint4 raw[IPT];
-  int64_t tok[IPT];
-  int head[IPT];
-#pragma unroll
-  for (int i = 0; i < IPT; ++i) {
-    const int64_t it = first + i < items ? first + i : items - 1;
-    tok[i] = it / heads;
-    head[i] = static_cast<int>(it - tok[i] * heads) + (a.skip_q ? a.H : 0);
-    raw[i] = *reinterpret_cast<const uint4*>(a.qkv + tok[i] * a.pitch + static_cast<int64_t>(head[i]) * D + sub * 8);
+  const int row0 = a.skip_q ? a.H : 0, rows = a.H + 2 * a.h - row0;
+  const int blocks = (rows + GROUPS * RPT - 1) / (GROUPS * RPT);  // of rows a token makes
+  const int hl = a.half / 8;  // lanes of a rotary half
+  const int from = sub < hl ? sub + hl : sub < 2 * hl ? sub - hl : sub;
+  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
+  if (a.wq) {
+    wq = *reinterpret_cast<const uint4*>(a.wq + sub * 8);
+    wk = *reinterpret_cast<const uint4*>(a.wk + sub * 8);
   }
+  uint4 raw[RPT], cs = make_uint4(0, 0, 0, 0), sn = cs;
+  auto fetch = [&](int64_t t, int blk) {
 #pragma unroll
-  for (int i = 0; i < IPT; ++i) {
-    if (first + i >= items) break;
-    const int64_t t = tok[i];
-    const bool is_q = head[i] < a.H, is_v = head[i] >= a.H + a.h;
-    float x[8];
-    unpack8(raw[i], x);
-    const __nv_bfloat16* w = is_v ? nullptr : is_q ? a.wq : a.wk;
-    if (w || (is_v && a.norm_v)) {
-      float ss = 0.f;
+    for (int i = 0; i < RPT; ++i) {
+      const int r = (blk * RPT + i) * GROUPS + group;
+      if (r < rows) raw[i] = *reinterpret_cast<const uint4*>(a.qkv + t * a.pitch + static_cast<int64_t>(row0 + r) * D + sub * 8);
+    }
+    if (sub < 2 * hl) {
+      const int64_t at = t * a.half + (sub < hl ? sub : sub - hl) * 8;
+      cs = *reinterpret_cast<const uint4*>(a.cos_t + at);
+      sn = *reinterpret_cast<const uint4*>(a.sin_t + at);
+    }
+  };
+  for (int64_t t0 = blockIdx.x; t0 < s.n; t0 += 256ll * gridDim.x) {
+    const int64_t left = (s.n - t0 + gridDim.x - 1) / gridDim.x;
+    const int steps = static_cast<int>(left < 256 ? left : 256) * blocks;
+    fetch(t0, 0);
+    {
+      const int64_t t = t0 + static_cast<int64_t>(threadIdx.x) * gridDim.x;
+      int pg = -1, in_page = 0;
+      if (t < s.n) {
+        int lo = 0, hi = s.B;  // the row's sequence: how many sequences end at or before it
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s.cu[mid + 1] <= t) lo = mid + 1;
+          else hi = mid;
+        }
+        if (lo < s.B && t >= s.cu[lo]) {  // (a row behind the last sequence, or before the first, has no slot)
+          const int slot = s.lens[lo] - s.cu[lo + 1] + static_cast<int>(t);
+          in_page = slot & ((1 << s.page_log2) - 1);
+          if (slot >= 0 && (slot >> s.page_log2) < a.width) pg = s.table[lo * s.table_pitch + (slot >> s.page_log2)];
+          if (pg < 0 || pg >= s.n_pages) {
+            pg = -1;
+            atomicCAS(status, 0, ST_BAD_INDEX);
+          }
+        }
+      }
+      __syncthreads();  // the last 256 tokens' places have been read
+      s_page[threadIdx.x] = pg;
+      s_row[threadIdx.x] = in_page;
+      __syncthreads();
+    }
+    int k = 0, blk = 0;
+    for (int step = 0; step < steps; ++step) {
+      const int64_t t = t0 + static_cast<int64_t>(k) * gridDim.x;
+      const int pg = s_page[k], in_page = s_row[k], r0 = blk * RPT * GROUPS + group;
+      uint4 cur[RPT];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+      for (int i = 0; i < RPT; ++i) cur[i] = raw[i];
+      float c[8], z[8];
+      unpack8(cs, c);
+      unpack8(sn, z);
+      if (++blk == blocks) blk = 0, ++k;
+      if (step + 1 < steps) fetch(t0 + static_cast<int64_t>(k) * gridDim.x, blk);
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(gmask, ss, o, LANES);
-      const float r = rsqrtf(ss * (1.f / D) + a.eps);
-      if (w) {
-        float wf[8];
-        unpack8(*reinterpret_cast<const uint4*>(w + sub * 8), wf);
+      for (int i = 0; i < RPT; ++i) {
+        const int r = r0 + i * GROUPS;
+        if (r >= rows) continue;
+        const int head = row0 + r;
+        const bool is_q = head < a.H, is_v = head >= a.H + a.h;
+        float x[8];
+        unpack8(cur[i], x);
+        if (is_v ? a.norm_v != 0 : a.wq != nullptr) {
+          float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (a.plus1 ? 1.f + wf[e] : wf[e]);
-      } else {
+          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= r;
+          for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(gmask, ss, o, LANES);
+          const float rs = rsqrtf(ss * (1.f / D) + a.eps);
+          if (is_v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= rs;
+          } else {
+            float wf[8];
+            unpack8(is_q ? wq : wk, wf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * rs * (a.plus1 ? 1.f + wf[e] : wf[e]);
+          }
+        }
+        if (a.half && !is_v) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(gmask, x[e], from, LANES);
+          if (sub < 2 * hl) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], c[e], (sub < hl ? -y[e] : y[e]) * z[e]);
+          }
+        }
+        const uint4 packed = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+        if (is_q) {
+          *reinterpret_cast<uint4*>(a.q_out + (t * a.H + head) * D + sub * 8) = packed;
+        } else if (pg >= 0) {
+          const int kh = head - a.H - (is_v ? a.h : 0);
+          __nv_bfloat16* dst = is_v ? a.v_pages + pg * a.v_page + kh * a.v_head + in_page * a.v_row
+                                    : a.k_pages + pg * a.k_page + kh * a.k_head + in_page * a.k_row;
+          *reinterpret_cast<uint4*>(dst + sub * 8) = packed;
+        }
       }
     }
-    if (a.half && !is_v) {
-      const int hl = a.half / 8;  // lanes of a rotary half
-      const int from = sub < hl ? sub + hl : sub < 2 * hl ? sub - hl : sub;
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(gmask, x[e], from, LANES);
-      if (sub < 2 * hl) {
-        const int64_t at = t * a.half + (sub < hl ? sub : sub - hl) * 8;
-        float c[8], sn[8];
-        unpack8(*reinterpret_cast<const uint4*>(a.cos_t + at), c);
-        unpack8(*reinterpret_cast<const uint4*>(a.sin_t + at), sn);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], c[e], (sub < hl ? -y[e] : y[e]) * sn[e]);
-      }
-    }
-    const uint4 packed = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-    if (is_q) {
-      *reinterpret_cast<uint4*>(a.q_out + (t * a.H + head[i]) * D + sub * 8) = packed;
-      continue;
-    }
-    // the row's sequence: how many sequences end at or before it
-    int b = 0;
-    for (int b0 = 0; b0 < s.B; b0 += LANES) {
-      const bool before = b0 + sub < s.B && s.cu[b0 + sub + 1] <= t;
-      b += __popc(__ballot_sync(gmask, before) & gmask);
-    }
-    if (b >= s.B || t < s.cu[b]) continue;  // a row behind the last sequence (or before the first) has no slot
-    const int slot = s.lens[b] - s.cu[b + 1] + static_cast<int>(t);
-    int pg = -1;
-    if (slot >= 0 && (slot >> s.page_log2) < a.width) pg = s.table[b * s.table_pitch + (slot >> s.page_log2)];
-    if (pg < 0 || pg >= s.n_pages) {
-      if (sub == 0) atomicCAS(status, 0, ST_BAD_INDEX);
-      continue;
-    }
-    const int in_page = slot & ((1 << s.page_log2) - 1);
-    const int kh = head[i] - a.H - (is_v ? a.h : 0);
-    __nv_bfloat16* dst = is_v ? a.v_pages + pg * a.v_page + kh * a.v_head + in_page * a.v_row
-                              : a.k_pages + pg * a.k_page + kh * a.k_head + in_page * a.k_row;
-    *reinterpret_cast<uint4*>(dst + sub * 8) = packed;
   }
 }
 
@@ -179,10 +214,8 @@ extern "C" int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int
   s.max_len = width * page;
   s.max_q = 0;  // the append sizes nothing by it
   s.n = n;
-  const int64_t items = n * (a.skip_q ? 2 * Hkv : H + 2 * Hkv);
-  const int64_t per_cta = (256 / (D / 8)) * 4;
-  const int64_t grid = (items + per_cta - 1) / per_cta;
-  if (grid >= (1ll << 31)) return SPINF_ERR_TOO_LARGE;
+  const int64_t most = 2ll * sm_count();  // two CTAs an SM
+  const int64_t grid = n < most ? n : most;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 256)
     paged_append_kernel<256><<<static_cast<unsigned>(grid), 256, 0, st>>>(a, s, status);
