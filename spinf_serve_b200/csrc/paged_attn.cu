@@ -12,7 +12,6 @@
 // shared memory, P goes to shared memory as bf16, and for P V each warp takes an eighth of the head dimensions over all 128 keys, so
 // the output needs no exchange and K and V are read from shared memory once. Running maximum and sum in fp32; P is rounded to bf16
 // for the product (its operands are 16 bit), which adds about what rounding the output to bf16 adds; the sum takes p unrounded.
-#include "gdn_mma.cuh"
 #include "paged_attn.cuh"
 
 #include <atomic>
@@ -90,89 +89,123 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 // The producer warp of both few-row kernels. Items are planned 32 at a time, one per lane, and an item's page indexes are fetched by
 // the lanes together, the next item's while this one is copied, so that no step of the copy loop waits for a load of its own. Order of
-// the stages: K and V of a unit in turn (STEP), or the two K units of a 128-key tile and then its two V units.
+// the stages: K and V of a unit in turn (STEP), or the two K units of a 128-key tile and then its two V units. One warp has to keep up
+// with the SM's share of HBM (a unit of 32 KB every 1 400 cycles at D 128), so the loop is written for few instructions: ring position
+// and phase are counted along, and units that lie inside the visible slots (all but the first and last) skip the box tests.
 template <int D, bool STEP, int NST, int STAGE, int Q_PITCH, int Q_SLOT, int NQ>
-__device__ __forceinline__ void produce_keys(const PagedSeqs& s, const PagedAttnArgs& a, const CUtensorMap* tmK, const CUtensorMap* tmV, const int* pre,
-                                             int total, uint8_t* ring, uint8_t* q_slots, KeyItem* items, KeyItem* plan, uint64_t* full, uint64_t* empty,
-                                             uint64_t* q_full, uint64_t* q_empty, const WaitCtx& wc, int* status) {
-  const int lane = threadIdx.x & 31;
-  const int br = s.page_log2 < 6 ? s.page_log2 : 6, box_rows = 1 << br, in_page = (1 << s.page_log2) - 1;
-  uint32_t cnt = 0, item_n = 0;
-  bool ok = true;
-  // page of box x of an item (boxes of 2^br slots from its first unit on): -1 where no row sees any of them, -2 for a bad index
-  auto page_of = [&](const KeyItem& w, int x) -> int {
+struct KeyProducer {
+  const PagedSeqs& s;
+  const PagedAttnArgs& a;
+  const CUtensorMap* tmK;
+  const CUtensorMap* tmV;
+  uint8_t* ring;
+  uint64_t* full;
+  uint64_t* empty;
+  const WaitCtx& wc;
+  int* status;
+  int br, in_page;
+  uint32_t st, ph, cnt;  // ring position, its phase, stages queued
+  static constexpr int UNITS = STEP ? 1 : 2;
+
+  __device__ __forceinline__ bool wanted(const KeyItem& w, int j) const {  // some row sees the box at slot j
+    return j < w.u1 * 64 && j < w.hi && j + (1 << br) > w.lo;
+  }
+  // table entry of box x of an item (boxes of 2^br slots from its first unit on). Nothing looks at it here: the first look waits for it
+  __device__ __forceinline__ int entry(const KeyItem& w, int x) const {
     const int j = (w.u0 * 64) + (x << br);
-    if (j >= w.u1 * 64 || j >= w.hi || j + box_rows <= w.lo) return -1;
-    const int pg = s.table[w.b * s.table_pitch + (j >> s.page_log2)];
-    return pg >= 0 && pg < s.n_pages ? pg : -2;
-  };
-  for (int k0 = 0; ok && static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(k0) * gridDim.x < total; k0 += PLAN) {
-    const int64_t mine = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(k0 + lane) * gridDim.x;
-    __syncwarp();
-    if (mine < total) plan[lane] = key_item<STEP>(s, a, pre, static_cast<int>(mine), status);
-    const int n_plan = __popc(__ballot_sync(0xffffffffu, mine < total));
-    __syncwarp();
-    int pages_next = page_of(plan[0], lane);
-    for (int k = 0; k < n_plan && ok; ++k, ++item_n) {
-      const KeyItem w = plan[k];
-      int pages = pages_next;
-      if (k + 1 < n_plan) pages_next = page_of(plan[k + 1], lane);
-      const uint32_t qs = item_n % NQ;
-      if (lane == 0) {
-        ok = mbar_wait(wc, &q_empty[qs], ((item_n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY);
-        if (ok) {
+    return wanted(w, j) ? s.table[w.b * s.table_pitch + (j >> s.page_log2)] : 0;
+  }
+  template <int BOXES>  // of a unit
+  __device__ __forceinline__ bool copy(const KeyItem& w, int pages, int lane) {
+    constexpr int ROWS = 64 / BOXES;
+    int x = 0;
+#pragma unroll 1
+    for (int u = w.u0; u < w.u1; u += UNITS, x += UNITS * BOXES) {
+      if (x && (x & 31) == 0) pages = entry(w, x + lane);
+      int pg[UNITS * BOXES], bytes[UNITS];
+      bool all = u * 64 >= w.lo && (u + UNITS) * 64 <= w.hi;
+#pragma unroll
+      for (int y = 0; y < UNITS * BOXES; ++y) {
+        pg[y] = __shfl_sync(0xffffffffu, pages, (x + y) & 31);
+        all = all && static_cast<unsigned>(pg[y]) < static_cast<unsigned>(s.n_pages);
+      }
+#pragma unroll
+      for (int v = 0; v < UNITS; ++v) bytes[v] = 64 * D * 2;
+      if (!all) {  // boxes that no row sees stay as they are (masked for K, cleared for V)
+#pragma unroll
+        for (int y = 0; y < UNITS * BOXES; ++y) {
+          const bool want = wanted(w, u * 64 + y * ROWS), good = static_cast<unsigned>(pg[y]) < static_cast<unsigned>(s.n_pages);
+          if (want && !good && lane == 0) atomicCAS(status, 0, ST_BAD_INDEX);
+          if (!want || !good) {
+            pg[y] = -1;
+            bytes[y / BOXES] -= ROWS * D * 2;
+          }
+        }
+      }
+#pragma unroll
+      for (int part = 0; part < 2 * UNITS; ++part) {
+        if (!__all_sync(0xffffffffu, mbar_wait(wc, &empty[st], ph ^ 1u, ST_TIMEOUT_EMPTY))) return false;
+        if (lane == 0) {
+          mbar_expect_tx(&full[st], bytes[part % UNITS]);
+#pragma unroll
+          for (int y = 0; y < BOXES; ++y)
+            if (pg[(part % UNITS) * BOXES + y] >= 0)
+              tma_load_5d(ring + st * STAGE + y * (ROWS * D * 2), part < UNITS ? tmK : tmV, 0, ((u + part % UNITS) * 64 + y * ROWS) & in_page, 0, w.g,
+                          pg[(part % UNITS) * BOXES + y], &full[st]);
+        }
+        if (++st == NST) st = 0, ph ^= 1u;
+        ++cnt;
+      }
+    }
+    return true;
+  }
+  __device__ __forceinline__ void run(const int* pre, int total, uint8_t* q_slots, KeyItem* items, KeyItem* plan, uint64_t* q_full, uint64_t* q_empty) {
+    const int lane = threadIdx.x & 31;
+    uint32_t item_n = 0;
+    bool ok = true;
+    for (int k0 = 0; ok && static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(k0) * gridDim.x < total; k0 += PLAN) {
+      const int64_t mine = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(k0 + lane) * gridDim.x;
+      __syncwarp();
+      if (mine < total) plan[lane] = key_item<STEP>(s, a, pre, static_cast<int>(mine), status);
+      const int n_plan = __popc(__ballot_sync(0xffffffffu, mine < total));
+      __syncwarp();
+      int pages_next = entry(plan[0], lane);
+      for (int k = 0; k < n_plan; ++k, ++item_n) {
+        const KeyItem w = plan[k];
+        const int pages = pages_next;
+        if (k + 1 < n_plan) pages_next = entry(plan[k + 1], lane);
+        const uint32_t qs = item_n % NQ;
+        ok = __all_sync(0xffffffffu, mbar_wait(wc, &q_empty[qs], ((item_n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY));
+        if (!ok) break;
+        if (lane == 0) {
           items[qs] = w;
           mbar_expect_tx(&q_full[qs], w.rows * D * 2);  // (an arrival: releases the item's numbers to the consumers as well)
         }
-      }
-      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
-      if (!ok) break;
-      for (int r = lane; r < w.rows; r += 32) {
-        const int rr = w.r0 + r;
-        bulk_load(q_slots + qs * Q_SLOT + r * Q_PITCH, a.q + (w.row0 + rr / a.group) * a.q_pitch + static_cast<int64_t>(w.g * a.group + rr % a.group) * D,
-                  D * 2, &q_full[qs]);
-      }
-      constexpr int UNITS = STEP ? 1 : 2;
-      const int boxes = 64 >> br;  // of a unit
-      for (int u = w.u0; u < w.u1 && ok; u += UNITS) {
-        const int x0 = (u - w.u0) * boxes;
-        if (x0 && (x0 & 31) == 0) pages = page_of(w, x0 + lane);
-        int pg[UNITS][4];
-#pragma unroll
-        for (int v = 0; v < UNITS; ++v)
-#pragma unroll
-          for (int y = 0; y < 4; ++y) pg[v][y] = __shfl_sync(0xffffffffu, pages, (x0 + v * boxes + y) & 31);
-        if (lane == 0) {
-#pragma unroll
-          for (int part = 0; part < 2 * UNITS; ++part, ++cnt) {
-            const int v = part % UNITS;
-            const uint32_t st = cnt % NST;
-            if (!mbar_wait(wc, &empty[st], ((cnt / NST) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-            int bytes = 0;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              if (y >= boxes) continue;
-              if (pg[v][y] == -2) atomicCAS(status, 0, ST_BAD_INDEX);
-              bytes += pg[v][y] >= 0 ? box_rows * D * 2 : 0;
-            }
-            mbar_expect_tx(&full[st], bytes);  // boxes that no row sees stay as they are (masked for K, cleared for V)
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (y < boxes && pg[v][y] >= 0)
-                tma_load_5d(ring + st * STAGE + y * box_rows * D * 2, part < UNITS ? tmK : tmV, 0, ((u + v) * 64 + y * box_rows) & in_page, 0, w.g, pg[v][y],
-                            &full[st]);
-          }
+        __syncwarp();
+        for (int r = lane; r < w.rows; r += 32) {
+          const int rr = w.r0 + r;
+          bulk_load(q_slots + qs * Q_SLOT + r * Q_PITCH, a.q + (w.row0 + rr / a.group) * a.q_pitch + static_cast<int64_t>(w.g * a.group + rr % a.group) * D,
+                    D * 2, &q_full[qs]);
         }
-        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+        ok = br == 6 ? copy<1>(w, pages, lane) : br == 5 ? copy<2>(w, pages, lane) : copy<4>(w, pages, lane);
+        if (!ok) break;
       }
     }
+    if (*wc.abort_flag && lane == 0) {  // bounded wait for copies that may still be in flight
+      for (uint32_t c = cnt > static_cast<uint32_t>(NST) ? cnt - NST : 0; c < cnt; ++c)
+        for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % NST], (c / NST) & 1u); ++spin) {}
+      for (uint32_t c = item_n > static_cast<uint32_t>(NQ) ? item_n - NQ : 0u; c <= item_n; ++c)
+        for (int spin = 0; spin < 4096 && !mbar_try_wait(&q_full[c % NQ], (c / NQ) & 1u); ++spin) {}
+    }
   }
-  if (*wc.abort_flag && lane == 0) {  // bounded wait for copies that may still be in flight
-    for (uint32_t c = cnt > static_cast<uint32_t>(NST) ? cnt - NST : 0; c < cnt; ++c)
-      for (int spin = 0; spin < 4096 && !mbar_try_wait(&full[c % NST], (c / NST) & 1u); ++spin) {}
-    for (uint32_t c = item_n > static_cast<uint32_t>(NQ) ? item_n - NQ : 0u; c <= item_n; ++c)
-      for (int spin = 0; spin < 4096 && !mbar_try_wait(&q_full[c % NQ], (c / NQ) & 1u); ++spin) {}
-  }
+};
+
+// D (16 x 8, fp32) += A (16 x 16, bf16, row) B (16 x 8, bf16, col). Not volatile: the fragment loads are, so the compiler may put the
+// loads of the next steps between a load and its product; with both volatile every step waited out its own loads.
+__device__ __forceinline__ void mma_free(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // byte offset of (key, 16-byte chunk of its row) in a stage: boxes of 2^br rows x all slabs, 128-byte swizzled
@@ -252,8 +285,8 @@ __device__ __forceinline__ bool rows_work(const PagedAttnArgs& a, const KeyItem&
           const int chunk = ks * 2 + (lane >> 4);
           const uint32_t qa = q_base + (m * 16 + (lane & 15)) * L::Q_PITCH + chunk * 16;
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(qf[0]), "=r"(qf[1]), "=r"(qf[2]), "=r"(qf[3]) : "r"(qa));
-          mma_bf16(sc[m][0], qf, kf[0], kf[1]);
-          mma_bf16(sc[m][1], qf, kf[2], kf[3]);
+          mma_free(sc[m][0], qf, kf[0], kf[1]);
+          mma_free(sc[m][1], qf, kf[2], kf[3]);
         }
       }
     }
@@ -371,8 +404,8 @@ __device__ __forceinline__ bool rows_work(const PagedAttnArgs& a, const KeyItem&
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(vf[0]), "=r"(vf[1]), "=r"(vf[2]), "=r"(vf[3]) : "r"(va));
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              mma_bf16(o[m][2 * np], pf[m], vf[0], vf[1]);
-              mma_bf16(o[m][2 * np + 1], pf[m], vf[2], vf[3]);
+              mma_free(o[m][2 * np], pf[m], vf[0], vf[1]);
+              mma_free(o[m][2 * np + 1], pf[m], vf[2], vf[3]);
             }
           }
         }
@@ -455,8 +488,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   KeyItem* items = reinterpret_cast<KeyItem*>(smem + L::ITEM_OFF);
 
   if (warp == 8) {
-    produce_keys<D, false, L::NST, L::STAGE, L::Q_PITCH, L::Q_SLOT, 1>(s, a, &tmK, &tmV, pre, total, smem, smem + L::Q_OFF, items, items + 1, full, empty,
-                                                                       q_full, q_empty, wc, status);
+    KeyProducer<D, false, L::NST, L::STAGE, L::Q_PITCH, L::Q_SLOT, 1> p{s, a, &tmK, &tmV, smem, full, empty, wc, status, br, (1 << s.page_log2) - 1, 0, 0, 0};
+    p.run(pre, total, smem + L::Q_OFF, items, items + 1, q_full, q_empty);
   } else {
     uint32_t cnt = 0, item_n = 0;
     for (int it = blockIdx.x; it < total; it += gridDim.x, ++item_n) {
@@ -477,16 +510,20 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 }
 
 // ---------------------------------------------------------------- few rows per kv head (at most 16): a decoding step
-static constexpr int SW = 7;                        // consumer warps; the eighth warp is the producer (8 warps: 255 registers a thread)
-static constexpr int STEP_THREADS = (SW + 1) * 32;
+// Consumer warps; one more is the producer. D 128: eight in two groups of four that take the 64-key units in turn, a warp 16 keys of
+// each; with an even number of units in the ring a stage always belongs to the same group. D 256: a warp's share of the output alone
+// is 128 registers (16 rows), so seven (8 warps of 255 registers), which take the units' 16-key pieces in turn.
+__host__ __device__ constexpr int step_warps(int D) { return D == 256 ? 7 : 8; }
+__host__ __device__ constexpr int step_threads(int D) { return (step_warps(D) + 1) * 32; }
 
 template <int D>
 struct StepSmem {
   static constexpr int STAGE = 64 * D * 2;          // 64 keys of K or V
-  static constexpr int NST = D == 256 ? 5 : 10;
+  static constexpr int NST = D == 256 ? 5 : 12;
   static constexpr int Q_PITCH = D * 2 + 16;        // a row of q; the 16 bytes spread the rows over the banks
   static constexpr int Q_SLOT = STEP_ROWS * Q_PITCH;
-  static constexpr int MR = D == 256 ? 4 : 8;       // rows merged at a time
+  static constexpr int SW = step_warps(D);
+  static constexpr int MR = 4;                      // rows merged at a time
   static constexpr int Q_OFF = NST * STAGE;
   static constexpr int MERGE_OFF = Q_OFF + 2 * Q_SLOT;
   static constexpr int ML_OFF = MERGE_OFF + SW * MR * D * 4;  // [SW][16] maxima, [SW][16] sums, [16] joined maxima, [16] joined sums
@@ -510,11 +547,11 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 }
 // NT: 8-row tiles of q. A row's arithmetic is the same for either.
 template <int D, int NT>
-__global__ void __launch_bounds__(STEP_THREADS, 1)
+__global__ void __launch_bounds__(step_threads(D), 1)
 paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedSeqs s, const PagedAttnArgs a,
                   int* __restrict__ status) {
   using L = StepSmem<D>;
-  constexpr int KS = D / 16;
+  constexpr int KS = D / 16, SW = L::SW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   int* pre = reinterpret_cast<int*>(smem + L::PRE_OFF);
@@ -529,7 +566,7 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NST; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], SW);
+      mbar_init(&empty[i], D == 256 ? SW : 4);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
@@ -540,14 +577,14 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  paged_item_prefix(s.B, pre, STEP_THREADS, [&](int b) { return key_items<true>(s, a, b, status); });
+  paged_item_prefix(s.B, pre, step_threads(D), [&](int b) { return key_items<true>(s, a, b, status); });
   const int total = pre[s.B];
   const int br = s.page_log2 < 6 ? s.page_log2 : 6;  // log2 of a box's rows
   KeyItem* items = reinterpret_cast<KeyItem*>(smem + L::ITEM_OFF);
 
   if (warp == SW) {
-    produce_keys<D, true, L::NST, L::STAGE, L::Q_PITCH, L::Q_SLOT, 2>(s, a, &tmK, &tmV, pre, total, smem, smem + L::Q_OFF, items, items + 2, full, empty,
-                                                                      q_full, q_empty, wc, status);
+    KeyProducer<D, true, L::NST, L::STAGE, L::Q_PITCH, L::Q_SLOT, 2> p{s, a, &tmK, &tmV, smem, full, empty, wc, status, br, (1 << s.page_log2) - 1, 0, 0, 0};
+    p.run(pre, total, smem + L::Q_OFF, items, items + 2, q_full, q_empty);
   } else {
     float* m_w = reinterpret_cast<float*>(smem + L::ML_OFF);  // [SW][16]
     float* l_w = m_w + SW * STEP_ROWS;
@@ -601,21 +638,27 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         m_run[n][0] = m_run[n][1] = -INFINITY;
         l_run[n][0] = l_run[n][1] = 0.f;
       }
-      // A unit is four pieces of 16 keys, piece after piece to the warps in turn. Every warp waits for every stage and lets it go, also
-      // where it has no piece: a barrier's parity tells a phase only from its neighbours, so no warp may be a phase ahead of one.
+      // A unit is four pieces of 16 keys. A barrier's parity tells a phase only from its neighbours, so a warp has to wait for every use
+      // of every stage it waits for at all. D 128: the groups' stages are their own. D 256: all warps wait for every stage and let it go,
+      // also where they have no piece. `me`: the warp's place in the item, which is where its keys are, whatever came before in the ring.
       const int units = w.u1 - w.u0;
-      int turn = warp;  // pieces from the unit's first on to this warp's next
-      for (int u = 0; u < units && ok; ++u, turn = turn < 4 ? turn + SW - 4 : turn - 4) {
+      const int me = D == 256 ? warp : ((((warp >> 2) ^ (cnt0 >> 1)) & 1) << 2) + (warp & 3);
+      int turn = D == 256 ? warp : warp & 3;  // pieces from the unit's first on to this warp's next
+      for (int u = D == 256 ? 0 : me >> 2; u < units && ok; u += D == 256 ? 1 : 2) {
         const uint32_t ck = cnt0 + 2 * u, stk = ck % L::NST, stv = (ck + 1) % L::NST;
         ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stk], (ck / L::NST) & 1u, ST_TIMEOUT_FULL));
         if (!ok) break;
-        if (turn >= 4) {
-          if (lane == 0) mbar_arrive(&empty[stk]);
-          ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stv], ((ck + 1) / L::NST) & 1u, ST_TIMEOUT_FULL));
-          if (ok && lane == 0) mbar_arrive(&empty[stv]);
-          continue;
+        const int piece = turn;
+        if (D == 256) {
+          turn = turn < 4 ? turn + SW - 4 : turn - 4;
+          if (piece >= 4) {
+            if (lane == 0) mbar_arrive(&empty[stk]);
+            ok = __all_sync(0xffffffffu, mbar_wait(wc, &full[stv], ((ck + 1) / L::NST) & 1u, ST_TIMEOUT_FULL));
+            if (ok && lane == 0) mbar_arrive(&empty[stv]);
+            continue;
+          }
         }
-        const int key0 = turn * 16, j0 = (w.u0 + u) * 64 + key0;
+        const int key0 = piece * 16, j0 = (w.u0 + u) * 64 + key0;
         float sc[2][NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -629,7 +672,7 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             uint32_t kf[4];
             ldsm4(kf, k_base + stage_offset<D>(key, ks * 2 + (lane >> 4), br));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_bf16(sc[ks & 1][n], kf, qf[n][ks][0], qf[n][ks][1]);
+            for (int n = 0; n < NT; ++n) mma_free(sc[ks & 1][n], kf, qf[n][ks][0], qf[n][ks][1]);
           }
         }
         __syncwarp();
@@ -705,14 +748,14 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             uint32_t vf[4];
             ldsm4_t(vf, v_base + stage_offset<D>(key, i * 2 + ((lane >> 3) & 1), br));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_bf16(o[i][n], vf, pf[n][0], pf[n][1]);
+            for (int n = 0; n < NT; ++n) mma_free(o[i][n], vf, pf[n][0], pf[n][1]);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stv]);
       }
       cnt0 += 2 * (w.u1 > w.u0 ? w.u1 - w.u0 : 0);
-      // ---- the warps' shares joined, in warp order
+      // ---- the warps' shares joined, in the order of their places
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -723,8 +766,8 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           l += __shfl_xor_sync(0xffffffffu, l, 16);
           if (r8 == 0) {
             const int r = n * 8 + 2 * c4 + x;
-            m_w[warp * STEP_ROWS + r] = m_run[n][x];
-            l_w[warp * STEP_ROWS + r] = l;
+            m_w[me * STEP_ROWS + r] = m_run[n][x];
+            l_w[me * STEP_ROWS + r] = l;
           }
         }
       if (!bar_red_and(1, SW * 32, ok)) break;
@@ -751,7 +794,7 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int x = 0; x < 2; ++x) {
             const int r = n * 8 + 2 * c4 + x;
             if (r >= rb && r < rb + L::MR && r < rows) {
-              float* dst = merge + (warp * L::MR + r - rb) * D + r8;
+              float* dst = merge + (me * L::MR + r - rb) * D + r8;
 #pragma unroll
               for (int i = 0; i < KS; ++i) dst[i * 16] = o[i][n][x] * f[n][x], dst[i * 16 + 8] = o[i][n][2 + x] * f[n][x];
             }
@@ -895,7 +938,10 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, co
   }
 }
 
-static constexpr int CHUNK_ROWS = 128;  // rows per kv head from which on the chunk kernel takes a sequence
+// A sequence with more rows per kv head than this is the chunk kernels', where a head set of it fills 256-row items: measured on 32
+// sequences of 2 000 tokens (16 / 8 heads of 256) 32 rows took 138 us in the few-row kernel and 168 there, 64 rows 253 and 172; with
+// three head sets per kv head (24 / 4 heads) 48 rows 106 and 237, 96 rows 250 and 240.
+__host__ __device__ constexpr int chunk_rows_of(int group) { return 32 * (group >> chunk_heads_log2(group)); }
 
 // what a call needs: sizes of the workspace's parts in bytes (256-byte multiples)
 struct PagedSizes {
@@ -909,8 +955,9 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   PagedSizes z = {};
   const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
   const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
-  z.chunk_rows = CHUNK_ROWS;
-  const int64_t group = H / h, most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
+  const int64_t group = H / h;
+  z.chunk_rows = chunk_rows_of(static_cast<int>(group));
+  const int64_t most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
   if (slots > 1) {
     const int64_t by_rows = (max_q < most ? max_q : most) * H * slots;  // every row in every split
     const int64_t by_items = static_cast<int64_t>(PG_SMS) * RT;  // every free slot one full row tile
@@ -956,9 +1003,9 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   }
   const unsigned grid = static_cast<unsigned>(sm_count());
   if (max_q * a.group <= 8)
-    paged_step_kernel<D, 1><<<grid, STEP_THREADS, StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+    paged_step_kernel<D, 1><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
   else
-    paged_step_kernel<D, 2><<<grid, STEP_THREADS, StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+    paged_step_kernel<D, 2><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
   SPINF_CUDA_OK(cudaGetLastError());
   if (max_q * a.group > STEP_ROWS)
     SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, 1, tmK, tmV, s, a, status));

@@ -1,4 +1,4 @@
-// Attention of a chunk of new tokens over the paged K/V cache (sequences with more than 128 query rows per kv head), tcgen05 + TMEM +
+// Attention of a chunk of new tokens over the paged K/V cache (sequences with more than 32 query rows per kv head and head set), tcgen05 + TMEM +
 // TMA.
 //
 // An item is 256 query rows of one kv head in two tiles of 128: `hp` heads that share it x 256 / hp tokens, the first half of the
@@ -902,9 +902,11 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ok = mbar_wait(wc, q_full, seg_n & 1u, ST_TIMEOUT_FULL) && mbar_wait(wc, &k_full[gt % NS], (gt / NS) & 1u, ST_TIMEOUT_FULL);
         if (!ok) break;
         tc_fence_after();
+        const bool both = g.tok0 + (128 >> a.hp_log2) < g.nq;  // few rows: the second tile has none, and no products
         // S of tile x may replace P of the last segment's end: its P V was issued before
         issue_s(0, gt);
-        issue_s(1, gt);
+        if (both) issue_s(1, gt);
+        else umma_commit(&s_done[NS + gt % NS]);
         for (int i = 0; i < n_tiles && ok; ++i) {
           const uint32_t gi = gt + i, st = gi % NS;
           const bool more = i + 1 < n_tiles;
@@ -919,6 +921,11 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (ok && i == 0 && seg_n > 0) ok = mbar_wait(wc, &o_free[tile], (seg_n - 1) & 1u, ST_TIMEOUT_OTHER);
             if (!ok) break;
             tc_fence_after();
+            if (tile == 1 && !both) {  // the copies wait for the second tile's barriers
+              umma_commit(&o_done[NS + st]);
+              if (more) umma_commit(&s_done[NS + (gi + 1) % NS]);
+              break;
+            }
 #pragma unroll
             for (int k = 0; k < 8; ++k)  // packed bf16 P: 16 keys per 8 columns
               umma_f16_ts(tmem_base + L::O_COL + tile * D, tmem_base + tile * 128 + (k >> 2) * CH_KH + 8 * (k & 3), vd + 128 * k, IDESC_O, (i | k) != 0);
@@ -954,6 +961,11 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         alive = __all_sync(0xffffffffu, mbar_wait(wc, &s_done[tile * NS + gi % NS], (gi / NS) & 1u, ST_TIMEOUT_TMEM));
         if (!alive) break;
         tc_fence_after();
+        if (tok_first >= g.nq) {  // no rows in this tile: only the barriers' phases are kept
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[tile]);
+          continue;
+        }
         const bool masked = jb + PG_TILE - 1 > hi_min || jb < lo_max;
         // p against the reference maximum as it stands, the scores' own maximum found on the way: no pass over the scores before the
         // exponentials. Only where a row outgrew the threshold (or has no maximum yet) is the half done again. The reference is a whole
@@ -1003,6 +1015,11 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       alive = __all_sync(0xffffffffu, mbar_wait(wc, &o_done[tile * NS + (gt - 1) % NS], ((gt - 1) / NS) & 1u, ST_TIMEOUT_TMEM));
       if (!alive) break;
       tc_fence_after();
+      if (tok_first >= g.nq) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[tile]);
+        continue;
+      }
       const float inv = l_run > 0.f ? 1.f / l_run : (l_run == 0.f ? 0.f : l_run);
       chunk_store<D, D>(a, g, o_tmem, 0, tile, qd, lane, inv, stage, [&] {
         tc_fence_before();
