@@ -106,7 +106,7 @@ __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttn
   c.quot = c.work / c.units;
   c.rem = c.work - c.quot * c.units;
   // many short items (a window): a cut would cost about as much as the imbalance it removes
-  c.whole = c.ntt * c.per_tt >= 2 * most && tiles <= 24 * c.ntt;
+  c.whole = 2 * c.ntt * c.per_tt >= most && tiles <= 24 * c.ntt;
   return c;
 }
 

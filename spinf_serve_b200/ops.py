@@ -606,53 +606,77 @@ def embed_scale(ids, emb, scale):
     return out
 
 
-# ---- paged K/V cache. A decoding step makes these calls once per layer, for a few microseconds of GPU work each: the checks are one
-# expression each on the way through, and say what is wrong only when one fails.
-_I32, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
+# ---- paged K/V cache. A decoding step makes these calls once per layer, for a few microseconds of GPU work each, so the host side is
+# kept short: everything that follows from shapes, strides and types is checked and worked out once per layout (the *_layout functions
+# below remember it by exactly those), and a call itself looks at devices and addresses only.
+_I32, _BF16, _F32, _U8 = torch.int32, torch.bfloat16, torch.float32, torch.uint8
 
 
-@functools.lru_cache(maxsize=256)
-def _page_layout(shape, k_stride, v_stride):
-    """a pool's shape and strides, checked -> (pages, kv heads, page, D, the strides of k and v for the C entry points)"""
-    n_pages, h, page, D = shape
-    if page < 16 or page > 256 or page & (page - 1) or D not in (128, 256):
-        raise SpinfError(f"pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {page} of {D}")
-    if k_stride[3] != 1 or v_stride[3] != 1 or any(x % 8 for x in k_stride[:3] + v_stride[:3]):
-        raise SpinfError(f"pages need unit stride over D and strides that are multiples of 8 elements, got {k_stride} and {v_stride}")
+def _layout(t):
+    return None if t is None else (t.dtype, t.shape, t.stride())
+
+
+def _page_layout(k, v, what):
+    """a pool's layout -> (pages, kv heads, page, D, the strides of k and v for the C entry points)"""
+    for name, t in (("k_pages", k), ("v_pages", v)):
+        if t[0] is not _BF16 or len(t[1]) != 4 or t[2][3] != 1 or any(x % 8 for x in t[2][:3]):
+            raise SpinfError(f"{what}: {name} must be a bf16 [pages, kv heads, page, D] tensor or view with unit stride over D and strides that are multiples of 8, got {t}")
+    if k[1] != v[1]:
+        raise SpinfError(f"{what}: k_pages and v_pages must agree in shape, got {tuple(k[1])} and {tuple(v[1])}")
+    n_pages, h, page, D = k[1]
+    if page < 16 or page > 256 or page & (page - 1) or D not in (128, 256) or n_pages < 1 or h < 1:
+        raise SpinfError(f"{what}: pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {tuple(k[1])}")
     i64x3 = ctypes.c_int64 * 3
-    return n_pages, h, page, D, i64x3(*k_stride[:3]), i64x3(*v_stride[:3])
+    return n_pages, h, page, D, i64x3(*k[2][:3]), i64x3(*v[2][:3])
 
 
-def _pages(k_pages, v_pages, what):
-    """the pools of a paged call, [pages, kv heads, page, D] with unit stride over D -> device index and _page_layout"""
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not _BF16 or t.dim() != 4:
-            raise SpinfError(f"{what}: {name} must be a CUDA bf16 [pages, kv heads, page, D] tensor or view")
-    if v_pages.shape != k_pages.shape or v_pages.get_device() != k_pages.get_device():
-        raise SpinfError(f"{what}: k_pages and v_pages must agree in shape and device")
-    idx = k_pages.get_device()
-    _lib.init(idx)
-    return idx, _page_layout(k_pages.shape, k_pages.stride(), v_pages.stride())
+def _index_layout(what, lens, table, cu=None, new_table=None):
+    """layouts of the index tensors -> (number of sequences, entries of a table's row, its pitch[, the same of new_table])"""
+    if any(x is not None and x[0] is not _I32 for x in (lens, table, cu, new_table)):
+        raise SpinfError(f"{what}: lens, cu and the page tables must be int32 tensors")
+    B = lens[1][0] if len(lens[1]) == 1 else -1
+    if B < 0 or (B > 1 and lens[2][0] != 1) or (cu is not None and (len(cu[1]) != 1 or cu[1][0] != B + 1 or (B > 0 and cu[2][0] != 1))):
+        raise SpinfError(f"{what}: lens must be a contiguous [B] tensor and cu a contiguous [B + 1] tensor, got {lens} and {cu}")
+    out = [B]
+    for x in (table, new_table):
+        if x is None:
+            continue
+        if len(x[1]) != 2 or x[1][0] != B or (x[1][1] > 1 and x[2][1] != 1) or (B > 1 and x[2][0] < x[1][1]):
+            raise SpinfError(f"{what}: a page table must be [B, pages] with contiguous rows for the {B} sequences of lens, got {x}")
+        out += [x[1][1], x[2][0] if B > 1 else x[1][1]]
+    return out
 
 
-def _paged_index(what, idx, lens, table, cu=None, new_table=None):
-    """the index tensors of a paged call: int32 on the pages' device, rows of the tables contiguous -> number of sequences"""
-    tensors = [x for x in (lens, table, cu, new_table) if x is not None]
-    if not all(isinstance(x, torch.Tensor) and x.dtype is _I32 and x.get_device() == idx for x in tensors):
-        raise SpinfError(f"{what}: lens, cu and the page tables must be int32 tensors on the pages' device")
-    B = lens.numel()
-    if lens.dim() != 1 or (cu is not None and (cu.dim() != 1 or cu.numel() != B + 1)):
-        raise SpinfError(f"{what}: lens must be [B] and cu [B + 1], got {tuple(lens.shape)}" + ("" if cu is None else f" and {tuple(cu.shape)}"))
-    for x in (table,) if new_table is None else (table, new_table):
-        if x.dim() != 2 or x.shape[0] != B or (x.shape[1] > 1 and x.stride(1) != 1) or (B > 1 and x.stride(0) < x.shape[1]):
-            raise SpinfError(f"{what}: a page table must be [B, pages] with contiguous rows for the {B} sequences of lens, got {tuple(x.shape)}, strides {x.stride()}")
-    if not lens.is_contiguous() or (cu is not None and not cu.is_contiguous()):
-        raise SpinfError(f"{what}: lens and cu must be contiguous")
-    return B
+def _row_layout(t, name, what, heads=None):
+    """[n, columns] rows or [n, heads, D] rows of contiguous heads -> row pitch"""
+    _, shape, stride = t
+    width = shape[1] if heads is None else heads * shape[2]
+    if stride[-1] != 1 and shape[-1] > 1 or (heads is not None and heads > 1 and stride[1] != shape[2]):
+        raise SpinfError(f"{what}: {name} needs rows without gaps (any row pitch), got {t}")
+    return stride[0] if shape[0] > 1 else width
 
 
-def _row_pitch(t, width):
-    return t.stride(0) if t.shape[0] > 1 else width
+@functools.lru_cache(maxsize=512)
+def _append_layout(qkv, H, Hkv, D, k, v, table, lens, cu, wq, wk, cos, sin):
+    what = "paged_append"
+    n_pages, h, page, Dp, ks, vs = _page_layout(k, v, what)
+    if qkv[0] is not _BF16 or len(qkv[1]) != 2 or H < 1 or h != Hkv or Dp != D or qkv[1][1] != (H + 2 * Hkv) * D:
+        raise SpinfError(f"{what}: qkv {qkv} and pages {tuple(k[1])} do not fit {H} / {Hkv} heads of {D} in bf16")
+    n = qkv[1][0]
+    if (wq is None) != (wk is None) or (cos is None) != (sin is None):
+        raise SpinfError(f"{what}: wq and wk, cos and sin come together")
+    for t in (wq, wk):
+        if t is not None and (t[0] is not _BF16 or tuple(t[1]) != (D,) or t[2] != (1,)):
+            raise SpinfError(f"{what}: wq and wk must be contiguous bf16 [{D}] tensors, got {t}")
+    rot = 0
+    for t in (cos, sin):
+        if t is None:
+            continue
+        rot = 2 * t[1][-1]
+        if t[0] is not _BF16 or t[1] != cos[1] or tuple(t[1]) != (n, rot // 2) or rot > D or rot % 16 or (n > 1 and t[2][0] != rot // 2) or (rot > 2 and t[2][1] != 1):
+            raise SpinfError(f"{what}: cos and sin must be contiguous bf16 [n, R/2] with R a multiple of 16 of at most D, got {cos} and {sin}")
+    B, width, pitch = _index_layout(what, lens, table, cu)
+    return n, _row_layout(qkv, "qkv", what), rot, n_pages, page, ks, vs, pitch, width, B
 
 
 def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=None, cos=None, sin=None, eps=1e-6, plus1=False, norm_v=False):
@@ -661,27 +685,10 @@ def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=
     1 + w); norm_v: norm of v without weight; cos, sin [n, R/2] bf16 (rope_table): rotary embedding over the first R dimensions.
     Without norms of q and rotation the returned q is a view of qkv."""
     what = "paged_append"
-    idx, (n_pages, h, page, Dp, ks, vs) = _pages(k_pages, v_pages, what)
-    if not isinstance(qkv, torch.Tensor) or qkv.dtype is not _BF16 or qkv.get_device() != idx or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
-        raise SpinfError(f"{what}: qkv must be a bf16 [n, (H + 2 Hkv) D] tensor on the pages' device with unit stride over its columns")
-    n, width = qkv.shape
-    if h != Hkv or Dp != D or H < 1 or width != (H + 2 * Hkv) * D:
-        raise SpinfError(f"{what}: qkv {tuple(qkv.shape)} and pages {tuple(k_pages.shape)} do not fit {H} / {Hkv} heads of {D}")
-    if (wq is None) != (wk is None) or (cos is None) != (sin is None):
-        raise SpinfError(f"{what}: wq and wk, cos and sin come together")
-    if wq is not None:
-        for t in (wq, wk):
-            if t.dtype is not _BF16 or t.get_device() != idx or t.dim() != 1 or t.numel() != D or not t.is_contiguous():
-                raise SpinfError(f"{what}: wq and wk must be contiguous bf16 [{D}] tensors on the pages' device")
-    rot = 0
-    if cos is not None:
-        rot = 2 * cos.shape[-1]
-        if cos.shape != (n, rot // 2) or sin.shape != cos.shape or rot > D or rot % 16:
-            raise SpinfError(f"{what}: cos and sin must be [n, R/2] with R a multiple of 16 of at most D, got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        for t in (cos, sin):
-            if t.dtype is not _BF16 or t.get_device() != idx or not t.is_contiguous():
-                raise SpinfError(f"{what}: cos and sin must be contiguous bf16 tensors on the pages' device")
-    B = _paged_index(what, idx, lens, table, cu)
+    n, q_pitch, rot, n_pages, page, ks, vs, pitch, width, B = _append_layout(
+        _layout(qkv), H, Hkv, D, _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cu), _layout(wq), _layout(wk), _layout(cos), _layout(sin)
+    )
+    idx = _paged_device(what, qkv, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin)
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
             return paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin, eps, plus1, norm_v)
@@ -689,15 +696,64 @@ def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=
     q = qkv.new_empty((n, H, D)) if moved else qkv[:, : H * D].view(n, H, D)
     check(
         _lib.lib().spinf_paged_append(
-            qkv.data_ptr(), _row_pitch(qkv, width), n, H, Hkv, D, wq.data_ptr() if wq is not None else None, wk.data_ptr() if wq is not None else None,
+            qkv.data_ptr(), q_pitch, n, H, Hkv, D, wq.data_ptr() if wq is not None else None, wk.data_ptr() if wq is not None else None,
             cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, rot, eps, plus1, norm_v, q.data_ptr() if moved else None,
-            k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(), _row_pitch(table, table.shape[1]), table.shape[1],
-            lens.data_ptr(), cu.data_ptr(), B, _lib.raw_stream(idx),
+            k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(), pitch, width, lens.data_ptr(), cu.data_ptr(), B,
+            _lib.raw_stream(idx),
         ),
         what,
     )
     COUNTS["launches"] += 1
     return q
+
+
+def _paged_device(what, *tensors):
+    """the one CUDA device of a paged call's tensors"""
+    idx = -2
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d != idx:
+                if idx != -2:
+                    raise SpinfError(f"{what}: the tensors lie on different devices")
+                idx = d
+    if idx < 0:
+        raise SpinfError(f"{what}: expected CUDA tensors (this library has no CPU path)")
+    _lib.init(idx)
+    return idx
+
+
+@functools.lru_cache(maxsize=512)
+def _attention_layout(q, k, v, table, lens, cu, max_q, window, w_in, w_out, max_len, out):
+    what = "paged_attention"
+    n_pages, h, page, D, ks, vs = _page_layout(k, v, what)
+    if q[0] is not _BF16 or len(q[1]) != 3 or q[1][2] != D:
+        raise SpinfError(f"{what}: q must be a bf16 [n, H, {D}] tensor, got {q}")
+    n, H = q[1][:2]
+    if H % h or H == 0:
+        raise SpinfError(f"{what}: {H} query heads do not share {h} key / value heads evenly")
+    if out is not None and (out[0] is not _BF16 or out[1] != q[1]):
+        raise SpinfError(f"{what}: out must be a bf16 tensor of q's shape, got {out}")
+    q_pitch = _row_layout(q, "q", what, H)
+    out_pitch = H * D if out is None else _row_layout(out, "out", what, H)
+    B, width, pitch = _index_layout(what, lens, table, cu)
+    room = width * page
+    max_len = room if max_len is None else max_len
+    if max_len < 0 or max_len > room or max_q < 0:
+        raise SpinfError(f"{what}: max_len {max_len} and max_q {max_q} must not be negative, nor max_len above what the table holds ({room})")
+    if window is not None and window < 1:
+        raise SpinfError(f"{what}: a window has at least one slot (None: no window)")
+    strides = None
+    if w_in is None and w_out is not None:
+        raise SpinfError(f"{what}: weights_out comes with weights")
+    if w_in is not None:
+        for t in (w_in, w_out):
+            if t[0] is not _F32 or len(t[1]) != 3 or tuple(t[1][:2]) != (B, h) or t[1][2] < max_len or (t[1][2] > 1 and t[2][2] != 1):
+                raise SpinfError(f"{what}: weights must be fp32 [{B}, {h}, at least {max_len}] tensors, contiguous over slots, got {t}")
+        strides = (ctypes.c_int64 * 4)(*w_in[2][:2], *w_out[2][:2])
+    need = int(_lib.lib().spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_in is not None))
+    check(need, what)
+    return n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, window or 0, strides, need
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=None, weights=None, weights_out=None, decay=1.0, max_len=None,
@@ -710,56 +766,49 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
     tensor reused between calls on one stream."""
     what = "paged_attention"
-    idx, (n_pages, h, page, D, ks, vs) = _pages(k_pages, v_pages, what)
-    if not isinstance(q, torch.Tensor) or q.dtype is not _BF16 or q.get_device() != idx or q.dim() != 3 or q.shape[2] != D:
-        raise SpinfError(f"{what}: q must be a bf16 [n, H, {D}] tensor on the pages' device")
-    n, H, _ = q.shape
-    if H % h or H == 0:
-        raise SpinfError(f"{what}: {H} query heads do not share {h} key / value heads evenly")
-    if out is not None and (out.dtype is not _BF16 or out.get_device() != idx or out.shape != q.shape):
-        raise SpinfError(f"{what}: out must be a bf16 tensor of q's shape on the pages' device")
-    for t in (q,) if out is None else (q, out):
-        if n and (t.stride(2) != 1 or (H > 1 and t.stride(1) != D)):
-            raise SpinfError(f"{what}: q and out need contiguous heads (any row pitch)")
-    B = _paged_index(what, idx, lens, table, cu)
-    room = table.shape[1] * page
-    if max_len is None:
-        max_len = room
-    if max_len < 0 or max_len > room or max_q < 0:
-        raise SpinfError(f"{what}: max_len {max_len} and max_q {max_q} must not be negative, nor max_len above what the table holds ({room})")
-    if window is not None and window < 1:
-        raise SpinfError(f"{what}: a window has at least one slot (None: no window)")
-    strides = w_in = w_out = None
-    if weights is None and weights_out is not None:
-        raise SpinfError(f"{what}: weights_out comes with weights")
-    if weights is not None:
-        if weights_out is None:
-            weights_out = weights
-        for t in (weights, weights_out):
-            if t.dtype is not _F32 or t.get_device() != idx or t.dim() != 3 or t.shape[:2] != (B, h) or t.shape[2] < max_len or (t.shape[2] > 1 and t.stride(2) != 1):
-                raise SpinfError(f"{what}: weights must be fp32 [{B}, {h}, at least {max_len}] tensors on the pages' device, contiguous over slots")
-        strides = (ctypes.c_int64 * 4)(weights.stride(0), weights.stride(1), weights_out.stride(0), weights_out.stride(1))
-        w_in, w_out = weights.data_ptr(), weights_out.data_ptr()
+    if weights is not None and weights_out is None:
+        weights_out = weights
+    n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, win, strides, need = _attention_layout(
+        _layout(q), _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cu), max_q, window, _layout(weights), _layout(weights_out),
+        max_len, _layout(out)
+    )
+    idx = _paged_device(what, q, k_pages, v_pages, table, lens, cu, weights, weights_out, out, workspace)
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
             return paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace)
     if out is None:
         out = q.new_empty((n, H, D))
-    lib = _lib.lib()
-    need = lib.spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_out is not None)
-    check(need, what)
-    if need and (workspace is None or workspace.numel() < need):
-        workspace = q.new_empty(need, dtype=torch.uint8)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = q.new_empty(need, dtype=_U8)
     check(
-        lib.spinf_paged_attention(
-            q.data_ptr(), _row_pitch(q, H * D), n, H, h, D, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(),
-            _row_pitch(table, table.shape[1]), lens.data_ptr(), cu.data_ptr(), B, max_q, max_len, window or 0, scale, w_in, w_out, strides, decay,
-            out.data_ptr(), _row_pitch(out, H * D), workspace.data_ptr() if need else None, need, _lib.raw_stream(idx),
+        _lib.lib().spinf_paged_attention(
+            q.data_ptr(), q_pitch, n, H, h, D, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(), pitch, lens.data_ptr(),
+            cu.data_ptr(), B, max_q, max_len, win, scale, None if weights is None else weights.data_ptr(), None if weights is None else weights_out.data_ptr(),
+            strides, decay, out.data_ptr(), out_pitch, workspace.data_ptr() if need else None, need, _lib.raw_stream(idx),
         ),
         what,
     )
     COUNTS["launches"] += 2 if weights is None else 3
     return out
+
+
+@functools.lru_cache(maxsize=512)
+def _evict_layout(k, v, table, lens, weights, keep, recent, new_table, max_len):
+    what = "paged_evict"
+    n_pages, h, page, D, ks, vs = _page_layout(k, v, what)
+    B, width, pitch, new_width, new_pitch = _index_layout(what, lens, table, None, new_table)
+    if keep < 1 or recent < 0 or recent > keep or keep > new_width * page:
+        raise SpinfError(f"{what}: keep {keep} needs at least one token and as many as new_table holds at most, recent {recent} between 0 and keep")
+    room, w_seq, w_head = width * page, 0, 0
+    if weights is not None:
+        if weights[0] is not _F32 or len(weights[1]) != 3 or tuple(weights[1][:2]) != (B, h) or (weights[1][2] > 1 and weights[2][2] != 1):
+            raise SpinfError(f"{what}: weights must be an fp32 [{B}, {h}, cap] tensor, contiguous over slots, got {weights}")
+        room = min(room, weights[1][2])
+        w_seq, w_head = weights[2][:2]
+    max_len = room if max_len is None else max_len
+    if max_len < 0 or max_len > room:
+        raise SpinfError(f"{what}: max_len {max_len} is more than the table and the weights hold ({room})")
+    return n_pages, h, page, D, ks, vs, B, pitch, new_pitch, max_len, w_seq, w_head, keep if weights is None else recent
 
 
 def paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table, max_len=None):
@@ -769,21 +818,10 @@ def paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table,
     name -> (new lens int32 [B], kept int32 [B, Hkv, keep]: the old slots, -1 behind the last, their weights [B, Hkv, keep] or None).
     The old pages are the caller's to reuse."""
     what = "paged_evict"
-    idx, (n_pages, h, page, D, ks, vs) = _pages(k_pages, v_pages, what)
-    B = _paged_index(what, idx, lens, table, None, new_table)
-    if keep < 1 or recent < 0 or recent > keep or keep > new_table.shape[1] * page:
-        raise SpinfError(f"{what}: keep {keep} needs at least one token and as many as new_table holds at most, recent {recent} between 0 and keep")
-    room = table.shape[1] * page
-    w_in, w_seq, w_head = None, 0, 0
-    if weights is not None:
-        if weights.dtype is not _F32 or weights.get_device() != idx or weights.dim() != 3 or weights.shape[:2] != (B, h) or (weights.shape[2] > 1 and weights.stride(2) != 1):
-            raise SpinfError(f"{what}: weights must be an fp32 [{B}, {h}, cap] tensor on the pages' device, contiguous over slots")
-        room = min(room, weights.shape[2])
-        w_in, w_seq, w_head = weights.data_ptr(), weights.stride(0), weights.stride(1)
-    if max_len is None:
-        max_len = room
-    if max_len < 0 or max_len > room:
-        raise SpinfError(f"{what}: max_len {max_len} is more than the table and the weights hold ({room})")
+    n_pages, h, page, D, ks, vs, B, pitch, new_pitch, max_len, w_seq, w_head, recent = _evict_layout(
+        _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(weights), keep, recent, _layout(new_table), max_len
+    )
+    idx = _paged_device(what, k_pages, v_pages, table, lens, weights, new_table)
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
             return paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table, max_len)
@@ -792,9 +830,9 @@ def paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table,
     w_out = None if weights is None else weights.new_empty((B, h, keep))
     check(
         _lib.lib().spinf_paged_evict(
-            k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, h, D, ks, vs, table.data_ptr(), _row_pitch(table, table.shape[1]), lens.data_ptr(), B,
-            max_len, w_in, w_seq, w_head, keep, keep if weights is None else recent, new_table.data_ptr(), _row_pitch(new_table, new_table.shape[1]),
-            new_lens.data_ptr(), kept.data_ptr(), None if w_out is None else w_out.data_ptr(), _lib.raw_stream(idx),
+            k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, h, D, ks, vs, table.data_ptr(), pitch, lens.data_ptr(), B, max_len,
+            None if weights is None else weights.data_ptr(), w_seq, w_head, keep, recent, new_table.data_ptr(), new_pitch, new_lens.data_ptr(),
+            kept.data_ptr(), None if w_out is None else w_out.data_ptr(), _lib.raw_stream(idx),
         ),
         what,
     )
