@@ -1278,7 +1278,6 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
       const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
       const int j = w.j0 + kt * PG_TILE + qd * 32 + lane, base = w.q.len - w.q.nq;
-      const int j_end = a.window > 0 ? j + a.window : 0x7fffffff;  // slots [j, j_end) see the key
       const int tile_lo = w.j0 + kt * PG_TILE;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       for (int set = 0; set < w.sets && ok; ++set)
@@ -1296,21 +1295,23 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
           const float4* lse = reinterpret_cast<const float4*>(lse_ring + sl * 64);
           const int slot0 = base + tt * w.tok;  // of the stage's first token
           const bool masked = slot0 < tile_lo + PG_TILE - 1 || (a.window > 0 && slot0 + w.tok - 1 >= tile_lo + a.window);
+          if (masked) {  // hidden scores to -inf ahead of the exponentials: no branch inside the unrolled loop
+            const int lo = j - slot0, hi = a.window > 0 ? lo + a.window : w.tok, tm = w.tok - 1;  // tokens [lo, hi) of the stage see the key; w.tok is a power of two
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const int t0 = c & tm, t1 = (c + 32) & tm;
+              v0[c] = t0 >= lo && t0 < hi ? v0[c] : 0xff800000u;
+              v1[c] = t1 >= lo && t1 < hi ? v1[c] : 0xff800000u;
+            }
+          }
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float4 z = lse[c];
-            const float zz[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int col = c * 4 + x;
-              const float sv = __uint_as_float(col < 32 ? v0[col & 31] : v1[col & 31]);
-              float p = fast_exp2(fmaf(sv, a.scale_log2, -zz[x]));
-              if (masked) {
-                const int slot = slot0 + (col & (w.tok - 1));  // w.tok is a power of two
-                p = slot >= j && slot < j_end ? p : 0.f;
-              }
-              sum[x] += p;
-            }
+            const uint32_t* v = c < 8 ? &v0[c * 4] : &v1[c * 4 - 32];
+            sum[0] += fast_exp2(fmaf(__uint_as_float(v[0]), a.scale_log2, -z.x));
+            sum[1] += fast_exp2(fmaf(__uint_as_float(v[1]), a.scale_log2, -z.y));
+            sum[2] += fast_exp2(fmaf(__uint_as_float(v[2]), a.scale_log2, -z.z));
+            sum[3] += fast_exp2(fmaf(__uint_as_float(v[3]), a.scale_log2, -z.w));
           }
           tc_fence_before();
           __syncwarp();
