@@ -1214,28 +1214,38 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     bool ok = true;
     for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
       const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+      // lse of the stage's rows r and r + 32, fetched a stage ahead (nothing looks at it before it is stored)
+      const int tl = 6 - a.hp_log2;  // log2 of a head's rows in a stage
+      float next[2] = {0.f, 0.f};
+      auto fetch = [&](int set, int tt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = lane + 32 * x, tok = (tt << tl) + (r & ((1 << tl) - 1));
+          next[x] = tok < w.q.nq ? a.lse[static_cast<int64_t>(w.q.row0 + tok) * a.H + w.g * a.group + (set << a.hp_log2) + (r >> tl)] : INFINITY;
+        }
+      };
+      if (w.tt0 < w.tt1) fetch(0, w.tt0);
       for (int set = 0; set < w.sets && ok; ++set)
         for (int tt = w.tt0; tt < w.tt1; ++tt, ++n) {
           const uint32_t st = n % NQ, sl = n % NS;
-          ok = __all_sync(0xffffffffu, mbar_wait(wc, &s_empty[sl], ((n / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY) &&
-                                           mbar_wait(wc, &q_empty[st], ((n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY));
+          ok = __all_sync(0xffffffffu, mbar_wait(wc, &q_empty[st], ((n / NQ) & 1u) ^ 1u, ST_TIMEOUT_EMPTY));
           if (!ok) break;
-          const int h0 = w.g * a.group + set * w.hp;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int r = lane + 32 * x, tok = tt * w.tok + r % w.tok;
-            float v = INFINITY;  // rows that are none, or see nothing, weigh nothing: exp2(s - inf) = 0
-            if (tok < w.q.nq) v = a.lse[static_cast<int64_t>(w.q.row0 + tok) * a.H + h0 + r / w.tok];
-            lse_ring[sl * 64 + r] = v == -INFINITY ? INFINITY : v;
-          }
-          __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&lse_full[sl]);
             mbar_expect_tx(&q_full[st], L::Q_STAGE);
             for (int hh = 0; hh < w.hp; ++hh)
               for (int x = 0; x < SLABS; ++x)
-                tma_load_2d(smem + L::Q_OFF + st * L::Q_STAGE + x * 64 * 128 + hh * w.tok * 128, &tmQ, (h0 + hh) * D + x * 64, w.q.row0 + tt * w.tok, &q_full[st]);
+                tma_load_2d(smem + L::Q_OFF + st * L::Q_STAGE + x * 64 * 128 + hh * w.tok * 128, &tmQ, (w.g * a.group + set * w.hp + hh) * D + x * 64,
+                            w.q.row0 + tt * w.tok, &q_full[st]);
           }
+          const float v0 = next[0], v1 = next[1];
+          if (tt + 1 < w.tt1) fetch(set, tt + 1);
+          else if (set + 1 < w.sets) fetch(set + 1, w.tt0);
+          ok = __all_sync(0xffffffffu, mbar_wait(wc, &s_empty[sl], ((n / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY));
+          if (!ok) break;
+          lse_ring[sl * 64 + lane] = v0 == -INFINITY ? INFINITY : v0;  // rows that are none, or see nothing, weigh nothing: exp2(s - inf) = 0
+          lse_ring[sl * 64 + lane + 32] = v1 == -INFINITY ? INFINITY : v1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&lse_full[sl]);
         }
     }
     if (*abort_flag && lane == 0)
