@@ -159,19 +159,28 @@ __global__ void __launch_bounds__(SEL_THREADS) paged_select_kernel(const PagedSe
   }
 }
 
+// Row blocks from the last one down, all sequences and heads of a block before the next: the `recent` rows, and all rows of a sequence
+// that keeps everything, move while the select is still at work; only the others wait for its answer.
 template <int D>
-__global__ void __launch_bounds__(256) paged_move_kernel(const PagedSeqs s, const EvictArgs a, int* __restrict__ status) {
+__global__ void __launch_bounds__(256) paged_move_kernel(const PagedSeqs s, const EvictArgs a, int blocks, int* __restrict__ status) {
   constexpr int LANES = D / 8, GROUPS = 256 / LANES, IPT = 4;
-  pdl_wait();
-  const int g = blockIdx.y, b = blockIdx.z, sub = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int per_block = s.B * a.h;
+  const int blk = blocks - 1 - static_cast<int>(blockIdx.x / per_block), bg = static_cast<int>(blockIdx.x % per_block);
+  const int b = bg / a.h, g = bg - b * a.h, sub = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  int len = s.lens[b];
+  len = len < 0 ? 0 : len > s.max_len ? s.max_len : len;  // (reported by the select)
+  const int quota = len > a.keep ? a.keep - a.recent : 0;  // rows the select chooses
+  const int shift = len > a.keep ? len - a.keep : 0;       // the others: old slot = row + shift
+  const int first = blk * GROUPS * IPT, i0 = first + group * IPT;
+  const bool wait = first < quota;
+  if (wait) pdl_wait();
   const int32_t* kept = a.kept + (static_cast<int64_t>(b) * a.h + g) * a.keep;
-  const int i0 = (blockIdx.x * GROUPS + group) * IPT;
-  const int in_page = (1 << s.page_log2) - 1;
+  const int in_page = (1 << s.page_log2) - 1, rows = len < a.keep ? len : a.keep;
   uint4 k[IPT], v[IPT];
   int to[IPT];
 #pragma unroll
   for (int x = 0; x < IPT; ++x) {
-    const int slot = i0 + x < a.keep ? kept[i0 + x] : -1;
+    const int slot = i0 + x >= rows ? -1 : i0 + x < quota ? kept[i0 + x] : i0 + x + shift;
     to[x] = -1;
     if (slot < 0) continue;
     const int src = s.table[b * s.table_pitch + (slot >> s.page_log2)], dst = a.new_table[b * a.new_pitch + ((i0 + x) >> s.page_log2)];
@@ -190,6 +199,7 @@ __global__ void __launch_bounds__(256) paged_move_kernel(const PagedSeqs s, cons
     *reinterpret_cast<uint4*>(const_cast<__nv_bfloat16*>(a.k) + to[x] * a.k_page + g * a.k_head + row * a.k_row + sub * 8) = k[x];
     *reinterpret_cast<uint4*>(const_cast<__nv_bfloat16*>(a.v) + to[x] * a.v_page + g * a.v_head + row * a.v_row + sub * 8) = v[x];
   }
+  if (!wait) pdl_wait();  // this kernel's end is the call's: not before the select's
 }
 
 }  // namespace spinf
@@ -208,7 +218,7 @@ extern "C" int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, 
   SPINF_CHECK_ARG(max_len >= 0 && max_len <= table_pitch * page && max_len < (1ll << 30));
   SPINF_CHECK_ARG(keep > 0 && recent >= 0 && recent <= keep && keep <= new_pitch * page && keep < (1ll << 30));
   SPINF_CHECK_ARG((weights != nullptr) == (weights_out != nullptr) && (weights || recent == keep));
-  if (B > 65535 || Hkv > 65535) return SPINF_ERR_TOO_LARGE;
+  if (B > 65535 || Hkv > 65535 || (keep / (32 * 256 / D) + 1) * Hkv * B >= (1ll << 31)) return SPINF_ERR_TOO_LARGE;
   uintptr_t bits = reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages);
   for (int i = 0; i < 3; ++i) bits |= static_cast<uintptr_t>(k_strides_host[i] | v_strides_host[i]) * 2;
   SPINF_CHECK_ARG((bits & 15) == 0);  // rows move 16 bytes at a time
@@ -240,9 +250,9 @@ extern "C" int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   paged_select_kernel<<<dim3(Hkv, B), SEL_THREADS, 0, st>>>(s, a, status);
   SPINF_CUDA_OK(cudaGetLastError());
-  const int64_t per_cta = (256 / (D / 8)) * 4;
-  const dim3 grid(static_cast<unsigned>((keep + per_cta - 1) / per_cta), Hkv, B);
-  SPINF_CUDA_OK(D == 256 ? launch_after(paged_move_kernel<256>, grid, dim3(256), st, 0, 1, s, a, status)
-                         : launch_after(paged_move_kernel<128>, grid, dim3(256), st, 0, 1, s, a, status));
+  const int64_t per_cta = (256 / (D / 8)) * 4, blocks = (keep + per_cta - 1) / per_cta;
+  const dim3 grid(static_cast<unsigned>(blocks * Hkv * B));
+  SPINF_CUDA_OK(D == 256 ? launch_after(paged_move_kernel<256>, grid, dim3(256), st, 0, 1, s, a, static_cast<int>(blocks), status)
+                         : launch_after(paged_move_kernel<128>, grid, dim3(256), st, 0, 1, s, a, static_cast<int>(blocks), status));
   return 0;
 }
