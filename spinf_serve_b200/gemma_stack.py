@@ -288,7 +288,7 @@ class GemmaStack:
         the stream layout. masks = {"full_attention": TileMask, "sliding_attention": TileMask} (attention.device_masks). Beyond the
         reference's signature: rows (int64 device tensor of stream positions) returns only those rows, [len(rows), hidden], the
         last norm running on them alone; taps: optional dict filled with per-layer intermediates (tests); attend(layer, kind, q, k,
-        v) -> [n, H, D] replaces the tree attention (the extraction decoder's steps: masks is unused then)."""
+        v) -> [n, H, D] replaces the tree attention (the extraction decoder's steps, the paged cache: masks is unused then)."""
         cfg, w = self.cfg, self.w
         H, K, D = cfg.heads, cfg.kv_heads, cfg.head_dim
         ids, pos = inputs["ids"].reshape(-1), inputs["pos"].reshape(-1)
@@ -297,6 +297,7 @@ class GemmaStack:
         fp8 = w.scheme in ("fp8row", "fp8", "fp8s")
         # a decoding step's few rows: the narrow projections run with their K dimension cut into slices
         row_gemm = ops.fp8_rowwise_gemm_small if attend is not None and n <= 128 else ops.fp8_rowwise_gemm
+        project = getattr(attend, "project", None)  # takes the bare projection: head norms and rotation are its own (paged.PagedReader)
         tables = {k: ops.rope_table(pos, f) for k, f in self.inv_freq.items()}
         h = ops.embed_scale(ids, w.embed, self.embed_scale)
         for start, obj in inputs.get("media", ()):  # the media rows over their placeholders, not scaled (gemma4.py:410-413)
@@ -316,7 +317,8 @@ class GemmaStack:
                 qkv = ops.fp8_gemm_qkv(x8, xs, L["qkv_w"], L["qkv_s"], H, K, D, L["q_norm"], L["k_norm"], cos, sin, cfg.eps)
             else:
                 qkv = ops.fp8_rowwise_gemm(x8, xs, L["qkv_w"], L["qkv_s"]) if fp8 else self._linear(r["norm"], L, "qkv", ("q", "k", "v"))
-                ops.qkv_norm_rope(qkv, H, K, D, L["q_norm"], L["k_norm"], cos, sin, cfg.eps)
+                if project is None:
+                    ops.qkv_norm_rope(qkv, H, K, D, L["q_norm"], L["k_norm"], cos, sin, cfg.eps)
             q = qkv[:, : H * D].view(n, H, D)
             k = qkv[:, H * D : (H + K) * D].view(n, K, D)
             v = qkv[:, (H + K) * D :].view(n, K, D)
@@ -326,7 +328,8 @@ class GemmaStack:
                     a0 = start + (max(0, cnt - keep) if kind == "sliding_attention" else 0)
                     self._cap["kv"].setdefault(key, {})[i] = (k[a0 : start + cnt].clone(), v[a0 : start + cnt].clone())
             if attend is not None:
-                a = attend(i, kind, q, k, v)
+                bare = project is not None and not (fp8 and self.fuse_qkv)
+                a = project(i, kind, qkv, L["q_norm"], L["k_norm"], cos, sin, cfg.eps) if bare else attend(i, kind, q, k, v)
                 amax = None
             else:
                 amax = torch.zeros(n, dtype=torch.float32, device=qkv.device) if row else None

@@ -1,0 +1,222 @@
+"""Reading a content once and asking about it later: a paged K/V cache for the attention layers of a stack, and the forward passes over
+it. The scoring pass reads a content and all its questions in one stream and forgets both; the extraction decoder keeps padded copies
+of what one pass captured. Here the keys and values stay in pages: a content is read in chunks of any length, questions that come
+later run as forks that share the content's pages, a sequence goes on token by token, and a cache that has grown too long is cut back
+to the slots that were attended to most (ops.paged_append, ops.paged_attention, ops.paged_evict).
+
+The host keeps the books (which pages a sequence holds, who shares them, how far it is); tables and lengths go to the device once per
+forward and serve all its layers."""
+
+from dataclasses import dataclass, field
+
+import torch
+
+from spinf_serve_b200 import ops
+
+
+@dataclass
+class Sequence:
+    """one cached sequence: its pages in slot order, cached slots, and the position of its next token (past `length` once slots were
+    evicted). weights: fp32 [layers, kv heads, cap] accumulated attention weight of every slot, where it is kept"""
+
+    pages: list = field(default_factory=list)
+    length: int = 0
+    position: int = 0
+    weights: torch.Tensor | None = None
+
+
+@dataclass
+class Step:
+    """the device side of one forward over some sequences' new tokens"""
+
+    table: torch.Tensor
+    lens: torch.Tensor
+    cu: torch.Tensor
+    pos: torch.Tensor
+    max_q: int
+    max_len: int
+
+
+class PagedCache:
+    """pools of pages for `layers` attention layers, [layers][pages, kv heads, page, D] for K and for V; a page index means the same
+    tokens in every layer"""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, n_pages: int, page: int = 64, device="cuda:0"):
+        if page < 16 or page > 256 or page & (page - 1) or head_dim not in (128, 256) or n_pages < 1:
+            raise RuntimeError(f"pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {n_pages} pages of {page} x {head_dim}")
+        self.page, self.n_pages, self.device = page, n_pages, torch.device(device)
+        self.k, self.v = (torch.empty((layers, n_pages, kv_heads, page, head_dim), dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        self.free = list(range(n_pages - 1, -1, -1))
+        self.refs = [0] * n_pages
+
+    def _take(self, n: int) -> list:
+        if n > len(self.free):
+            raise RuntimeError(f"the cache is out of pages: {n} wanted, {len(self.free)} of {self.n_pages} free")
+        out = [self.free.pop() for _ in range(n)]
+        for p in out:
+            self.refs[p] = 1
+        return out
+
+    def _release(self, pages) -> None:
+        for p in pages:
+            self.refs[p] -= 1
+            if self.refs[p] == 0:
+                self.free.append(p)
+
+    def open(self) -> Sequence:
+        return Sequence()
+
+    def close(self, seq: Sequence) -> None:
+        self._release(seq.pages)
+        seq.pages, seq.length, seq.position, seq.weights = [], 0, 0, None
+
+    def fork(self, seq: Sequence) -> Sequence:
+        """a sequence that goes on from where `seq` is: full pages are shared, a begun one is copied (both may go on writing)"""
+        whole = seq.length // self.page
+        last = self._take(1) if seq.length % self.page else []
+        for p in seq.pages[:whole]:
+            self.refs[p] += 1
+        if last:
+            old = seq.pages[whole]
+            for pool in (self.k, self.v):
+                pool[:, last[0]].copy_(pool[:, old])
+        return Sequence(seq.pages[:whole] + last, seq.length, seq.position)
+
+    def grow(self, seqs: list, counts: list) -> Step:
+        """room for counts[i] new tokens of seqs[i] (0: the sequence sits this one out) -> the forward's tables. The same sequence
+        twice in one call is an error: its tokens would take the same slots"""
+        if len(seqs) != len(counts) or not seqs or any(c < 0 for c in counts):
+            raise RuntimeError("one count of new tokens per sequence, none negative")
+        if len({id(s) for s in seqs}) != len(seqs):
+            raise RuntimeError("a sequence can be extended once per forward")
+        need = [-(-(s.length + c) // self.page) - len(s.pages) for s, c in zip(seqs, counts)]
+        pages = self._take(sum(need))  # all or none
+        cu, pos = [0], []
+        for s, c, n in zip(seqs, counts, need):
+            s.pages += [pages.pop() for _ in range(n)]
+            pos += range(s.position, s.position + c)
+            s.length += c
+            s.position += c
+            cu.append(cu[-1] + c)
+        width = max(1, max(len(s.pages) for s in seqs))
+        table = torch.tensor([s.pages + [0] * (width - len(s.pages)) for s in seqs], dtype=torch.int32)
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
+        return Step(table.to(self.device), i32([s.length for s in seqs]), i32(cu), i32(pos), max(counts), max(s.length for s in seqs))
+
+    def evict(self, seq: Sequence, keep: int, recent: int, by_weight: list) -> list | None:
+        """cuts the sequence back to `keep` slots in every layer: by accumulated weight where by_weight[layer], else the last `keep`.
+        Its pages are left to whoever shares them, what stays goes to new ones -> per layer the kept old slots [kv heads, keep]
+        (None: nothing to cut)"""
+        if not 0 <= recent <= keep or keep < 1:
+            raise RuntimeError(f"keep {keep} and recent {recent}: at least one slot, and no more recent ones than kept ones")
+        if seq.length <= keep:
+            return None
+        if any(by_weight) and seq.weights is None:
+            raise RuntimeError("the sequence was read without its slots' weights")
+        pages = self._take(-(-keep // self.page))
+        i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=self.device)  # noqa: E731
+        table, new_table, lens = i32(seq.pages), i32(pages), torch.tensor([seq.length], dtype=torch.int32, device=self.device)
+        kept = []
+        for li in range(self.k.shape[0]):
+            w = seq.weights[li][None] if by_weight[li] else None
+            _, slots, w_new = ops.paged_evict(self.k[li], self.v[li], table, lens, w, keep, recent, new_table, max_len=seq.length)
+            if w is not None:
+                seq.weights[li, :, :keep] = w_new[0]
+            kept.append(slots[0])
+        self._release(seq.pages)
+        seq.pages, seq.length = pages, keep
+        return kept
+
+
+class PagedReader:
+    """forward passes of a GemmaStack over a PagedCache. `read` takes a content in, `ask` runs questions that share it, `forward` is one
+    pass over new tokens of any sequences, `evict` cuts a sequence back"""
+
+    def __init__(self, stack, n_pages: int, page: int = 64, chunk: int = 2048):
+        cfg = stack.cfg
+        if getattr(stack, "hybrid", False):
+            raise RuntimeError("the paged cache holds attention layers only: a hybrid stack's recurrent states are the decoder's (decode.HybridDecoder)")
+        self.stack, self.chunk = stack, chunk
+        self.cache = PagedCache(stack.n_layers, cfg.kv_heads, cfg.head_dim, n_pages, page, stack.w.embed.device)
+        self.scaling = 1.0  # the Gemma-style layers norm q and k and attend with scaling 1
+        self._step, self._weights = None, None
+
+    # ---- the stack's attention (GemmaStack.forward, `attend`)
+    def _attend(self, i, kind, q):
+        st, c, cfg = self._step, self.cache, self.stack.cfg
+        sliding = kind == "sliding_attention"
+        w = None if self._weights is None or sliding else self._weights[i][None]
+        return ops.paged_attention(q, c.k[i], c.v[i], st.table, st.lens, st.cu, st.max_q, self.scaling, window=cfg.window if sliding else None,
+                                   weights=w, max_len=st.max_len)
+
+    def __call__(self, i, kind, q, k, v):
+        """q, k, v normed and rotated, side by side in one projection's rows: k and v into the pages, then the attention"""
+        c, cfg, st = self.cache, self.stack.cfg, self._step
+        qkv = torch.as_strided(q, (q.shape[0], (cfg.heads + 2 * cfg.kv_heads) * cfg.head_dim), (q.stride(0), 1))
+        ops.paged_append(qkv, cfg.heads, cfg.kv_heads, cfg.head_dim, c.k[i], c.v[i], st.table, st.lens, st.cu)
+        return self._attend(i, kind, q)
+
+    def project(self, i, kind, qkv, wq, wk, cos, sin, eps):
+        """the same from the bare projection: head norms and rotation on the way into the pages"""
+        c, cfg, st = self.cache, self.stack.cfg, self._step
+        q = ops.paged_append(qkv, cfg.heads, cfg.kv_heads, cfg.head_dim, c.k[i], c.v[i], st.table, st.lens, st.cu, wq, wk, cos, sin, eps, norm_v=True)
+        return self._attend(i, kind, q)
+
+    def forward(self, seqs: list, ids: list, last: bool = True, weigh: bool = False):
+        """one pass over new tokens: ids[i] (token ids) goes on from seqs[i] -> hidden states after the last norm at every sequence's
+        last new token [len(seqs), hidden] (last=False: at all new tokens, sequence after sequence). weigh: the slots' attention
+        weights are added up (one sequence, full-attention layers). The attention runs in calls of at most 1 024 sequences"""
+        if weigh and len(seqs) != 1:
+            raise RuntimeError("weights are kept for a sequence that is read alone")
+        if not all(len(x) for x in ids) or len(seqs) > 1024:
+            raise RuntimeError("every sequence of a forward (at most 1024) needs new tokens")
+        st = self.cache.grow(seqs, [len(x) for x in ids])
+        dev = self.cache.device
+        if weigh:
+            seq, cap = seqs[0], len(seqs[0].pages) * self.cache.page
+            if seq.weights is None or seq.weights.shape[2] < cap:
+                old = seq.weights
+                seq.weights = torch.zeros((self.stack.n_layers, self.stack.cfg.kv_heads, -(-cap // 1024) * 1024), dtype=torch.float32, device=dev)
+                if old is not None:
+                    seq.weights[:, :, : old.shape[2]] = old
+            seq.weights[:, :, seq.length - len(ids[0]) : seq.length] = 0.0
+        self._step, self._weights = st, seqs[0].weights if weigh else None
+        try:
+            inputs = {"ids": torch.cat([torch.as_tensor(x, dtype=torch.int64) for x in ids]).to(dev), "pos": st.pos}
+            rows = (st.cu[1:].long() - 1) if last else None
+            out = self.stack.forward(None, None, inputs, None, rows=rows, attend=self)
+        except BaseException:
+            for s, x in zip(seqs, ids):  # the sequences stay where they were (their new pages are kept for the next try)
+                s.length -= len(x)
+                s.position -= len(x)
+            raise
+        finally:
+            self._step = self._weights = None
+        return out if last else out[0]
+
+    def read(self, ids, weigh: bool = False) -> Sequence:
+        """a content's tokens into a new sequence, `chunk` at a time"""
+        seq = self.cache.open()
+        for at in range(0, len(ids), self.chunk):
+            self.forward([seq], [ids[at : at + self.chunk]], weigh=weigh)
+        return seq
+
+    def ask(self, seq: Sequence, branches: list):
+        """questions (token ids each) about a content that was read: every branch attends to the content and itself only, as in the
+        scoring pass -> hidden states at the branches' last tokens [len(branches), hidden]. The sequence itself stays as it is"""
+        forks = []
+        try:
+            for _ in branches:
+                forks.append(self.cache.fork(seq))
+            return self.forward(forks, branches)
+        finally:
+            for f in forks:
+                self.cache.close(f)
+
+    def evict(self, seq: Sequence, keep: int, recent: int):
+        """cuts the sequence back to `keep` slots: on full-attention layers the last `recent` and, of the others, those with the largest
+        accumulated weight; sliding layers keep the last `keep`, which has to cover their window"""
+        kinds = [self.stack.cfg.layer_types[i] for i in range(self.stack.n_layers)]
+        if "sliding_attention" in kinds and keep < self.stack.cfg.window and seq.length > keep:
+            raise RuntimeError(f"keep {keep} is less than the sliding layers' window {self.stack.cfg.window}")
+        return self.cache.evict(seq, keep, recent, [k != "sliding_attention" for k in kinds])

@@ -1,0 +1,182 @@
+"""The paged cache without a GPU: the book-keeping of pages, and what the operators refuse before any CUDA work."""
+
+import ctypes
+
+import pytest
+import torch
+
+from spinf_serve_b200 import _lib, ops
+from spinf_serve_b200.paged import PagedCache
+
+
+def _cache(n=12, page=16):
+    return PagedCache(2, 3, 128, n, page, device="cpu")
+
+
+def test_pages_are_shared_copied_and_returned():
+    c = _cache()
+    a = c.open()
+    st = c.grow([a], [40])
+    assert len(a.pages) == 3 and a.length == a.position == 40 and st.table.tolist() == [a.pages] and st.lens.tolist() == [40] and st.cu.tolist() == [0, 40]
+    assert st.pos.tolist() == list(range(40)) and (st.max_q, st.max_len) == (40, 40)
+    c.k[:, a.pages[2]], c.v[:, a.pages[2]] = 5.0, 6.0
+    b = c.fork(a)
+    assert b.pages[:2] == a.pages[:2] and b.pages[2] != a.pages[2]  # the begun page is copied
+    assert (c.k[:, b.pages[2]] == 5.0).all() and (c.v[:, b.pages[2]] == 6.0).all()
+    assert [c.refs[p] for p in a.pages] == [2, 2, 1]
+    st = c.grow([a, b], [0, 9])
+    assert a.length == 40 and b.length == 49 and len(b.pages) == 4 and st.table.shape == (2, 4) and st.cu.tolist() == [0, 0, 9] and st.pos.tolist() == list(range(40, 49))
+    c.close(a)
+    assert c.refs[b.pages[0]] == 1 and len(c.free) == 12 - 4
+    c.close(b)
+    assert sorted(c.free) == list(range(12)) and b.pages == []
+
+
+def test_a_fork_of_whole_pages_shares_them_all():
+    c = _cache()
+    a = c.open()
+    c.grow([a], [32])
+    b = c.fork(a)
+    assert b.pages == a.pages
+    c.grow([b], [1])
+    assert len(b.pages) == 3 and len(a.pages) == 2
+
+
+def test_running_out_of_pages_changes_nothing():
+    c = _cache(4)
+    a, b = c.open(), c.open()
+    c.grow([a], [20])
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c.grow([a, b], [30, 17])
+    assert a.length == 20 and len(a.pages) == 2 and b.pages == [] and len(c.free) == 2
+    c.grow([a, b], [12, 17])
+    assert len(c.free) == 0
+
+
+def test_refused_steps():
+    c = _cache()
+    a = c.open()
+    for seqs, counts in (([a], [1, 2]), ([], []), ([a], [-1]), ([a, a], [1, 1])):
+        with pytest.raises(RuntimeError):
+            c.grow(seqs, counts)
+    c.grow([a], [30])
+    for keep, recent in ((0, 0), (5, 6), (5, -1)):
+        with pytest.raises(RuntimeError):
+            c.evict(a, keep, recent, [False, False])
+    with pytest.raises(RuntimeError, match="weights"):
+        c.evict(a, 5, 2, [True, False])
+    assert c.evict(a, 30, 4, [True, True]) is None and a.length == 30
+    for args in ((2, 3, 128, 4, 24), (2, 3, 64, 4, 16), (2, 3, 128, 0, 16), (2, 3, 128, 4, 512)):
+        with pytest.raises(RuntimeError):
+            PagedCache(*args, device="cpu")
+
+
+def _call(**kw):
+    """a well-formed attention call but for the device"""
+    a = dict(q=torch.zeros((5, 4, 128), dtype=torch.bfloat16), k_pages=torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16),
+             v_pages=torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16), table=torch.zeros((2, 3), dtype=torch.int32),
+             lens=torch.tensor([20, 30], dtype=torch.int32), cu=torch.tensor([0, 2, 5], dtype=torch.int32), max_q=3, scale=0.1)
+    return ops.paged_attention(**{**a, **kw})
+
+
+@pytest.mark.parametrize("kw,what", [
+    ({}, "CUDA"),
+    ({"q": torch.zeros((5, 4, 128))}, "bf16"),
+    ({"q": torch.zeros((5, 3, 128), dtype=torch.bfloat16)}, "evenly"),
+    ({"q": torch.zeros((5, 128, 4), dtype=torch.bfloat16).transpose(1, 2)}, "without gaps"),
+    ({"k_pages": torch.zeros((6, 2, 24, 128), dtype=torch.bfloat16), "v_pages": torch.zeros((6, 2, 24, 128), dtype=torch.bfloat16)}, "pages hold"),
+    ({"v_pages": torch.zeros((6, 2, 32, 128), dtype=torch.bfloat16)}, "agree"),
+    ({"k_pages": torch.zeros((6, 2, 16, 132), dtype=torch.bfloat16)[..., :128]}, "multiples of 8"),
+    ({"table": torch.zeros((2, 3), dtype=torch.int64)}, "int32"),
+    ({"table": torch.zeros((3, 3), dtype=torch.int32)}, "page table"),
+    ({"table": torch.zeros((3, 2), dtype=torch.int32).t()}, "page table"),
+    ({"cu": torch.tensor([0, 5], dtype=torch.int32)}, "cu"),
+    ({"lens": torch.zeros(4, dtype=torch.int32)[::2]}, "contiguous"),
+    ({"max_len": 49}, "max_len"),
+    ({"max_q": -1}, "max_q"),
+    ({"window": 0}, "window"),
+    ({"weights": torch.zeros((2, 2, 40))}, "weights"),
+    ({"weights": torch.zeros((2, 2, 48), dtype=torch.float64)}, "weights"),
+    ({"weights_out": torch.zeros((2, 2, 48))}, "comes with"),
+    ({"out": torch.zeros((5, 4, 128))}, "out"),
+])
+def test_attention_refusals(kw, what):
+    with pytest.raises(_lib.SpinfError, match=what):
+        _call(**kw)
+
+
+def _append(**kw):
+    a = dict(qkv=torch.zeros((5, 8 * 128), dtype=torch.bfloat16), H=4, Hkv=2, D=128, k_pages=torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16),
+             v_pages=torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16), table=torch.zeros((2, 3), dtype=torch.int32),
+             lens=torch.tensor([20, 30], dtype=torch.int32), cu=torch.tensor([0, 2, 5], dtype=torch.int32))
+    return ops.paged_append(**{**a, **kw})
+
+
+@pytest.mark.parametrize("kw,what", [
+    ({}, "CUDA"),
+    ({"H": 5}, "fit"),
+    ({"qkv": torch.zeros((5, 8 * 128))}, "fit"),
+    ({"wq": torch.zeros(128, dtype=torch.bfloat16)}, "together"),
+    ({"wq": torch.zeros(64, dtype=torch.bfloat16), "wk": torch.zeros(64, dtype=torch.bfloat16)}, "wq and wk"),
+    ({"cos": torch.zeros((5, 20), dtype=torch.bfloat16), "sin": torch.zeros((5, 20), dtype=torch.bfloat16)}, "multiple of 16"),
+    ({"cos": torch.zeros((4, 64), dtype=torch.bfloat16), "sin": torch.zeros((4, 64), dtype=torch.bfloat16)}, "cos and sin"),
+    ({"cos": torch.zeros((5, 64), dtype=torch.bfloat16), "sin": torch.zeros((5, 32), dtype=torch.bfloat16)}, "cos and sin"),
+])
+def test_append_refusals(kw, what):
+    with pytest.raises(_lib.SpinfError, match=what):
+        _append(**kw)
+
+
+def _evict(**kw):
+    a = dict(k_pages=torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16), v_pages=torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16),
+             table=torch.zeros((2, 3), dtype=torch.int32), lens=torch.tensor([20, 30], dtype=torch.int32), weights=torch.zeros((2, 2, 48)), keep=16, recent=4,
+             new_table=torch.zeros((2, 1), dtype=torch.int32))
+    return ops.paged_evict(**{**a, **kw})
+
+
+@pytest.mark.parametrize("kw,what", [
+    ({}, "CUDA"),
+    ({"keep": 0}, "keep"), ({"keep": 17}, "keep"), ({"recent": 17}, "recent"), ({"recent": -1}, "recent"),
+    ({"weights": torch.zeros((2, 3, 48))}, "weights"),
+    ({"weights": torch.zeros((2, 2, 40)), "max_len": 41}, "max_len"),
+    ({"new_table": torch.zeros((1, 1), dtype=torch.int32)}, "page table"),
+])
+def test_evict_refusals(kw, what):
+    with pytest.raises(_lib.SpinfError, match=what):
+        _evict(**kw)
+
+
+def test_the_c_entry_points_refuse_on_the_host():
+    lib = _lib.lib()
+    p, N = ctypes.c_void_p(256), None
+    st = (ctypes.c_int64 * 3)(4096, 2048, 128)
+    odd = (ctypes.c_int64 * 3)(4096, 2048, 130)
+
+    def attn(n=2, H=4, h=2, D=128, page=16, q=p, table=p, width=4, B=1, max_q=2, max_len=64, window=0, scale=1.0, w_in=N, w_out=N, strides=N, decay=1.0, ws=N, ws_bytes=0, k=st):
+        return lib.spinf_paged_attention(q, H * D, n, H, h, D, p, p, 8, page, k, st, table, width, p, p, B, max_q, max_len, window, scale, w_in, w_out, strides, decay, p, H * D, ws, ws_bytes, N)
+
+    assert attn(B=0) == 0 and attn(n=0, q=N) == 0  # nothing to do
+    for bad in (dict(q=N), dict(table=N), dict(H=3), dict(D=64), dict(page=24), dict(page=8), dict(max_len=65), dict(max_q=-1), dict(window=-1), dict(scale=0.0),
+                dict(w_out=p), dict(w_out=p, strides=(ctypes.c_int64 * 4)(), decay=1.0), dict(width=64, max_len=1024)):  # (the last: splits need a workspace)
+        assert attn(**bad) == -1, bad
+    assert attn(B=2000) == -4
+    assert lib.spinf_paged_attention_workspace_bytes(4, 2000, 4, 2, 128, 1, 64, 0) == -1
+    assert lib.spinf_paged_attention_workspace_bytes(4, 2, 4, 3, 128, 1, 64, 0) == -1
+    need = [lib.spinf_paged_attention_workspace_bytes(64, 64, 16, 8, 256, 1, n, w) for n, w in ((100, 0), (8192, 0), (8192, 1))]
+    assert need[0] == 0 and 0 < need[1] < need[2]
+
+    def append(n=2, H=4, h=2, D=128, pitch=1024, page=16, wq=N, wk=N, cos=N, sin=N, rot=0, q=N, width=4, k=st, B=1, qkv=p):
+        return lib.spinf_paged_append(qkv, pitch, n, H, h, D, wq, wk, cos, sin, rot, 1e-6, 0, 0, q, p, p, 8, page, k, st, p, width, width, p, p, B, N)
+
+    assert append(n=0, qkv=N) == 0 and append(B=0) == 0
+    for bad in (dict(qkv=N), dict(D=64), dict(pitch=1000), dict(page=20), dict(wq=p), dict(cos=p, sin=p), dict(cos=p, sin=p, rot=24, q=p), dict(cos=p, sin=p, rot=256, q=p),
+                dict(wq=p, wk=p), dict(width=0), dict(k=odd)):
+        assert append(**bad) == -1, bad
+    assert append(B=1025) == -4
+
+    def evict(keep=16, recent=4, w=p, w_out=p, new_pitch=1, max_len=64, D=128, page=16, k=st, B=1, kept=p):
+        return lib.spinf_paged_evict(p, p, 8, page, 2, D, k, st, p, 4, p, B, max_len, w, 128, 64, keep, recent, p, new_pitch, p, kept, w_out, N)
+
+    assert evict(B=0) == 0
+    for bad in (dict(keep=0), dict(keep=17), dict(recent=17), dict(recent=-1), dict(w=N), dict(w=N, w_out=N), dict(w_out=N), dict(max_len=65), dict(D=64), dict(page=48), dict(k=odd), dict(kept=N)):
+        assert evict(**bad) == -1, bad
