@@ -118,9 +118,10 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, int
       : "memory");
 }
 
-// a launch that may start before the kernel ahead of it on the stream has ended (its pdl_wait holds it back)
+// a launch that, with `early`, may start before the kernel ahead of it on the stream has ended (its pdl_wait holds it back); the first
+// kernel of a call must not: what is ahead of it is not ours
 template <class... Params, class... Args>
-inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t st, int smem, int cluster, Args... args) {
+inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t st, int smem, int cluster, bool early, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -128,7 +129,7 @@ inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, 
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;

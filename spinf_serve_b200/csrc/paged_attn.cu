@@ -51,7 +51,7 @@ struct alignas(4) KeyItem {
 template <bool STEP>
 __device__ __forceinline__ int key_items(const PagedSeqs& s, const PagedAttnArgs& a, int b, int* status) {
   const PagedSeq q = paged_seq(s, b, status);
-  if (!(STEP ? step_class(q, a.group) : rows_class(q, a))) return 0;
+  if (!(STEP ? step_class(q, a) : rows_class(q, a))) return 0;
   const PagedCut c = STEP ? step_cut(q, a) : rows_cut(q, a);
   return a.h * c.row_tiles * c.splits;
 }
@@ -969,9 +969,10 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
     const int hl = chunk_heads_log2(static_cast<int>(group)), tl = 8 - hl;
     const int64_t work = ((max_q + (1 << tl) - 1) >> tl) * (H >> hl) * (tiles > 0 ? tiles : 1);
     if (work >= (1ll << 31)) z.too_large = true;  // the chunk kernels count (item, key tile) pairs in 32 bits
-    int64_t units = work / CHUNK_MIN_TILES;
-    units = units < 1 ? 1 : units > chunk_units_of(D) ? chunk_units_of(D) : units;
-    const int64_t seqs = n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
+    // (an item makes a unit, or a unit holds CHUNK_MIN_TILES pairs, or a part of an item four)
+    int64_t units = work / 4 + ((max_q + (1 << tl) - 1) >> tl) * (H >> hl);
+    units = units > chunk_units_of(D) ? chunk_units_of(D) : units;
+    const int64_t seqs = B == 1 ? 1 : n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
     z.max_units = static_cast<int>(seqs * units);
     z.chunk_o = up256(seqs * units * 512 * D * 4);
     z.chunk_ml = up256(seqs * units * 512 * 8);
@@ -1002,22 +1003,26 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
     attr_set[dev].store(true, std::memory_order_release);
   }
   const unsigned grid = static_cast<unsigned>(sm_count());
-  if (max_q * a.group <= 8)
-    paged_step_kernel<D, 1><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
-  else
-    paged_step_kernel<D, 2><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
-  SPINF_CUDA_OK(cudaGetLastError());
-  if (max_q * a.group > STEP_ROWS)
-    SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, 1, tmK, tmV, s, a, status));
-  if (max_splits > 1) {
+  // with one sequence its kernel is known here: the others' launches fall away
+  const bool step = a.only ? a.only == 1 : true, rows = a.only ? a.only == 2 : max_q * a.group > STEP_ROWS;
+  const bool chunk = a.only ? a.only == 3 : max_q * a.group > a.chunk_rows;
+  if (step) {
+    if (max_q * a.group <= 8)
+      paged_step_kernel<D, 1><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+    else
+      paged_step_kernel<D, 2><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+    SPINF_CUDA_OK(cudaGetLastError());
+  }
+  if (rows) SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, 1, step, tmK, tmV, s, a, status));
+  if (max_splits > 1 && (step || rows)) {
     const int64_t most = a.chunk_rows / a.group;  // tokens of a sequence that is not the chunk kernel's
     int64_t gx = (max_q < most ? max_q : most) * a.H;
     if (gx > 1024) gx = 1024;
-    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, s, a, status));
+    SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, true, s, a, status));
   }
-  if (max_q * a.group > a.chunk_rows && (r = paged_chunk_launch(D, kp, vp, s, a, w, max_q, st, dev, status))) return r;
-  if (w)
-    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, 1, s, a, *w, status));
+  if (chunk && (r = paged_chunk_launch(D, kp, vp, s, a, w, step || rows, st, dev, status))) return r;
+  if (w && a.only != 3)
+    SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, 1, true, s, a, *w, status));
   return 0;
 }
 
@@ -1083,6 +1088,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.scale_log2 = scale * 1.4426950408889634f;
   a.seq_parts = z.seq_parts;
   a.chunk_rows = z.chunk_rows;
+  a.only = B == 1 && mq > 0 ? class_of(mq * a.group, z.chunk_rows) : 0;
   a.max_units = z.max_units;
   auto take = [&](int64_t bytes) {
     uint8_t* p = ws;

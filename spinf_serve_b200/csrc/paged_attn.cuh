@@ -15,6 +15,7 @@ struct PagedAttnArgs {
   int H, h, D, group, window;
   int hp_log2, sets;  // chunk kernels: heads of an item, items of a kv head and token tile
   float scale_log2;
+  int only;        // one sequence in the call: the kernel its row limit asks for (1 step, 2 few rows, 3 chunk) takes it; 0: by rows
   int chunk_rows;  // sequences with more query rows per kv head than this are the chunk kernel's
   // split keys, few rows: part_o [B][seq_parts][D], part_ml [B][seq_parts] (maximum in log2 units, sum)
   float* part_o;
@@ -42,20 +43,25 @@ struct PagedWeightArgs {
 static constexpr int RT = 64;         // query rows of an item of the few-row kernel
 static constexpr int STEP_ROWS = 16;  // rows per kv head a decoding step's kernel takes
 
-__device__ __forceinline__ bool step_class(const PagedSeq& q, int group) { return q.nq > 0 && q.nq * group <= STEP_ROWS; }
-__device__ __forceinline__ bool chunk_class(const PagedSeq& q, const PagedAttnArgs& a) { return q.nq * a.group > a.chunk_rows; }
-__device__ __forceinline__ bool rows_class(const PagedSeq& q, const PagedAttnArgs& a) { return q.nq * a.group > STEP_ROWS && !chunk_class(q, a); }
+__host__ __device__ inline int class_of(int64_t rows, int chunk_rows) { return rows <= STEP_ROWS ? 1 : rows > chunk_rows ? 3 : 2; }
+__device__ __forceinline__ int seq_class(const PagedSeq& q, const PagedAttnArgs& a) {
+  return q.nq == 0 ? 0 : a.only ? a.only : class_of(q.nq * a.group, a.chunk_rows);
+}
+__device__ __forceinline__ bool step_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 1; }
+__device__ __forceinline__ bool rows_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 2; }
+__device__ __forceinline__ bool chunk_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 3; }
 __device__ __forceinline__ PagedCut step_cut(const PagedSeq& q, const PagedAttnArgs& a) { return paged_cut(q, a.window, 1, a.h, PG_SMS, 1); }
 __device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
   const int rt = (q.nq * a.group + RT - 1) / RT;
   return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 4);  // splits of at least 4 tiles: up to 64 rows of partial results each
 }
-__device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a.group) ? step_cut(q, a) : rows_cut(q, a); }
+__device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a) ? step_cut(q, a) : rows_cut(q, a); }
 
 // ---- the chunk kernel: items of 256 rows (hp heads x 256 / hp tokens), their key tiles dealt out in equal units
 // units of a sequence: one per CTA pair (D 256) or CTA (D 128)
 __host__ __device__ constexpr int chunk_units_of(int D) { return D == 256 ? PG_SMS / 2 : PG_SMS; }
-static constexpr int CHUNK_MIN_TILES = 8;       // least (item, tile) pairs of a unit: below that a cut costs more than it spreads
+static constexpr int CHUNK_MIN_TILES = 8;       // least (item, tile) pairs of a unit that begins anywhere: below that a cut costs more than it spreads
+static constexpr int CHUNK_SHORT = 24;          // key tiles of an item that is not worth cutting where there are items enough
 
 // heads of an item, as a power of two: the largest that divides the group, at most 8 (16 rows of a head in one tile); more heads per
 // item mean fewer tokens, so less of the causal triangle is padding
@@ -66,6 +72,7 @@ struct ChunkCut {
   int work;                   // (item, key tile) pairs
   int units, quot, rem;       // unit u takes quot pairs, the first `rem` units one more
   bool whole;                 // units take whole items: those that begin in their range
+  int parts;                  // not 0: no more items than the GPU runs at once, every unit is one of the `parts` equal parts of an item
 
   __device__ __forceinline__ void slots(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& lo, int& hi) const {
     const int base = q.len - q.nq, first = base + (tt << tok_log2);
@@ -101,12 +108,28 @@ __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttn
     tiles += nt;
   }
   c.work = tiles * c.per_tt;  // (the host has checked that this fits)
-  const int u = c.work / CHUNK_MIN_TILES, most = chunk_units_of(a.D);
+  const int most = chunk_units_of(a.D), items = c.ntt * c.per_tt;
+  const bool brief = tiles <= CHUNK_SHORT * c.ntt;
+  c.parts = 0;
+  c.whole = false;
+  if (items <= most && (c.ntt == 1 || brief)) {
+    // few items: one unit each, or (a single token tile) as many equal parts as there is room for, of at least four tiles
+    int k = 1;
+    if (c.ntt == 1) {
+      k = most / items;
+      k = k < tiles / 4 ? k : tiles / 4;
+      k = k > 1 ? k : 1;
+    }
+    c.parts = k;
+    c.units = items * k;
+    c.quot = c.rem = 0;
+    return c;
+  }
+  const int u = c.work / CHUNK_MIN_TILES;
   c.units = u < 1 ? 1 : u > most ? most : u;
   c.quot = c.work / c.units;
   c.rem = c.work - c.quot * c.units;
-  // many short items (a window): a cut would cost about as much as the imbalance it removes
-  c.whole = 2 * c.ntt * c.per_tt >= most && tiles <= 24 * c.ntt;
+  c.whole = brief && 2 * items >= most;  // many short items (a window): a cut would cost about as much as the imbalance it removes
   return c;
 }
 
@@ -126,7 +149,7 @@ __device__ __forceinline__ int chunk_page(const PagedSeqs& s, const int32_t* pag
   return s.n_pages;
 }
 
-int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, bool early,
                        cudaStream_t st, int dev, int* status);
 
 }  // namespace spinf

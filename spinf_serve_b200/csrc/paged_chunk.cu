@@ -85,15 +85,32 @@ struct ChunkWalk {
     c = chunk_cut(q, a);
     it = unit;
     const int u = unit - pre[b];
-    w = c.begin(u);
-    w_end = c.begin(u + 1);
     first = true;
     tt = 0, w_tt = 0;
+    ChunkJoin join;
+    join.pieces = 0;
+    if (c.parts) {
+      const int i = u / c.parts, part = u - i * c.parts;
+      tt = i / c.per_tt;
+      c.tiles(q, a, tt, t0, nt);
+      const int item = i - tt * c.per_tt;
+      w = item * nt + nt * part / c.parts;  // (pairs counted from the token tile's first)
+      w_end = item * nt + nt * (part + 1) / c.parts;
+      if (part == 1) {  // parts are the first segments of their units
+        join.pieces = c.parts;
+        join.first = (unit - 1) * 2;
+        join.row0 = q.row0, join.nq = q.nq;
+        join.tok0 = tt << c.tok_log2;
+        join.h0 = item / a.sets * a.group + (item % a.sets << a.hp_log2);
+      }
+      a.joins[unit] = join;
+      return;
+    }
+    w = c.begin(u);
+    w_end = c.begin(u + 1);
     c.tiles(q, a, 0, t0, nt);
     advance(a);
     const int item = (w - w_tt) / nt, off = w - w_tt - item * nt;
-    ChunkJoin join;
-    join.pieces = 0;
     if (off) {
       if (c.whole) {
         w += nt - off;
@@ -118,7 +135,7 @@ struct ChunkWalk {
   }
   __device__ __forceinline__ bool next(const PagedAttnArgs& a, ChunkSeg& g) {
     if (w >= w_end) return false;
-    advance(a);
+    if (!c.parts) advance(a);
     const int item = (w - w_tt) / nt, off = w - w_tt - item * nt;
     const int len = !c.whole && w_end - w < nt - off ? w_end - w : nt - off;
     g.b = b, g.row0 = q.row0, g.nq = q.nq, g.base = q.len - q.nq;
@@ -1177,7 +1194,7 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   }
   paged_item_prefix(s.B, pre, CHUNK_WEIGHT_THREADS, [&](int b) {
     const PagedSeq q = paged_seq(s, b, status);
-    return chunk_class(q, a) ? a.h * ((q.len + 255) / 256) : 0;
+    return a.only == 3 || chunk_class(q, a) ? a.h * ((q.len + 255) / 256) : 0;  // (alone in the call: also without new rows)
   });
   const int total = pre[s.B];
   pdl_wait();  // lse is the kernels' ahead
@@ -1343,7 +1360,7 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 }
 
 template <int D>
-static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, bool early,
                         cudaStream_t st, int dev, int* status) {
   using L = ChunkSmem<D>;
   CUtensorMap tmQ, tmK, tmV;
@@ -1365,20 +1382,20 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
     attr_set[dev].store(true, std::memory_order_release);
   }
   SPINF_CUDA_OK(launch_after(kern, dim3(static_cast<unsigned>(D == 256 ? sm_count() / 2 * 2 : sm_count())), dim3(CHUNK_THREADS), st, L::TOTAL,
-                             D == 256 ? 2 : 1, tmQ, tmK, tmV, s, a, status));
-  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, a));
+                             D == 256 ? 2 : 1, early, tmQ, tmK, tmV, s, a, status));
+  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, true, a));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
   if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;
   if ((r = make_tmap_pages(&tmKw, kp, vrows, vrows == PG_TILE ? D / 64 : 1))) return r;
-  SPINF_CUDA_OK(launch_after(paged_chunk_weight_kernel<D>, dim3(static_cast<unsigned>(sm_count())), dim3(CHUNK_WEIGHT_THREADS), st, ChunkWeightSmem<D>::TOTAL, 1,
+  SPINF_CUDA_OK(launch_after(paged_chunk_weight_kernel<D>, dim3(static_cast<unsigned>(sm_count())), dim3(CHUNK_WEIGHT_THREADS), st, ChunkWeightSmem<D>::TOTAL, 1, true,
                              tmQw, tmKw, s, a, *w, status));
   return 0;
 }
 
-int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
+int paged_chunk_launch(int D, const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, bool early,
                        cudaStream_t st, int dev, int* status) {
-  return D == 256 ? launch_chunk<256>(kp, vp, s, a, w, max_q, st, dev, status) : launch_chunk<128>(kp, vp, s, a, w, max_q, st, dev, status);
+  return D == 256 ? launch_chunk<256>(kp, vp, s, a, w, early, st, dev, status) : launch_chunk<128>(kp, vp, s, a, w, early, st, dev, status);
 }
 
 }  // namespace spinf

@@ -252,7 +252,7 @@ extern "C" int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, 
   SPINF_CUDA_OK(cudaGetLastError());
   const int64_t per_cta = (256 / (D / 8)) * 4, blocks = (keep + per_cta - 1) / per_cta;
   const dim3 grid(static_cast<unsigned>(blocks * Hkv * B));
-  SPINF_CUDA_OK(D == 256 ? launch_after(paged_move_kernel<256>, grid, dim3(256), st, 0, 1, s, a, static_cast<int>(blocks), status)
-                         : launch_after(paged_move_kernel<128>, grid, dim3(256), st, 0, 1, s, a, static_cast<int>(blocks), status));
+  SPINF_CUDA_OK(D == 256 ? launch_after(paged_move_kernel<256>, grid, dim3(256), st, 0, 1, true, s, a, static_cast<int>(blocks), status)
+                         : launch_after(paged_move_kernel<128>, grid, dim3(256), st, 0, 1, true, s, a, static_cast<int>(blocks), status));
   return 0;
 }

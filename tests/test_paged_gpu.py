@@ -228,6 +228,25 @@ def test_long_items_of_a_step(dev, H, h, D, page):
         assert ((first[b].double().view_as(want) - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("max_q", [3, 14, 200])
+@pytest.mark.parametrize("nq", [0, 1, 3])
+def test_one_sequence_with_a_loose_row_limit(dev, max_q, nq):
+    """a sequence alone goes to the kernel its row limit asks for, whatever its rows: padded batches, also without rows at all"""
+    c = Call(dev, 8, 4, 128, 64, [(300, nq)], seed=max_q + nq, extra_rows=max_q - nq)
+    out = torch.full((c.n, 8, 128), 7.0, dtype=torch.bfloat16, device=dev)
+    old = torch.rand((1, 4, 320), generator=c.gen)
+    w = old.to(dev)
+    o = c.on
+    ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], max_q, 128**-0.5, weights=w, decay=0.25, out=out)
+    want, weights, mag, big = c.expect()
+    if nq:
+        check_out(c, out, want, mag, big)
+    assert (out[nq:] == 7.0).all()
+    ref = 0.25 * old[0, :, :300].double() + weights[0]
+    rel = (float(score_noise(c, big, 300).max()) if nq else 0.0) + 2.0**-20
+    assert ((w[0, :, :300].double().cpu() - ref).abs() <= rel * ref).all() and torch.equal(w[0, :, 300:].cpu(), old[0, :, 300:])
+
+
 def test_attention_views_streams_and_a_graph(dev):
     c = Call(dev, 8, 2, 128, 64, [(300, 3), (129, 1)], seed=5)
     want, _, mag, big = c.expect()
