@@ -1058,50 +1058,54 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 // ---------------------------------------------------------------- join of the cut items
-// CTAs (it, y): the item that unit `it` is the first to begin inside of, as the planning warps have left word; 64 of its 256 rows, a
-// warp per row, the pieces added in the order of the units
+// CTAs (x, y) over units `it`: the item that the unit is the first to begin inside of, as the planning warps have left word; 16 of its 256 rows, a
+// warp per row, the pieces added in the order of the units (an item in nine parts is a chain of loads for a row, so rows side by side)
+static constexpr int JOIN_ROWS = 16;
 template <int D>
 __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedAttnArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int V = D / 128;  // float4 per lane
-  const int it = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int total = *a.n_units;
-  const ChunkJoin join = a.joins[it];  // (read with the count, used only below it)
-  if (it >= total || join.pieces == 0) return;
-  const int last = it + join.pieces - 2 < a.max_units ? join.pieces - 2 : a.max_units - 1 - it;
-  const int ql = 7 - a.hp_log2;
-  const int64_t first = static_cast<int64_t>(join.first) * 256;
-  for (int r = blockIdx.y * 64 + warp; r < blockIdx.y * 64 + 64; r += 8) {
-    const int in = r & 127, tok = join.tok0 + ((r >> 7) << ql) + (in & ((1 << ql) - 1)), head = join.h0 + (in >> ql);
-    if (tok >= join.nq) continue;
-    const int64_t at0 = first + r, at = static_cast<int64_t>(it) * 512 + r;  // further pieces: 512 rows apart
-    float m = a.chunk_ml[at0].x;
-    for (int y = 0; y <= last; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
-    const float neg_m = m == -INFINITY ? 0.f : -m;
-    float l = 0.f;
-    float4 acc[V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int total = *a.n_units, ql = 7 - a.hp_log2;
+  for (int it = blockIdx.x; it < total; it += gridDim.x) {
+    const ChunkJoin join = a.joins[it];
+    if (join.pieces == 0) continue;
+    const int last = it + join.pieces - 2 < a.max_units ? join.pieces - 2 : a.max_units - 1 - it;
+    const int64_t first = static_cast<int64_t>(join.first) * 256;
+    for (int r = blockIdx.y * JOIN_ROWS + warp; r < (blockIdx.y + 1) * JOIN_ROWS; r += 8) {
+      const int in = r & 127, tok = join.tok0 + ((r >> 7) << ql) + (in & ((1 << ql) - 1)), head = join.h0 + (in >> ql);
+      if (tok >= join.nq) continue;
+      const int64_t at0 = first + r, at = static_cast<int64_t>(it) * 512 + r;  // further pieces: 512 rows apart
+      float m = a.chunk_ml[at0].x;
+#pragma unroll 4
+      for (int y = 0; y <= last; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
+      const float neg_m = m == -INFINITY ? 0.f : -m;
+      float l = 0.f;
+      float4 acc[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int y = -1; y <= last; ++y) {
-      const int64_t from = y < 0 ? at0 : at + y * 512;
-      const float2 ml = a.chunk_ml[from];
-      const float f = fast_exp2(ml.x + neg_m);
-      l = fmaf(f, ml.y, l);
-      const float4* src = reinterpret_cast<const float4*>(a.chunk_o + from * D);
+      for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int y = -1; y <= last; ++y) {
+        const int64_t from = y < 0 ? at0 : at + y * 512;
+        const float2 ml = a.chunk_ml[from];
+        const float f = fast_exp2(ml.x + neg_m);
+        l = fmaf(f, ml.y, l);
+        const float4* src = reinterpret_cast<const float4*>(a.chunk_o + from * D);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float4 z = src[v * 32 + lane];
-        acc[v].x = fmaf(f, z.x, acc[v].x), acc[v].y = fmaf(f, z.y, acc[v].y), acc[v].z = fmaf(f, z.z, acc[v].z), acc[v].w = fmaf(f, z.w, acc[v].w);
+        for (int v = 0; v < V; ++v) {
+          const float4 z = src[v * 32 + lane];
+          acc[v].x = fmaf(f, z.x, acc[v].x), acc[v].y = fmaf(f, z.y, acc[v].y), acc[v].z = fmaf(f, z.z, acc[v].z), acc[v].w = fmaf(f, z.w, acc[v].w);
+        }
       }
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    __nv_bfloat16* dst = a.out + (join.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      __nv_bfloat16* dst = a.out + (join.row0 + tok) * a.out_pitch + static_cast<int64_t>(head) * D;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
-          make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv), pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
-    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(join.row0 + tok) * a.H + head] = m + log2f(l);
+      for (int v = 0; v < V; ++v)
+        *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
+            make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv), pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
+      if (a.lse && lane == 0) a.lse[static_cast<int64_t>(join.row0 + tok) * a.H + head] = m + log2f(l);
+    }
   }
 }
 
@@ -1383,7 +1387,7 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   }
   SPINF_CUDA_OK(launch_after(kern, dim3(static_cast<unsigned>(D == 256 ? sm_count() / 2 * 2 : sm_count())), dim3(CHUNK_THREADS), st, L::TOTAL,
                              D == 256 ? 2 : 1, early, tmQ, tmK, tmV, s, a, status));
-  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units), 4), dim3(256), st, 0, 1, true, a));
+  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units < PG_SMS ? a.max_units : PG_SMS), 256 / JOIN_ROWS), dim3(256), st, 0, 1, true, a));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
   if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;
