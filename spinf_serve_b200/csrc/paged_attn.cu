@@ -1032,7 +1032,8 @@ using namespace spinf;
 
 extern "C" int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
                                                          int32_t weights) {
-  if (n < 0 || B < 0 || B > PG_MAX_SEQS || H <= 0 || Hkv <= 0 || H % Hkv || (D != 128 && D != 256) || max_q < 0 || max_len < 0) return SPINF_ERR_BAD_ARGUMENT;
+  if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
+  if (n < 0 || B < 0 || H <= 0 || Hkv <= 0 || H % Hkv || (D != 128 && D != 256) || max_q < 0 || max_len < 0) return SPINF_ERR_BAD_ARGUMENT;
   const PagedSizes z = paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0);
   return z.too_large ? SPINF_ERR_TOO_LARGE : z.total;
 }

@@ -764,7 +764,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     0). max_q, max_len: no sequence has more rows / tokens (max_len None: what the table can hold).
     weights (fp32 [B, Hkv, cap], cap >= max_len): each slot's accumulated attention weight, weights_out = decay * weights + this
     call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
-    tensor reused between calls on one stream."""
+    tensor reused between calls on one stream; out must not overlap q."""
     what = "paged_attention"
     if weights is not None and weights_out is None:
         weights_out = weights
@@ -778,6 +778,8 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
             return paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace)
     if out is None:
         out = q.new_empty((n, H, D))
+    elif n and out.data_ptr() == q.data_ptr():
+        raise SpinfError(f"{what}: out must not be q: its rows are read until the call has ended")
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = q.new_empty(need, dtype=_U8)
     check(

@@ -418,3 +418,61 @@ def test_out_of_range_entries_are_reported_not_followed(dev):
     assert _lib.last_status(raise_on_error=False) == 5
     ops.paged_evict(o["k"], o["v"], table, o["lens_t"], None, 64, 64, c.free[:2].view(2, 1).to(dev))
     assert _lib.last_status(raise_on_error=False) == 5
+
+
+def test_a_captured_chain(dev):
+    """append, attention with weights and eviction in one graph, replayed on new rows: as the calls one by one"""
+    H, h, D, page = 8, 4, 128, 32
+    c = Call(dev, H, h, D, page, [(200, 70), (300, 3), (150, 0)], seed=21, spare=12)
+    o = c.on
+    new_table = c.free[:9].view(3, 3).to(dev)
+    g = torch.Generator().manual_seed(0)
+    rows = [torch.randn((c.n, (H + 2 * h) * D), generator=g).to(torch.bfloat16).to(dev) for _ in range(3)]
+    w0 = torch.rand((3, h, 320), generator=g).to(dev)
+    qkv, w, k, v = rows[0].clone(), w0.clone(), o["k"].clone(), o["v"].clone()
+
+    def chain():
+        q = ops.paged_append(qkv, H, h, D, k, v, o["table"], o["lens_t"], o["cu"], norm_v=True)
+        out = ops.paged_attention(q, k, v, o["table"], o["lens_t"], o["cu"], 70, D**-0.5, weights=w)
+        return (out,) + ops.paged_evict(k, v, o["table"], o["lens_t"], w, 90, 30, new_table)
+
+    want = []
+    for r in rows:
+        qkv.copy_(r)
+        w.copy_(w0)
+        want.append([x.clone() for x in chain()] + [k.clone(), v.clone()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = chain()
+    for r, x in zip(rows, want):
+        qkv.copy_(r)
+        w.copy_(w0)
+        graph.replay()
+        for a, b in zip(list(res) + [k, v], x):
+            assert torch.equal(a.view(torch.int16) if a.dtype is torch.bfloat16 else a, b.view(torch.int16) if b.dtype is torch.bfloat16 else b)
+
+
+def test_as_many_sequences_as_a_call_takes(dev):
+    B, H, h, D, page = 1024, 4, 2, 128, 16
+    g = torch.Generator(device=dev).manual_seed(4)
+    lens = torch.randint(1, 60, (B,), generator=g, device=dev).to(torch.int32)
+    n_new = torch.minimum(lens, torch.randint(0, 4, (B,), generator=g, device=dev).to(torch.int32))
+    n_new[500] = lens[500] = 40  # one chunk among the steps
+    cu = torch.zeros(B + 1, dtype=torch.int32, device=dev)
+    cu[1:] = n_new.cumsum(0)
+    table = torch.randperm(4 * B, generator=g, device=dev).to(torch.int32).view(B, 4)
+    both = torch.randn((4 * B, 2, h, page, D), generator=g, device=dev, dtype=torch.bfloat16)  # K and V side by side in one tensor
+    k, v = both[:, 0], both[:, 1]
+    q = torch.randn((int(cu[-1]), H, D), generator=g, device=dev, dtype=torch.bfloat16)
+    out = ops.paged_attention(q, k, v, table, lens, cu, 40, D**-0.5)
+    for b in (0, 1, 17, 499, 500, 501, 1023):
+        r0, r1, L = int(cu[b]), int(cu[b + 1]), int(lens[b])
+        want, _, mag, big = OP.attention(q[r0:r1].cpu(), k.cpu(), v.cpu(), table[b : b + 1].cpu(), [L], [0, r1 - r0], D**-0.5)
+        rel = torch.expm1(2 * (D + 8) * 2.0**-24 * big) + 128 * 2.0**-24 + 2.0**-21
+        assert ((out[r0:r1].double().cpu() - want).abs() <= BF * want.abs() + (BF * 1.01 + rel[..., None]) * mag * 1.01 + 1e-30).all()
+    with pytest.raises(_lib.SpinfError, match="maximum"):
+        z = torch.zeros(1025, dtype=torch.int32, device=dev)
+        ops.paged_attention(q, k, v, torch.zeros((1025, 4), dtype=torch.int32, device=dev), z, torch.zeros(1026, dtype=torch.int32, device=dev), 1, 1.0)
+    with pytest.raises(_lib.SpinfError, match="must not be q"):
+        ops.paged_attention(q, k, v, table, lens, cu, 40, D**-0.5, out=q)

@@ -160,7 +160,7 @@ def test_the_c_entry_points_refuse_on_the_host():
                 dict(w_out=p), dict(w_out=p, strides=(ctypes.c_int64 * 4)(), decay=1.0), dict(width=64, max_len=1024)):  # (the last: splits need a workspace)
         assert attn(**bad) == -1, bad
     assert attn(B=2000) == -4
-    assert lib.spinf_paged_attention_workspace_bytes(4, 2000, 4, 2, 128, 1, 64, 0) == -1
+    assert lib.spinf_paged_attention_workspace_bytes(4, 2000, 4, 2, 128, 1, 64, 0) == -4
     assert lib.spinf_paged_attention_workspace_bytes(4, 2, 4, 3, 128, 1, 64, 0) == -1
     need = [lib.spinf_paged_attention_workspace_bytes(64, 64, 16, 8, 256, 1, n, w) for n, w in ((100, 0), (8192, 0), (8192, 1))]
     assert need[0] == 0 and 0 < need[1] < need[2]
