@@ -436,15 +436,16 @@ int spinf_gdn_epilogue(const void* o, const void* z, int64_t z_pitch, const void
  *
  * A pool is [n_pages, Hkv, page, D] bf16 with any strides between pages, heads and rows (strides_host: those three, in elements;
  * multiples of 8; D contiguous), page a power of two from 16 to 256, D 128 or 256. Sequence b of a call (B <= 1024) has rows
- * cu[b] .. cu[b+1] of the n rows (int32 [B+1], ascending; rows behind cu[B] are left alone) and lens[b] cached tokens, the call's
+ * cu[b] .. cu[b+1] of the n rows (int32 [B+1], ascending; rows of no sequence take part in nothing) and lens[b] cached tokens, the call's
  * own included: row i of the sequence sits in slot lens[b] - (cu[b+1] - cu[b]) + i, and slot s is row s % page of page
  * table[b * table_pitch + s / page]. Tables may share pages as long as nothing writes to a shared one. A page index, length or row
  * range outside the pool, max_len, max_q or n is skipped and reported as SPINF_ST_BAD_INDEX.
  *
  * spinf_paged_append: rows of a fused projection [H q | Hkv k | Hkv v] x D -> norms of the q and k heads (wq, wk [D]; both null:
  * none; plus1: weights 1 + w), of the v heads (norm_v, without weight), rotary embedding of q and k over the first rot_dim
- * dimensions (cos, sin bf16 [n, rot_dim / 2]; 0 and null: none), q to q_out [n, H, D] (null: not touched, only without norms and
- * rotation), k and v to their slots. fp32 throughout, rounded once. */
+ * dimensions (cos, sin bf16 [n, rot_dim / 2]; 0 and null: none), q to q_out [n, H, D] (all n rows; null: not touched, only without
+ * norms and rotation), k and v of the sequences' rows to their slots. fp32 throughout, rounded once. q_out, the pools and qkv lie
+ * apart; no slot of the pools is written twice. */
 int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* wq, const void* wk,
                        const void* cos_t, const void* sin_t, int32_t rot_dim, float eps, int32_t plus1, int32_t norm_v, void* q_out,
                        void* k_pages, void* v_pages, int64_t n_pages, int32_t page, const int64_t* k_strides_host,
@@ -457,8 +458,11 @@ int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int32_t H, int
  * (they size the workspace; 256-byte aligned). weights_out (optional, fp32; weight_strides_host: sequence and head strides of
  * weights_in, then of weights_out): weights_out[b, g, j] = decay * weights_in[b, g, j] + the sum of the attention weights of slot j
  * over the sequence's rows and the heads that share kv head g, for j < lens[b]; the two may be the same tensor; with decay 0
- * weights_in is not read. A sequence's results do not depend on the other sequences of the call. Values in slots that no row of a
- * sequence's 64-row tile sees never reach its results; inside a tile's range they have to be finite. */
+ * weights_in is not read. out lies apart from q, its rows behind cu[B] are left as they were. A sequence's results do not depend on
+ * the other sequences of the call (a call of one sequence takes the kernel that max_q asks for, a call of several each sequence's
+ * own rows). The rows that share an item of work (up to 256 rows of neighbouring tokens) share their slots' values: those that none
+ * of them sees never reach a result, whatever they hold; a value that is not finite in a slot that one of them sees makes all of
+ * them NaN. */
 int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
                                               int32_t weights);
 int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* k_pages,
@@ -471,7 +475,7 @@ int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, 
 /* Cuts every sequence with more than `keep` tokens back to `keep`, per kv head: the last `recent` slots stay, and of the others the
  * keep - recent with the largest weight (weights [b * w_seq + g * w_head + slot] fp32; ties: the lowest slot; NaN below all numbers; null: recent
  * has to equal keep). What stays is copied in slot order to the pages of new_table [B, new_pitch], which must not hold any page that
- * `table` still names. Out: new_lens [B], kept [B, Hkv, keep] the old slots (-1 behind the last), weights_out [B, Hkv, keep] their
+ * `table` still names, nor one page twice. Out (apart from what is read): new_lens [B], kept [B, Hkv, keep] the old slots (-1 behind the last), weights_out [B, Hkv, keep] their
  * weights (0 behind the last; null without weights). */
 int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, int32_t page, int32_t Hkv, int32_t D, const int64_t* k_strides_host,
                       const int64_t* v_strides_host, const int32_t* table, int64_t table_pitch, const int32_t* lens, int32_t B,

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256, 2) paged_append_kernel(const AppendArgs a
           if (s.cu[mid + 1] <= t) lo = mid + 1;
           else hi = mid;
         }
-        if (lo < s.B && t >= s.cu[lo]) {  // (a row behind the last sequence, or before the first, has no slot)
+        if (lo < s.B && t >= s.cu[lo]) {  // (a row behind the last sequence, or before the first, has no slot: its q is made, nothing else)
           const int slot = s.lens[lo] - s.cu[lo + 1] + static_cast<int>(t);
           in_page = slot & ((1 << s.page_log2) - 1);
           if (slot >= 0 && (slot >> s.page_log2) < a.width) pg = s.table[lo * s.table_pitch + (slot >> s.page_log2)];

@@ -1021,7 +1021,7 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
     SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, true, s, a, status));
   }
   if (chunk && (r = paged_chunk_launch(D, kp, vp, s, a, w, step || rows, st, dev, status))) return r;
-  if (w && a.only != 3)
+  if (w && a.only != 3 && s.max_len > 0)
     SPINF_CUDA_OK(launch_after(paged_weight_kernel, dim3(static_cast<unsigned>((s.max_len + 1023) / 1024), a.h, s.B), dim3(256), st, 0, 1, true, s, a, *w, status));
   return 0;
 }
@@ -1083,7 +1083,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.h = Hkv;
   a.D = D;
   a.group = H / Hkv;
-  a.window = window;
+  a.window = window < max_len ? window : 0;  // (no row has more slots before it: the same, and sums with it stay in 32 bits)
   a.hp_log2 = chunk_heads_log2(a.group);
   a.sets = a.group >> a.hp_log2;
   a.scale_log2 = scale * 1.4426950408889634f;

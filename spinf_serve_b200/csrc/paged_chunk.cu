@@ -541,6 +541,9 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       }
     }
+    if (*abort_flag && lane == 0)  // bounded wait for copies that may still be in flight (the leader's barriers count both CTAs')
+      for (uint32_t c = cnt > static_cast<uint32_t>(NS) ? cnt - NS : 0; c <= cnt; ++c)
+        for (int spin = 0; spin < 4096 && !mbar_try_wait(&k_full[c % NS], (c / NS) & 1u); ++spin) {}
   } else if (warp == 2) {
     const int rl = s.page_log2 < 7 ? s.page_log2 : 7, rows = 1 << rl;  // rows of a V box
     uint32_t cnt = 0, seg_n = 0;
@@ -595,6 +598,11 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       }
+    }
+    if (*abort_flag && lane == 0) {
+      for (uint32_t c = cnt > static_cast<uint32_t>(NS) ? cnt - NS : 0; c <= cnt; ++c)
+        for (int spin = 0; spin < 4096 && !mbar_try_wait(&v_full[c % NS], (c / NS) & 1u); ++spin) {}
+      for (int spin = 0; seg_n && spin < 4096 && !mbar_try_wait(q_full, (seg_n - 1) & 1u); ++spin) {}
     }
   } else if (warp == 3) {
     uint32_t cnt = 0, edges[NS];  // boundary tiles each stage has held

@@ -616,7 +616,17 @@ def _layout(t):
     return None if t is None else (t.dtype, t.shape, t.stride())
 
 
-def _page_layout(k, v, what):
+def _apart(shape, stride):
+    """no two elements of the layout share a place (so that a kernel may write to it)"""
+    extent = 1
+    for st, sz in sorted((st, sz) for st, sz in zip(stride, shape) if sz > 1):
+        if st < extent:
+            return False
+        extent += st * (sz - 1)
+    return True
+
+
+def _page_layout(k, v, what, written=False):
     """a pool's layout -> (pages, kv heads, page, D, the strides of k and v for the C entry points)"""
     for name, t in (("k_pages", k), ("v_pages", v)):
         if t[0] is not _BF16 or len(t[1]) != 4 or t[2][3] != 1 or any(x % 8 for x in t[2][:3]):
@@ -626,6 +636,8 @@ def _page_layout(k, v, what):
     n_pages, h, page, D = k[1]
     if page < 16 or page > 256 or page & (page - 1) or D not in (128, 256) or n_pages < 1 or h < 1:
         raise SpinfError(f"{what}: pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {tuple(k[1])}")
+    if written and not (_apart(*k[1:]) and _apart(*v[1:])):
+        raise SpinfError(f"{what}: k_pages and v_pages are written to, rows must not share places: {k}, {v}")
     i64x3 = ctypes.c_int64 * 3
     return n_pages, h, page, D, i64x3(*k[2][:3]), i64x3(*v[2][:3])
 
@@ -659,7 +671,7 @@ def _row_layout(t, name, what, heads=None):
 @functools.lru_cache(maxsize=512)
 def _append_layout(qkv, H, Hkv, D, k, v, table, lens, cu, wq, wk, cos, sin):
     what = "paged_append"
-    n_pages, h, page, Dp, ks, vs = _page_layout(k, v, what)
+    n_pages, h, page, Dp, ks, vs = _page_layout(k, v, what, True)
     if qkv[0] is not _BF16 or len(qkv[1]) != 2 or H < 1 or h != Hkv or Dp != D or qkv[1][1] != (H + 2 * Hkv) * D:
         raise SpinfError(f"{what}: qkv {qkv} and pages {tuple(k[1])} do not fit {H} / {Hkv} heads of {D} in bf16")
     n = qkv[1][0]
@@ -683,12 +695,14 @@ def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=
     """a step's rows into the paged cache: qkv [n, (H + 2 Hkv) D] bf16 (rows of any pitch) -> q [n, H, D]; k and v go to the slots of
     their sequences (spinf_paged_append in include/spinf_b200.h has the layout). wq, wk [D]: head norms of q and k (plus1: weights
     1 + w); norm_v: norm of v without weight; cos, sin [n, R/2] bf16 (rope_table): rotary embedding over the first R dimensions.
-    Without norms of q and rotation the returned q is a view of qkv."""
+    Without norms of q and rotation the returned q is a view of qkv. q has all n rows; k and v are written for the rows of sequences only."""
     what = "paged_append"
     n, q_pitch, rot, n_pages, page, ks, vs, pitch, width, B = _append_layout(
         _layout(qkv), H, Hkv, D, _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cu), _layout(wq), _layout(wk), _layout(cos), _layout(sin)
     )
     idx = _paged_device(what, qkv, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin)
+    if k_pages.data_ptr() == v_pages.data_ptr():
+        raise SpinfError(f"{what}: k_pages and v_pages are the same memory")
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
             return paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin, eps, plus1, norm_v)
@@ -750,10 +764,13 @@ def _attention_layout(q, k, v, table, lens, cu, max_q, window, w_in, w_out, max_
         for t in (w_in, w_out):
             if t[0] is not _F32 or len(t[1]) != 3 or tuple(t[1][:2]) != (B, h) or t[1][2] < max_len or (t[1][2] > 1 and t[2][2] != 1):
                 raise SpinfError(f"{what}: weights must be fp32 [{B}, {h}, at least {max_len}] tensors, contiguous over slots, got {t}")
+        if not _apart(*w_out[1:]):
+            raise SpinfError(f"{what}: weights_out is written to, slots must not share places: {w_out}")
         strides = (ctypes.c_int64 * 4)(*w_in[2][:2], *w_out[2][:2])
     need = int(_lib.lib().spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_in is not None))
     check(need, what)
-    return n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, window or 0, strides, need
+    win = window if window is not None and window < max_len else 0  # (a window that holds everything is none)
+    return n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, win, strides, need
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=None, weights=None, weights_out=None, decay=1.0, max_len=None,
@@ -797,7 +814,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
 @functools.lru_cache(maxsize=512)
 def _evict_layout(k, v, table, lens, weights, keep, recent, new_table, max_len):
     what = "paged_evict"
-    n_pages, h, page, D, ks, vs = _page_layout(k, v, what)
+    n_pages, h, page, D, ks, vs = _page_layout(k, v, what, True)
     B, width, pitch, new_width, new_pitch = _index_layout(what, lens, table, None, new_table)
     if keep < 1 or recent < 0 or recent > keep or keep > new_width * page:
         raise SpinfError(f"{what}: keep {keep} needs at least one token and as many as new_table holds at most, recent {recent} between 0 and keep")

@@ -186,7 +186,9 @@ class PagedReader:
             rows = (st.cu[1:].long() - 1) if last else None
             out = self.stack.forward(None, None, inputs, None, rows=rows, attend=self)
         except BaseException:
-            for s, x in zip(seqs, ids):  # the sequences stay where they were (their new pages are kept for the next try)
+            # the sequences stay where they were (their new pages are kept for the next try; weights that layers before the failure
+            # have added up stay added)
+            for s, x in zip(seqs, ids):
                 s.length -= len(x)
                 s.position -= len(x)
             raise

@@ -476,3 +476,52 @@ def test_as_many_sequences_as_a_call_takes(dev):
         ops.paged_attention(q, k, v, torch.zeros((1025, 4), dtype=torch.int32, device=dev), z, torch.zeros(1026, dtype=torch.int32, device=dev), 1, 1.0)
     with pytest.raises(_lib.SpinfError, match="must not be q"):
         ops.paged_attention(q, k, v, table, lens, cu, 40, D**-0.5, out=q)
+
+
+def test_windows_that_hold_everything_are_none(dev):
+    """also those whose sum with a slot would leave 32 bits; with more rows than cached tokens, and with weights"""
+    for seqs in ([(300, 70), (20, 25), (260, 3)], [(40, 90)]):
+        c = Call(dev, 8, 2, 128, 16, seqs, seed=33)
+        w = torch.zeros((len(seqs), 2, 512), device=dev)
+        want, want_w = c.attend(weights=w, weights_out=torch.zeros_like(w)), torch.zeros_like(w)
+        c.attend(weights=w, weights_out=want_w)
+        for window in (c.table.shape[1] * 16, 2**30, 2**31 - 1, 2**32 + 5):
+            got_w = torch.zeros_like(w)
+            got = c.attend(window=window, weights=w, weights_out=got_w)
+            assert torch.equal(got, want) and torch.equal(got_w, want_w)
+
+
+def test_weights_of_an_empty_cache(dev):
+    c = Call(dev, 4, 2, 128, 16, [(20, 4)], seed=3)
+    o, w = c.on, torch.ones((1, 2, 32), device=dev)
+    out = ops.paged_attention(o["q"], o["k"], o["v"], o["table"], torch.zeros_like(o["lens_t"]), o["cu"], 4, 1.0, weights=w, max_len=0)
+    assert (out == 0).all() and (w == 1).all()
+    # rows of q that belong to no sequence (as many as a chunk has): the weights only decay
+    c = Call(dev, 4, 2, 128, 16, [(20, 0)], seed=3, extra_rows=90)
+    o = c.on
+    w = torch.ones((1, 2, 32), device=dev)
+    out = torch.full((90, 4, 128), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 90, 1.0, weights=w, decay=0.5, out=out)
+    assert (out == 7.0).all() and (w[..., :20] == 0.5).all() and (w[..., 20:] == 1).all()
+
+
+def test_append_of_rows_that_belong_to_no_sequence(dev):
+    H, h, D, page = 4, 2, 128, 16
+    c = Call(dev, H, h, D, page, [(20, 4), (9, 9)], seed=5)
+    o = c.on
+    cu = o["cu"] + 2  # two rows ahead of the first sequence, three behind the last
+    n = c.n + 5
+    qkv = torch.randn((n, (H + 2 * h) * D), device=dev).to(torch.bfloat16)
+    w = torch.ones(D, dtype=torch.bfloat16, device=dev)
+    before = o["k"].clone()
+    q = ops.paged_append(qkv, H, h, D, o["k"], o["v"], o["table"], o["lens_t"], cu, wq=w, wk=w)
+    assert _lib.last_status(raise_on_error=False) == 0
+    x = qkv[:, : H * D].double().view(n, H, D)
+    want_q = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-6)
+    assert ((q.double() - want_q).abs() <= (BF + 2.0**-19) * want_q.abs()).all()
+    moved = (before.view(torch.int16) != o["k"].view(torch.int16)).any(-1).any(1)  # [pages, slots]
+    want = torch.zeros_like(moved)
+    for b, (L, k) in enumerate([(20, 4), (9, 9)]):
+        for s in range(L - k, L):
+            want[int(c.table[b, s // page]), s % page] = True
+    assert torch.equal(moved, want)

@@ -180,3 +180,23 @@ def test_the_c_entry_points_refuse_on_the_host():
     assert evict(B=0) == 0
     for bad in (dict(keep=0), dict(keep=17), dict(recent=17), dict(recent=-1), dict(w=N), dict(w=N, w_out=N), dict(w_out=N), dict(max_len=65), dict(D=64), dict(page=48), dict(k=odd), dict(kept=N)):
         assert evict(**bad) == -1, bad
+
+
+def test_written_layouts_that_share_places_are_refused():
+    one = torch.zeros((1, 2, 16, 128), dtype=torch.bfloat16).expand(6, -1, -1, -1)
+    half = torch.as_strided(torch.zeros(6 * 4096, dtype=torch.bfloat16), (6, 2, 16, 128), (2048, 2048, 128, 1))
+    for pool in (one, half):
+        with pytest.raises(_lib.SpinfError, match="share places"):
+            _append(k_pages=pool)
+        with pytest.raises(_lib.SpinfError, match="share places"):
+            _evict(v_pages=pool)
+        with pytest.raises(_lib.SpinfError, match="CUDA"):  # reading them is fine
+            _call(k_pages=pool)
+    w = torch.zeros((2, 1, 48)).expand(-1, 2, -1)
+    with pytest.raises(_lib.SpinfError, match="share places"):
+        _call(weights=w)
+    with pytest.raises(_lib.SpinfError, match="CUDA"):
+        _call(weights=w, weights_out=torch.zeros((2, 2, 48)))
+    with pytest.raises(_lib.SpinfError, match="CUDA"):  # K and V side by side in one tensor, token-major weights' rows apart
+        both = torch.zeros((6, 2, 2, 16, 128), dtype=torch.bfloat16)
+        _append(k_pages=both[:, 0], v_pages=both[:, 1])
