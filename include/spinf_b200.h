@@ -461,8 +461,8 @@ int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int32_t H, int
  * weights_in is not read. out lies apart from q, its rows behind cu[B] are left as they were. A sequence's results do not depend on
  * the other sequences of the call (a call of one sequence takes the kernel that max_q asks for, a call of several each sequence's
  * own rows). The rows that share an item of work (up to 256 rows of neighbouring tokens) share their slots' values: those that none
- * of them sees never reach a result, whatever they hold; a value that is not finite in a slot that one of them sees makes all of
- * them NaN. */
+ * of them sees never reach a result, whatever they hold; a value that is not finite in a slot that one of them sees may make
+ * all of them NaN. */
 int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
                                               int32_t weights);
 int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* k_pages,

@@ -1,17 +1,29 @@
-// Attention of new tokens over the paged K/V cache: out = softmax(scale q K^T) V over the slots a row sees.
+// Attention of new tokens over the paged K/V cache: out = softmax(scale q K^T) V over the slots a row sees. Here: the sequences with few
+// rows per key / value head (rows = new tokens x heads that share it), and the call's C entry points; paged_chunk.cu has the others.
 //
-//   paged_rows_kernel     sequences with few rows per key / value head (at most 64 = tokens x heads that share it): a decoding step,
-//                         a question branch. Bound by reading K and V once.
-//   paged_join_kernel     joins the splits of a sequence: out = sum_c e^(m_c - m) O_c / sum_c e^(m_c - m) l_c
-//   paged_weight_kernel   adds each key's attention weight, sum over rows and heads of p, from the scores the first kernel kept
+//   paged_step_kernel    at most 16 rows: a decoding step
+//   paged_rows_kernel    up to 32 rows per head set: a question branch, a short chunk
+//   paged_join_kernel    joins the splits of a sequence: out = sum_c e^(m_c - m) O_c / sum_c e^(m_c - m) l_c
+//   paged_weight_kernel  adds each slot's attention weight, the sum over rows and heads of p, from the scores the first two kept
 //
-// paged_rows_kernel: persistent CTAs, one per SM; an item is (sequence, 64-row tile, kv head, split of the keys). One producer lane
-// brings K and V pages in with TMA, 64 keys at a time, into one ring that runs ahead across items; eight warps work on tiles of 128
-// keys. S: each warp takes 16 keys of the tile against all rows (warp-level mma.sync: at most 64 rows, so the products are far from
-// bounding: a tile of 128 keys takes about 5 700 cycles to arrive at an SM's share of HBM). The row maxima are exchanged through
-// shared memory, P goes to shared memory as bf16, and for P V each warp takes an eighth of the head dimensions over all 128 keys, so
-// the output needs no exchange and K and V are read from shared memory once. Running maximum and sum in fp32; P is rounded to bf16
-// for the product (its operands are 16 bit), which adds about what rounding the output to bf16 adds; the sum takes p unrounded.
+// Both attention kernels: persistent CTAs, one per SM; an item is (sequence, 64-row tile, kv head, split of the keys). A producer warp
+// brings K and V pages in with TMA, 64 keys a stage, into one ring that runs ahead across items; the others compute with warp-level
+// products (a 128-row tensor-core tile would be 8 to 16 times empty) and a running maximum and sum in fp32. P is rounded to bf16 for
+// the product (its operands are 16 bit), which adds about what rounding the output to bf16 adds; the sum takes p unrounded.
+//
+// paged_step_kernel: each warp takes 16 keys against all rows and keeps a maximum, a sum and an output of its own, so that nothing but
+// the ring's barriers stands between a key's arrival and its use; the warps' shares are joined once per item. (With a shared maximum,
+// as in the rows kernel, 64 sequences of up to 8 192 tokens took 714 us, so 394.) S^T = K Q^T with the keys as rows: P^T is turned into
+// the second product's operand between lanes, without shared memory. Bound by HBM: 64 ragged steps (32 / 16 heads of 128) 394 us, 6.2
+// TB/s of K and V; 131 072 slots (24 / 4 heads of 256) 90 us, 6.0 TB/s; a few short sequences by latency: 4 x 1 501 tokens 19 us, of
+// which about 7 are the launches of the kernel and the join. Pages of 64 tokens and more are one copy a stage; of 32 tokens two (6.2
+// TB/s instead of 6.5), of 16 four (4.8 TB/s).
+//
+// paged_rows_kernel: S: each warp takes 16 keys of a 128-key tile against all rows. The row maxima are exchanged through shared memory,
+// P goes to shared memory as bf16, and for P V each warp takes an eighth of the head dimensions over all 128 keys, so the output needs
+// no exchange and K and V are read from shared memory once. Bound by the warp-level products (one m16n8k16 takes a scheduler about 13
+// cycles: 24 rows padded to 32 and D 256 make a tile 5 900 cycles, and an item costs about 4 000 more): 56 branches of 12 tokens over
+// 2 012 (16 / 8 heads of 256) 224 us.
 #include "paged_attn.cuh"
 
 #include <atomic>
@@ -907,8 +919,10 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedSeqs s, c
   }
 }
 
-// weights_out[b][g][j] = decay weights[b][g][j] + sum over the sequence's rows of kv head g of p(row, j), for j < len; a thread owns a
-// key and adds its rows in order
+// weights_out[b][g][j] = decay weights[b][g][j] + sum over the sequence's rows of kv head g of p(row, j), for j < len; a thread owns
+// four keys, 256 apart, and adds their rows in order. Bound by reading the scores back (L2): 16 steps over up to 4 096 tokens (16 / 8 heads of
+// 256) 78 us with the attention, 6 us of them here. Scores are written and read once because the attention cannot weigh a key before
+// its row's last key is known; for a chunk they would be the larger part, so there they are computed again (paged_chunk.cu).
 __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, const PagedAttnArgs a, const PagedWeightArgs w, int* __restrict__ status) {
   pdl_trigger();
   pdl_wait();

@@ -1,17 +1,21 @@
-// Attention of a chunk of new tokens over the paged K/V cache (sequences with more than 32 query rows per kv head and head set), tcgen05 + TMEM +
-// TMA.
+// Attention of a chunk of new tokens over the paged K/V cache (sequences with more than 32 query rows per kv head and head set), on
+// tcgen05, TMEM and TMA.
 //
 // An item is 256 query rows of one kv head in two tiles of 128: `hp` heads that share it x 256 / hp tokens, the first half of the
 // tokens in one tile and the second in the other. The key tiles some row sees are walked 128 keys at a time; S = Q K^T and O += P V
-// on the tensor cores with P read from tensor memory, the softmax thread per row in fp32 with P rounded to bf16 for the product.
+// on the tensor cores with P read from tensor memory, the softmax thread per row in fp32 with P rounded to bf16 for the product. A
+// row's reference maximum moves (and O is scaled) only when its maximum has outgrown it by more than 2^24.
 //   D 256 (paged_pair_kernel): a CTA pair, one tile of rows each (O takes half of tensor memory). The pair is there for K and V: 128
 //       rows alone would need 128 keys from L2 every 2 048 cycles, 64 bytes per cycle and SM, more than L2 delivers. Two S buffers; two
-//       groups of four softmax warps, each half the keys of every row.
+//       groups of four softmax warps, each half the keys of every row. 2 048 tokens over 18 432 (16 / 8 heads of 256): 546 us, 2 970
+//       cycles a tile where the products take 2 048; the tensor pipe is 61 to 70 % busy, at a clock that the power limit has brought
+//       to about 1.6 GHz: 1 037 TFLOP/s of visible pairs.
 //   D 128 (paged_two_kernel): one CTA holds both tiles (S and O of each fill tensor memory) and a group of four softmax warps per tile.
 //       The exponentials take as long as the products here (128 x 128 at 16 per cycle and SM: 1 024 cycles); with two independent tiles
-//       one tile's softmax runs under the other's products and waits, where the pair form leaves its chain of waits exposed (2 434
-//       cycles per 128 x 128 and SM).
-// Bound by the tensor pipe (4 D flops per row and key).
+//       one tile's softmax runs under the other's products and waits, where the pair form left its chain of waits exposed. About
+//       4 000 cycles for two tiles (the pair form: 4 870): 2 000 of softmax arithmetic, the rest waits for the products. 1 024 tokens
+//       over 8 192 (32 / 16 heads of 128) 150 us; seven chunks of up to 1 501 tokens, window 1 024, 254 us.
+// Bound by the chain product - softmax - product; the tensor pipe (4 D flops per row and key) is the floor.
 //
 // A sequence's work, the (item, key tile) pairs in order, is dealt out in equal contiguous units, one per CTA pair / CTA of the GPU
 // (fewer for little work): the causal triangle, ragged tails and few items of many tiles balance by themselves. An item cut by
@@ -1122,7 +1126,10 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedAttnAr
 // pass over Q K^T, this time with the keys as the rows of the product, so that a key's sum stays in one thread: S^T = K Q^T, thread =
 // key, 64 query rows a stage along its columns. No reduction across threads, no atomics: a key adds its rows in one fixed order.
 // Item = 256 keys of a (sequence, kv head), both tiles of K resident in shared memory while the rows that see any of them stream by.
-// Bound by the exponentials (256 x 64 a stage at 16 per cycle and SM: 1 024 cycles, the products 512 at D 128 and 1 024 at D 256).
+// Bound by the exponentials and what surrounds them (256 x 64 a stage at 16 per cycle and SM: 1 024 cycles, the products 512 at D 128
+// and 1 024 at D 256; measured 2 050 a stage: reading S out of tensor memory and the instructions around each exponential share the
+// issue slots). 1 024 tokens over 8 192 (32 / 16 heads of 128): 285 us with the attention, about 130 of them here; scores kept in memory
+// and read back took 2 500 for the same.
 template <int D>
 struct ChunkWeightSmem {
   static constexpr int SLABS = D / 64;
