@@ -460,15 +460,17 @@ int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int32_t H, int
  * over the sequence's rows and the heads that share kv head g, for j < lens[b]; the two may be the same tensor; with decay 0
  * weights_in is not read. out lies apart from q, its rows behind cu[B] are left as they were. A sequence's results do not depend on
  * the other sequences of the call (a call of one sequence takes the kernel that max_q asks for, a call of several each sequence's
- * own rows). The rows that share an item of work (up to 256 rows of neighbouring tokens) share their slots' values: those that none
+ * own rows), with `shared` but for the sequences it shares pages with. shared: look for neighbouring sequences (with up to 128 rows per
+ * kv head and head set) whose tables begin with the same pages, at least 1 024 tokens of them and 128 MB of reading saved, and read
+ * those once for all of their rows (the same sums, added in another order; without window and weights). The rows that share an item of work (up to 256 rows of neighbouring tokens) share their slots' values: those that none
  * of them sees never reach a result, whatever they hold; a value that is not finite in a slot that one of them sees may make
  * all of them NaN. */
 int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
-                                              int32_t weights);
+                                              int32_t weights, int32_t shared);
 int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* k_pages,
                           const void* v_pages, int64_t n_pages, int32_t page, const int64_t* k_strides_host,
                           const int64_t* v_strides_host, const int32_t* table, int64_t table_pitch, const int32_t* lens,
-                          const int32_t* cu, int32_t B, int64_t max_q, int64_t max_len, int32_t window, float scale,
+                          const int32_t* cu, int32_t B, int64_t max_q, int64_t max_len, int32_t window, int32_t shared, float scale,
                           const float* weights_in, float* weights_out, const int64_t* weight_strides_host, float decay, void* out,
                           int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream);
 

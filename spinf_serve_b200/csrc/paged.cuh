@@ -24,11 +24,16 @@ struct PagedSeqs {
   int max_len;  // longest sequence the caller's buffers are sized for
   int max_q;    // most new rows of a sequence they are sized for
   int64_t n;    // rows of q
+  const int32_t* share;  // [2][B], or null: key tiles of each sequence that its group reads together; behind a group's first, at B + b, its end
 };
 
 struct PagedSeq {
   int row0, nq, len;
+  int skip;  // key tiles at the front that are another item's work (0: none)
+  int cap;   // slots from here on are another item's work (a group's common front; INT_MAX otherwise)
 };
+static constexpr int PG_NO_CAP = 0x7fffffff;
+static constexpr int PG_SKIP_SPLITS = 4;  // most splits behind a shared front: little is left there, and the parts of up to four times the rows take room
 
 // the sequence's numbers, cut to what the buffers hold: one that lies outside them is reported and treated as
 // shorter, or as having no new rows
@@ -38,6 +43,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedSeqs& s, int b, int* st
   r.len = s.lens[b];
   r.row0 = r0;
   r.nq = r1 - r0;
+  r.skip = s.share ? s.share[b] : 0;
+  r.cap = PG_NO_CAP;
   if (r0 < 0 || r1 < r0 || r1 > s.n || r.nq > s.max_q) {
     r.row0 = r.nq = 0;
     atomicCAS(status, 0, ST_BAD_INDEX);
@@ -63,12 +70,12 @@ __device__ __forceinline__ PagedCut paged_cut(const PagedSeq& q, int window, int
   PagedCut c;
   c.row_tiles = row_tiles;
   const int first = q.len - q.nq + 1 - window;
-  c.t_lo = window > 0 && first > 0 ? first / PG_TILE : 0;
+  c.t_lo = window > 0 && first > 0 ? first / PG_TILE : q.skip;
   c.t_hi = (q.len + PG_TILE - 1) / PG_TILE;
   const int tiles = c.t_hi > c.t_lo ? c.t_hi - c.t_lo : 0;
   int s = slots / (items_per_split > 0 ? items_per_split : 1);
   s = s < tiles / min_tiles ? s : tiles / min_tiles;
-  s = s < 1 ? 1 : s;
+  s = s < 1 ? 1 : q.skip && s > PG_SKIP_SPLITS ? PG_SKIP_SPLITS : s;
   c.tiles_per_split = (tiles + s - 1) / s;
   c.splits = c.tiles_per_split > 0 ? (tiles + c.tiles_per_split - 1) / c.tiles_per_split : 1;
   return c;

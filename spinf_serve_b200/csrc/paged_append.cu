@@ -204,7 +204,7 @@ extern "C" int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int
   a.k_page = k_strides_host[0], a.k_head = k_strides_host[1], a.k_row = k_strides_host[2];
   a.v_page = v_strides_host[0], a.v_head = v_strides_host[1], a.v_row = v_strides_host[2];
   a.width = width;
-  PagedSeqs s;
+  PagedSeqs s = {};
   s.table = table;
   s.table_pitch = table_pitch;
   s.lens = lens;

@@ -24,6 +24,10 @@
 // no exchange and K and V are read from shared memory once. Bound by the warp-level products (one m16n8k16 takes a scheduler about 13
 // cycles: 24 rows padded to 32 and D 256 make a tile 5 900 cycles, and an item costs about 4 000 more): 56 branches of 12 tokens over
 // 2 012 (16 / 8 heads of 256) 224 us.
+//
+//   paged_share_kernel   finds neighbouring sequences that begin with the same pages (branches of one content). Their common front is then
+//                        read once for all of their rows, by the chunk kernels; the kernels here begin behind it: the 56 branches 98 us
+//                        (looking 6, few-row part 39, front 40, joins 13), 12 tokens over 16 384 each 1 500 -> 293 us.
 #include "paged_attn.cuh"
 
 #include <atomic>
@@ -78,7 +82,7 @@ __device__ __forceinline__ KeyItem key_item(const PagedSeqs& s, const PagedAttnA
   if (!STEP) x /= c.row_tiles;
   w.g = x % a.h;
   w.split = x / a.h;
-  w.splits = c.splits;
+  w.splits = c.splits + (q.skip ? 1 : 0);  // (what the sequence shares with others counts as a split: the item's result is a part)
   w.row0 = q.row0, w.nq = q.nq, w.base = q.len - q.nq;
   const int all = q.nq * a.group;
   w.rows = STEP || all - w.r0 < RT ? all - w.r0 : RT;
@@ -574,6 +578,7 @@ paged_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(q_empty + 2);
   const WaitCtx wc{abort_flag, status};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (s.share) pdl_wait();  // the groups are the kernel's ahead; all kernels behind this one start after this
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NST; ++i) {
@@ -851,7 +856,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedSeqs s, c
   pdl_wait();
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSeq q = paged_seq(s, b, status);
-  if (q.nq == 0 || chunk_class(q, a)) return;
+  if (q.nq == 0 || q.skip || chunk_class(q, a)) return;
   const PagedCut c = attn_cut(q, a);
   if (c.splits == 1) return;
   const int all = q.nq * a.group, rows = q.nq * a.H;
@@ -952,6 +957,74 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, co
   }
 }
 
+// Finds the groups: runs of neighbouring sequences, none of them a long chunk, whose tables begin with the same pages. share[b]: key tiles of
+// b's group (0: none), share[B + b]: behind a group's first sequence its end. One CTA: a warp compares two tables, then one thread walks
+// the runs. A run ends where the common front changes by more than a factor of two (another content behind a prompt that both share),
+// and a group whose units the workspace has no room for is left as it is.
+__global__ void __launch_bounds__(1024) paged_share_kernel(const PagedSeqs s, const PagedAttnArgs a, int32_t* __restrict__ share, int units,
+                                                           int* __restrict__ status) {
+  __shared__ int lim[PG_MAX_SEQS], link[PG_MAX_SEQS], out[2 * PG_MAX_SEQS];
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int b = tid; b < s.B; b += 1024) {
+    const PagedSeq q = paged_seq(s, b, status);
+    lim[b] = q.nq > 0 && q.nq * a.group <= SHARE_ROWS * a.chunk_rows && q.len > q.nq ? (q.len - q.nq) / PG_TILE : 0;
+    link[b] = out[b] = out[s.B + b] = 0;
+  }
+  __syncthreads();
+  for (int b = warp; b + 1 < s.B; b += 32) {
+    const int most = lim[b] < lim[b + 1] ? lim[b] : lim[b + 1];
+    if (most < SHARE_TILES) continue;
+    const int pages = (most * PG_TILE + (1 << s.page_log2) - 1) >> s.page_log2;
+    const int32_t* x = s.table + b * s.table_pitch;
+    const int32_t* y = x + s.table_pitch;
+    int common = pages;
+    for (int p0 = 0; p0 < pages && common == pages; p0 += 128) {
+      bool same[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) same[u] = p0 + u * 32 + lane >= pages || x[p0 + u * 32 + lane] == y[p0 + u * 32 + lane];
+#pragma unroll
+      for (int u = 3; u >= 0; --u) {
+        const uint32_t off = __ballot_sync(0xffffffffu, !same[u]);
+        if (off) common = p0 + u * 32 + __ffs(off) - 1;
+      }
+    }
+    const int64_t tiles = (static_cast<int64_t>(common) << s.page_log2) / PG_TILE;
+    if (lane == 0) link[b] = tiles < most ? static_cast<int>(tiles) : most;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int used = 0;
+    for (int b = 0; b + 1 < s.B;) {
+      int t = link[b], e = b + 1;
+      if (t < SHARE_TILES) {
+        ++b;
+        continue;
+      }
+      for (; e + 1 < s.B && link[e] >= SHARE_TILES && 2 * link[e] >= t && link[e] <= 2 * t; ++e) t = link[e] < t ? link[e] : t;
+      if (!share_pays(e + 1 - b, t * PG_TILE, a.h, a.D)) {
+        b = e;
+        continue;
+      }
+      PagedSeq q;
+      q.row0 = s.cu[b];
+      q.nq = s.cu[e + 1] - q.row0;
+      q.skip = t;
+      q.cap = t * PG_TILE;
+      q.len = q.cap + q.nq;
+      const int need = chunk_cut(q, a).units;
+      if (used + need <= units) {
+        used += need;
+        for (int i = b; i <= e; ++i) out[i] = t;
+        out[s.B + b] = e + 1;
+      }
+      b = e + 1;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < 2 * s.B; i += 1024) share[i] = out[i];
+}
+
 // A sequence with more rows per kv head than this is the chunk kernels', where a head set of it fills 256-row items: measured on 32
 // sequences of 2 000 tokens (16 / 8 heads of 256) 32 rows took 138 us in the few-row kernel and 168 there, 64 rows 253 and 172; with
 // three head sets per kv head (24 / 4 heads) 48 rows 106 and 237, 96 rows 250 and 240.
@@ -959,13 +1032,13 @@ __host__ __device__ constexpr int chunk_rows_of(int group) { return 32 * (group 
 
 // what a call needs: sizes of the workspace's parts in bytes (256-byte multiples)
 struct PagedSizes {
-  int64_t seq_parts, part_o, part_ml, chunk_o, chunk_ml, joins, lse, scores, total;
+  int64_t seq_parts, part_o, part_ml, chunk_o, chunk_ml, joins, share, lse, scores, total;
   int64_t score_pitch;
-  int tok_cap, chunk_rows, max_units;
+  int tok_cap, chunk_rows, max_units, share_units;
   bool too_large;
 };
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
-static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights) {
+static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights, bool shared) {
   PagedSizes z = {};
   const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
   const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
@@ -977,20 +1050,37 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
     const int64_t by_items = static_cast<int64_t>(PG_SMS) * RT;  // every free slot one full row tile
     z.seq_parts = by_rows < by_items ? by_rows : by_items;
   }
+  shared = shared && !weights && B > 1 && tiles > SHARE_TILES && share_pays(B, max_len, h, D);
+  if (shared) {  // a sequence of a group leaves parts in any case
+    const int64_t one = (max_q < SHARE_ROWS * most ? max_q : SHARE_ROWS * most) * H;
+    const int64_t parts = one * (slots < 1 ? 1 : slots < PG_SKIP_SPLITS ? slots : PG_SKIP_SPLITS);
+    z.seq_parts = z.seq_parts > parts ? z.seq_parts : parts;
+  }
   z.part_o = up256(B * z.seq_parts * D * 4);
   z.part_ml = up256(B * z.seq_parts * 8);
+  const int hl = chunk_heads_log2(static_cast<int>(group)), tl = 8 - hl;
+  int64_t all_units = 0;
   if (max_q > most) {
-    const int hl = chunk_heads_log2(static_cast<int>(group)), tl = 8 - hl;
     const int64_t work = ((max_q + (1 << tl) - 1) >> tl) * (H >> hl) * (tiles > 0 ? tiles : 1);
     if (work >= (1ll << 31)) z.too_large = true;  // the chunk kernels count (item, key tile) pairs in 32 bits
     // (an item makes a unit, or a unit holds CHUNK_MIN_TILES pairs, or a part of an item four)
     int64_t units = work / 4 + ((max_q + (1 << tl) - 1) >> tl) * (H >> hl);
     units = units > chunk_units_of(D) ? chunk_units_of(D) : units;
     const int64_t seqs = B == 1 ? 1 : n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
-    z.max_units = static_cast<int>(seqs * units);
-    z.chunk_o = up256(seqs * units * 512 * D * 4);
-    z.chunk_ml = up256(seqs * units * 512 * 8);
-    z.joins = up256(seqs * units * static_cast<int64_t>(sizeof(ChunkJoin)) + 16);
+    all_units = seqs * units;
+  }
+  if (shared) {
+    // a unit per item of a group, or up to one per CTA (pair) for a group of few items: room for four such groups
+    const int64_t items = ((n >> tl) + B / 2) * (H >> hl) + 4 * chunk_units_of(D);
+    z.share_units = static_cast<int>(items < 4 * PG_SMS ? items : 4 * PG_SMS);
+    z.share = up256(B * 8);
+    all_units += z.share_units;
+  }
+  z.max_units = static_cast<int>(all_units);
+  if (all_units > 0) {
+    z.chunk_o = up256(all_units * 512 * D * 4);
+    z.chunk_ml = up256(all_units * 512 * 8);
+    z.joins = up256(all_units * static_cast<int64_t>(sizeof(ChunkJoin)) + 16);
   }
   if (weights) {
     z.lse = up256(n * H * 4);
@@ -998,13 +1088,13 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
     z.tok_cap = static_cast<int>(max_q < most ? max_q : most);
     z.scores = up256(B * z.tok_cap * H * z.score_pitch * 4);
   }
-  z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.joins + z.lse + z.scores;
+  z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.joins + z.share + z.lse + z.scores;
   return z;
 }
 
 template <int D>
 static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeqs& s, const PagedAttnArgs& a, const PagedWeightArgs* w, int64_t max_q,
-                        int max_splits, cudaStream_t st, int dev, int* status) {
+                        int max_splits, int share_units, cudaStream_t st, int dev, int* status) {
   CUtensorMap tmK, tmV;
   int r;
   const uint32_t box = kp.page < 64 ? static_cast<uint32_t>(kp.page) : 64u;
@@ -1019,19 +1109,23 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   const unsigned grid = static_cast<unsigned>(sm_count());
   // with one sequence its kernel is known here: the others' launches fall away
   const bool step = a.only ? a.only == 1 : true, rows = a.only ? a.only == 2 : max_q * a.group > STEP_ROWS;
-  const bool chunk = a.only ? a.only == 3 : max_q * a.group > a.chunk_rows;
-  if (step) {
-    if (max_q * a.group <= 8)
-      paged_step_kernel<D, 1><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
-    else
-      paged_step_kernel<D, 2><<<grid, step_threads(D), StepSmem<D>::TOTAL, st>>>(tmK, tmV, s, a, status);
+  const bool chunk = a.only ? a.only == 3 : max_q * a.group > a.chunk_rows || share_units > 0;
+  if (share_units > 0) {
+    PagedSeqs plain = s;
+    plain.share = nullptr;
+    paged_share_kernel<<<1, 1024, 0, st>>>(plain, a, const_cast<int32_t*>(s.share), share_units, status);
     SPINF_CUDA_OK(cudaGetLastError());
+  }
+  if (step) {
+    const auto kern = max_q * a.group <= 8 ? paged_step_kernel<D, 1> : paged_step_kernel<D, 2>;
+    SPINF_CUDA_OK(launch_after(kern, dim3(grid), dim3(step_threads(D)), st, StepSmem<D>::TOTAL, 1, share_units > 0, tmK, tmV, s, a, status));
   }
   if (rows) SPINF_CUDA_OK(launch_after(paged_rows_kernel<D>, dim3(grid), dim3(ROWS_THREADS), st, RowsSmem<D>::TOTAL, 1, step, tmK, tmV, s, a, status));
   if (max_splits > 1 && (step || rows)) {
     const int64_t most = a.chunk_rows / a.group;  // tokens of a sequence that is not the chunk kernel's
     int64_t gx = (max_q < most ? max_q : most) * a.H;
-    if (gx > 1024) gx = 1024;
+    const int64_t fill = 8 * PG_SMS / s.B > 16 ? 8 * PG_SMS / s.B : 16;  // (CTAs of many sequences that have nothing to join cost 10 us to start)
+    if (gx > fill) gx = fill;
     SPINF_CUDA_OK(launch_after(paged_join_kernel<D>, dim3(static_cast<unsigned>(gx), s.B), dim3(256), st, 0, 1, true, s, a, status));
   }
   if (chunk && (r = paged_chunk_launch(D, kp, vp, s, a, w, step || rows, st, dev, status))) return r;
@@ -1045,17 +1139,17 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
 using namespace spinf;
 
 extern "C" int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
-                                                         int32_t weights) {
+                                                         int32_t weights, int32_t shared) {
   if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
   if (n < 0 || B < 0 || H <= 0 || Hkv <= 0 || H % Hkv || (D != 128 && D != 256) || max_q < 0 || max_len < 0) return SPINF_ERR_BAD_ARGUMENT;
-  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0);
+  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0, shared != 0);
   return z.too_large ? SPINF_ERR_TOO_LARGE : z.total;
 }
 
 extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, int32_t H, int32_t Hkv, int32_t D, const void* k_pages,
                                      const void* v_pages, int64_t n_pages, int32_t page, const int64_t* k_strides_host,
                                      const int64_t* v_strides_host, const int32_t* table, int64_t table_pitch, const int32_t* lens,
-                                     const int32_t* cu, int32_t B, int64_t max_q, int64_t max_len, int32_t window, float scale,
+                                     const int32_t* cu, int32_t B, int64_t max_q, int64_t max_len, int32_t window, int32_t shared, float scale,
                                      const float* weights_in, float* weights_out, const int64_t* weight_strides_host, float decay,
                                      void* out, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
   if (B == 0 || (n == 0 && !weights_out)) return 0;  // nothing to do: the row pointers may be null
@@ -1069,14 +1163,15 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   SPINF_CHECK_ARG(!weights_out || (weight_strides_host && (weights_in || decay == 0.f)));
   if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
   const int64_t mq = max_q < n ? max_q : n;
-  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr);
+  const bool narrow = window > 0 && window < max_len;  // (a window of max_len slots holds everything: no window)
+  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr, shared && !narrow);
   if (z.too_large) return SPINF_ERR_TOO_LARGE;
   SPINF_CHECK_ARG(z.total == 0 || (workspace && workspace_bytes >= z.total && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0));
   int dev = 0;
   SPINF_CUDA_OK(cudaGetDevice(&dev));
   int* status = status_word(dev);
   if (!status) return SPINF_ERR_CUDA;
-  PagedSeqs s;
+  PagedSeqs s = {};
   s.table = table;
   s.table_pitch = table_pitch;
   s.lens = lens;
@@ -1097,7 +1192,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.h = Hkv;
   a.D = D;
   a.group = H / Hkv;
-  a.window = window < max_len ? window : 0;  // (no row has more slots before it: the same, and sums with it stay in 32 bits)
+  a.window = narrow ? window : 0;  // (sums with it stay in 32 bits)
   a.hp_log2 = chunk_heads_log2(a.group);
   a.sets = a.group >> a.hp_log2;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -1116,6 +1211,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.chunk_ml = reinterpret_cast<float2*>(take(z.chunk_ml));
   a.n_units = reinterpret_cast<int32_t*>(take(z.joins));
   a.joins = reinterpret_cast<ChunkJoin*>(a.n_units + 4);
+  if (z.share_units) s.share = reinterpret_cast<int32_t*>(take(z.share));
   if (weights_out) {
     a.lse = reinterpret_cast<float*>(take(z.lse));
     a.scores = reinterpret_cast<float*>(take(z.scores));
@@ -1134,6 +1230,6 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   const PagedPool vp = {v_pages, n_pages, page, Hkv, D, v_strides_host[0], v_strides_host[1], v_strides_host[2]};
   const int max_splits = z.seq_parts ? 2 : 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return D == 256 ? launch_paged<256>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, st, dev, status)
-                  : launch_paged<128>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, st, dev, status);
+  return D == 256 ? launch_paged<256>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, z.share_units, st, dev, status)
+                  : launch_paged<128>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, z.share_units, st, dev, status);
 }

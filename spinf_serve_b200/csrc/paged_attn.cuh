@@ -45,7 +45,9 @@ static constexpr int STEP_ROWS = 16;  // rows per kv head a decoding step's kern
 
 __host__ __device__ inline int class_of(int64_t rows, int chunk_rows) { return rows <= STEP_ROWS ? 1 : rows > chunk_rows ? 3 : 2; }
 __device__ __forceinline__ int seq_class(const PagedSeq& q, const PagedAttnArgs& a) {
-  return q.nq == 0 ? 0 : a.only ? a.only : class_of(q.nq * a.group, a.chunk_rows);
+  if (q.nq == 0 || a.only) return q.nq == 0 ? 0 : a.only;
+  const int c = class_of(q.nq * a.group, a.chunk_rows);
+  return c == 3 && q.skip ? 2 : c;  // (behind a front that a group shares little is left: few-row work)
 }
 __device__ __forceinline__ bool step_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 1; }
 __device__ __forceinline__ bool rows_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 2; }
@@ -79,6 +81,7 @@ struct ChunkCut {
     const int end = (tt + 1) << tok_log2 < q.nq ? base + ((tt + 1) << tok_log2) : q.len;
     lo = a.window > 0 && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
     hi = end > 0 ? end : 0;
+    hi = hi < q.cap ? hi : q.cap;
   }
   // key tiles [t0, t0 + nt) of a token tile; one (fully masked) where nothing is seen, so that its rows are written
   __device__ __forceinline__ void tiles(const PagedSeq& q, const PagedAttnArgs& a, int tt, int& t0, int& nt) const {
@@ -109,15 +112,17 @@ __device__ __forceinline__ ChunkCut chunk_cut(const PagedSeq& q, const PagedAttn
   }
   c.work = tiles * c.per_tt;  // (the host has checked that this fits)
   const int most = chunk_units_of(a.D), items = c.ntt * c.per_tt;
-  const bool brief = tiles <= CHUNK_SHORT * c.ntt;
+  const bool brief = tiles <= CHUNK_SHORT * c.ntt, front = q.cap != PG_NO_CAP;
   c.parts = 0;
   c.whole = false;
-  if (items <= most && (c.ntt == 1 || brief)) {
-    // few items: one unit each, or (a single token tile) as many equal parts as there is room for, of at least four tiles
+  if (front || (items <= most && (c.ntt == 1 || brief))) {
+    // few items: one unit each, or (a single token tile; a group's front, whose items are all alike) as many equal parts as there is
+    // room for, of at least four tiles
     int k = 1;
-    if (c.ntt == 1) {
+    if (c.ntt == 1 || front) {
+      const int each = tiles / c.ntt / 4;
       k = most / items;
-      k = k < tiles / 4 ? k : tiles / 4;
+      k = k < each ? k : each;
       k = k > 1 ? k : 1;
     }
     c.parts = k;
@@ -138,7 +143,29 @@ struct alignas(16) ChunkJoin {
   int pieces;             // partial results of the item, the first of them not the unit's own
   int first;              // the one before (in units of 256 rows); the others are 2 it, 2 it + 2, ..
   int row0, nq, tok0, h0;
+  int b0, b1;             // a group's front: the rows belong to these sequences, whose own splits are joined here, too (b1 = 0: none)
 };
+
+// ---- the common front of neighbouring sequences (branches of one content): read once for all of their rows, by the chunk kernels, as
+// if it were one sequence whose rows see all of it; the sequences' own kernels begin behind it, and the chunk join adds the two.
+static constexpr int SHARE_TILES = 8;  // least key tiles of a front (56 sequences of 40 new tokens over 512: 127 us, read together 182; over 1 024: 252, 194)
+static constexpr int SHARE_ROWS = 4;   // a group's sequences have up to so many times the rows that make a chunk
+// The further kernels cost about 20 us, which the reading they save has to outweigh: measured without / with (us), new tokens over a
+// front of that many: 16 / 8 heads of 256, one new token each: 8 over 2 048 (117 MB saved) 36 / 36, 8 over 1 024 (59 MB) 23 / 30, 16
+// over 2 048 (252 MB) 60 / 42; twelve new tokens: 6 over 2 048 (84 MB) 47 / 46; 24 / 4 heads of 256, one each: 8 over 4 096 (117 MB)
+// 45 / 44; 8 / 8 heads of 128: 8 over 4 096 (117 MB) 31 / 32, 16 over 4 096 (252 MB) 51 / 42. Further up: 56 of 40 new tokens over 4 096
+// 796 / 285, 56 of one over 16 384 681 / 118.
+__host__ __device__ inline bool share_pays(int64_t seqs, int64_t tokens, int h, int D) { return (seqs - 1) * tokens * h * D * 4 >= 1 << 27; }
+// what the chunk kernels make of index b: a chunk's sequence, a group's front (at its first sequence), or nothing
+__device__ __forceinline__ bool chunk_seq(const PagedSeqs& s, const PagedAttnArgs& a, int b, PagedSeq& q, int* status) {
+  q = paged_seq(s, b, status);
+  const int end = s.share ? s.share[s.B + b] : 0;
+  if (end == 0) return chunk_class(q, a);
+  q.nq = s.cu[end] - q.row0;
+  q.cap = q.skip * PG_TILE;
+  q.len = q.cap + q.nq;
+  return true;
+}
 
 // page of the `rows` slots from j on, or one past the last page (the copy then brings zeros) where no row sees any of them
 __device__ __forceinline__ int chunk_page(const PagedSeqs& s, const int32_t* pages, int j, int rows, int lo, int hi, int* status) {

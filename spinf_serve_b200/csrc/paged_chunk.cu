@@ -20,7 +20,8 @@
 // A sequence's work, the (item, key tile) pairs in order, is dealt out in equal contiguous units, one per CTA pair / CTA of the GPU
 // (fewer for little work): the causal triangle, ragged tails and few items of many tiles balance by themselves. An item cut by
 // a unit's border leaves partial rows (maximum, sum, O in fp32), which the join adds in order. The cut depends on the sequence's own
-// lengths only, so its results do not depend on the rest of the call.
+// lengths only, so its results do not depend on the rest of the call. A front that several sequences share is cut and computed like a
+// sequence whose rows see all of it; its items always leave parts, and the join adds the sequences' own splits to them.
 #include "paged_attn.cuh"
 
 #include <atomic>
@@ -85,7 +86,7 @@ struct ChunkWalk {
 
   __device__ __forceinline__ void start(const PagedSeqs& s, const PagedAttnArgs& a, const int* pre, int unit, int* status) {
     b = paged_find(pre, s.B, unit);
-    q = paged_seq(s, b, status);
+    chunk_seq(s, a, b, q, status);
     c = chunk_cut(q, a);
     it = unit;
     const int u = unit - pre[b];
@@ -93,6 +94,8 @@ struct ChunkWalk {
     tt = 0, w_tt = 0;
     ChunkJoin join;
     join.pieces = 0;
+    join.b0 = b;
+    join.b1 = q.cap != PG_NO_CAP ? s.share[s.B + b] : 0;
     if (c.parts) {
       const int i = u / c.parts, part = u - i * c.parts;
       tt = i / c.per_tt;
@@ -100,9 +103,10 @@ struct ChunkWalk {
       const int item = i - tt * c.per_tt;
       w = item * nt + nt * part / c.parts;  // (pairs counted from the token tile's first)
       w_end = item * nt + nt * (part + 1) / c.parts;
-      if (part == 1) {  // parts are the first segments of their units
+      // parts are the first segments of their units. A front is never whole: its one part is joined with the sequences' own splits
+      if (part == 1 || (join.b1 && c.parts == 1)) {
         join.pieces = c.parts;
-        join.first = (unit - 1) * 2;
+        join.first = (unit - part) * 2;
         join.row0 = q.row0, join.nq = q.nq;
         join.tok0 = tt << c.tok_log2;
         join.h0 = item / a.sets * a.group + (item % a.sets << a.hp_log2);
@@ -149,7 +153,7 @@ struct ChunkWalk {
     g.ta = t0 + off;
     g.tb = g.ta + len;
     c.slots(q, a, tt, g.lo, g.hi);
-    g.part = len == nt ? -1 : it * 2 + (first ? 0 : 1);
+    g.part = len == nt && q.cap == PG_NO_CAP ? -1 : it * 2 + (first ? 0 : 1);
     first = false;
     w += len;
     return true;
@@ -422,8 +426,8 @@ __device__ __forceinline__ bool chunk_edge(const ChunkSeg& g, int t) { return t 
 // unit counts of the sequences, and for the join their sum
 __device__ __forceinline__ int chunk_units(const PagedSeqs& s, const PagedAttnArgs& a, int* pre, int* status) {
   paged_item_prefix(s.B, pre, CHUNK_THREADS, [&](int b) {
-    const PagedSeq q = paged_seq(s, b, status);
-    return chunk_class(q, a) ? chunk_cut(q, a).units : 0;
+    PagedSeq q;
+    return chunk_seq(s, a, b, q, status) ? chunk_cut(q, a).units : 0;
   });
   int total = pre[s.B];
   if (total > a.max_units) {  // rows of q that several sequences claim: more units than n rows can make
@@ -1074,7 +1078,7 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 // warp per row, the pieces added in the order of the units (an item in nine parts is a chain of loads for a row, so rows side by side)
 static constexpr int JOIN_ROWS = 16;
 template <int D>
-__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
   pdl_trigger();
   pdl_wait();
   constexpr int V = D / 128;  // float4 per lane
@@ -1092,6 +1096,18 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedAttnAr
       float m = a.chunk_ml[at0].x;
 #pragma unroll 4
       for (int y = 0; y <= last; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
+      int splits = 0;  // the row's own, behind the front it shares
+      int64_t own = 0, own_step = 0;
+      if (join.b1) {
+        int b = join.b0 - 1;  // the last sequence that begins at or before the row (the lanes look at 32 at a time: no chain of loads)
+        for (int b0 = join.b0; b0 < join.b1; b0 += 32) b += __popc(__ballot_sync(0xffffffffu, b0 + lane < join.b1 && s.cu[b0 + lane] <= join.row0 + tok));
+        const PagedSeq q = paged_seq(s, b, status);
+        const int all = q.nq * a.group;
+        splits = attn_cut(q, a).splits;
+        own_step = static_cast<int64_t>(a.h) * all;
+        own = b * a.seq_parts + static_cast<int64_t>(head / a.group) * all + (join.row0 + tok - q.row0) * a.group + head % a.group;
+        for (int y = 0; y < splits; ++y) m = fmaxf(m, a.part_ml[own + y * own_step].x);
+      }
       const float neg_m = m == -INFINITY ? 0.f : -m;
       float l = 0.f;
       float4 acc[V];
@@ -1104,6 +1120,19 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedAttnAr
         const float f = fast_exp2(ml.x + neg_m);
         l = fmaf(f, ml.y, l);
         const float4* src = reinterpret_cast<const float4*>(a.chunk_o + from * D);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float4 z = src[v * 32 + lane];
+          acc[v].x = fmaf(f, z.x, acc[v].x), acc[v].y = fmaf(f, z.y, acc[v].y), acc[v].z = fmaf(f, z.z, acc[v].z), acc[v].w = fmaf(f, z.w, acc[v].w);
+        }
+      }
+#pragma unroll 2
+      for (int y = 0; y < splits; ++y) {
+        const int64_t from = own + y * own_step;
+        const float2 ml = a.part_ml[from];
+        const float f = fast_exp2(ml.x + neg_m);
+        l = fmaf(f, ml.y, l);
+        const float4* src = reinterpret_cast<const float4*>(a.part_o + from * D);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float4 z = src[v * 32 + lane];
@@ -1402,7 +1431,7 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   }
   SPINF_CUDA_OK(launch_after(kern, dim3(static_cast<unsigned>(D == 256 ? sm_count() / 2 * 2 : sm_count())), dim3(CHUNK_THREADS), st, L::TOTAL,
                              D == 256 ? 2 : 1, early, tmQ, tmK, tmV, s, a, status));
-  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units < PG_SMS ? a.max_units : PG_SMS), 256 / JOIN_ROWS), dim3(256), st, 0, 1, true, a));
+  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units < PG_SMS ? a.max_units : PG_SMS), 256 / JOIN_ROWS), dim3(256), st, 0, 1, true, s, a, status));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
   if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;

@@ -610,6 +610,7 @@ def embed_scale(ids, emb, scale):
 # kept short: everything that follows from shapes, strides and types is checked and worked out once per layout (the *_layout functions
 # below remember it by exactly those), and a call itself looks at devices and addresses only.
 _I32, _BF16, _F32, _U8 = torch.int32, torch.bfloat16, torch.float32, torch.uint8
+SHARE_BYTES = 1 << 27  # reading saved from which paged_attention reads a common front once (share_pays in csrc/paged_attn.cuh)
 
 
 def _layout(t):
@@ -738,7 +739,7 @@ def _paged_device(what, *tensors):
 
 
 @functools.lru_cache(maxsize=512)
-def _attention_layout(q, k, v, table, lens, cu, max_q, window, w_in, w_out, max_len, out):
+def _attention_layout(q, k, v, table, lens, cu, max_q, window, w_in, w_out, max_len, out, shared):
     what = "paged_attention"
     n_pages, h, page, D, ks, vs = _page_layout(k, v, what)
     if q[0] is not _BF16 or len(q[1]) != 3 or q[1][2] != D:
@@ -767,32 +768,37 @@ def _attention_layout(q, k, v, table, lens, cu, max_q, window, w_in, w_out, max_
         if not _apart(*w_out[1:]):
             raise SpinfError(f"{what}: weights_out is written to, slots must not share places: {w_out}")
         strides = (ctypes.c_int64 * 4)(*w_in[2][:2], *w_out[2][:2])
-    need = int(_lib.lib().spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_in is not None))
-    check(need, what)
     win = window if window is not None and window < max_len else 0  # (a window that holds everything is none)
-    return n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, win, strides, need
+    if shared is None:
+        shared = B * max_len > 4 * n_pages * page
+    shared = bool(shared) and win == 0 and w_in is None
+    need = int(_lib.lib().spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_in is not None, shared))
+    check(need, what)
+    return n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, win, strides, need, shared
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=None, weights=None, weights_out=None, decay=1.0, max_len=None,
-                    out=None, workspace=None):
+                    out=None, workspace=None, shared=None):
     """attention of new tokens over the paged cache: q [n, H, D] bf16 (a view with contiguous heads and any row pitch), sequence b's
     rows cu[b] .. cu[b + 1] over its lens[b] cached tokens, of which its own rows are the last; causal, with a window only the last
     `window` slots of a row -> [n, H, D] (rows behind cu[B]: undefined in a new tensor, untouched in `out`; a row that sees nothing:
     0). max_q, max_len: no sequence has more rows / tokens (max_len None: what the table can hold).
     weights (fp32 [B, Hkv, cap], cap >= max_len): each slot's accumulated attention weight, weights_out = decay * weights + this
     call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
-    tensor reused between calls on one stream; out must not overlap q."""
+    tensor reused between calls on one stream; out must not overlap q. shared: look for neighbouring sequences whose tables begin with
+    the same pages (branches of one content) and read those once for all of them (None: where the pool has less than a quarter of the
+    pages that this many sequences of max_len tokens would need; looking in vain costs up to 20 us)."""
     what = "paged_attention"
     if weights is not None and weights_out is None:
         weights_out = weights
-    n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, win, strides, need = _attention_layout(
+    n, H, h, D, q_pitch, out_pitch, n_pages, page, ks, vs, pitch, B, max_len, win, strides, need, shared = _attention_layout(
         _layout(q), _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cu), max_q, window, _layout(weights), _layout(weights_out),
-        max_len, _layout(out)
+        max_len, _layout(out), shared
     )
     idx = _paged_device(what, q, k_pages, v_pages, table, lens, cu, weights, weights_out, out, workspace)
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
-            return paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace)
+            return paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace, shared)
     if out is None:
         out = q.new_empty((n, H, D))
     elif n and out.data_ptr() == q.data_ptr():
@@ -802,7 +808,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     check(
         _lib.lib().spinf_paged_attention(
             q.data_ptr(), q_pitch, n, H, h, D, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, ks, vs, table.data_ptr(), pitch, lens.data_ptr(),
-            cu.data_ptr(), B, max_q, max_len, win, scale, None if weights is None else weights.data_ptr(), None if weights is None else weights_out.data_ptr(),
+            cu.data_ptr(), B, max_q, max_len, win, shared, scale, None if weights is None else weights.data_ptr(), None if weights is None else weights_out.data_ptr(),
             strides, decay, out.data_ptr(), out_pitch, workspace.data_ptr() if need else None, need, _lib.raw_stream(idx),
         ),
         what,

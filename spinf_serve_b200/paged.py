@@ -35,6 +35,7 @@ class Step:
     pos: torch.Tensor
     max_q: int
     max_len: int
+    shared: bool = False  # the sequences' tables begin with so many of the same pages that reading them once pays
 
 
 class PagedCache:
@@ -46,6 +47,7 @@ class PagedCache:
             raise RuntimeError(f"pages hold 16, 32, 64, 128 or 256 tokens of 128 or 256 dimensions, got {n_pages} pages of {page} x {head_dim}")
         self.page, self.n_pages, self.device = page, n_pages, torch.device(device)
         self.k, self.v = (torch.empty((layers, n_pages, kv_heads, page, head_dim), dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        self.row_bytes = 4 * kv_heads * head_dim  # a token's K and V in one layer
         self.free = list(range(n_pages - 1, -1, -1))
         self.refs = [0] * n_pages
 
@@ -62,6 +64,15 @@ class PagedCache:
             self.refs[p] -= 1
             if self.refs[p] == 0:
                 self.free.append(p)
+
+    def common_front(self, seqs: list) -> int:
+        """tokens of the pages that all of the sequences begin with"""
+        n = 0
+        for pages in zip(*(s.pages for s in seqs)):
+            if len(set(pages)) > 1:
+                break
+            n += 1
+        return n * self.page
 
     def open(self) -> Sequence:
         return Sequence()
@@ -147,7 +158,7 @@ class PagedReader:
         sliding = kind == "sliding_attention"
         w = None if self._weights is None or sliding else self._weights[i][None]
         return ops.paged_attention(q, c.k[i], c.v[i], st.table, st.lens, st.cu, st.max_q, self.scaling, window=cfg.window if sliding else None,
-                                   weights=w, max_len=st.max_len)
+                                   weights=w, max_len=st.max_len, shared=st.shared)
 
     def __call__(self, i, kind, q, k, v):
         """q, k, v normed and rotated, side by side in one projection's rows: k and v into the pages, then the attention"""
@@ -171,6 +182,7 @@ class PagedReader:
         if not all(len(x) for x in ids) or len(seqs) > 1024:
             raise RuntimeError("every sequence of a forward (at most 1024) needs new tokens")
         st = self.cache.grow(seqs, [len(x) for x in ids])
+        st.shared = self.cache.common_front(seqs) * (len(seqs) - 1) * self.cache.row_bytes >= ops.SHARE_BYTES
         dev = self.cache.device
         if weigh:
             seq, cap = seqs[0], len(seqs[0].pages) * self.cache.page

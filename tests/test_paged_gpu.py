@@ -525,3 +525,134 @@ def test_append_of_rows_that_belong_to_no_sequence(dev):
         for s in range(L - k, L):
             want[int(c.table[b, s // page]), s % page] = True
     assert torch.equal(moved, want)
+
+
+class Fronts(Call):
+    """sequences in groups (common tokens, [(length, new rows) ..]) whose tables begin with the same pages, others between the groups"""
+
+    def __init__(self, dev, H, h, D, page, groups, between=(), seed=0):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        seqs, self.first = [], []
+        for i, (_, members) in enumerate(groups):
+            self.first.append(len(seqs))
+            seqs += members
+            seqs += between[i : i + 1]
+        self.H, self.h, self.D, self.page, self.dev = H, h, D, page, dev
+        self.lens, news = [x for x, _ in seqs], [n for _, n in seqs]
+        pages = [-(-x // page) for x in self.lens]
+        start = torch.tensor([0] + pages).cumsum(0)
+        order = torch.randperm(int(start[-1]) + 2, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        self.table = torch.full((len(seqs), max(pages)), -7, dtype=torch.int32)
+        for b, n in enumerate(pages):
+            self.table[b, :n] = order[int(start[b]) : int(start[b]) + n]
+        for b0, (common, members) in zip(self.first, groups):
+            self.table[b0 : b0 + len(members), : common // page] = self.table[b0, : common // page]
+        used = self.table[self.table >= 0].unique()
+        place = torch.full((len(order),), -7, dtype=torch.int32)
+        place[used.long()] = torch.randperm(len(used), generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        self.table = torch.where(self.table >= 0, place[self.table.clamp_min(0).long()], self.table)
+        self.on = {"k": torch.randn((len(used), h, page, D), generator=g, device=dev).to(torch.bfloat16)}
+        self.on["v"] = torch.randn((len(used), h, page, D), generator=g, device=dev).to(torch.bfloat16)
+        for b, x in enumerate(self.lens):
+            if x % page:
+                for pool in (self.on["k"], self.on["v"]):
+                    pool[int(self.table[b, x // page]), :, x % page :] = math.nan
+        self.cu = torch.tensor([0] + news).cumsum(0).to(torch.int32)
+        self.n, self.max_q = int(self.cu[-1]) + 1, max(news)
+        self.q = torch.randn((self.n, H, D), generator=g, device=dev).to(torch.bfloat16).cpu()
+        self.lens_t = torch.tensor(self.lens, dtype=torch.int32)
+        self.on |= {x: getattr(self, x).to(dev) for x in ("table", "cu", "q", "lens_t")}
+        self.k, self.v = self.on["k"].cpu(), self.on["v"].cpu()
+
+    def rows(self, x, b, k=1):
+        return x[int(self.cu[b]) : int(self.cu[b + k])]
+
+    def check(self, got, seqs):
+        for b in seqs:
+            cu = torch.tensor([0, int(self.cu[b + 1] - self.cu[b])])
+            want, _, mag, big = OP.attention(self.rows(self.q, b), self.k, self.v, self.table[b : b + 1], self.lens[b : b + 1], cu, self.D**-0.5)
+            rel = score_noise(self, big, max(self.lens))[..., None]
+            tol = BF * want.abs() + (BF * (1 + BF) + rel) * mag * (1 + BF) + 1e-30
+            off = ((self.rows(got, b).double().cpu() - want).abs() / tol).max()
+            assert off <= 1.0, f"sequence {b}: {float(off)} of the tolerance"
+
+
+def _worth(seqs, h, D):
+    """the shortest front, in tokens, that a group of so many sequences reads together"""
+    return max(1024, -(-(2**27) // ((seqs - 1) * h * D * 4 * 128)) * 128)
+
+
+@pytest.mark.parametrize("H,h,D,page", [(16, 8, 256, 64), (32, 4, 128, 16), (24, 4, 256, 32), (8, 8, 128, 128), (32, 16, 128, 256)])
+def test_common_fronts_are_read_once(dev, H, h, D, page):
+    few = max(1, 32 // (H // h))  # rows of a sequence that is no chunk
+    fa, fb = _worth(9, h, D), _worth(20, h, D)
+    pad = lambda x: -(-x // page) * page  # noqa: E731
+    a = [(pad(fa) + 1 + few + 37 * i, 1 + (3 * i) % few) for i in range(9)]
+    b = [(pad(fb) + few + 5 * (i % 7), few) for i in range(20)]
+    c = Fronts(dev, H, h, D, page, [(pad(fa), a), (pad(fb), b)], between=[(400, 70), (900, 1)], seed=H + D)
+    a0, b0 = c.first
+    out = torch.full((c.n, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    got, apart = c.attend(shared=True, out=out), c.attend(shared=False)
+    assert (got[-1:] == 7.0).all()
+    c.check(got, [0, 4, 8, 9, b0, b0 + 11, b0 + 19])
+    assert not torch.equal(c.rows(got, a0, 9), c.rows(apart, a0, 9)) and not torch.equal(c.rows(got, b0, 20), c.rows(apart, b0, 20))  # it did look
+    for i in (9, 30):  # the others' bits stay
+        assert torch.equal(c.rows(got, i), c.rows(apart, i))
+    assert torch.equal(c.attend(shared=True)[:-1], got[:-1])
+    # a group's results do not depend on what else is in the call
+    o = c.on
+    alone = ops.paged_attention(c.rows(o["q"], b0, 20).clone(), o["k"], o["v"], o["table"][b0 : b0 + 20], o["lens_t"][b0 : b0 + 20], o["cu"][b0 : b0 + 21] - o["cu"][b0],
+                                few, D**-0.5, shared=True)
+    assert torch.equal(alone, c.rows(got, b0, 20))
+
+
+def test_fronts_that_do_not_make_a_group(dev):
+    """too little in common, a chunk or a sequence without new rows among them, a window, weights: the same bits as without looking"""
+    H, h, D, page = 16, 8, 256, 64
+    f = _worth(9, h, D)
+    one = (f + 20, 2)
+    little = [(f - 128 + 70, 3)] * 9
+    broken = [one] * 4 + [(f + 150, 100)] + [one] * 4 + [(f + 20, 0)] + [one] * 3
+    c = Fronts(dev, H, h, D, page, [(f - 128, little), (f, broken)], seed=2)
+    assert torch.equal(c.attend(shared=True)[:-1], c.attend(shared=False)[:-1])
+    c = Fronts(dev, H, h, D, page, [(f, [one] * 9)], seed=3)
+    assert not torch.equal(c.attend(shared=True)[:-1], c.attend(shared=False)[:-1])
+    assert torch.equal(c.attend(window=300, shared=True)[:-1], c.attend(window=300, shared=False)[:-1])
+    w = torch.zeros((9, h, f + 128), device=dev)
+    assert torch.equal(c.attend(weights=w.clone(), shared=True)[:-1], c.attend(weights=w.clone(), shared=False)[:-1])
+
+
+def test_fronts_within_fronts(dev):
+    """nine sequences with a long common front, then eleven that share only its first part with them; rows right behind the front; a page
+    index that lies outside the pool in the part that is read together"""
+    H, h, D, page = 16, 8, 256, 64
+    f = _worth(9, h, D)
+    c = Fronts(dev, H, h, D, page, [(1088, [(3 * f + 2, 2)] * 9 + [(1088 + 1 + 3 * i, 1) for i in range(11)])], seed=4)
+    c.table[:9, : 3 * f // page] = c.table[0, : 3 * f // page]
+    c.on["table"] = c.table.to(dev)
+    got = c.attend(shared=True)
+    c.check(got, [0, 8, 9, 19])
+    assert not torch.equal(c.rows(got, 0, 9), c.rows(c.attend(shared=False), 0, 9))
+    assert _lib.last_status(raise_on_error=False) == 0
+    c.on["table"][:9, 5] = 10**6
+    c.attend(shared=True)
+    assert _lib.last_status(raise_on_error=False) == 5
+
+
+def test_many_fronts_and_a_graph(dev):
+    """more groups than the workspace has room for (the last ones stay apart); two calls in one graph, each with a workspace of its own"""
+    H, h, D, page = 8, 8, 128, 64
+    f = _worth(9, h, D)
+    c = Fronts(dev, H, h, D, page, [(f, [(f + 9 + i, 2) for i in range(9)]) for _ in range(12)], seed=1)
+    got, apart = c.attend(shared=True), c.attend(shared=False)
+    same = [torch.equal(c.rows(got, b, 9), c.rows(apart, b, 9)) for b in c.first]
+    assert not any(same[:9]) and all(same[-1:])
+    c.check(got, [0, 80, 107])
+    assert torch.equal(c.attend()[:-1], got[:-1])  # (a pool of less than a quarter of these sequences' pages: it looks by itself)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one, two = c.attend(shared=True), c.attend(shared=True)
+    for _ in range(2):
+        one.zero_(), two.zero_()
+        graph.replay()
+        assert torch.equal(one[:-1], got[:-1]) and torch.equal(two[:-1], got[:-1])

@@ -153,16 +153,16 @@ def test_the_c_entry_points_refuse_on_the_host():
     odd = (ctypes.c_int64 * 3)(4096, 2048, 130)
 
     def attn(n=2, H=4, h=2, D=128, page=16, q=p, table=p, width=4, B=1, max_q=2, max_len=64, window=0, scale=1.0, w_in=N, w_out=N, strides=N, decay=1.0, ws=N, ws_bytes=0, k=st):
-        return lib.spinf_paged_attention(q, H * D, n, H, h, D, p, p, 8, page, k, st, table, width, p, p, B, max_q, max_len, window, scale, w_in, w_out, strides, decay, p, H * D, ws, ws_bytes, N)
+        return lib.spinf_paged_attention(q, H * D, n, H, h, D, p, p, 8, page, k, st, table, width, p, p, B, max_q, max_len, window, 0, scale, w_in, w_out, strides, decay, p, H * D, ws, ws_bytes, N)
 
     assert attn(B=0) == 0 and attn(n=0, q=N) == 0  # nothing to do
     for bad in (dict(q=N), dict(table=N), dict(H=3), dict(D=64), dict(page=24), dict(page=8), dict(max_len=65), dict(max_q=-1), dict(window=-1), dict(scale=0.0),
                 dict(w_out=p), dict(w_out=p, strides=(ctypes.c_int64 * 4)(), decay=1.0), dict(width=64, max_len=1024)):  # (the last: splits need a workspace)
         assert attn(**bad) == -1, bad
     assert attn(B=2000) == -4
-    assert lib.spinf_paged_attention_workspace_bytes(4, 2000, 4, 2, 128, 1, 64, 0) == -4
-    assert lib.spinf_paged_attention_workspace_bytes(4, 2, 4, 3, 128, 1, 64, 0) == -1
-    need = [lib.spinf_paged_attention_workspace_bytes(64, 64, 16, 8, 256, 1, n, w) for n, w in ((100, 0), (8192, 0), (8192, 1))]
+    assert lib.spinf_paged_attention_workspace_bytes(4, 2000, 4, 2, 128, 1, 64, 0, 0) == -4
+    assert lib.spinf_paged_attention_workspace_bytes(4, 2, 4, 3, 128, 1, 64, 0, 0) == -1
+    need = [lib.spinf_paged_attention_workspace_bytes(64, 64, 16, 8, 256, 1, n, w, 0) for n, w in ((100, 0), (8192, 0), (8192, 1))]
     assert need[0] == 0 and 0 < need[1] < need[2]
 
     def append(n=2, H=4, h=2, D=128, pitch=1024, page=16, wq=N, wk=N, cos=N, sin=N, rot=0, q=N, width=4, k=st, B=1, qkv=p):
@@ -200,3 +200,23 @@ def test_written_layouts_that_share_places_are_refused():
     with pytest.raises(_lib.SpinfError, match="CUDA"):  # K and V side by side in one tensor, token-major weights' rows apart
         both = torch.zeros((6, 2, 2, 16, 128), dtype=torch.bfloat16)
         _append(k_pages=both[:, 0], v_pages=both[:, 1])
+
+
+def test_the_front_that_sequences_have_in_common():
+    c = _cache(24)
+    a = c.open()
+    c.grow([a], [40])
+    forks = [c.fork(a) for _ in range(3)]
+    assert c.common_front(forks) == 32 and c.common_front([a]) == 48 and c.common_front([a, c.open()]) == 0
+    c.grow(forks, [9, 1, 30])
+    assert c.common_front(forks) == 32
+    b = c.open()
+    c.grow([b], [20])
+    assert c.common_front(forks + [b]) == 0
+
+
+def test_workspace_of_a_call_that_looks_for_fronts():
+    need = lambda B, n, max_q, max_len, w, shared: _lib.lib().spinf_paged_attention_workspace_bytes(n, B, 16, 8, 256, max_q, max_len, w, shared)  # noqa: E731
+    assert need(56, 672, 12, 2048, 0, 1) > need(56, 672, 12, 2048, 0, 0) > 0
+    for args in ((56, 672, 12, 2048, 1), (1, 12, 12, 65536, 0), (2, 24, 12, 2048, 0), (56, 672, 12, 256, 0)):  # weights, one sequence, too little to save
+        assert need(*args, 1) == need(*args, 0)

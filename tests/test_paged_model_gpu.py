@@ -153,3 +153,23 @@ def test_reading_with_weights_evicting_and_going_on(dev):
     assert sorted(reader.cache.free) == list(range(80))
     with pytest.raises(RuntimeError, match="out of pages"):
         reader.read(rng.integers(5, 4096, 3000).tolist())
+
+
+def test_many_questions_on_a_long_content(dev, monkeypatch):
+    """enough branches on enough content that the full-attention layers read it once for all of them: the same answers but for roundings (p
+    to bf16 against another reference, once each way, and the output's: three times half a step of 2^-8 at most, relative)"""
+    _, _, _, stack = _stack(dev, "bf16")
+    rng = np.random.default_rng(8)
+    reader = PagedReader(stack, n_pages=200, page=32)
+    seq = reader.read(rng.integers(5, 4096, 2210).tolist())
+    branches = [rng.integers(5, 4096, int(rng.integers(1, 12))).tolist() for _ in range(70)]
+    seen = []
+    attend = ops.paged_attention
+    monkeypatch.setattr(ops, "paged_attention", lambda *a, **kw: (seen.append(kw["shared"]), attend(*a, **kw))[1])
+    got = reader.ask(seq, branches)
+    assert seen == [True] * 3
+    monkeypatch.setattr(ops, "SHARE_BYTES", 1 << 40)
+    apart = reader.ask(seq, branches)
+    assert seen == [True] * 3 + [False] * 3
+    off = ((got.double() - apart.double()).norm(dim=1) / apart.double().norm(dim=1)).max()
+    assert 0 < off < 3 * 2.0**-8
