@@ -24,7 +24,7 @@ struct PagedSeqs {
   int max_len;  // longest sequence the caller's buffers are sized for
   int max_q;    // most new rows of a sequence they are sized for
   int64_t n;    // rows of q
-  const int32_t* share;  // [2][B], or null: key tiles of each sequence that its group reads together; behind a group's first, at B + b, its end
+  const int32_t* share;  // [2][B] and the number of groups, or null: key tiles of each sequence that its group reads together; behind a group's first, at B + b, its end
 };
 
 struct PagedSeq {

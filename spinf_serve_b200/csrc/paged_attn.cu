@@ -994,7 +994,7 @@ __global__ void __launch_bounds__(1024) paged_share_kernel(const PagedSeqs s, co
   }
   __syncthreads();
   if (tid == 0) {
-    int used = 0;
+    int used = 0, groups = 0;
     for (int b = 0; b + 1 < s.B;) {
       int t = link[b], e = b + 1;
       if (t < SHARE_TILES) {
@@ -1015,11 +1015,13 @@ __global__ void __launch_bounds__(1024) paged_share_kernel(const PagedSeqs s, co
       const int need = chunk_cut(q, a).units;
       if (used + need <= units) {
         used += need;
+        ++groups;
         for (int i = b; i <= e; ++i) out[i] = t;
         out[s.B + b] = e + 1;
       }
       b = e + 1;
     }
+    share[2 * s.B] = groups;
   }
   __syncthreads();
   for (int i = tid; i < 2 * s.B; i += 1024) share[i] = out[i];
@@ -1073,7 +1075,7 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
     // a unit per item of a group, or up to one per CTA (pair) for a group of few items: room for four such groups
     const int64_t items = ((n >> tl) + B / 2) * (H >> hl) + 4 * chunk_units_of(D);
     z.share_units = static_cast<int>(items < 4 * PG_SMS ? items : 4 * PG_SMS);
-    z.share = up256(B * 8);
+    z.share = up256(B * 8 + 4);
     all_units += z.share_units;
   }
   z.max_units = static_cast<int>(all_units);
@@ -1200,6 +1202,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.chunk_rows = z.chunk_rows;
   a.only = B == 1 && mq > 0 ? class_of(mq * a.group, z.chunk_rows) : 0;
   a.max_units = z.max_units;
+  a.fronts_only = z.share_units > 0 && mq * a.group <= z.chunk_rows;
   auto take = [&](int64_t bytes) {
     uint8_t* p = ws;
     ws += bytes;

@@ -31,6 +31,7 @@ struct PagedAttnArgs {
   float* scores;  // [B][tok_cap][H][score_pitch] log2 units, or null: kept for the weights
   int64_t score_pitch;
   int tok_cap;
+  int fronts_only;  // no sequence of the call can be a chunk: the chunk kernels have the groups' fronts only
 };
 
 struct PagedWeightArgs {
@@ -156,6 +157,13 @@ static constexpr int SHARE_ROWS = 4;   // a group's sequences have up to so many
 // 45 / 44; 8 / 8 heads of 128: 8 over 4 096 (117 MB) 31 / 32, 16 over 4 096 (252 MB) 51 / 42. Further up: 56 of 40 new tokens over 4 096
 // 796 / 285, 56 of one over 16 384 681 / 118.
 __host__ __device__ inline bool share_pays(int64_t seqs, int64_t tokens, int h, int D) { return (seqs - 1) * tokens * h * D * 4 >= 1 << 27; }
+// nothing for the chunk kernels: no chunk, and no group found. Their CTAs leave before they set anything up
+__device__ __forceinline__ bool chunk_idle(const PagedSeqs& s, const PagedAttnArgs& a) {
+  if (!a.fronts_only || s.share[2 * s.B] != 0) return false;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_units = 0;
+  if (threadIdx.x == 0) pdl_wait();  // (the kernels behind this one need what the kernels ahead of it wrote)
+  return true;
+}
 // what the chunk kernels make of index b: a chunk's sequence, a group's front (at its first sequence), or nothing
 __device__ __forceinline__ bool chunk_seq(const PagedSeqs& s, const PagedAttnArgs& a, int b, PagedSeq& q, int* status) {
   q = paged_seq(s, b, status);

@@ -480,6 +480,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t rank = cluster_ctarank();
   const int n_pairs = static_cast<int>(gridDim.x) >> 1, pair = static_cast<int>(blockIdx.x) >> 1;
   pdl_trigger();
+  if (chunk_idle(s, a)) return;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -806,6 +807,7 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WaitCtx wc{abort_flag, status};
   pdl_trigger();
+  if (chunk_idle(s, a)) return;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);

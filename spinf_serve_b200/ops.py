@@ -770,7 +770,7 @@ def _attention_layout(q, k, v, table, lens, cu, max_q, window, w_in, w_out, max_
         strides = (ctypes.c_int64 * 4)(*w_in[2][:2], *w_out[2][:2])
     win = window if window is not None and window < max_len else 0  # (a window that holds everything is none)
     if shared is None:
-        shared = B * max_len > 4 * n_pages * page
+        shared = B * max_len > 8 * n_pages * page
     shared = bool(shared) and win == 0 and w_in is None
     need = int(_lib.lib().spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, w_in is not None, shared))
     check(need, what)
@@ -786,7 +786,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     weights (fp32 [B, Hkv, cap], cap >= max_len): each slot's accumulated attention weight, weights_out = decay * weights + this
     call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
     tensor reused between calls on one stream; out must not overlap q. shared: look for neighbouring sequences whose tables begin with
-    the same pages (branches of one content) and read those once for all of them (None: where the pool has less than a quarter of the
+    the same pages (branches of one content) and read those once for all of them (None: where the pool has less than an eighth of the
     pages that this many sequences of max_len tokens would need; looking in vain costs up to 20 us)."""
     what = "paged_attention"
     if weights is not None and weights_out is None:
@@ -813,7 +813,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
         ),
         what,
     )
-    COUNTS["launches"] += 2 if weights is None else 3
+    COUNTS["launches"] += 6 if shared else 2 if weights is None else 3
     return out
 
 

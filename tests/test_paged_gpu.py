@@ -648,7 +648,7 @@ def test_many_fronts_and_a_graph(dev):
     same = [torch.equal(c.rows(got, b, 9), c.rows(apart, b, 9)) for b in c.first]
     assert not any(same[:9]) and all(same[-1:])
     c.check(got, [0, 80, 107])
-    assert torch.equal(c.attend()[:-1], got[:-1])  # (a pool of less than a quarter of these sequences' pages: it looks by itself)
+    assert torch.equal(c.attend()[:-1], got[:-1])  # (a pool of less than an eighth of these sequences' pages: it looks by itself)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         one, two = c.attend(shared=True), c.attend(shared=True)
