@@ -694,8 +694,7 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint8_t* stage = smem + L::OUT_OFF + (warp - 4) * 2048;
     const uint32_t p_bar = map_to_cta(p_ready, 0), free_bar = map_to_cta(o_free, 0);
     uint32_t gt = 0;
-    while (__all_sync(0xffffffffu, ring.next(wc, g))) {
-      __syncwarp();
+    while (bar_red_and(1 + qd, 64, ring.next(wc, g))) {  // (two warps share these rows and their barrier: they leave together)
       if (lane == 0) ring.done(); else ++ring.n;
       const int n_tiles = g.tb - g.ta, qrows = 128 >> a.hp_log2;
       const int head = g.h0 + (row >> (7 - a.hp_log2));
