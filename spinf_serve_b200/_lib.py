@@ -10,6 +10,7 @@ import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "csrc", "libspinf_b200.so")
+BIND_PATH = os.path.join(os.path.dirname(LIB_PATH), "paged_bind.so")
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -114,6 +115,7 @@ STATUS = {
 
 _lock = threading.Lock()
 _lib = None
+_bind = None
 _inited = set()
 
 
@@ -136,6 +138,26 @@ def lib():
                     fn.argtypes = args
                 _lib = handle
     return _lib
+
+
+def paged_bind():
+    """the paged operators' short way into the library (csrc/paged_bind.cpp)"""
+    global _bind
+    if _bind is None:
+        import importlib.util
+
+        import torch  # noqa: F401 (the module links to it)
+
+        lib()
+        with _lock:
+            if _bind is None:
+                if not os.path.exists(BIND_PATH):
+                    raise SpinfError(f"{BIND_PATH} is missing: build it with `python -m spinf_serve_b200.csrc.build`")
+                spec = importlib.util.spec_from_file_location("paged_bind", BIND_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _bind = module
+    return _bind
 
 
 def check(code: int, what: str) -> None:

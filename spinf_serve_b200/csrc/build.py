@@ -1,4 +1,5 @@
-"""Builds libspinf_b200.so (the C-ABI library of sm_100a kernels) in place with nvcc.
+"""Builds libspinf_b200.so (the C-ABI library of sm_100a kernels) in place with nvcc, and paged_bind.so (the paged operators' short way
+from Python into it, against torch's C++ headers) with g++.
 
     python -m spinf_serve_b200.csrc.build [--force] [--verbose]
 
@@ -12,6 +13,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libspinf_b200.so")
+BIND = os.path.join(HERE, "paged_bind.so")
+CXX = os.environ.get("CXX", "g++")
 SOURCES = ["host_util.cpp", "abi.cpp", "tile_desc.cpp", "gemm.cu", "glue.cu", "attn_tree.cu", "w4_gemm.cu", "gdn.cu", "gdn_chunk.cu", "gdn_tree.cu", "gdn_tree_tc.cu", "x_attn.cu", "w4_small.cu",
            "paged_append.cu", "paged_attn.cu", "paged_chunk.cu", "paged_evict.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -70,7 +73,27 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_bind(force)
     return LIB
+
+
+def _build_bind(force):
+    src = os.path.join(HERE, "paged_bind.cpp")
+    if not (force or _stale(BIND, [src, __file__, _headers()[-1]])):
+        return
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(NVCC), "..", "include")
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += ["-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    cmd += ["-isystem", sysconfig.get_paths()["include"], "-isystem", cuda, src, "-o", BIND, "-L" + HERE, "-lspinf_b200", "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for paged_bind.cpp:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

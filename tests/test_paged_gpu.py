@@ -656,3 +656,51 @@ def test_many_fronts_and_a_graph(dev):
         one.zero_(), two.zero_()
         graph.replay()
         assert torch.equal(one[:-1], got[:-1]) and torch.equal(two[:-1], got[:-1])
+
+
+def test_known_layouts(dev):
+    """calls whose layout has been seen are made without the checks' way round: other layouts in between, addresses that do not fit, a
+    workspace that is too small, and out = q are noticed all the same"""
+    H, h, D, page = 4, 2, 128, 16
+    c = Call(dev, H, h, D, page, [(300, 2), (40, 1)], seed=6)
+    o = c.on
+    want = c.attend()
+    wide = torch.zeros((c.n, H * D + 64), dtype=torch.bfloat16, device=dev)
+    wide[:, : H * D] = o["q"].view(c.n, -1)
+    views = [o["q"], wide[:, : H * D].view(c.n, H, D), o["q"].clone()]
+    kept = [o["k"], o["k"].transpose(1, 2).contiguous().transpose(1, 2)]
+    for _ in range(3):
+        for q in views:
+            for k in kept:
+                for ws in (None, torch.empty(16, dtype=torch.uint8, device=dev), torch.empty(1 << 22, dtype=torch.uint8, device=dev)):
+                    got = ops.paged_attention(q, k, o["v"], o["table"], o["lens_t"], o["cu"], 2, D**-0.5, workspace=ws)
+                    assert torch.equal(got, want)
+    out = torch.empty_like(want)
+    assert ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 2, D**-0.5, out=out) is not None and torch.equal(out, want)
+    with pytest.raises(_lib.SpinfError, match="must not be q"):
+        ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 2, D**-0.5, out=o["q"])
+    odd = torch.zeros(c.n * H * D + 8, dtype=torch.bfloat16, device=dev)[1 : 1 + c.n * H * D].view(c.n, H, D)  # the layout of q at an address that does not fit
+    with pytest.raises(_lib.SpinfError, match="bad argument"):
+        ops.paged_attention(odd, o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 2, D**-0.5)
+    with pytest.raises(_lib.SpinfError, match="bad argument"):
+        ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 2, -1.0)
+    with pytest.raises(_lib.SpinfError, match="different devices|CUDA"):
+        ops.paged_attention(o["q"], o["k"], o["v"], c.table, o["lens_t"], o["cu"], 2, D**-0.5)
+    qkv = torch.randn((c.n, 8 * D), device=dev).to(torch.bfloat16)
+    for _ in range(2):
+        q = ops.paged_append(qkv, H, h, D, o["k"], o["v"], o["table"], o["lens_t"], o["cu"])
+        assert q.data_ptr() == qkv.data_ptr() and torch.equal(q, qkv[:, : H * D].view(c.n, H, D))
+    with pytest.raises(_lib.SpinfError, match="same memory"):
+        ops.paged_append(qkv, H, h, D, o["k"], o["k"], o["table"], o["lens_t"], o["cu"])
+    new_table = c.free[:2].view(2, 1).to(dev)
+    first = ops.paged_evict(o["k"], o["v"], o["table"], o["lens_t"], None, 16, 16, new_table)
+    again = ops.paged_evict(o["k"], o["v"], o["table"], o["lens_t"], None, 16, 16, new_table)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1]) and first[2] is again[2] is None
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)
+        fresh = o["q"] * 1.0
+        got = ops.paged_attention(fresh, o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 2, D**-0.5)
+    side.synchronize()
+    assert torch.equal(got, c.attend())
