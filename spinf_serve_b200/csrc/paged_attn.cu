@@ -1030,7 +1030,10 @@ __global__ void __launch_bounds__(1024) paged_share_kernel(const PagedSeqs s, co
 // A sequence with more rows per kv head than this is the chunk kernels', where a head set of it fills 256-row items: measured on 32
 // sequences of 2 000 tokens (16 / 8 heads of 256) 32 rows took 138 us in the few-row kernel and 168 there, 64 rows 253 and 172; with
 // three head sets per kv head (24 / 4 heads) 48 rows 106 and 237, 96 rows 250 and 240.
-__host__ __device__ constexpr int chunk_rows_of(int group) { return 32 * (group >> chunk_heads_log2(group)); }
+// Where the slots' weights are kept the border is 32 rows for any number of head sets: the few-row kernel's scores go out to memory and back,
+// the chunk kernels' second product costs less (24 / 4 heads of 256: three sequences of 14 tokens over 275 67 us there, 38 here; five of up to
+// 23 over up to 3 656, window 1 024, 132 and 85).
+__host__ __device__ constexpr int chunk_rows_of(int group, bool weights) { return weights ? 32 : 32 * (group >> chunk_heads_log2(group)); }
 
 // what a call needs: sizes of the workspace's parts in bytes (256-byte multiples)
 struct PagedSizes {
@@ -1045,7 +1048,7 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
   const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
   const int64_t group = H / h;
-  z.chunk_rows = chunk_rows_of(static_cast<int>(group));
+  z.chunk_rows = chunk_rows_of(static_cast<int>(group), weights);
   const int64_t most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
   if (slots > 1) {
     const int64_t by_rows = (max_q < most ? max_q : most) * H * slots;  // every row in every split

@@ -54,9 +54,12 @@ __device__ __forceinline__ bool step_class(const PagedSeq& q, const PagedAttnArg
 __device__ __forceinline__ bool rows_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 2; }
 __device__ __forceinline__ bool chunk_class(const PagedSeq& q, const PagedAttnArgs& a) { return seq_class(q, a) == 3; }
 __device__ __forceinline__ PagedCut step_cut(const PagedSeq& q, const PagedAttnArgs& a) { return paged_cut(q, a.window, 1, a.h, PG_SMS, 1); }
+// Splits of at least two tiles: shorter ones answer few sequences sooner and cost many more, since every split leaves up to 64 rows of
+// partial results (12 new tokens, 24 / 4 heads of 256, splits of at least 4 / 2 / 1 tiles: one sequence of 2 048 38 / 27 / 21 us, 16 of them
+// 148 / 168 / 195, 56 of them 441 / 537 / 628).
 __device__ __forceinline__ PagedCut rows_cut(const PagedSeq& q, const PagedAttnArgs& a) {
   const int rt = (q.nq * a.group + RT - 1) / RT;
-  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 4);  // splits of at least 4 tiles: up to 64 rows of partial results each
+  return paged_cut(q, a.window, rt, a.h * rt, PG_SMS, 2);
 }
 __device__ __forceinline__ PagedCut attn_cut(const PagedSeq& q, const PagedAttnArgs& a) { return step_class(q, a) ? step_cut(q, a) : rows_cut(q, a); }
 

@@ -1257,8 +1257,9 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     if (lane == 0) {
       const int rows = s.page_log2 < 7 ? 1 << s.page_log2 : PG_TILE;
       uint32_t n = 0;
-      for (int it = blockIdx.x; it < total; it += gridDim.x, ++n) {
+      for (int it = blockIdx.x; it < total; it += gridDim.x) {
         const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+        if (w.tt0 >= w.tt1) continue;  // keys that no row sees: only the decay is left
         const int32_t* pages = s.table + w.b * s.table_pitch;
         const uint32_t st = n % NK;
         if (!mbar_wait(wc, &k_empty[st], ((n / NK) & 1u) ^ 1u, ST_TIMEOUT_EMPTY)) break;
@@ -1270,6 +1271,7 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
             uint8_t* dst = smem + (st * 2 + t) * L::K_TILE + x * rows * 128;
             for (int y = 0; y < (rows == PG_TILE ? 1 : SLABS); ++y) tma_load_5d(dst + y * PG_TILE * 128, &tmK, 0, j & in_page, y, w.g, pg, &k_full[st]);
           }
+        ++n;
       }
       if (*abort_flag)  // bounded wait for copies that may still be in flight
         for (uint32_t c = n > static_cast<uint32_t>(NK) ? n - NK : 0; c < n; ++c)
@@ -1321,8 +1323,9 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     if (lane == 0) {
       uint32_t n = 0, k = 0;
       bool ok = true;
-      for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+      for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
         const ChunkWeightItem w = chunk_weight_item(s, a, pre, it, status);
+        if (w.tt0 >= w.tt1) continue;
         if (!mbar_wait(wc, &k_full[k % NK], (k / NK) & 1u, ST_TIMEOUT_FULL)) break;
         const uint32_t k_addr = smem_u32(smem) + (k % NK) * 2 * L::K_TILE;
         const int stages = w.sets * (w.tt1 - w.tt0);
@@ -1344,6 +1347,7 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
           umma_commit(&s_full[n % NS]);
         }
         if (ok) umma_commit(&k_empty[k % NK]);
+        ++k;
       }
     }
   } else {
