@@ -55,7 +55,7 @@ void* data(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 enum { APPEND, ATTENTION, EVICT };
 struct Call {
   Key key;
-  const std::vector<int64_t>* layout = nullptr;
+  std::vector<int64_t> layout;  // (a copy: what the call allocates may run other code that learns)
   bool plain = true;  // the arguments are ones that a key can be made of
   void find() {
     if (!plain || PyErr_Occurred()) {
@@ -64,7 +64,7 @@ struct Call {
       return;
     }
     const auto it = g_layouts.find(key.bytes);
-    if (it != g_layouts.end() && key.device == c10::cuda::current_device()) layout = &it->second;
+    if (it != g_layouts.end() && key.device == c10::cuda::current_device()) layout = it->second;
   }
 };
 constexpr int TENSORS = 10;
@@ -95,8 +95,8 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (wrong_count(n_args, 16)) return nullptr;
   const at::Tensor* t[TENSORS];
   const Call c = make_call(APPEND, args, 10, 3, t);
-  if (!c.layout || data(t[1]) == data(t[2])) Py_RETURN_NONE;
-  const int64_t* x = c.layout->data();  // n, pitch, rot, pages, page, k strides, v strides, table pitch, width, B
+  if (c.layout.empty() || data(t[1]) == data(t[2])) Py_RETURN_NONE;
+  const int64_t* x = c.layout.data();  // n, pitch, rot, pages, page, k strides, v strides, table pitch, width, B
   const int64_t H = PyLong_AsLongLong(args[10]), h = PyLong_AsLongLong(args[11]), D = PyLong_AsLongLong(args[12]);
   const double eps = PyFloat_AsDouble(args[13]);
   const int plus1 = PyObject_IsTrue(args[14]), norm_v = PyObject_IsTrue(args[15]);
@@ -121,14 +121,14 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   std::memcpy(in, args, 9 * sizeof(PyObject*));
   std::memcpy(in + 9, args + 10, 4 * sizeof(PyObject*));
   const Call c = make_call(ATTENTION, in, 9, 4, t);
-  if (!c.layout) Py_RETURN_NONE;
+  if (c.layout.empty()) Py_RETURN_NONE;
   if (args[9] != Py_None) {
     if (!THPVariable_Check(args[9])) Py_RETURN_NONE;
     t[9] = &THPVariable_Unpack(args[9]);
     if (!t[9]->is_cuda() || t[9]->get_device() != c.key.device) Py_RETURN_NONE;
   }
   // n, H, h, D, q pitch, out pitch, pages, page, k strides, v strides, table pitch, B, max_len, window, workspace, shared, weight strides
-  const int64_t* x = c.layout->data();
+  const int64_t* x = c.layout.data();
   if (t[8] && x[0] && data(t[8]) == data(t[0])) Py_RETURN_NONE;
   const double scale = PyFloat_AsDouble(args[14]), decay = PyFloat_AsDouble(args[15]);
   const int64_t max_q = PyLong_AsLongLong(args[10]);
@@ -153,8 +153,8 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (wrong_count(n_args, 9)) return nullptr;
   const at::Tensor* t[TENSORS];
   const Call c = make_call(EVICT, args, 6, 3, t);
-  if (!c.layout) Py_RETURN_NONE;
-  const int64_t* x = c.layout->data();  // pages, h, page, D, k strides, v strides, B, table pitch, new pitch, max_len, weight strides, recent
+  if (c.layout.empty()) Py_RETURN_NONE;
+  const int64_t* x = c.layout.data();  // pages, h, page, D, k strides, v strides, B, table pitch, new pitch, max_len, weight strides, recent
   const int64_t keep = PyLong_AsLongLong(args[6]);
   at::Tensor lens = make({x[10]}, at::kInt, *t[0]), kept = make({x[10], x[1], keep}, at::kInt, *t[0]), w;
   if (t[4]) w = make({x[10], x[1], keep}, at::kFloat, *t[0]);

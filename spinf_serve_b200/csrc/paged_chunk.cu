@@ -1158,7 +1158,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s
 // Item = 256 keys of a (sequence, kv head), both tiles of K resident in shared memory while the rows that see any of them stream by.
 // Bound by the exponentials and what surrounds them (256 x 64 a stage at 16 per cycle and SM: 1 024 cycles, the products 512 at D 128
 // and 1 024 at D 256; measured 2 050 a stage: reading S out of tensor memory and the instructions around each exponential share the
-// issue slots). 1 024 tokens over 8 192 (32 / 16 heads of 128): 285 us with the attention, about 130 of them here; scores kept in memory
+// issue slots). 1 024 tokens over 8 192 (32 / 16 heads of 128): 290 us with the attention, about 135 of them here; scores kept in memory
 // and read back took 2 500 for the same.
 template <int D>
 struct ChunkWeightSmem {

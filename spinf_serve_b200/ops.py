@@ -610,7 +610,8 @@ def embed_scale(ids, emb, scale):
 # by a first call (*_first) that goes through ctypes; _lib.paged_bind() remembers the layout by exactly those and makes the further
 # calls (host time of an append 15 -> 6 us, of an eviction 19 -> 10).
 _I32, _BF16, _F32, _U8 = torch.int32, torch.bfloat16, torch.float32, torch.uint8
-SHARE_BYTES = 1 << 27  # reading saved from which paged_attention reads a common front once (share_pays in csrc/paged_attn.cuh)
+# reading saved, and tokens, from which paged_attention reads a common front once (share_pays, SHARE_TILES in csrc/paged_attn.cuh)
+SHARE_BYTES, SHARE_TOKENS = 1 << 27, 1024
 
 
 def _layout(t):

@@ -65,10 +65,10 @@ class PagedCache:
             if self.refs[p] == 0:
                 self.free.append(p)
 
-    def common_front(self, seqs: list) -> int:
-        """tokens of the pages that all of the sequences begin with"""
+    def common_front(self, seqs: list, most: int | None = None) -> int:
+        """tokens of the pages that all of the sequences begin with (of their first `most` pages)"""
         n = 0
-        for pages in zip(*(s.pages for s in seqs)):
+        for pages in zip(*(s.pages[:most] for s in seqs)):
             if len(set(pages)) > 1:
                 break
             n += 1
@@ -182,7 +182,9 @@ class PagedReader:
         if not all(len(x) for x in ids) or len(seqs) > 1024:
             raise RuntimeError("every sequence of a forward (at most 1024) needs new tokens")
         st = self.cache.grow(seqs, [len(x) for x in ids])
-        st.shared = self.cache.common_front(seqs) * (len(seqs) - 1) * self.cache.row_bytes >= ops.SHARE_BYTES
+        if len(seqs) > 1:
+            front = max(ops.SHARE_TOKENS, -(-ops.SHARE_BYTES // ((len(seqs) - 1) * self.cache.row_bytes)))
+            st.shared = self.cache.common_front(seqs, -(-front // self.cache.page)) >= front
         dev = self.cache.device
         if weigh:
             seq, cap = seqs[0], len(seqs[0].pages) * self.cache.page

@@ -220,3 +220,23 @@ def test_workspace_of_a_call_that_looks_for_fronts():
     assert need(56, 672, 12, 2048, 0, 1) > need(56, 672, 12, 2048, 0, 0) > 0
     for args in ((56, 672, 12, 2048, 1), (1, 12, 12, 65536, 0), (2, 24, 12, 2048, 0), (56, 672, 12, 256, 0)):  # weights, one sequence, too little to save
         assert need(*args, 1) == need(*args, 0)
+
+
+def test_the_common_front_of_the_first_pages():
+    c = _cache(24)
+    a = c.open()
+    c.grow([a], [80])
+    forks = [c.fork(a) for _ in range(3)]
+    assert [c.common_front(forks, n) for n in (None, 0, 2, 9)] == [80, 0, 32, 80]
+
+
+def test_the_short_way_wants_the_right_arguments():
+    bind = _lib.paged_bind()
+    x = torch.zeros((5, 8 * 128), dtype=torch.bfloat16)
+    for f in (bind.append, bind.attention, bind.evict, bind.learn):
+        with pytest.raises(TypeError):
+            f(x)
+    with pytest.raises(TypeError):
+        bind.learn(0, (x,), (1,))
+    assert bind.append(*[x] * 10, 4, 2, 128, 1e-6, False, False) is None  # not on a CUDA device: left to the checks
+    assert bind.evict(*[None] * 6, 16, 16, None) is None and bind.evict(*["x"] * 6, 16, 16, None) is None
