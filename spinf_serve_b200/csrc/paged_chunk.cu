@@ -1205,6 +1205,13 @@ __device__ __forceinline__ ChunkWeightItem chunk_weight_item(const PagedSeqs& s,
   return w;
 }
 
+// A row's lse as it is subtracted from its scores, hidden ones of which are -inf: their p has to come out as 0 whatever the lse is. A row
+// whose scores are all -inf weighs nothing (exp2(-inf - inf) = 0). One whose sum is NaN gets the lowest number instead: the slots it sees become
+// infinite, which no sum of p is (weight_sum makes it NaN again), and a hidden score of -inf stays -inf.
+static constexpr float NAN_LSE = -3.402823466e38f;
+__device__ __forceinline__ float weight_lse(float x) { return x != x ? NAN_LSE : x == -INFINITY ? INFINITY : x; }
+__device__ __forceinline__ float weight_sum(float x) { return x == INFINITY ? NAN : x; }
+
 template <int D>
 __global__ void __launch_bounds__(CHUNK_WEIGHT_THREADS, 1)
 paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const PagedSeqs s, const PagedAttnArgs a,
@@ -1310,8 +1317,8 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
           else if (set + 1 < w.sets) fetch(set + 1, w.tt0);
           ok = __all_sync(0xffffffffu, mbar_wait(wc, &s_empty[sl], ((n / NS) & 1u) ^ 1u, ST_TIMEOUT_EMPTY));
           if (!ok) break;
-          lse_ring[sl * 64 + lane] = v0 == -INFINITY ? INFINITY : v0;  // rows that are none, or see nothing, weigh nothing: exp2(s - inf) = 0
-          lse_ring[sl * 64 + lane + 32] = v1 == -INFINITY ? INFINITY : v1;
+          lse_ring[sl * 64 + lane] = weight_lse(v0);
+          lse_ring[sl * 64 + lane + 32] = weight_lse(v1);
           __syncwarp();
           if (lane == 0) mbar_arrive(&lse_full[sl]);
         }
@@ -1374,9 +1381,11 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
           tmem_wait_ld();
           const float4* lse = reinterpret_cast<const float4*>(lse_ring + sl * 64);
           const int slot0 = base + tt * w.tok;  // of the stage's first token
-          const bool masked = slot0 < tile_lo + PG_TILE - 1 || (a.window > 0 && slot0 + w.tok - 1 >= tile_lo + a.window);
+          const int left = w.q.nq - tt * w.tok;  // tokens of the stage that are the sequence's: the rows behind them are a neighbour's or none's
+          const bool masked = left < w.tok || slot0 < tile_lo + PG_TILE - 1 || (a.window > 0 && slot0 + w.tok - 1 >= tile_lo + a.window);
           if (masked) {  // hidden scores to -inf ahead of the exponentials: no branch inside the unrolled loop
-            const int lo = j - slot0, hi = a.window > 0 ? lo + a.window : w.tok, tm = w.tok - 1;  // tokens [lo, hi) of the stage see the key; w.tok is a power of two
+            const int lo = j - slot0, tm = w.tok - 1;  // tokens [lo, hi) of the stage see the key; w.tok is a power of two
+            const int end = a.window > 0 ? lo + a.window : w.tok, hi = end < left ? end : left;
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
               const int t0 = c & tm, t1 = (c + 32) & tm;
@@ -1399,7 +1408,7 @@ paged_chunk_weight_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         }
       if (ok && j < w.q.len) {
         const float old = wa.decay != 0.f ? wa.in[w.b * wa.in_seq + w.g * wa.in_head + j] * wa.decay : 0.f;
-        wa.out[w.b * wa.out_seq + w.g * wa.out_head + j] = old + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        wa.out[w.b * wa.out_seq + w.g * wa.out_head + j] = old + weight_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
       }
     }
   }

@@ -704,3 +704,36 @@ def test_known_layouts(dev):
         got = ops.paged_attention(fresh, o["k"], o["v"], o["table"], o["lens_t"], o["cu"], 2, D**-0.5)
     side.synchronize()
     assert torch.equal(got, c.attend())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("window", [None, 150])
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (8, 4, 128), (6, 1, 256), (8, 1, 128)])
+def test_weights_of_a_chunk_beside_rows_that_are_not_finite(dev, H, h, D, window, bad):
+    """rows of q that belong to no sequence, or to a neighbour, take no part in a chunk's weights, whatever they hold; a row of the chunk
+    itself reaches the slots that it sees and no others"""
+    seqs = [(700, 161), (300, 75), (520, 141), (9, 2), (333, 70)]
+    c = Call(dev, H, h, D, 64, seqs, seed=H + D, spare=0, extra_rows=70)
+    cap = 704
+    old, w = torch.rand((len(seqs), h, cap), generator=c.gen).to(dev), torch.empty((len(seqs), h, cap), device=dev)
+    run = lambda: c.attend(window, weights=old, weights_out=w.zero_())  # noqa: E731
+    out = run()
+    clean = w.clone()
+    q, cu = c.on["q"], c.cu.tolist()
+    q[cu[-1] :] = bad
+    q[cu[1] : cu[2]] = bad  # all of the second sequence
+    got = run()
+    for b in (0, 2, 3, 4):
+        assert torch.equal(w[b], clean[b]), f"sequence {b}"
+        assert torch.equal(got[cu[b] : cu[b + 1]], out[cu[b] : cu[b + 1]])
+    # one row in the middle of the third: what it sees, and nothing else
+    at = 97
+    slot = 520 - 141 + at
+    q[cu[2] + at] = bad
+    got = run()
+    lo = max(0, slot - window + 1) if window else 0
+    assert torch.isnan(w[2, :, lo : slot + 1]).all()
+    assert torch.equal(w[2, :, :lo], clean[2, :, :lo]) and torch.equal(w[2, :, slot + 1 :], clean[2, :, slot + 1 :])
+    keep = [i for i in range(cu[2], cu[3]) if i != cu[2] + at]
+    assert torch.equal(got[keep], out[keep])
+    assert torch.equal(w[0], clean[0]) and torch.equal(w[4], clean[4])
