@@ -100,19 +100,27 @@ class PagedCache:
             raise RuntimeError("one count of new tokens per sequence, none negative")
         if len({id(s) for s in seqs}) != len(seqs):
             raise RuntimeError("a sequence can be extended once per forward")
-        need = [-(-(s.length + c) // self.page) - len(s.pages) for s, c in zip(seqs, counts)]
+        need = [max(0, -(-(s.length + c) // self.page) - len(s.pages)) for s, c in zip(seqs, counts)]  # (pages of a failed forward may be left)
         pages = self._take(sum(need))  # all or none
-        cu, pos = [0], []
-        for s, c, n in zip(seqs, counts, need):
-            s.pages += [pages.pop() for _ in range(n)]
-            pos += range(s.position, s.position + c)
+        try:
+            tables, cu, pos, at = [], [0], [], 0
+            for s, c, n in zip(seqs, counts, need):
+                tables.append(s.pages + pages[at : at + n])
+                pos += range(s.position, s.position + c)
+                cu.append(cu[-1] + c)
+                at += n
+            width = max(1, max(len(t) for t in tables))
+            lens = [s.length + c for s, c in zip(seqs, counts)]
+            i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
+            step = Step(i32([t + [0] * (width - len(t)) for t in tables]), i32(lens), i32(cu), i32(pos), max(counts), max(lens))
+        except BaseException:
+            self._release(pages)
+            raise
+        for s, c, t in zip(seqs, counts, tables):  # nothing has changed up to here
+            s.pages = t
             s.length += c
             s.position += c
-            cu.append(cu[-1] + c)
-        width = max(1, max(len(s.pages) for s in seqs))
-        table = torch.tensor([s.pages + [0] * (width - len(s.pages)) for s in seqs], dtype=torch.int32)
-        i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
-        return Step(table.to(self.device), i32([s.length for s in seqs]), i32(cu), i32(pos), max(counts), max(s.length for s in seqs))
+        return step
 
     def evict(self, seq: Sequence, keep: int, recent: int, by_weight: list) -> list | None:
         """cuts the sequence back to `keep` slots in every layer: by accumulated weight where by_weight[layer], else the last `keep`.

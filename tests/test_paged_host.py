@@ -240,3 +240,32 @@ def test_the_short_way_wants_the_right_arguments():
         bind.learn(0, (x,), (1,))
     assert bind.append(*[x] * 10, 4, 2, 128, 1e-6, False, False) is None  # not on a CUDA device: left to the checks
     assert bind.evict(*[None] * 6, 16, 16, None) is None and bind.evict(*["x"] * 6, 16, 16, None) is None
+
+
+def _back(seq, n):
+    """what a failed forward does: the sequence stays where it was, the pages that grow gave it are kept"""
+    seq.length -= n
+    seq.position -= n
+
+
+def test_pages_kept_from_a_failed_forward_serve_their_own_sequence_only():
+    c = _cache(8)
+    a, b = c.open(), c.open()
+    c.grow([a], [64])
+    _back(a, 64)
+    st = c.grow([a, b], [1, 40])
+    assert a.length == 1 and b.length == 40 and len(a.pages) == 4 and len(b.pages) == 3 and len(c.free) == 1
+    assert st.table[1, :3].tolist() == b.pages and not set(a.pages) & set(b.pages)
+    c.close(a)
+    c.close(b)
+    assert sorted(c.free) == list(range(8))
+
+
+def test_a_step_that_cannot_be_built_changes_nothing():
+    c = _cache(8)
+    a, b = c.open(), c.open()
+    c.grow([a], [20])
+    c.device = "no such device"  # the tables cannot be made there
+    with pytest.raises(RuntimeError):
+        c.grow([a, b], [30, 17])
+    assert (a.length, a.position, len(a.pages), b.length, b.pages, len(c.free)) == (20, 20, 2, 0, [], 6)
