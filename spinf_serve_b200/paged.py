@@ -221,8 +221,12 @@ class PagedReader:
     def read(self, ids, weigh: bool = False) -> Sequence:
         """a content's tokens into a new sequence, `chunk` at a time"""
         seq = self.cache.open()
-        for at in range(0, len(ids), self.chunk):
-            self.forward([seq], [ids[at : at + self.chunk]], weigh=weigh)
+        try:
+            for at in range(0, len(ids), self.chunk):
+                self.forward([seq], [ids[at : at + self.chunk]], weigh=weigh)
+        except BaseException:
+            self.cache.close(seq)
+            raise
         return seq
 
     def ask(self, seq: Sequence, branches: list):

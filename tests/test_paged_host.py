@@ -269,3 +269,70 @@ def test_a_step_that_cannot_be_built_changes_nothing():
     with pytest.raises(RuntimeError):
         c.grow([a, b], [30, 17])
     assert (a.length, a.position, len(a.pages), b.length, b.pages, len(c.free)) == (20, 20, 2, 0, [], 6)
+
+
+class _Stack:
+    """a stack that calls the reader's attention for every layer but computes nothing: `fail` raises in the layer of that number"""
+
+    hybrid, n_layers = False, 2
+    fail = None
+
+    def __init__(self):
+        from types import SimpleNamespace
+
+        self.cfg = SimpleNamespace(kv_heads=3, head_dim=128, heads=3, window=4, layer_types=["sliding_attention", "full_attention"])
+        self.w = SimpleNamespace(embed=torch.zeros(1))
+
+    def forward(self, sc, b, inputs, masks, rows=None, attend=None):
+        n = inputs["ids"].numel()
+        for i, kind in enumerate(self.cfg.layer_types):
+            if i == self.fail:
+                raise ValueError("out of memory")
+            attend.project(i, kind, torch.zeros((n, 9 * 128), dtype=torch.bfloat16), None, None, None, None, 1e-6)
+        out = torch.zeros((1, n, 4))
+        return out if rows is None else out[0][rows]
+
+
+@pytest.fixture
+def reader(monkeypatch):
+    """a PagedReader without a GPU: the operators stand in (weights: one more for every slot)"""
+    from spinf_serve_b200.paged import PagedReader
+
+    def attend(q, k, v, table, lens, cu, max_q, scale, weights=None, weights_out=None, **kw):
+        if weights is not None:
+            n = int(lens[0])
+            (weights if weights_out is None else weights_out)[:, :, :n] = weights[:, :, :n] + 1.0
+        return q
+
+    def evict(k, v, table, lens, weights, keep, recent, new_table, max_len=None):
+        n, h = int(lens[0]), k.shape[1]
+        if evict.fail:
+            evict.fail -= 1
+            if not evict.fail:
+                raise _lib.SpinfError("paged_evict: refused")
+        if weights is None:
+            kept = torch.arange(n - keep, n).expand(h, -1)[None]
+            return None, kept, None
+        kept = torch.stack([torch.cat([weights[0, x, : n - recent].sort(descending=True, stable=True).indices[: keep - recent].sort().values, torch.arange(n - recent, n)]) for x in range(h)])[None]
+        return None, kept, torch.gather(weights, 2, kept)
+
+    evict.fail = 0
+    monkeypatch.setattr(ops, "paged_append", lambda qkv, H, h, D, *a, **kw: qkv[:, : H * D].view(-1, H, D))
+    monkeypatch.setattr(ops, "paged_attention", attend)
+    monkeypatch.setattr(ops, "paged_evict", evict)
+    r = PagedReader(_Stack(), n_pages=12, page=16, chunk=32)
+    r.evict_op = evict
+    return r
+
+
+def test_a_reading_that_fails_gives_its_pages_back(reader):
+    with pytest.raises(RuntimeError, match="out of pages"):
+        reader.read(list(range(200)))
+    assert sorted(reader.cache.free) == list(range(12)) and reader.cache.refs == [0] * 12
+    reader.stack.fail = 1
+    with pytest.raises(ValueError):
+        reader.read(list(range(20)))
+    assert len(reader.cache.free) == 12
+    reader.stack.fail = None
+    seq = reader.read(list(range(100)))
+    assert seq.length == 100 and len(reader.cache.free) == 5
