@@ -133,15 +133,21 @@ class PagedCache:
         if any(by_weight) and seq.weights is None:
             raise RuntimeError("the sequence was read without its slots' weights")
         pages = self._take(-(-keep // self.page))
-        i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=self.device)  # noqa: E731
-        table, new_table, lens = i32(seq.pages), i32(pages), torch.tensor([seq.length], dtype=torch.int32, device=self.device)
-        kept = []
-        for li in range(self.k.shape[0]):
-            w = seq.weights[li][None] if by_weight[li] else None
-            _, slots, w_new = ops.paged_evict(self.k[li], self.v[li], table, lens, w, keep, recent, new_table, max_len=seq.length)
-            if w is not None:
-                seq.weights[li, :, :keep] = w_new[0]
-            kept.append(slots[0])
+        kept, moved = [], {}
+        try:
+            i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=self.device)  # noqa: E731
+            table, new_table, lens = i32(seq.pages), i32(pages), torch.tensor([seq.length], dtype=torch.int32, device=self.device)
+            for li in range(self.k.shape[0]):
+                w = seq.weights[li][None] if by_weight[li] else None
+                _, slots, w_new = ops.paged_evict(self.k[li], self.v[li], table, lens, w, keep, recent, new_table, max_len=seq.length)
+                if w is not None:
+                    moved[li] = w_new[0]
+                kept.append(slots[0])
+        except BaseException:  # the old pages still hold everything
+            self._release(pages)
+            raise
+        for li, w in moved.items():
+            seq.weights[li, :, :keep] = w
         self._release(seq.pages)
         seq.pages, seq.length = pages, keep
         return kept

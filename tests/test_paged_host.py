@@ -336,3 +336,29 @@ def test_a_reading_that_fails_gives_its_pages_back(reader):
     reader.stack.fail = None
     seq = reader.read(list(range(100)))
     assert seq.length == 100 and len(reader.cache.free) == 5
+
+
+def test_an_eviction_that_fails_changes_nothing(reader):
+    seq = reader.read(list(range(90)), weigh=True)
+    pages, weights, free = list(seq.pages), seq.weights.clone(), list(reader.cache.free)
+    for layer in (1, 2):
+        reader.evict_op.fail = layer
+        with pytest.raises(_lib.SpinfError):
+            reader.evict(seq, 40, 8)
+        assert seq.pages == pages and seq.length == seq.position == 90 and torch.equal(seq.weights, weights)
+        assert sorted(reader.cache.free) == sorted(free)
+    kept = reader.evict(seq, 40, 8)
+    assert seq.length == 40 and len(seq.pages) == 3 and len(reader.cache.free) == 9
+    assert torch.equal(seq.weights[1, :, :40], torch.gather(weights[1], 1, kept[1]))
+
+
+def test_a_weight_layer_behind_one_that_failed_is_not_half_moved(reader):
+    """both layers by weight: the second's failure leaves the first's weights as they were"""
+    reader.stack.cfg.layer_types = ["full_attention", "full_attention"]
+    seq = reader.read(list(range(90)), weigh=True)
+    seq.weights[:, :, :90] = torch.randperm(90).float()
+    weights = seq.weights.clone()
+    reader.evict_op.fail = 2
+    with pytest.raises(_lib.SpinfError):
+        reader.evict(seq, 40, 8)
+    assert torch.equal(seq.weights, weights) and len(reader.cache.free) == 6
