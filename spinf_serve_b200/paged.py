@@ -17,7 +17,8 @@ from spinf_serve_b200 import ops
 @dataclass
 class Sequence:
     """one cached sequence: its pages in slot order, cached slots, and the position of its next token (past `length` once slots were
-    evicted). weights: fp32 [layers, kv heads, cap] accumulated attention weight of every slot, where it is kept"""
+    evicted). weights: fp32 [layers, kv heads, cap] attention weight of every slot, added up over the forwards that weigh (a slot begins at
+    zero), where it is kept"""
 
     pages: list = field(default_factory=list)
     length: int = 0
@@ -65,6 +66,15 @@ class PagedCache:
             if self.refs[p] == 0:
                 self.free.append(p)
 
+    def _weights_room(self, weights, slots: int):
+        """the weights with room for so many slots (None: new ones, all zero)"""
+        if weights is not None and weights.shape[2] >= slots:
+            return weights
+        out = torch.zeros((self.k.shape[0], self.k.shape[2], -(-slots // 1024) * 1024), dtype=torch.float32, device=self.device)
+        if weights is not None:
+            out[:, :, : weights.shape[2]] = weights
+        return out
+
     def common_front(self, seqs: list, most: int | None = None) -> int:
         """tokens of the pages that all of the sequences begin with (of their first `most` pages)"""
         n = 0
@@ -81,8 +91,10 @@ class PagedCache:
         self._release(seq.pages)
         seq.pages, seq.length, seq.position, seq.weights = [], 0, 0, None
 
-    def fork(self, seq: Sequence) -> Sequence:
-        """a sequence that goes on from where `seq` is: full pages are shared, a begun one is copied (both may go on writing)"""
+    def fork(self, seq: Sequence, weights: bool = True) -> Sequence:
+        """a sequence that goes on from where `seq` is: full pages are shared, a begun one is copied (both may go on writing), and so are the
+        slots' weights where they are kept (weights=False: the fork has none)"""
+        own = seq.weights.clone() if weights and seq.weights is not None else None
         whole = seq.length // self.page
         last = self._take(1) if seq.length % self.page else []
         for p in seq.pages[:whole]:
@@ -91,7 +103,7 @@ class PagedCache:
             old = seq.pages[whole]
             for pool in (self.k, self.v):
                 pool[:, last[0]].copy_(pool[:, old])
-        return Sequence(seq.pages[:whole] + last, seq.length, seq.position)
+        return Sequence(seq.pages[:whole] + last, seq.length, seq.position, own)
 
     def grow(self, seqs: list, counts: list) -> Step:
         """room for counts[i] new tokens of seqs[i] (0: the sequence sits this one out) -> the forward's tables. The same sequence
@@ -112,6 +124,10 @@ class PagedCache:
             width = max(1, max(len(t) for t in tables))
             lens = [s.length + c for s, c in zip(seqs, counts)]
             i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
+            for s, c, t in zip(seqs, counts, tables):
+                if s.weights is not None:
+                    s.weights = self._weights_room(s.weights, len(t) * self.page)
+                    s.weights[:, :, s.length : s.length + c] = 0.0
             step = Step(i32([t + [0] * (width - len(t)) for t in tables]), i32(lens), i32(cu), i32(pos), max(counts), max(lens))
         except BaseException:
             self._release(pages)
@@ -133,23 +149,22 @@ class PagedCache:
         if any(by_weight) and seq.weights is None:
             raise RuntimeError("the sequence was read without its slots' weights")
         pages = self._take(-(-keep // self.page))
-        kept, moved = [], {}
+        kept = []
         try:
+            moved = None if seq.weights is None else torch.zeros_like(seq.weights)
             i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=self.device)  # noqa: E731
             table, new_table, lens = i32(seq.pages), i32(pages), torch.tensor([seq.length], dtype=torch.int32, device=self.device)
             for li in range(self.k.shape[0]):
                 w = seq.weights[li][None] if by_weight[li] else None
                 _, slots, w_new = ops.paged_evict(self.k[li], self.v[li], table, lens, w, keep, recent, new_table, max_len=seq.length)
-                if w is not None:
-                    moved[li] = w_new[0]
+                if moved is not None:  # (without `w` the last slots stay, and their weights with them)
+                    moved[li, :, :keep] = seq.weights[li, :, seq.length - keep : seq.length] if w is None else w_new[0]
                 kept.append(slots[0])
         except BaseException:  # the old pages still hold everything
             self._release(pages)
             raise
-        for li, w in moved.items():
-            seq.weights[li, :, :keep] = w
         self._release(seq.pages)
-        seq.pages, seq.length = pages, keep
+        seq.pages, seq.length, seq.weights = pages, keep, moved
         return kept
 
 
@@ -200,14 +215,8 @@ class PagedReader:
             front = max(ops.SHARE_TOKENS, -(-ops.SHARE_BYTES // ((len(seqs) - 1) * self.cache.row_bytes)))
             st.shared = self.cache.common_front(seqs, -(-front // self.cache.page)) >= front
         dev = self.cache.device
-        if weigh:
-            seq, cap = seqs[0], len(seqs[0].pages) * self.cache.page
-            if seq.weights is None or seq.weights.shape[2] < cap:
-                old = seq.weights
-                seq.weights = torch.zeros((self.stack.n_layers, self.stack.cfg.kv_heads, -(-cap // 1024) * 1024), dtype=torch.float32, device=dev)
-                if old is not None:
-                    seq.weights[:, :, : old.shape[2]] = old
-            seq.weights[:, :, seq.length - len(ids[0]) : seq.length] = 0.0
+        if weigh and seqs[0].weights is None:
+            seqs[0].weights = self.cache._weights_room(None, len(seqs[0].pages) * self.cache.page)
         self._step, self._weights = st, seqs[0].weights if weigh else None
         try:
             inputs = {"ids": torch.cat([torch.as_tensor(x, dtype=torch.int64) for x in ids]).to(dev), "pos": st.pos}
@@ -241,7 +250,7 @@ class PagedReader:
         forks = []
         try:
             for _ in branches:
-                forks.append(self.cache.fork(seq))
+                forks.append(self.cache.fork(seq, weights=False))
             return self.forward(forks, branches)
         finally:
             for f in forks:

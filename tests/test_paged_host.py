@@ -362,3 +362,57 @@ def test_a_weight_layer_behind_one_that_failed_is_not_half_moved(reader):
     with pytest.raises(_lib.SpinfError):
         reader.evict(seq, 40, 8)
     assert torch.equal(seq.weights, weights) and len(reader.cache.free) == 6
+
+
+def test_weights_are_those_of_the_tokens_that_are_there(reader):
+    """weigh, evict, read on without and with weights: no slot has what an evicted token had in its place. (Rows that are read without
+    weights add none; their slots begin at zero like any others)"""
+    seq = reader.read(list(range(90)), weigh=True)
+    assert (seq.weights[1, :, :90] >= 1.0).all() and (seq.weights[1, :, 90:] == 0).all()
+    reader.evict(seq, 40, 8)
+    assert (seq.weights[1, :, :40] >= 1.0).all()
+    reader.forward([seq], [[1] * 20])
+    assert (seq.weights[1, :, :40] >= 1.0).all() and (seq.weights[1, :, 40:60] == 0).all()
+    reader.forward([seq], [[1] * 20], weigh=True)
+    assert (seq.weights[1, :, 40:80] == 1.0).all()
+    kept = reader.evict(seq, 30, 25)
+    assert all(x < 40 for x in kept[1][:, :5].flatten().tolist())  # the old tokens have the larger weights
+
+
+def test_growing_without_weights_past_their_room(reader):
+    seq = reader.read([1] * 20, weigh=True)
+    seq.weights = seq.weights[:, :, :32].clone()  # (as if the cache had been that short)
+    reader.forward([seq], [[1] * 60])
+    assert seq.weights.shape[2] >= 80 and (seq.weights[1, :, :20] == 1).all() and (seq.weights[1, :, 20:80] == 0).all()
+    reader.evict(seq, 30, 8)
+    assert seq.length == 30 and len(reader.cache.free) == 10
+
+
+def test_weighing_the_last_tokens_only(reader):
+    seq = reader.read([1] * 20)
+    reader.forward([seq], [[1] * 4], weigh=True)
+    assert (seq.weights[1, :, :24] == 1).all()
+    reader.evict(seq, 10, 4)
+    assert seq.length == 10
+
+
+def test_a_fork_has_its_own_copy_of_the_weights(reader):
+    seq = reader.read([1] * 50, weigh=True)
+    before = seq.weights.clone()
+    fork = reader.cache.fork(seq)
+    reader.forward([fork], [[1] * 4], weigh=True)
+    assert torch.equal(seq.weights, before) and torch.equal(fork.weights[1, :, :50], before[1, :, :50] + 1) and (fork.weights[1, :, 50:54] == 1).all()
+    reader.evict(fork, 30, 8)
+    assert torch.equal(seq.weights, before) and fork.length == 30
+    plain = reader.cache.fork(reader.read([1] * 5))
+    assert plain.weights is None
+    reader.ask(seq, [[1], [2, 3]])
+    assert torch.equal(seq.weights, before)
+
+
+def test_cutting_by_place_moves_the_weights_along(reader):
+    """an eviction that keeps the last slots of a weighed sequence: each slot's weight goes with it"""
+    seq = reader.read([1] * 60, weigh=True)
+    seq.weights[:, :, :60] = torch.arange(60.0)
+    reader.cache.evict(seq, 24, 0, [False, False])
+    assert (seq.weights[:, :, :24] == torch.arange(36.0, 60.0)).all() and (seq.weights[:, :, 24:] == 0).all()
