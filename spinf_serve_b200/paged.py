@@ -211,26 +211,28 @@ class PagedReader:
         if not all(len(x) for x in ids) or len(seqs) > 1024:
             raise RuntimeError("every sequence of a forward (at most 1024) needs new tokens")
         st = self.cache.grow(seqs, [len(x) for x in ids])
-        if len(seqs) > 1:
-            front = max(ops.SHARE_TOKENS, -(-ops.SHARE_BYTES // ((len(seqs) - 1) * self.cache.row_bytes)))
-            st.shared = self.cache.common_front(seqs, -(-front // self.cache.page)) >= front
-        dev = self.cache.device
-        if weigh and seqs[0].weights is None:
-            seqs[0].weights = self.cache._weights_room(None, len(seqs[0].pages) * self.cache.page)
-        self._step, self._weights = st, seqs[0].weights if weigh else None
+        weights = None
         try:
-            inputs = {"ids": torch.cat([torch.as_tensor(x, dtype=torch.int64) for x in ids]).to(dev), "pos": st.pos}
+            if len(seqs) > 1:
+                front = max(ops.SHARE_TOKENS, -(-ops.SHARE_BYTES // ((len(seqs) - 1) * self.cache.row_bytes)))
+                st.shared = self.cache.common_front(seqs, -(-front // self.cache.page)) >= front
+            if weigh:  # added up in a copy, so that a failure half way through the layers leaves none of it
+                old = seqs[0].weights
+                weights = old.clone() if old is not None else self.cache._weights_room(None, len(seqs[0].pages) * self.cache.page)
+            self._step, self._weights = st, weights
+            inputs = {"ids": torch.cat([torch.as_tensor(x, dtype=torch.int64) for x in ids]).to(self.cache.device), "pos": st.pos}
             rows = (st.cu[1:].long() - 1) if last else None
             out = self.stack.forward(None, None, inputs, None, rows=rows, attend=self)
         except BaseException:
-            # the sequences stay where they were (their new pages are kept for the next try; weights that layers before the failure
-            # have added up stay added)
+            # the sequences stay where they were (their new pages are kept for the next try)
             for s, x in zip(seqs, ids):
                 s.length -= len(x)
                 s.position -= len(x)
             raise
         finally:
             self._step = self._weights = None
+        if weigh:
+            seqs[0].weights = weights
         return out if last else out[0]
 
     def read(self, ids, weigh: bool = False) -> Sequence:

@@ -416,3 +416,41 @@ def test_cutting_by_place_moves_the_weights_along(reader):
     seq.weights[:, :, :60] = torch.arange(60.0)
     reader.cache.evict(seq, 24, 0, [False, False])
     assert (seq.weights[:, :, :24] == torch.arange(36.0, 60.0)).all() and (seq.weights[:, :, 24:] == 0).all()
+
+
+def test_a_weighing_forward_that_fails_adds_nothing(reader):
+    """the first layer has added its weights when the second fails: the next try counts them once"""
+    reader.stack.cfg.layer_types = ["full_attention", "full_attention"]
+    seq = reader.read([1] * 20, weigh=True)
+    before = seq.weights.clone()
+    reader.stack.fail = 1
+    with pytest.raises(ValueError):
+        reader.forward([seq], [[1] * 15], weigh=True)
+    assert seq.length == seq.position == 20 and torch.equal(seq.weights[:, :, :20], before[:, :, :20])
+    reader.stack.fail = None
+    reader.forward([seq], [[1] * 15], weigh=True)
+    assert (seq.weights[:, :, :20] == before[:, :, :20] + 1).all() and (seq.weights[:, :, 20:35] == 1).all() and (seq.weights[:, :, 35:] == 0).all()
+
+
+def test_a_weighing_forward_that_fails_first_keeps_none(reader):
+    seq = reader.cache.open()
+    reader.stack.fail = 1
+    with pytest.raises(ValueError):
+        reader.forward([seq], [[1] * 15], weigh=True)
+    assert seq.weights is None and seq.length == 0
+
+
+def test_a_forward_that_fails_before_its_layers(reader):
+    """token ids that are none, or weights that do not fit in: the sequences stay where they were"""
+    a, b = reader.read([1] * 20), reader.read([1] * 5)
+    with pytest.raises((TypeError, ValueError)):
+        reader.forward([a, b], [[1, 2], ["x"]])
+    assert (a.length, a.position, b.length, b.position) == (20, 20, 5, 5)
+
+    def full(*a):
+        raise MemoryError
+
+    reader.cache._weights_room = full
+    with pytest.raises(MemoryError):
+        reader.forward([a], [[1, 2]], weigh=True)
+    assert (a.length, a.position, a.weights) == (20, 20, None)
