@@ -125,7 +125,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (args[9] != Py_None) {
     if (!THPVariable_Check(args[9])) Py_RETURN_NONE;
     t[9] = &THPVariable_Unpack(args[9]);
-    if (!t[9]->is_cuda() || t[9]->get_device() != c.key.device) Py_RETURN_NONE;
+    if (!t[9]->is_cuda() || t[9]->get_device() != c.key.device || !t[9]->is_contiguous()) Py_RETURN_NONE;
   }
   // n, H, h, D, q pitch, out pitch, pages, page, k strides, v strides, table pitch, B, max_len, window, workspace, shared, weight strides
   const int64_t* x = c.layout.data();

@@ -794,7 +794,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     `window` slots of a row -> [n, H, D] (rows behind cu[B]: undefined in a new tensor, untouched in `out`; a row that sees nothing:
     0). max_q, max_len: no sequence has more rows / tokens (max_len None: what the table can hold).
     weights (fp32 [B, Hkv, cap], cap >= max_len): each slot's accumulated attention weight, weights_out = decay * weights + this
-    call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional uint8
+    call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional contiguous uint8
     tensor reused between calls on one stream; out must not overlap q. shared: look for neighbouring sequences whose tables begin with
     the same pages (branches of one content) and read those once for all of them (None: where the pool has less than an eighth of the
     pages that this many sequences of max_len tokens would need; looking in vain costs up to 20 us)."""
@@ -817,6 +817,8 @@ def _attention_first(q, k_pages, v_pages, table, lens, cu, max_q, scale, window,
         _layout(q), _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cu), max_q, window, _layout(weights), _layout(weights_out),
         max_len, _layout(out), shared
     )
+    if workspace is not None and not workspace.is_contiguous():
+        raise SpinfError(f"{what}: workspace must be contiguous, got strides {workspace.stride()} of {tuple(workspace.shape)}")
     idx = _paged_device(what, q, k_pages, v_pages, table, lens, cu, weights, weights_out, out, workspace)
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):

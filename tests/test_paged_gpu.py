@@ -737,3 +737,14 @@ def test_weights_of_a_chunk_beside_rows_that_are_not_finite(dev, H, h, D, window
     keep = [i for i in range(cu[2], cu[3]) if i != cu[2] + at]
     assert torch.equal(got[keep], out[keep])
     assert torch.equal(w[0], clean[0]) and torch.equal(w[4], clean[4])
+
+
+def test_a_workspace_with_gaps_is_refused_in_a_known_layout(dev):
+    c = Call(dev, 4, 2, 128, 16, [(300, 2), (40, 1)], seed=6)
+    room = torch.empty(1 << 22, dtype=torch.uint8, device=dev)
+    want = c.attend(workspace=room)
+    assert torch.equal(c.attend(workspace=room.view(2, -1)), want)
+    for ws in (room[:1].expand(1 << 22), room.view(-1, 2)[:, 0]):
+        with pytest.raises(_lib.SpinfError, match="contiguous"):
+            c.attend(workspace=ws)
+    assert torch.equal(c.attend(), want)

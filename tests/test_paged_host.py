@@ -454,3 +454,10 @@ def test_a_forward_that_fails_before_its_layers(reader):
     with pytest.raises(MemoryError):
         reader.forward([a], [[1, 2]], weigh=True)
     assert (a.length, a.position, a.weights) == (20, 20, None)
+
+
+@pytest.mark.parametrize("ws", [torch.empty(1, dtype=torch.uint8).expand(1 << 30), torch.empty((64, 64), dtype=torch.uint8)[:, ::2], torch.empty((8, 8)).t()])
+def test_a_workspace_with_gaps_is_refused(ws):
+    """its number of bytes is not the room that it has"""
+    with pytest.raises(_lib.SpinfError, match="contiguous"):
+        _call(workspace=ws)
