@@ -166,10 +166,11 @@ extern "C" int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int
                                   int32_t norm_v, void* q_out, void* k_pages, void* v_pages, int64_t n_pages, int32_t page,
                                   const int64_t* k_strides_host, const int64_t* v_strides_host, const int32_t* table,
                                   int64_t table_pitch, int32_t width, const int32_t* lens, const int32_t* cu, int32_t B, void* stream) {
-  if (n == 0 || B == 0) return 0;  // nothing to do: the row pointers may be null
-  SPINF_CHECK_ARG(qkv && k_pages && v_pages && k_strides_host && v_strides_host && table && lens && cu && n > 0 && B > 0);
+  if (n == 0 || (B == 0 && !q_out)) return 0;  // nothing to do: the row pointers may be null
+  SPINF_CHECK_ARG(qkv && k_pages && v_pages && k_strides_host && v_strides_host && n > 0 && B >= 0);
+  SPINF_CHECK_ARG(B == 0 || (table && lens && cu && width > 0 && table_pitch >= width));  // (no sequence: q's rows are made all the same)
   SPINF_CHECK_ARG(H > 0 && Hkv > 0 && (D == 128 || D == 256) && n < (1ll << 31) && pitch >= static_cast<int64_t>(H + 2 * Hkv) * D && pitch % 8 == 0);
-  SPINF_CHECK_ARG(page >= 16 && page <= 256 && (page & (page - 1)) == 0 && n_pages > 0 && n_pages < (1ll << 31) && width > 0 && table_pitch >= width);
+  SPINF_CHECK_ARG(page >= 16 && page <= 256 && (page & (page - 1)) == 0 && n_pages > 0 && n_pages < (1ll << 31));
   SPINF_CHECK_ARG(static_cast<int64_t>(width) * page < (1ll << 31));
   SPINF_CHECK_ARG((wq != nullptr) == (wk != nullptr) && (cos_t != nullptr) == (sin_t != nullptr) && (cos_t != nullptr) == (rot_dim != 0));
   SPINF_CHECK_ARG(rot_dim >= 0 && rot_dim <= D && rot_dim % 16 == 0);

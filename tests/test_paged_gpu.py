@@ -748,3 +748,20 @@ def test_a_workspace_with_gaps_is_refused_in_a_known_layout(dev):
         with pytest.raises(_lib.SpinfError, match="contiguous"):
             c.attend(workspace=ws)
     assert torch.equal(c.attend(), want)
+
+
+def test_append_of_no_sequences_makes_q(dev):
+    """q has all n rows, also where none of them is a sequence's"""
+    H, h, D, page = 4, 2, 128, 16
+    c = Call(dev, H, h, D, page, [(20, 4)], seed=5)
+    qkv = torch.randn((9, (H + 2 * h) * D), generator=c.gen).to(torch.bfloat16).to(dev)
+    w = (1 + 0.1 * torch.randn(D, generator=c.gen)).to(torch.bfloat16).to(dev)
+    k, v = c.on["k"].clone(), c.on["v"].clone()
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    for width in (0, 3):
+        held = torch.full((9, H, D), 7.0, dtype=torch.bfloat16, device=dev)  # where the allocator finds room for q again
+        del held
+        q = ops.paged_append(qkv, H, h, D, c.on["k"], c.on["v"], torch.zeros((0, width), dtype=torch.int32, device=dev), none, torch.zeros(1, dtype=torch.int32, device=dev), wq=w, wk=w)
+        want = OP.append(qkv.cpu(), H, h, D, w.cpu(), w.cpu())[0]
+        assert ((q.double().cpu() - want).abs() <= (BF + 2.0**-19) * want.abs()).all()
+    assert torch.equal(k.view(torch.int16), c.on["k"].view(torch.int16)) and torch.equal(v.view(torch.int16), c.on["v"].view(torch.int16))
