@@ -439,7 +439,8 @@ int spinf_gdn_epilogue(const void* o, const void* z, int64_t z_pitch, const void
  * cu[b] .. cu[b+1] of the n rows (int32 [B+1], ascending; rows of no sequence take part in nothing) and lens[b] cached tokens, the call's
  * own included: row i of the sequence sits in slot lens[b] - (cu[b+1] - cu[b]) + i, and slot s is row s % page of page
  * table[b * table_pitch + s / page]. Tables may share pages as long as nothing writes to a shared one. A page index, length or row
- * range outside the pool, max_len, max_q or n is skipped and reported as SPINF_ST_BAD_INDEX.
+ * range outside the pool, max_len, max_q or n is skipped and reported as SPINF_ST_BAD_INDEX (keys and values on a page that is none
+ * count as zeros).
  *
  * spinf_paged_append: rows of a fused projection [H q | Hkv k | Hkv v] x D -> norms of the q and k heads (wq, wk [D]; both null:
  * none; plus1: weights 1 + w), of the v heads (norm_v, without weight), rotary embedding of q and k over the first rot_dim

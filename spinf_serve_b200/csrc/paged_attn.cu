@@ -151,10 +151,12 @@ struct KeyProducer {
 #pragma unroll
         for (int y = 0; y < UNITS * BOXES; ++y) {
           const bool want = wanted(w, u * 64 + y * ROWS), good = static_cast<unsigned>(pg[y]) < static_cast<unsigned>(s.n_pages);
-          if (want && !good && lane == 0) atomicCAS(status, 0, ST_BAD_INDEX);
-          if (!want || !good) {
+          if (!want) {
             pg[y] = -1;
             bytes[y / BOXES] -= ROWS * D * 2;
+          } else if (!good) {  // one past the last page: the copy brings zeros
+            pg[y] = s.n_pages;
+            if (lane == 0) atomicCAS(status, 0, ST_BAD_INDEX);
           }
         }
       }

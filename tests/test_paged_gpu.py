@@ -765,3 +765,27 @@ def test_append_of_no_sequences_makes_q(dev):
         want = OP.append(qkv.cpu(), H, h, D, w.cpu(), w.cpu())[0]
         assert ((q.double().cpu() - want).abs() <= (BF + 2.0**-19) * want.abs()).all()
     assert torch.equal(k.view(torch.int16), c.on["k"].view(torch.int16)) and torch.equal(v.view(torch.int16), c.on["v"].view(torch.int16))
+
+
+@pytest.mark.parametrize("bad", [-1, 2**30])
+@pytest.mark.parametrize("H,h,D,page", [(16, 8, 256, 64), (8, 4, 128, 16), (6, 1, 256, 128), (32, 4, 128, 32)])
+def test_a_page_outside_the_pool_counts_as_zeros(dev, H, h, D, page, bad):
+    """in every kernel, and not as whatever another sequence's keys have left behind; the call is reported"""
+    seqs = [(700, 1), (700, 3), (700, 130), (520, 1)]
+    c = Call(dev, H, h, D, page, seqs, seed=H, spare=1)
+    o, w = c.on, torch.zeros((4, h, 768), device=dev)
+    zero = int(c.free[0])
+    o["k"][zero], o["v"][zero] = 0.0, 0.0
+    got = {}
+    for entry in (zero, bad):
+        table = o["table"].clone()
+        for b in range(3):
+            table[b, 2], table[b, (700 - 1) // page] = entry, entry
+        got[entry] = []
+        for weights in (None, w):
+            for window in (None, 300):
+                into = None if weights is None else torch.zeros_like(w)
+                got[entry] += [ops.paged_attention(o["q"], o["k"], o["v"], table, o["lens_t"], o["cu"], 130, D**-0.5, window=window, weights=weights, weights_out=into), into]
+        assert _lib.last_status(raise_on_error=False) == (0 if entry == zero else 5)
+    for x, y in zip(got[zero], got[bad]):
+        assert x is y is None or torch.equal(x, y)
