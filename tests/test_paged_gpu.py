@@ -789,3 +789,24 @@ def test_a_page_outside_the_pool_counts_as_zeros(dev, H, h, D, page, bad):
         assert _lib.last_status(raise_on_error=False) == (0 if entry == zero else 5)
     for x, y in zip(got[zero], got[bad]):
         assert x is y is None or torch.equal(x, y)
+
+
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (8, 1, 128)])
+@pytest.mark.parametrize("n", [1, 3, 90])
+def test_a_row_whose_scores_are_all_minus_infinity_weighs_nothing(dev, H, h, D, n):
+    """as a row that sees nothing: 0, and no weight for any slot"""
+    c = Call(dev, H, h, D, 32, [(300, n)], seed=n)
+    o = c.on
+    o["k"][..., 0] = o["k"][..., 0].abs()  # (behind the sequence they stay NaN)
+    q = o["q"]
+    q[n - 1] = 0.0
+    q[n - 1, :, 0] = -math.inf
+    w = torch.zeros((1, h, 320), device=dev)
+    got = c.attend(weights=w)
+    assert (got[n - 1] == 0).all()
+    q[n - 1] = math.nan  # the same call with that row taken out: its cu ends before it, the last slot is still there
+    rest = torch.zeros_like(w)
+    if n > 1:
+        cu, lens = torch.tensor([0, n - 1], dtype=torch.int32, device=dev), o["lens_t"] - 1
+        ops.paged_attention(q, o["k"], o["v"], o["table"], lens, cu, c.max_q, D**-0.5, weights=rest)
+    assert torch.equal(w[..., :300], rest[..., :300])
