@@ -1053,7 +1053,8 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   const int64_t group = H / h;
   z.chunk_rows = chunk_rows_of(static_cast<int>(group), weights);
   const int64_t most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
-  if (slots > 1) {
+  const bool chunk_only = B == 1 && max_q > most;  // the few-row kernels are not launched
+  if (slots > 1 && !chunk_only) {
     const int64_t by_rows = (max_q < most ? max_q : most) * H * slots;  // every row in every split
     const int64_t by_items = static_cast<int64_t>(PG_SMS) * RT;  // every free slot one full row tile
     z.seq_parts = by_rows < by_items ? by_rows : by_items;
@@ -1090,8 +1091,8 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
     z.chunk_ml = up256(all_units * 512 * 8);
     z.joins = up256(all_units * static_cast<int64_t>(sizeof(ChunkJoin)) + 16);
   }
-  if (weights) {
-    z.lse = up256(n * H * 4);
+  if (weights) z.lse = up256(n * H * 4);
+  if (weights && !chunk_only) {
     z.score_pitch = tiles * PG_TILE;
     z.tok_cap = static_cast<int>(max_q < most ? max_q : most);
     z.scores = up256(B * z.tok_cap * H * z.score_pitch * 4);

@@ -461,3 +461,16 @@ def test_a_workspace_with_gaps_is_refused(ws):
     """its number of bytes is not the room that it has"""
     with pytest.raises(_lib.SpinfError, match="contiguous"):
         _call(workspace=ws)
+
+
+def _room(n, B, H, h, D, max_q, max_len, weights=0, shared=0):
+    return _lib.lib().spinf_paged_attention_workspace_bytes(n, B, H, h, D, max_q, max_len, weights, shared)
+
+
+@pytest.mark.parametrize("H,h,D", [(32, 16, 128), (16, 8, 256), (8, 1, 128)])
+def test_a_chunk_alone_asks_for_no_scores(H, h, D):
+    """its kernels compute them again: beside the parts of its items there is the rows' lse only"""
+    for max_len in (4096, 131072, 1 << 20):
+        assert _room(2048, 1, H, h, D, 2048, max_len, 1) - _room(2048, 1, H, h, D, 2048, max_len, 0) <= 2048 * H * 4
+        assert _room(2048, 1, H, h, D, 2048, max_len, 1) <= 150 * 512 * (D * 4 + 8 + 32) + 2048 * H * 4
+    assert _room(1, 1, H, h, D, 1, 4096, 1) > 4096 * H * 4  # a step keeps its scores
