@@ -456,7 +456,9 @@ int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int32_t H, int
 /* Attention of the call's rows over their sequences' slots: row i sees the slots up to its own, with window > 0 only the last
  * `window` of them; out = softmax(scale q k) v, 0 for a row that sees nothing (a sequence with more rows than cached tokens).
  * q, out: rows of q_pitch / out_pitch elements, head j at j * D. max_q, max_len: no sequence of the call has more rows or tokens
- * (they size the workspace; 256-byte aligned). weights_out (optional, fp32; weight_strides_host: sequence and head strides of
+ * (they size the workspace; 256-byte aligned). A call whose sequences' parts would take more than 2 GB is made in launches of as many
+ * sequences as that holds, with the same results (a common front ends where a launch ends); beside that the workspace has n * H floats
+ * where weights are kept. weights_out (optional, fp32; weight_strides_host: sequence and head strides of
  * weights_in, then of weights_out): weights_out[b, g, j] = decay * weights_in[b, g, j] + the sum of the attention weights of slot j
  * over the sequence's rows and the heads that share kv head g, for j < lens[b]; the two may be the same tensor; with decay 0
  * weights_in is not read. out lies apart from q, its rows behind cu[B] are left as they were. A sequence's results do not depend on

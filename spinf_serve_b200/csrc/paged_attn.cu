@@ -1042,18 +1042,25 @@ __host__ __device__ constexpr int chunk_rows_of(int group, bool weights) { retur
 struct PagedSizes {
   int64_t seq_parts, part_o, part_ml, chunk_o, chunk_ml, joins, share, lse, scores, total;
   int64_t score_pitch;
-  int tok_cap, chunk_rows, max_units, share_units;
+  int tok_cap, chunk_rows, max_units, share_units, unit_slots;
   bool too_large;
 };
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
-static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights, bool shared) {
+// alone: the call has one sequence (B: those of a launch); window 0: none
+static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, int64_t window, bool weights, bool shared, bool alone) {
   PagedSizes z = {};
+  // key tiles that so many neighbouring rows see at most: their window's slots, wherever in a tile they begin
+  const auto seen = [=](int64_t rows, int64_t tiles) {
+    const int64_t w = window > 0 ? (rows - 1 + window + 2 * PG_TILE - 2) / PG_TILE : tiles;
+    return w < tiles ? w : tiles;
+  };
   const int64_t tiles = (max_len + PG_TILE - 1) / PG_TILE;
-  const int64_t slots = tiles < PG_SMS / h ? tiles : PG_SMS / h;  // most splits of a sequence
   const int64_t group = H / h;
   z.chunk_rows = chunk_rows_of(static_cast<int>(group), weights);
   const int64_t most = z.chunk_rows / group;  // tokens of a sequence that is not the chunk kernel's
-  const bool chunk_only = B == 1 && max_q > most;  // the few-row kernels are not launched
+  const int64_t few = seen(max_q < most ? max_q : most, tiles);
+  const int64_t slots = few < PG_SMS / h ? few : PG_SMS / h;  // most splits of a sequence
+  const bool chunk_only = alone && max_q > most;  // the few-row kernels are not launched
   if (slots > 1 && !chunk_only) {
     const int64_t by_rows = (max_q < most ? max_q : most) * H * slots;  // every row in every split
     const int64_t by_items = static_cast<int64_t>(PG_SMS) * RT;  // every free slot one full row tile
@@ -1068,27 +1075,34 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   z.part_o = up256(B * z.seq_parts * D * 4);
   z.part_ml = up256(B * z.seq_parts * 8);
   const int hl = chunk_heads_log2(static_cast<int>(group)), tl = 8 - hl;
+  const int64_t most_units = chunk_units_of(D), per_tt = H >> hl, ntt = (max_q + (1 << tl) - 1) >> tl;
+  // items of one token tile (and fronts) are cut into parts, a unit each: one slot of 256 rows; other units end one item and begin the next
+  z.unit_slots = ntt <= 1 && per_tt <= most_units ? 1 : 2;
   int64_t all_units = 0;
   if (max_q > most) {
-    const int64_t work = ((max_q + (1 << tl) - 1) >> tl) * (H >> hl) * (tiles > 0 ? tiles : 1);
+    const int64_t each = seen(max_q < 1 << tl ? max_q : 1 << tl, tiles), work = ntt * per_tt * (each > 0 ? each : 1);
     if (work >= (1ll << 31)) z.too_large = true;  // the chunk kernels count (item, key tile) pairs in 32 bits
     // (an item makes a unit, or a unit holds CHUNK_MIN_TILES pairs, or a part of an item four)
-    int64_t units = work / 4 + ((max_q + (1 << tl) - 1) >> tl) * (H >> hl);
-    units = units > chunk_units_of(D) ? chunk_units_of(D) : units;
+    int64_t units = work / 4 + ntt * per_tt;
+    if (z.unit_slots == 1) {
+      const int64_t parts = most_units / per_tt < each / 4 ? most_units / per_tt : each / 4;
+      units = per_tt * (parts > 1 ? parts : 1);
+    }
+    units = units > most_units ? most_units : units;
     const int64_t seqs = B == 1 ? 1 : n / (most + 1) < B ? n / (most + 1) : B;  // so many can be the chunk kernel's
     all_units = seqs * units;
   }
   if (shared) {
     // a unit per item of a group, or up to one per CTA (pair) for a group of few items: room for four such groups
-    const int64_t items = ((n >> tl) + B / 2) * (H >> hl) + 4 * chunk_units_of(D);
+    const int64_t items = ((n >> tl) + B / 2) * per_tt + 4 * most_units;
     z.share_units = static_cast<int>(items < 4 * PG_SMS ? items : 4 * PG_SMS);
     z.share = up256(B * 8 + 4);
     all_units += z.share_units;
   }
   z.max_units = static_cast<int>(all_units);
   if (all_units > 0) {
-    z.chunk_o = up256(all_units * 512 * D * 4);
-    z.chunk_ml = up256(all_units * 512 * 8);
+    z.chunk_o = up256(all_units * z.unit_slots * 256 * D * 4);
+    z.chunk_ml = up256(all_units * z.unit_slots * 256 * 8);
     z.joins = up256(all_units * static_cast<int64_t>(sizeof(ChunkJoin)) + 16);
   }
   if (weights) z.lse = up256(n * H * 4);
@@ -1099,6 +1113,30 @@ static PagedSizes paged_sizes(int64_t n, int64_t B, int H, int h, int D, int64_t
   }
   z.total = z.part_o + z.part_ml + z.chunk_o + z.chunk_ml + z.joins + z.share + z.lse + z.scores;
   return z;
+}
+
+// Parts are sized for every sequence of a launch at once (1 024 of 40 new tokens over 4 096 would ask for 21 GB), so a call of many
+// sequences is made in launches of as many as this holds, one behind the other over the same workspace: by then each of them fills the GPU many
+// times over. A sequence's cuts are its own, so its results stay the same; a common front ends where a launch ends.
+static constexpr int64_t PG_ROOM = 2ll << 30;
+struct PagedPlan {
+  PagedSizes z;
+  int64_t seqs;  // of a launch
+};
+static PagedPlan paged_plan(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, int64_t window, bool weights, bool shared, int64_t room) {
+  PagedPlan p = {paged_sizes(n, B, H, h, D, max_q, max_len, window, weights, shared, B == 1), B};
+  int64_t launches = 1;
+  while (p.seqs > 1 && p.z.total - p.z.lse > room) {
+    const int64_t by_size = (p.z.total - p.z.lse) * launches / room;  // (rounded down: the least that could do)
+    launches = by_size > launches ? by_size : launches + 1;
+    p.seqs = (B + launches - 1) / launches;
+    p.z = paged_sizes(n, p.seqs, H, h, D, max_q, max_len, window, weights, shared, false);
+  }
+  return p;
+}
+// what the caller has been told to bring knows no window
+static PagedPlan paged_plan(int64_t n, int64_t B, int H, int h, int D, int64_t max_q, int64_t max_len, bool weights, bool shared) {
+  return paged_plan(n, B, H, h, D, max_q, max_len, 0, weights, shared, PG_ROOM);
 }
 
 template <int D>
@@ -1151,7 +1189,7 @@ extern "C" int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, i
                                                          int32_t weights, int32_t shared) {
   if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
   if (n < 0 || B < 0 || H <= 0 || Hkv <= 0 || H % Hkv || (D != 128 && D != 256) || max_q < 0 || max_len < 0) return SPINF_ERR_BAD_ARGUMENT;
-  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0, shared != 0);
+  const PagedSizes z = paged_plan(n, B, H, Hkv, D, max_q < n ? max_q : n, max_len, weights != 0, shared != 0).z;
   return z.too_large ? SPINF_ERR_TOO_LARGE : z.total;
 }
 
@@ -1173,7 +1211,9 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
   const int64_t mq = max_q < n ? max_q : n;
   const bool narrow = window > 0 && window < max_len;  // (a window of max_len slots holds everything: no window)
-  const PagedSizes z = paged_sizes(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr, shared && !narrow);
+  PagedPlan plan = paged_plan(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr, shared && !narrow);
+  if (narrow) plan = paged_plan(n, B, H, Hkv, D, mq, max_len, window, weights_out != nullptr, false, plan.z.total - plan.z.lse);  // more sequences fit in
+  const PagedSizes& z = plan.z;
   if (z.too_large) return SPINF_ERR_TOO_LARGE;
   SPINF_CHECK_ARG(z.total == 0 || (workspace && workspace_bytes >= z.total && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0));
   int dev = 0;
@@ -1185,7 +1225,6 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   s.table_pitch = table_pitch;
   s.lens = lens;
   s.cu = cu;
-  s.B = B;
   s.n_pages = static_cast<int>(n_pages);
   s.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   s.max_len = static_cast<int>(max_len);
@@ -1208,6 +1247,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   a.seq_parts = z.seq_parts;
   a.chunk_rows = z.chunk_rows;
   a.only = B == 1 && mq > 0 ? class_of(mq * a.group, z.chunk_rows) : 0;
+  a.unit_slots = z.unit_slots;
   a.max_units = z.max_units;
   a.fronts_only = z.share_units > 0 && mq * a.group <= z.chunk_rows;
   auto take = [&](int64_t bytes) {
@@ -1240,6 +1280,18 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   const PagedPool vp = {v_pages, n_pages, page, Hkv, D, v_strides_host[0], v_strides_host[1], v_strides_host[2]};
   const int max_splits = z.seq_parts ? 2 : 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return D == 256 ? launch_paged<256>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, z.share_units, st, dev, status)
-                  : launch_paged<128>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, z.share_units, st, dev, status);
+  for (int64_t b = 0; b < B; b += plan.seqs) {
+    s.B = static_cast<int>(plan.seqs < B - b ? plan.seqs : B - b);
+    s.table = table + b * table_pitch;
+    s.lens = lens + b;
+    s.cu = cu + b;
+    if (weights_out) {
+      w.in = weights_in ? weights_in + b * w.in_seq : nullptr;
+      w.out = weights_out + b * w.out_seq;
+    }
+    const int r = D == 256 ? launch_paged<256>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, z.share_units, st, dev, status)
+                           : launch_paged<128>(kp, vp, s, a, weights_out ? &w : nullptr, mq, max_splits, z.share_units, st, dev, status);
+    if (r) return r;
+  }
+  return 0;
 }

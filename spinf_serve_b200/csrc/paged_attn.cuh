@@ -21,7 +21,8 @@ struct PagedAttnArgs {
   float* part_o;
   float2* part_ml;
   int64_t seq_parts;
-  // cut items of the chunk kernel: 256 rows twice per unit, and what to join
+  // cut items of the chunk kernel: 256 rows once or twice per unit, and what to join
+  int unit_slots;
   float* chunk_o;
   float2* chunk_ml;
   ChunkJoin* joins;  // [max_units]

@@ -106,7 +106,7 @@ struct ChunkWalk {
       // parts are the first segments of their units. A front is never whole: its one part is joined with the sequences' own splits
       if (part == 1 || (join.b1 && c.parts == 1)) {
         join.pieces = c.parts;
-        join.first = (unit - part) * 2;
+        join.first = (unit - part) * a.unit_slots;
         join.row0 = q.row0, join.nq = q.nq;
         join.tok0 = tt << c.tok_log2;
         join.h0 = item / a.sets * a.group + (item % a.sets << a.hp_log2);
@@ -125,7 +125,7 @@ struct ChunkWalk {
       } else if (c.begin(u - 1) <= w - off) {  // the first unit that begins inside this item
         const int w0 = w - off;
         join.pieces = c.unit_of(w0 + nt - 1) - u + 2;
-        join.first = (unit - 1) * 2 + (c.begin(u - 1) < w0 ? 1 : 0);
+        join.first = (unit - 1) * a.unit_slots + (c.begin(u - 1) < w0 ? 1 : 0);
         join.row0 = q.row0, join.nq = q.nq;
         join.tok0 = tt << c.tok_log2;
         join.h0 = item / a.sets * a.group + (item % a.sets << a.hp_log2);
@@ -153,7 +153,7 @@ struct ChunkWalk {
     g.ta = t0 + off;
     g.tb = g.ta + len;
     c.slots(q, a, tt, g.lo, g.hi);
-    g.part = len == nt && q.cap == PG_NO_CAP ? -1 : it * 2 + (first ? 0 : 1);
+    g.part = len == nt && q.cap == PG_NO_CAP ? -1 : it * a.unit_slots + (first ? 0 : 1);  // (one slot: units are parts, of one segment each)
     first = false;
     w += len;
     return true;
@@ -1078,12 +1078,13 @@ paged_two_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 // CTAs (x, y) over units `it`: the item that the unit is the first to begin inside of, as the planning warps have left word; 16 of its 256 rows, a
 // warp per row, the pieces added in the order of the units (an item in nine parts is a chain of loads for a row, so rows side by side)
 static constexpr int JOIN_ROWS = 16;
-template <int D>
+template <int D, int SLOTS>  // of 256 rows a unit has
 __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s, const PagedAttnArgs a, int* __restrict__ status) {
   pdl_trigger();
   pdl_wait();
   constexpr int V = D / 128;  // float4 per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int APART = SLOTS * 256;  // rows between an item's further pieces
   const int total = *a.n_units, ql = 7 - a.hp_log2;
   for (int it = blockIdx.x; it < total; it += gridDim.x) {
     const ChunkJoin join = a.joins[it];
@@ -1093,10 +1094,10 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s
     for (int r = blockIdx.y * JOIN_ROWS + warp; r < (blockIdx.y + 1) * JOIN_ROWS; r += 8) {
       const int in = r & 127, tok = join.tok0 + ((r >> 7) << ql) + (in & ((1 << ql) - 1)), head = join.h0 + (in >> ql);
       if (tok >= join.nq) continue;
-      const int64_t at0 = first + r, at = static_cast<int64_t>(it) * 512 + r;  // further pieces: 512 rows apart
+      const int64_t at0 = first + r, at = static_cast<int64_t>(it) * APART + r;
       float m = a.chunk_ml[at0].x;
 #pragma unroll 4
-      for (int y = 0; y <= last; ++y) m = fmaxf(m, a.chunk_ml[at + y * 512].x);
+      for (int y = 0; y <= last; ++y) m = fmaxf(m, a.chunk_ml[at + y * APART].x);
       int splits = 0;  // the row's own, behind the front it shares
       int64_t own = 0, own_step = 0;
       if (join.b1) {
@@ -1116,7 +1117,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s
       for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int y = -1; y <= last; ++y) {
-        const int64_t from = y < 0 ? at0 : at + y * 512;
+        const int64_t from = y < 0 ? at0 : at + y * APART;
         const float2 ml = a.chunk_ml[from];
         const float f = fast_exp2(ml.x + neg_m);
         l = fmaf(f, ml.y, l);
@@ -1445,7 +1446,8 @@ static int launch_chunk(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   }
   SPINF_CUDA_OK(launch_after(kern, dim3(static_cast<unsigned>(D == 256 ? sm_count() / 2 * 2 : sm_count())), dim3(CHUNK_THREADS), st, L::TOTAL,
                              D == 256 ? 2 : 1, early, tmQ, tmK, tmV, s, a, status));
-  SPINF_CUDA_OK(launch_after(paged_chunk_join_kernel<D>, dim3(static_cast<unsigned>(a.max_units < PG_SMS ? a.max_units : PG_SMS), 256 / JOIN_ROWS), dim3(256), st, 0, 1, true, s, a, status));
+  const auto join = a.unit_slots == 1 ? paged_chunk_join_kernel<D, 1> : paged_chunk_join_kernel<D, 2>;
+  SPINF_CUDA_OK(launch_after(join, dim3(static_cast<unsigned>(a.max_units < PG_SMS ? a.max_units : PG_SMS), 256 / JOIN_ROWS), dim3(256), st, 0, 1, true, s, a, status));
   if (!w) return 0;
   CUtensorMap tmQw, tmKw;
   if ((r = make_tmap_2d(&tmQw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, s.n, static_cast<uint64_t>(a.H) * D, a.q_pitch * 2, 64, 64 / hp))) return r;

@@ -810,3 +810,47 @@ def test_a_row_whose_scores_are_all_minus_infinity_weighs_nothing(dev, H, h, D, 
         cu, lens = torch.tensor([0, n - 1], dtype=torch.int32, device=dev), o["lens_t"] - 1
         ops.paged_attention(q, o["k"], o["v"], o["table"], lens, cu, c.max_q, D**-0.5, weights=rest)
     assert torch.equal(w[..., :300], rest[..., :300])
+
+
+@pytest.mark.parametrize("window", [None, 1000])
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (32, 16, 128)])
+def test_more_sequences_than_one_launch_holds(dev, H, h, D, window):
+    """chunks, branches, steps and sequences without rows whose parts pass the workspace's bound: the call is made in several launches, and
+    every sequence's bits are those it has alone; with weights, and asked to look for common fronts"""
+    B, page, L = 400, 64, 4100
+    g = torch.Generator(device=dev).manual_seed(D)
+    width = -(-(L + 41) // page)
+    shared = 4096 // page
+    k, v = (torch.randn((shared + 2 * B, h, page, D), generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    table = torch.full((B, width), -1, dtype=torch.int32, device=dev)
+    table[:, :shared] = torch.arange(shared, device=dev)
+    own = shared + torch.arange(2 * B, device=dev).view(B, 2)
+    table[:, shared:] = own[:, : width - shared].to(torch.int32)
+    news = torch.tensor([(40, 33, 1, 12, 0, 40, 40, 17)[b % 8] for b in range(B)])
+    lens = (4096 + news + torch.arange(B) % 5).to(torch.int32).to(dev)
+    cu = torch.zeros(B + 1, dtype=torch.int32)
+    cu[1:] = news.cumsum(0)
+    n = int(cu[-1]) + 3
+    q = torch.randn((n, H, D), generator=g, device=dev, dtype=torch.bfloat16)
+    assert _lib.lib().spinf_paged_attention_workspace_bytes(n, B // 3, H, h, D, 40, width * page, 0, 0) > 1 << 29  # (the whole of it would pass the bound)
+    out = torch.full((n, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    on = cu.to(dev)
+    ops.paged_attention(q, k, v, table, lens, on, 40, D**-0.5, window=window, out=out, shared=False)
+    w, w_out = torch.rand((B, h, width * page), generator=g, device=dev), torch.full((B, h, width * page), -3.0, device=dev)
+    weighed = ops.paged_attention(q, k, v, table, lens, on, 40, D**-0.5, window=window, weights=w, weights_out=w_out, decay=0.5)
+    assert (out[int(cu[-1]) :] == 7.0).all()
+    together = ops.paged_attention(q, k, v, table, lens, on, 40, D**-0.5, window=window, shared=True)
+    for b in sorted({0, 1, 2, 3, 4, 5, 99, 100, 131, 132, 133, 134, 135, 199, 200, 201, 265, 266, 267, 268, 269, 397, 398, 399}):
+        r0, r1 = int(cu[b]), int(cu[b + 1])
+        cu1 = torch.tensor([0, r1 - r0], dtype=torch.int32, device=dev)
+        for weights in (None, w[b : b + 1]):
+            w1 = None if weights is None else torch.full_like(weights, -3.0)
+            # (beside an empty neighbour, so that it takes the kernel of its own rows)
+            one = ops.paged_attention(q[r0:r1], k, v, table[[b, b]], torch.stack([lens[b], lens[b] * 0]), torch.cat([cu1, cu1[1:]]), 40, D**-0.5, window=window, shared=False,
+                                      weights=None if weights is None else weights.repeat(2, 1, 1), weights_out=None if weights is None else (w2 := w1.repeat(2, 1, 1)), decay=0.5)
+            assert torch.equal(one, (out if weights is None else weighed)[r0:r1]), b
+            if weights is not None:
+                assert torch.equal(w2[0], w_out[b]), b
+        off = (together[r0:r1].double() - out[r0:r1].double()).abs()
+        assert r0 == r1 or off.max() <= 3 * BF * float(v.abs().max()), b  # (the same sums in another order, p rounded against another maximum)
+    assert torch.equal(together[: int(cu[-1])], out[: int(cu[-1])]) == (window is not None)

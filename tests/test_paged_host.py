@@ -474,3 +474,18 @@ def test_a_chunk_alone_asks_for_no_scores(H, h, D):
         assert _room(2048, 1, H, h, D, 2048, max_len, 1) - _room(2048, 1, H, h, D, 2048, max_len, 0) <= 2048 * H * 4
         assert _room(2048, 1, H, h, D, 2048, max_len, 1) <= 150 * 512 * (D * 4 + 8 + 32) + 2048 * H * 4
     assert _room(1, 1, H, h, D, 1, 4096, 1) > 4096 * H * 4  # a step keeps its scores
+
+
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (32, 16, 128), (24, 4, 256), (8, 1, 128)])
+def test_the_workspace_of_many_sequences_is_bounded(H, h, D):
+    """whatever the number of sequences: beside the rows' lse two gigabytes (a sequence alone may need more, where it is very long and
+    its scores are kept)"""
+    for B in (56, 256, 1024):
+        for max_q, max_len in ((1, 4096), (12, 2012), (40, 4136), (300, 20000), (2048, 131072), (1, 1 << 20)):
+            n = min(B * max_q, 1 << 20)
+            for shared in (0, 1):
+                assert 0 <= _room(n, B, H, h, D, max_q, max_len, 0, shared) <= 2 << 30, (B, max_q, max_len)
+            if max_len < 1 << 20:
+                assert 0 < _room(n, B, H, h, D, max_q, max_len, 1) <= (2 << 30) + n * H * 4 + 256
+    # 56 questions of 40 tokens over 4 096: one slot of 256 rows per part, as many parts as are made
+    assert _room(56 * 40, 56, 16, 8, 256, 40, 4136) < 1300 << 20
