@@ -463,10 +463,12 @@ int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int32_t H, int
  * over the sequence's rows and the heads that share kv head g, for j < lens[b]; the two may be the same tensor; with decay 0
  * weights_in is not read. out lies apart from q, its rows behind cu[B] are left as they were. A sequence's results do not depend on
  * the other sequences of the call (a call of one sequence takes the kernel that max_q asks for, a call of several each sequence's
- * own rows), with `shared` but for the sequences it shares pages with. shared: look for neighbouring sequences (with up to 128 rows per
- * kv head and head set) whose tables begin with the same pages, at least 1 024 tokens of them and 128 MB of reading saved, and read
- * those once for all of their rows (the same sums, added in another order; without window and weights). The rows that share an item of work (up to 256 rows of neighbouring tokens) share their slots' values: those that none
- * of them sees never reach a result, whatever they hold; a value that is not finite in a slot that one of them sees may make
+ * own rows). shared: look for neighbouring sequences (with up to 128 rows per kv head and head set) whose tables begin with the same
+ * pages, at least 1 024 tokens of them and 128 MB of reading saved, and read those once for all of their rows (the same sums, added in
+ * another order; without window and weights). Which sequences are read together then depends on the call: on their neighbours' tables,
+ * and on the room, which the groups take in the call's order (the last ones of many, and one of very many rows, stay apart); so the
+ * last bits of a result may, too. The rows that share an item of work (up to 256 rows of neighbouring tokens) share their slots'
+ * values: those that none of them sees never reach a result, whatever they hold; a value that is not finite in a slot that one of them sees may make
  * all of them NaN. */
 int64_t spinf_paged_attention_workspace_bytes(int64_t n, int64_t B, int32_t H, int32_t Hkv, int32_t D, int64_t max_q, int64_t max_len,
                                               int32_t weights, int32_t shared);

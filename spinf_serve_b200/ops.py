@@ -797,7 +797,9 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
     call's sums over rows and heads of the group, for the slots below lens[b] (weights_out None: in place). workspace: optional contiguous uint8
     tensor reused between calls on one stream; out must not overlap q. shared: look for neighbouring sequences whose tables begin with
     the same pages (branches of one content) and read those once for all of them (None: where the pool has less than an eighth of the
-    pages that this many sequences of max_len tokens would need; looking in vain costs up to 20 us)."""
+    pages that this many sequences of max_len tokens would need; looking in vain costs up to 20 us). A sequence's bits depend on its own
+    tokens only, where it is read together with others on which they are, too: on its neighbours in the call, and on the room that groups
+    ahead of its own have left."""
     if weights is not None and weights_out is None:
         weights_out = weights
     got = _lib.paged_bind().attention(q, k_pages, v_pages, table, lens, cu, weights, weights_out, out, workspace, max_q, window, max_len, shared, scale, decay)

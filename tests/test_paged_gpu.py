@@ -854,3 +854,20 @@ def test_more_sequences_than_one_launch_holds(dev, H, h, D, window):
         off = (together[r0:r1].double() - out[r0:r1].double()).abs()
         assert r0 == r1 or off.max() <= 3 * BF * float(v.abs().max()), b  # (the same sums in another order, p rounded against another maximum)
     assert torch.equal(together[: int(cu[-1])], out[: int(cu[-1])]) == (window is not None)
+
+
+def test_a_group_that_finds_no_room_stays_apart(dev):
+    """what the documentation says of `shared`: a group alone is read together, behind others that have taken the room it is not; either way
+    it is right, and the call repeats itself"""
+    H, h, D, page = 8, 8, 128, 64
+    f = _worth(9, h, D)
+    c = Fronts(dev, H, h, D, page, [(f, [(f + 9 + i, 2) for i in range(9)]) for _ in range(12)], seed=2)
+    got, apart, o = c.attend(shared=True), c.attend(shared=False), c.on
+    for b0, in_call in ((c.first[0], got), (c.first[-1], None)):
+        alone = ops.paged_attention(c.rows(o["q"], b0, 9).clone(), o["k"], o["v"], o["table"][b0 : b0 + 9], o["lens_t"][b0 : b0 + 9], o["cu"][b0 : b0 + 10] - o["cu"][b0], 2,
+                                    D**-0.5, shared=True)
+        assert not torch.equal(alone, c.rows(apart, b0, 9))
+        assert torch.equal(alone, c.rows(got, b0, 9)) == (in_call is not None)
+    assert torch.equal(c.rows(got, c.first[-1], 9), c.rows(apart, c.first[-1], 9))
+    c.check(got, [0, 99, 107])
+    assert torch.equal(c.attend(shared=True)[:-1], got[:-1])
