@@ -489,6 +489,9 @@ int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, int32_t pag
                       int64_t max_len, const float* weights, int64_t w_seq, int64_t w_head, int64_t keep, int64_t recent,
                       const int32_t* new_table, int64_t new_pitch, int32_t* new_lens, int32_t* kept, float* weights_out, void* stream);
 
+/* Kernels that the calling thread's last spinf_paged_append, _attention or _evict has launched. */
+int64_t spinf_paged_launches(void);
+
 #ifdef __cplusplus
 }
 #endif

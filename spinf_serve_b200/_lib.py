@@ -91,6 +91,7 @@ SIGNATURES = {
         ctypes.c_int,
         [_p, _i64, _i64, _i32, _i32, _i32, _p, _p, _i64, _i32, _p, _p, _p, _i64, _p, _p, _i32, _i64, _i64, _i32, _i32, _f32, _p, _p, _p, _f32, _p, _i64, _p, _i64, _p],
     ),
+    "spinf_paged_launches": (_i64, []),
     "spinf_paged_evict": (
         ctypes.c_int,
         [_p, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _i64, _p, _i32, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p],

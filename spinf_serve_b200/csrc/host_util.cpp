@@ -64,6 +64,8 @@ int make_tmap_3d(CUtensorMap* out, CUtensorMapDataType dt, int elem_bytes, const
   return r == CUDA_SUCCESS ? 0 : SPINF_ERR_TENSORMAP;
 }
 
+thread_local int64_t paged_launches = 0;
+
 // (64 dims, rows of a page, 64-dim slabs of a head's row, heads, pages): rank 5, the most a tensor map has
 int make_tmap_pages(CUtensorMap* out, const PagedPool& p, uint32_t box_rows, uint32_t box_slabs) {
   EncodeTiledFn fn = encode_tiled_fn();

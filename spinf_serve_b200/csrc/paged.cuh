@@ -142,6 +142,7 @@ inline cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
+  ++paged_launches;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

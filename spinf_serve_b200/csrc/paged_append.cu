@@ -166,6 +166,7 @@ extern "C" int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int
                                   int32_t norm_v, void* q_out, void* k_pages, void* v_pages, int64_t n_pages, int32_t page,
                                   const int64_t* k_strides_host, const int64_t* v_strides_host, const int32_t* table,
                                   int64_t table_pitch, int32_t width, const int32_t* lens, const int32_t* cu, int32_t B, void* stream) {
+  paged_launches = 0;
   if (n == 0 || (B == 0 && !q_out)) return 0;  // nothing to do: the row pointers may be null
   SPINF_CHECK_ARG(qkv && k_pages && v_pages && k_strides_host && v_strides_host && n > 0 && B >= 0);
   SPINF_CHECK_ARG(B == 0 || (table && lens && cu && width > 0 && table_pitch >= width));  // (no sequence: q's rows are made all the same)
@@ -219,6 +220,7 @@ extern "C" int spinf_paged_append(const void* qkv, int64_t pitch, int64_t n, int
   const int64_t most = 2ll * sm_count();  // two CTAs an SM
   const int64_t grid = n < most ? n : most;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ++paged_launches;
   if (D == 256)
     paged_append_kernel<256><<<static_cast<unsigned>(grid), 256, 0, st>>>(a, s, status);
   else

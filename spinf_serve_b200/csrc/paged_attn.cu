@@ -1160,6 +1160,7 @@ static int launch_paged(const PagedPool& kp, const PagedPool& vp, const PagedSeq
   if (share_units > 0) {
     PagedSeqs plain = s;
     plain.share = nullptr;
+    ++paged_launches;
     paged_share_kernel<<<1, 1024, 0, st>>>(plain, a, const_cast<int32_t*>(s.share), share_units, status);
     SPINF_CUDA_OK(cudaGetLastError());
   }
@@ -1199,6 +1200,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
                                      const int32_t* cu, int32_t B, int64_t max_q, int64_t max_len, int32_t window, int32_t shared, float scale,
                                      const float* weights_in, float* weights_out, const int64_t* weight_strides_host, float decay,
                                      void* out, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
+  paged_launches = 0;
   if (B == 0 || (n == 0 && !weights_out)) return 0;  // nothing to do: the row pointers may be null
   SPINF_CHECK_ARG(k_pages && v_pages && k_strides_host && v_strides_host && table && lens && cu && n >= 0 && B > 0);
   SPINF_CHECK_ARG(n == 0 || (q && out));
@@ -1295,3 +1297,5 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   }
   return 0;
 }
+
+extern "C" int64_t spinf_paged_launches(void) { return paged_launches; }

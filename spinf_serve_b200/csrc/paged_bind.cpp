@@ -168,6 +168,9 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// kernels that this thread's last call has launched, whichever way it went
+PyObject* launches(PyObject*, PyObject*) { return PyLong_FromLongLong(spinf_paged_launches()); }
+
 // (operator, its tensors and the numbers of its key, the checked layout): the next call with this key is made from here
 PyObject* learn(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
@@ -197,6 +200,7 @@ PyMethodDef METHODS[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(evict)), METH_FASTCALL, nullptr},
+    {"launches", launches, METH_NOARGS, nullptr},
     {"learn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(learn)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -213,6 +213,7 @@ extern "C" int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, 
                                  const int32_t* lens, int32_t B, int64_t max_len, const float* weights, int64_t w_seq, int64_t w_head,
                                  int64_t keep, int64_t recent, const int32_t* new_table, int64_t new_pitch, int32_t* new_lens,
                                  int32_t* kept, float* weights_out, void* stream) {
+  paged_launches = 0;
   if (B == 0) return 0;  // nothing to do: the pointers may be null
   SPINF_CHECK_ARG(k_pages && v_pages && k_strides_host && v_strides_host && table && lens && new_table && new_lens && kept && B > 0);
   SPINF_CHECK_ARG(Hkv > 0 && (D == 128 || D == 256) && n_pages > 0 && n_pages < (1ll << 31));
@@ -250,6 +251,7 @@ extern "C" int spinf_paged_evict(void* k_pages, void* v_pages, int64_t n_pages, 
   a.k_page = k_strides_host[0], a.k_head = k_strides_host[1], a.k_row = k_strides_host[2];
   a.v_page = v_strides_host[0], a.v_head = v_strides_host[1], a.v_row = v_strides_host[2];
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ++paged_launches;
   paged_select_kernel<<<dim3(Hkv, B), SEL_THREADS, 0, st>>>(s, a, status);
   SPINF_CUDA_OK(cudaGetLastError());
   const int64_t per_cta = (256 / (D / 8)) * 4, blocks = (keep + per_cta - 1) / per_cta;

@@ -702,7 +702,7 @@ def paged_append(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq=None, wk=
         q = _append_first(qkv, H, Hkv, D, k_pages, v_pages, table, lens, cu, wq, wk, cos, sin, eps, plus1, norm_v)
     elif type(q) is int:
         check(q, "paged_append")
-    COUNTS["launches"] += 1
+    COUNTS["launches"] += _lib.paged_bind().launches()
     return q
 
 
@@ -807,7 +807,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, cu, max_q, scale, window=N
         got = _attention_first(q, k_pages, v_pages, table, lens, cu, max_q, scale, window, weights, weights_out, decay, max_len, out, workspace, shared)
     elif type(got) is int:
         check(got, "paged_attention")
-    COUNTS["launches"] += 2 if weights is None else 3
+    COUNTS["launches"] += _lib.paged_bind().launches()
     return got
 
 
@@ -873,7 +873,7 @@ def paged_evict(k_pages, v_pages, table, lens, weights, keep, recent, new_table,
         got = _evict_first(k_pages, v_pages, table, lens, weights, keep, recent, new_table, max_len)
     elif type(got) is int:
         check(got, "paged_evict")
-    COUNTS["launches"] += 2
+    COUNTS["launches"] += _lib.paged_bind().launches()
     return got
 
 

@@ -871,3 +871,40 @@ def test_a_group_that_finds_no_room_stays_apart(dev):
     assert torch.equal(c.rows(got, c.first[-1], 9), c.rows(apart, c.first[-1], 9))
     c.check(got, [0, 99, 107])
     assert torch.equal(c.attend(shared=True)[:-1], got[:-1])
+
+
+def test_launches_are_counted(dev):
+    """COUNTS["launches"] against the kernels that the profiler sees"""
+    from torch.profiler import ProfilerActivity, profile
+
+    def kernels(f):
+        f()
+        torch.cuda.synchronize()
+        before = ops.COUNTS["launches"]
+        with profile(activities=[ProfilerActivity.CUDA]) as prof:
+            f()
+            torch.cuda.synchronize()
+        return ops.COUNTS["launches"] - before, sum(e.count for e in prof.key_averages() if "paged_" in e.key)
+
+    H, h, D, page = 16, 8, 256, 64
+    one, chunk, mixed = (Call(dev, H, h, D, page, x, seed=1) for x in ([(70, 1)], [(700, 200)], [(300, 1), (200, 12), (400, 100)]))
+    f = _worth(9, h, D)
+    fronts = Fronts(dev, H, h, D, page, [(f, [(f + 20, 2)] * 9)], seed=3)
+    seen = []
+    for call in (lambda: one.attend(), lambda: chunk.attend(), lambda: mixed.attend(), lambda: mixed.attend(weights=torch.zeros((3, h, 448), device=dev)),
+                 lambda: chunk.attend(weights=torch.zeros((1, h, 704), device=dev)), lambda: fronts.attend(shared=True)):
+        got, want = kernels(call)
+        if want == 0:
+            pytest.skip("the profiler sees no kernels here")
+        assert got == want
+        seen.append(got)
+    assert len(set(seen)) > 3, seen
+    c = Call(dev, H, h, D, page, [(300, 2)], seed=2, spare=4)
+    o = c.on
+    qkv = torch.randn((2, (H + 2 * h) * D), device=dev).to(torch.bfloat16)
+    new = c.free[:2].view(1, 2).to(dev)
+    for call in (lambda: ops.paged_append(qkv, H, h, D, o["k"], o["v"], o["table"], o["lens_t"], o["cu"]),
+                 lambda: ops.paged_append(qkv[:0], H, h, D, o["k"], o["v"], o["table"], o["lens_t"], o["cu"] * 0),
+                 lambda: ops.paged_evict(o["k"], o["v"], o["table"], o["lens_t"], None, 100, 100, new)):
+        got, want = kernels(call)
+        assert got == want
