@@ -141,6 +141,15 @@ def lib():
     return _lib
 
 
+def bind_made_for() -> str:
+    """what paged_bind.so is compiled against"""
+    import sys
+
+    import torch
+
+    return f"torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
 def paged_bind():
     """the paged operators' short way into the library (csrc/paged_bind.cpp)"""
     global _bind
@@ -155,8 +164,14 @@ def paged_bind():
                 if not os.path.exists(BIND_PATH):
                     raise SpinfError(f"{BIND_PATH} is missing: build it with `python -m spinf_serve_b200.csrc.build`")
                 spec = importlib.util.spec_from_file_location("paged_bind", BIND_PATH)
-                module = importlib.util.module_from_spec(spec)
-                spec.loader.exec_module(module)
+                try:
+                    module = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(module)
+                    made_for = module.made_for
+                except (ImportError, AttributeError) as e:
+                    made_for = str(e)
+                if made_for != bind_made_for():
+                    raise SpinfError(f"{BIND_PATH} is not made for {bind_made_for()} ({made_for}): build it with `python -m spinf_serve_b200.csrc.build`")
                 _bind = module
     return _bind
 

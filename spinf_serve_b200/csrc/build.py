@@ -11,6 +11,8 @@ import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
 
+from spinf_serve_b200._lib import bind_made_for
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libspinf_b200.so")
 BIND = os.path.join(HERE, "paged_bind.so")
@@ -77,9 +79,17 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def bind_stale() -> bool:
+    """paged_bind.so is missing, older than its sources, or made for another torch or interpreter (it says which)"""
+    if _stale(BIND, [os.path.join(HERE, "paged_bind.cpp"), __file__, _headers()[-1]]):
+        return True
+    with open(BIND, "rb") as f:
+        return bind_made_for().encode() + b"\0" not in f.read()
+
+
 def _build_bind(force):
     src = os.path.join(HERE, "paged_bind.cpp")
-    if not (force or _stale(BIND, [src, __file__, _headers()[-1]])):
+    if not (force or bind_stale()):
         return
     import sysconfig
 
@@ -88,7 +98,7 @@ def _build_bind(force):
     root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(NVCC), "..", "include")
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    cmd += ["-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    cmd += [f'-DSPINF_MADE_FOR="{bind_made_for()}"', "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include")]
     cmd += ["-isystem", sysconfig.get_paths()["include"], "-isystem", cuda, src, "-o", BIND, "-L" + HERE, "-lspinf_b200", "-Wl,-rpath,$ORIGIN"]
     cmd += ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -208,4 +208,8 @@ PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "paged_bind", nullptr, -1, METHODS,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_paged_bind() { return PyModule_Create(&MODULE); }
+PyMODINIT_FUNC PyInit_paged_bind() {
+  PyObject* m = PyModule_Create(&MODULE);
+  if (m) PyModule_AddStringConstant(m, "made_for", SPINF_MADE_FOR);  // (the loader and the build look at it)
+  return m;
+}

@@ -489,3 +489,16 @@ def test_the_workspace_of_many_sequences_is_bounded(H, h, D):
                 assert 0 < _room(n, B, H, h, D, max_q, max_len, 1) <= (2 << 30) + n * H * 4 + 256
     # 56 questions of 40 tokens over 4 096: one slot of 256 rows per part, as many parts as are made
     assert _room(56 * 40, 56, 16, 8, 256, 40, 4136) < 1300 << 20
+
+
+def test_the_binding_is_made_anew_for_another_torch(monkeypatch):
+    """its layout follows torch's headers and the interpreter: neither the build nor the loader takes one that was made for others"""
+    from spinf_serve_b200.csrc import build
+
+    monkeypatch.setattr(build, "_stale", lambda *a: False)  # (by their times it is newer than its sources)
+    assert not build.bind_stale()
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    assert build.bind_stale()
+    monkeypatch.setattr(_lib, "_bind", None)
+    with pytest.raises(_lib.SpinfError, match="1.0.0"):
+        _lib.paged_bind()
