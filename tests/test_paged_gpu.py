@@ -908,3 +908,67 @@ def test_launches_are_counted(dev):
                  lambda: ops.paged_evict(o["k"], o["v"], o["table"], o["lens_t"], None, 100, 100, new)):
         got, want = kernels(call)
         assert got == want
+
+
+def _levels(kind, n, g):
+    """score level of every slot, in nats: what a row's maximum does as its tiles go by"""
+    s = torch.arange(n) / n
+    if kind == "rising":
+        return -85 + 170 * s
+    if kind == "falling":
+        return 85 - 170 * s
+    if kind == "steps":  # a level of its own for every 64 slots: up by more than the threshold, down, up by less
+        return ((torch.rand((n + 63) // 64, generator=g) - 0.5) * 170).repeat_interleave(64)[:n]
+    return torch.where(torch.arange(n) % 190 == 100, 60.0 * s, -60.0 + 0 * s)  # peaks
+
+
+@pytest.mark.parametrize("kind", ["normed", "rising", "falling", "steps", "peaks"])
+@pytest.mark.parametrize("window", [None, 300])
+@pytest.mark.parametrize("H,h,D", [(16, 8, 256), (8, 4, 128), (6, 1, 256), (8, 1, 128)])
+def test_scores_that_spread_widely(dev, H, h, D, window, kind):
+    """heads of unit mean square attended to with scale 1, as the stacks do, and levels that move a row's reference maximum up, by much and by
+    little, from tile to tile, part to part and half to half: outputs and weights of every kernel against the definition"""
+    seqs = [(900, 161), (700, 1), (650, 3), (1200, 40), (333, 333), (520, 12)]
+    c = Call(dev, H, h, D, 64, seqs, seed=D + H, spare=0)
+    g, e = c.gen, torch.where(torch.rand(D, generator=c.gen) < 0.5, -1.0, 1.0)
+    k, q = torch.full(c.k.shape, math.nan), None
+    for b, L in enumerate(c.lens):
+        s = torch.arange(L)
+        if kind == "normed":
+            rows = torch.randn((L, h, D), generator=g)
+            rows = rows / rows.pow(2).mean(-1, keepdim=True).sqrt()
+        else:
+            rows = e * _levels(kind, L, g)[:, None, None] / D + 0.02 * torch.randn((L, h, D), generator=g)
+        k[c.table[b].long()[s // 64], :, s % 64] = rows
+    if kind == "normed":
+        q = torch.randn((c.n, H, D), generator=g)
+        q = q / q.pow(2).mean(-1, keepdim=True).sqrt()
+    else:
+        q = e * torch.tensor([1.0, 0.75, 0.5, 0.125])[torch.randint(0, 4, (c.n, H, 1), generator=g)]
+    c.k, c.q = k.to(torch.bfloat16), q.to(torch.bfloat16)
+    c.on["k"], c.on["q"] = c.k.to(dev), c.q.to(dev)
+    o, w = c.on, torch.zeros((len(seqs), h, 1216), device=dev)
+    want, weights, mag, big = OP.attention(c.q, c.k, c.v, c.table, c.lens, c.cu, 1.0, window)
+    check_out(c, ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], c.max_q, 1.0, window=window), want, mag, big)
+    check_out(c, ops.paged_attention(o["q"], o["k"], o["v"], o["table"], o["lens_t"], o["cu"], c.max_q, 1.0, window=window, weights=w, max_len=1200), want, mag, big)
+    rel = float(score_noise(c, big, 1200).max()) + 2.0**-20 + 1600 * 2.0**-24
+    for b, (L, n) in enumerate(seqs):
+        ref = weights[b]
+        assert ((w[b, :, :L].double().cpu() - ref).abs() <= rel * ref + 2.0**-126 * max(1, n) * H).all(), b  # (a p below the normal numbers is 0)
+        if n > 40:  # alone: an item in several parts, or none
+            cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+            rows = slice(int(c.cu[b]), int(c.cu[b]) + n)
+            one = ops.paged_attention(o["q"][rows], o["k"], o["v"], o["table"][b : b + 1], o["lens_t"][b : b + 1], cu, n, 1.0, window=window)
+            tol = BF * want[rows].abs() + (BF * (1 + BF) + score_noise(c, big[rows], 1200)[..., None]) * mag[rows] * (1 + BF) + 1e-30
+            assert ((one.double().cpu() - want[rows]).abs() <= tol).all(), b
+
+
+@pytest.mark.parametrize("H,h,D,page", [(16, 8, 256, 64), (32, 16, 128, 64)])
+def test_common_fronts_of_scores_that_spread_widely(dev, H, h, D, page):
+    f = _worth(20, h, D)
+    c = Fronts(dev, H, h, D, page, [(f, [(f + 12 + 9 * i, 12) for i in range(20)])], seed=D)
+    c.q *= 16  # (exact)
+    c.on["q"] *= 16
+    got = c.attend(shared=True)
+    assert not torch.equal(got[:-1], c.attend(shared=False)[:-1])
+    c.check(got, [0, 7, 19])
