@@ -941,8 +941,8 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, co
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int r = 0; r < all; ++r) {
     const int tok = r / a.group, hd = g * a.group + r % a.group, hi = base + tok, lo = a.window > 0 ? hi - a.window + 1 : 0;
-    const float lse = a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd];
-    if (lse == -INFINITY) continue;  // the row sees nothing, or all its scores are -inf: its output is 0, and it weighs nothing
+    const float l = a.lse[static_cast<int64_t>(q.row0 + tok) * a.H + hd];
+    const float lse = l == -INFINITY ? INFINITY : l;  // the row sees nothing, or all its scores are -inf: its output is 0, and it weighs nothing
     const float* src = a.scores + ((static_cast<int64_t>(b) * a.tok_cap + tok) * a.H + hd) * a.score_pitch + first + threadIdx.x;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
