@@ -3,8 +3,8 @@
 //   r = rsqrt(mean(x^2) + eps),  y = x r w,  y1' = y1 cos - y2 sin,  y2' = y2 cos + y1 sin  (halves of the rotary dimensions)
 // Everything in fp32 with one rounding at the end. (qkv_norm_rope rounds after every module's output, as the module code it stands
 // in for does; nothing else reads what this writes before the attention, so the intermediate roundings would only lose bits.)
-// A group of D / 8 lanes owns one head's row, 16 bytes a lane. Bound by HBM: 8 192 rows (32 / 16 heads of 128, rotary, norms) 62.8 us,
-// 270 MB read and written at 4.3 TB/s; one row each of 64 sequences 4.4 us, a launch and one chain of loads.
+// A group of D / 8 lanes owns one head's row, 16 bytes a lane. 8 192 rows (32 / 16 heads of 128, rotary, norms) 62.8 us, 270 MB read and
+// written at 4.3 TB/s where a copy has 6.5: one token ahead in flight, a page's rows written by many SMs at different moments; one row each of 64 sequences 4.4 us, a launch and one chain of loads.
 #include "common.cuh"
 #include "host_util.h"
 #include "paged.cuh"

@@ -8,12 +8,13 @@
 //
 // Both attention kernels: persistent CTAs, one per SM; an item is (sequence, 64-row tile, kv head, split of the keys). A producer warp
 // brings K and V pages in with TMA, 64 keys a stage, into one ring that runs ahead across items; the others compute with warp-level
-// products (a 128-row tensor-core tile would be 8 to 16 times empty) and a running maximum and sum in fp32. P is rounded to bf16 for
+// products (with the rows of q along M a 128-row tensor-core tile would be 8 to 16 times empty; with the keys there, as the weights of
+// chunks have them, it was not built) and a running maximum and sum in fp32. P is rounded to bf16 for
 // the product (its operands are 16 bit), which adds about what rounding the output to bf16 adds; the sum takes p unrounded.
 //
 // paged_step_kernel: each warp takes 16 keys against all rows and keeps a maximum, a sum and an output of its own, so that nothing but
 // the ring's barriers stands between a key's arrival and its use; the warps' shares are joined once per item. (With a shared maximum,
-// as in the rows kernel, 64 sequences of up to 8 192 tokens took 714 us, so 394.) S^T = K Q^T with the keys as rows: P^T is turned into
+// as in the rows kernel, 64 sequences of up to 8 192 tokens took 714 us, so 394 to 400.) S^T = K Q^T with the keys as rows: P^T is turned into
 // the second product's operand between lanes, without shared memory. Bound by HBM: 64 ragged steps (32 / 16 heads of 128) 394 us, 6.2
 // TB/s of K and V; 131 072 slots (24 / 4 heads of 256) 90 us, 6.0 TB/s; a few short sequences by latency: 4 x 1 501 tokens 19 us, of
 // which about 7 are the launches of the kernel and the join. Pages of 64 tokens and more are one copy a stage; of 32 tokens two (6.2
@@ -26,7 +27,7 @@
 // 2 012 (16 / 8 heads of 256) 224 us.
 //
 //   paged_share_kernel   finds neighbouring sequences that begin with the same pages (branches of one content). Their common front is then
-//                        read once for all of their rows, by the chunk kernels; the kernels here begin behind it: the 56 branches 98 us
+//                        read once for all of their rows, by the chunk kernels; the kernels here begin behind it: the 56 branches 100 us
 //                        (looking 6, few-row part 39, front 40, joins 13), 12 tokens over 16 384 each 1 500 -> 293 us.
 #include "paged_attn.cuh"
 
@@ -928,7 +929,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedSeqs s, c
 
 // weights_out[b][g][j] = decay weights[b][g][j] + sum over the sequence's rows of kv head g of p(row, j), for j < len; a thread owns
 // four keys, 256 apart, and adds their rows in order. Bound by reading the scores back (L2): 16 steps over up to 4 096 tokens (16 / 8 heads of
-// 256) 78 us with the attention, 6 us of them here. Scores are written and read once because the attention cannot weigh a key before
+// 256) 80 us with the attention, 6 us of them here. Scores are written and read once because the attention cannot weigh a key before
 // its row's last key is known; for a chunk they would be the larger part, so there they are computed again (paged_chunk.cu).
 __global__ void __launch_bounds__(256) paged_weight_kernel(const PagedSeqs s, const PagedAttnArgs a, const PagedWeightArgs w, int* __restrict__ status) {
   pdl_trigger();

@@ -7,7 +7,7 @@
 // row's reference maximum moves (and O is scaled) only when its maximum has outgrown it by more than 2^24.
 //   D 256 (paged_pair_kernel): a CTA pair, one tile of rows each (O takes half of tensor memory). The pair is there for K and V: 128
 //       rows alone would need 128 keys from L2 every 2 048 cycles, 64 bytes per cycle and SM, more than L2 delivers. Two S buffers; two
-//       groups of four softmax warps, each half the keys of every row. 2 048 tokens over 18 432 (16 / 8 heads of 256): 546 us, 2 970
+//       groups of four softmax warps, each half the keys of every row. 2 048 tokens over 18 432 (16 / 8 heads of 256): 508 to 558 us, about 2 970
 //       cycles a tile where the products take 2 048; the tensor pipe is 61 to 70 % busy, at a clock that the power limit has brought
 //       to about 1.6 GHz: 1 037 TFLOP/s of visible pairs.
 //   D 128 (paged_two_kernel): one CTA holds both tiles (S and O of each fill tensor memory) and a group of four softmax warps per tile.
@@ -1159,7 +1159,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedSeqs s
 // Item = 256 keys of a (sequence, kv head), both tiles of K resident in shared memory while the rows that see any of them stream by.
 // Bound by the exponentials and what surrounds them (256 x 64 a stage at 16 per cycle and SM: 1 024 cycles, the products 512 at D 128
 // and 1 024 at D 256; measured 2 050 a stage: reading S out of tensor memory and the instructions around each exponential share the
-// issue slots). 1 024 tokens over 8 192 (32 / 16 heads of 128): 290 us with the attention, about 135 of them here; scores kept in memory
+// issue slots). 1 024 tokens over 8 192 (32 / 16 heads of 128): 295 us with the attention, about 137 of them here; scores kept in memory
 // and read back took 2 500 for the same.
 template <int D>
 struct ChunkWeightSmem {
