@@ -7,6 +7,7 @@ to the slots that were attended to most (ops.paged_append, ops.paged_attention, 
 The host keeps the books (which pages a sequence holds, who shares them, how far it is); tables and lengths go to the device once per
 forward and serve all its layers."""
 
+import threading
 from dataclasses import dataclass, field
 
 import torch
@@ -170,7 +171,8 @@ class PagedCache:
 
 class PagedReader:
     """forward passes of a GemmaStack over a PagedCache. `read` takes a content in, `ask` runs questions that share it, `forward` is one
-    pass over new tokens of any sequences, `evict` cuts a sequence back"""
+    pass over new tokens of any sequences, `evict` cuts a sequence back. One call at a time, all on one stream: pages that are given back
+    are taken again without waiting for kernels that other streams still run on them"""
 
     def __init__(self, stack, n_pages: int, page: int = 64, chunk: int = 2048):
         cfg = stack.cfg
@@ -179,7 +181,7 @@ class PagedReader:
         self.stack, self.chunk = stack, chunk
         self.cache = PagedCache(stack.n_layers, cfg.kv_heads, cfg.head_dim, n_pages, page, stack.w.embed.device)
         self.scaling = 1.0  # the Gemma-style layers norm q and k and attend with scaling 1
-        self._step, self._weights = None, None
+        self._step, self._weights, self._busy = None, None, threading.Lock()
 
     # ---- the stack's attention (GemmaStack.forward, `attend`)
     def _attend(self, i, kind, q):
@@ -210,6 +212,14 @@ class PagedReader:
             raise RuntimeError("weights are kept for a sequence that is read alone")
         if not all(len(x) for x in ids) or len(seqs) > 1024:
             raise RuntimeError("every sequence of a forward (at most 1024) needs new tokens")
+        if not self._busy.acquire(blocking=False):
+            raise RuntimeError("a reader runs one forward at a time")
+        try:
+            return self._forward(seqs, ids, last, weigh)
+        finally:
+            self._busy.release()
+
+    def _forward(self, seqs, ids, last, weigh):
         st = self.cache.grow(seqs, [len(x) for x in ids])
         weights = None
         try:

@@ -502,3 +502,22 @@ def test_the_binding_is_made_anew_for_another_torch(monkeypatch):
     monkeypatch.setattr(_lib, "_bind", None)
     with pytest.raises(_lib.SpinfError, match="1.0.0"):
         _lib.paged_bind()
+
+
+def test_a_forward_inside_a_forward_is_refused(reader):
+    """(or beside it, from another thread: the layers would find the other's tables)"""
+    a, b = reader.read([1] * 20), reader.read([1] * 5)
+    plain, got = reader.stack.forward, []
+
+    def forward(*args, **kw):
+        with pytest.raises(RuntimeError, match="one forward at a time"):
+            reader.forward([b], [[1]])
+        got.append(1)
+        return plain(*args, **kw)
+
+    reader.stack.forward = forward
+    reader.forward([a], [[1, 2]])
+    assert got == [1] and (a.length, b.length) == (22, 5)
+    reader.stack.forward = plain
+    reader.forward([b], [[1]])
+    assert b.length == 6
