@@ -1214,7 +1214,7 @@ extern "C" int spinf_paged_attention(const void* q, int64_t q_pitch, int64_t n, 
   if (B > PG_MAX_SEQS) return SPINF_ERR_TOO_LARGE;
   const int64_t mq = max_q < n ? max_q : n;
   const bool narrow = window > 0 && window < max_len;  // (a window of max_len slots holds everything: no window)
-  PagedPlan plan = paged_plan(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr, shared && !narrow);
+  PagedPlan plan = paged_plan(n, B, H, Hkv, D, mq, max_len, weights_out != nullptr, shared != 0);
   if (narrow) plan = paged_plan(n, B, H, Hkv, D, mq, max_len, window, weights_out != nullptr, false, plan.z.total - plan.z.lse);  // more sequences fit in
   const PagedSizes& z = plan.z;
   if (z.too_large) return SPINF_ERR_TOO_LARGE;

@@ -972,3 +972,26 @@ def test_common_fronts_of_scores_that_spread_widely(dev, H, h, D, page):
     got = c.attend(shared=True)
     assert not torch.equal(got[:-1], c.attend(shared=False)[:-1])
     c.check(got, [0, 7, 19])
+
+
+def test_the_workspace_asked_for_is_enough_under_a_window(dev):
+    """at the C entry point, asked to look for common fronts too: the query knows no window, and the call no fronts under one"""
+    import ctypes
+
+    B, n_new, max_len, page, D = 256, 13, 1 << 20, 256, 256
+    g = torch.Generator(device=dev).manual_seed(3)
+    k, v = (torch.randn((B, 1, page, D), generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    table = torch.zeros((B, max_len // page), dtype=torch.int32, device=dev)
+    table[:, 0] = torch.arange(B, device=dev)
+    lens = torch.full((B,), 200, dtype=torch.int32, device=dev)
+    cu = (torch.arange(B + 1, device=dev) * n_new).to(torch.int32)
+    q = torch.randn((B * n_new, 1, D), generator=g, device=dev, dtype=torch.bfloat16)
+    lib, out = _lib.lib(), torch.zeros_like(q)
+    need = lib.spinf_paged_attention_workspace_bytes(B * n_new, B, 1, 1, D, 40, max_len, 0, 1)
+    room = torch.empty(need, dtype=torch.uint8, device=dev)
+    st = (ctypes.c_int64 * 3)(*k.stride()[:3])
+    for window in (0, 100, 1 << 19):
+        assert lib.spinf_paged_attention(q.data_ptr(), D, B * n_new, 1, 1, D, k.data_ptr(), v.data_ptr(), B, page, st, st, table.data_ptr(), table.stride(0), lens.data_ptr(),
+                                         cu.data_ptr(), B, 40, max_len, window, 1, D**-0.5, None, None, None, 1.0, out.data_ptr(), D, room.data_ptr(), need, _lib.raw_stream(0)) == 0
+        want = ops.paged_attention(q, k, v, table[:, :1].contiguous(), lens, cu, 40, D**-0.5, window=window or None, shared=False)
+        assert torch.equal(out, want)
